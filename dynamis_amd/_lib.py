@@ -16,7 +16,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # different options); the default is the in-tree build.
 LIB_PATH = os.environ.get("DYNAMIS_GRAPH_LIB") or os.path.join(_HERE, "libdynamis_graph.so")
 
-DG_F32, DG_F64, DG_I64, DG_I32 = 0, 1, 2, 3
+DG_F32, DG_F64, DG_I64, DG_I32, DG_BF16 = 0, 1, 2, 3, 4
+DG_NEIGHBOR_PAD = 64
 DG_OK, DG_ERR_INVALID, DG_ERR_WORKSPACE, DG_ERR_HIP, DG_ERR_RANGE, DG_ERR_CAPACITY = range(6)
 
 
@@ -62,6 +63,67 @@ class BatchDesc(ctypes.Structure):
     ]
 
 
+class NeighborDesc(ctypes.Structure):
+    """dg_neighbor_desc."""
+
+    _fields_ = [
+        ("n_edges", ctypes.c_int64),
+        ("n_nodes", ctypes.c_int64),
+        ("n_targets", ctypes.c_int64),
+        ("n_boundaries", ctypes.c_int32),
+        ("dist_dtype", ctypes.c_int32),
+    ]
+
+
+class NeighborTotals(ctypes.Structure):
+    """dg_neighbor_totals."""
+
+    _fields_ = [
+        ("n_entries", ctypes.c_int64),
+        ("longest", ctypes.c_int64),
+        ("long_rows", ctypes.c_int64),
+        ("long_entries", ctypes.c_int64),
+        ("grouped", ctypes.c_int32),
+        ("symmetric", ctypes.c_int32),
+    ]
+
+
+class NeighborLists(ctypes.Structure):
+    """dg_neighbor_lists."""
+
+    _fields_ = [
+        ("n_rows", ctypes.c_int64),
+        ("n_items", ctypes.c_int64),
+        ("order", ctypes.c_void_p),
+        ("ptr", ctypes.c_void_p),
+        ("idx", ctypes.c_void_p),
+        ("bucket", ctypes.c_void_p),
+        ("item_slot", ctypes.c_void_p),
+        ("item_first", ctypes.c_void_p),
+        ("chunk", ctypes.c_int32),
+        ("pad_", ctypes.c_int32),
+    ]
+
+
+class AttentionDesc(ctypes.Structure):
+    """dg_attention_desc."""
+
+    _fields_ = [
+        ("n_targets", ctypes.c_int64),
+        ("n_nodes", ctypes.c_int64),
+        ("ld_q", ctypes.c_int64),
+        ("ld_k", ctypes.c_int64),
+        ("ld_v", ctypes.c_int64),
+        ("ld_g", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("n_buckets", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 _lib = None
 
 _p = ctypes.c_void_p
@@ -80,6 +142,7 @@ def lib():
             "(python -m dynamis_amd.build, or __graft_entry__.build())")
     L = ctypes.CDLL(LIB_PATH)
     D = ctypes.POINTER(GraphDesc)
+    ND, NL, AD = ctypes.POINTER(NeighborDesc), ctypes.POINTER(NeighborLists), ctypes.POINTER(AttentionDesc)
     sig = {
         "dg_graph_workspace_size": (_sz, [D]),
         "dg_graph_count": (_i32, [D, _p, _p, _p, _sz, _p, _p]),
@@ -117,6 +180,16 @@ def lib():
         "dg_batch_count": (_i32, [ctypes.POINTER(BatchDesc), _p, _p, _p, _p, _p, _sz, _p]),
         "dg_batch_read_totals": (_i32, [ctypes.POINTER(BatchDesc), _p, ctypes.POINTER(_i64), ctypes.POINTER(_i64), _p]),
         "dg_batch_write": (_i32, [ctypes.POINTER(BatchDesc), _p, _p, _sz, _i64, _p, _p, _p, _p, _p]),
+        "dg_neighbors_workspace_size": (_sz, [ND]),
+        "dg_neighbors_by_target": (_i32, [ND, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _p, _sz, _p]),
+        "dg_neighbors_read_totals": (_i32, [ND, _p, ctypes.POINTER(NeighborTotals), _p]),
+        "dg_neighbors_sort_workspace_size": (_sz, [_i64]),
+        "dg_neighbors_by_source": (_i32, [ND, _i64, _p, _p, _p, _p, _p, _p, _sz, _p, _sz, _p]),
+        "dg_neighbors_parts_workspace_size": (_sz, [_i64]),
+        "dg_neighbors_parts": (_i32, [_p, _i64, _i32, _i64, _p, _p, _p, _sz, _p]),
+        "dg_attention_workspace_size": (_sz, [AD, NL, NL]),
+        "dg_attention_forward": (_i32, [AD, NL] + [_p] * 9 + [_sz, _p]),
+        "dg_attention_backward": (_i32, [AD, NL, NL] + [_p] * 12 + [_sz, _p]),
         "dg_last_error": (ctypes.c_char_p, []),
         "dg_version": (ctypes.c_char_p, []),
     }

@@ -1,0 +1,289 @@
+"""What a model runs on a built neighbour list: attention of every atom over its neighbours
+with a learned bias by distance, and linear maps whose weights go by group.
+
+    ei, _, nn, _, vec, dist = impl.radius_graph_pbc_vectors(pos, cell, pbc, 6.0)
+    plan = neighbor_plan(ei, num_nodes=len(pos), distances=dist, boundaries=edges)
+    y = grouped_linear(x, weight, sizes)                  # rows by structure, species, expert
+    out = neighbor_attention(q, k, v, plan, bias_table)   # differentiable in q, k, v, bias_table
+
+No counterpart in the reference, whose force models bring their own layers.  The kernels are
+those of libdynamis_graph.so (dg_neighbors_*, dg_attention_*, dg_grouped_*); there is no CPU
+path.  Everything runs on the current stream; tensors follow torch's rules for streams, and a
+plan made on one stream may be read on another once the caller has ordered the two.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from .. import _lib as L
+from .dynamis_state_impl import _check, _shape, sfc_order
+
+_DTYPES = {torch.float32: L.DG_F32, torch.bfloat16: L.DG_BF16}
+_NULL = ctypes.c_void_p(0)
+
+
+class _Rows:
+    """One direction's index lists, as the kernels take them."""
+
+    def __init__(self, order, ptr, idx, bucket):
+        self.order, self.ptr, self.idx, self.bucket = order, ptr, idx, bucket
+        self.item_slot = self.item_first = None
+        c = self.c = L.NeighborLists()
+        c.n_rows = order.numel()
+        c.order, c.ptr, c.idx = order.data_ptr(), ptr.data_ptr(), idx.data_ptr()
+        c.bucket = bucket.data_ptr() if bucket is not None else None
+        self.byref = ctypes.byref(c)
+
+    def split(self, long_rows, long_entries, stream):
+        """Rows above DG_NEIGHBOR_SPLIT entries in parts: as many entries as give every SIMD of
+        the card a few parts, at least 128 (a part's result costs as much as some entries)."""
+        if not long_rows:
+            return
+        lib, dev, c = L.lib(), self.ptr.device, self.c
+        c.chunk = min(2048, max(128, -(-long_entries // 4096 + 31) // 32 * 32))
+        c.n_items = long_entries // c.chunk + long_rows
+        self.item_slot = torch.empty(c.n_items, dtype=torch.int32, device=dev)
+        self.item_first = torch.empty(c.n_rows + 1, dtype=torch.int32, device=dev)
+        c.item_slot, c.item_first = self.item_slot.data_ptr(), self.item_first.data_ptr()
+        wsb = lib.dg_neighbors_parts_workspace_size(c.n_rows)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        L.check(lib.dg_neighbors_parts(L.ptr(self.ptr), c.n_rows, c.chunk, c.n_items, L.ptr(self.item_first),
+                                       L.ptr(self.item_slot), L.ptr(ws), wsb, stream), "neighbor_plan")
+
+    def tensors(self):
+        return [t for t in (self.order, self.ptr, self.idx, self.bucket, self.item_slot, self.item_first)
+                if t is not None]
+
+
+class NeighborPlan:
+    """Index lists of a graph for ``neighbor_attention`` (see ``neighbor_plan``).
+
+    num_nodes, num_targets, num_edges (those kept), num_buckets (0: made without distances),
+    symmetric (the lists by source are those by target)."""
+
+    def __init__(self, device, num_nodes, num_targets, num_edges, num_buckets, by_target, by_source, symmetric):
+        self.device = device
+        self.num_nodes, self.num_targets = num_nodes, num_targets
+        self.num_edges, self.num_buckets = num_edges, num_buckets
+        self.by_target, self.by_source, self.symmetric = by_target, by_source, symmetric
+        self._stream = torch.cuda.current_stream(device)
+
+    def _use(self):
+        """Keeps the lists' memory from being handed out again while the current stream reads it."""
+        s = torch.cuda.current_stream(self.device)
+        if s != self._stream:
+            self.record_stream(s)
+
+    def record_stream(self, stream):
+        for rows in {id(r): r for r in (self.by_target, self.by_source) if r is not None}.values():
+            for t in rows.tensors():
+                t.record_stream(stream)
+
+
+def neighbor_plan(edge_index, num_nodes, num_targets=None, distances=None, boundaries=None, edge_mask=None,
+                  backward=True):
+    """Index lists of an edge list, made once and read by every layer.
+
+    edge_index [2, E] int64 (sources, targets) as the builders here return it.  Nodes are
+    [0, num_nodes), targets [0, num_targets) (default: all nodes; a rank's own atoms come first,
+    then its ghosts).  Edges of a target need not be together, but then they are sorted first.
+    distances [E] with boundaries [B - 1], ascending and of the same type, put an edge into
+    bucket #{boundaries <= distance} of B <= 128.  edge_mask [E] bool leaves edges out (a list
+    with a skin, cut to the radius).  backward=False leaves out the lists that only gradients
+    need.  One host synchronisation; E < 2^31 - 256.
+    """
+    _check(isinstance(edge_index, torch.Tensor) and edge_index.is_cuda, "edge_index must be a CUDA tensor")
+    _check(edge_index.dim() == 2 and edge_index.size(0) == 2,
+           f"edge_index must have shape [2, E], got {_shape(edge_index)}")
+    _check(edge_index.dtype == torch.int64, f"edge_index must be int64, got {edge_index.dtype}")
+    dev, E = edge_index.device, edge_index.size(1)
+    num_nodes = int(num_nodes)
+    num_targets = num_nodes if num_targets is None else int(num_targets)
+    _check(0 <= num_targets <= num_nodes, f"num_targets must be in [0, num_nodes], got {num_targets}")
+    n_bounds = 0
+    if distances is not None:
+        _check(distances.device == dev and distances.dim() == 1 and distances.size(0) == E,
+               f"distances must have shape [{E}] on {dev}, got {_shape(distances)} on {distances.device}")
+        _check(distances.dtype in (torch.float32, torch.float64),
+               f"distances must be float32 or float64, got {distances.dtype}")
+        _check(boundaries is not None, "distances come with boundaries")
+        boundaries = torch.as_tensor(boundaries, dtype=distances.dtype, device=dev).contiguous()
+        _check(boundaries.dim() == 1, f"boundaries must be 1-D, got {_shape(boundaries)}")
+        n_bounds = boundaries.numel()
+        _check(n_bounds <= 127, f"at most 127 boundaries (128 buckets), got {n_bounds}")
+        distances = distances.detach().contiguous()
+    else:
+        _check(boundaries is None, "boundaries come with distances")
+    if edge_mask is not None:
+        _check(edge_mask.device == dev and edge_mask.dtype == torch.bool and edge_mask.dim() == 1
+               and edge_mask.size(0) == E, f"edge_mask must be bool [{E}] on {dev}")
+        edge_mask = edge_mask.contiguous()
+    lib = L.lib()
+    edge_index = edge_index.contiguous()
+    d = L.NeighborDesc(E, num_nodes, num_targets, n_bounds,
+                       L.DG_F64 if distances is not None and distances.dtype == torch.float64 else L.DG_F32)
+    wsb = lib.dg_neighbors_workspace_size(d)
+    if wsb == 0:
+        raise RuntimeError(f"neighbor_plan: {lib.dg_last_error().decode()}")
+    with torch.cuda.device(dev):
+        s = L.stream_of(dev)
+        pad = L.DG_NEIGHBOR_PAD
+        new = lambda n, t=torch.int32: torch.empty(n, dtype=t, device=dev)  # noqa: E731
+        ws, order, ptr, idx = new(wsb, torch.uint8), new(num_nodes), new(num_nodes + 1), new(E + pad)
+        bucket = new(E + pad, torch.uint8) if distances is not None else None
+        base = edge_index.data_ptr()
+        L.check(lib.dg_neighbors_by_target(d, ctypes.c_void_p(base), ctypes.c_void_p(base + 8 * E), L.ptr(edge_mask),
+                                           L.ptr(distances), L.ptr(boundaries), L.ptr(order), L.ptr(ptr), L.ptr(idx),
+                                           L.ptr(bucket), int(backward), L.ptr(ws), wsb, s), "neighbor_plan")
+        t = L.NeighborTotals()
+        L.check(lib.dg_neighbors_read_totals(d, L.ptr(ws), t, s), "neighbor_plan")
+        if not t.grouped:
+            perm = sfc_order(edge_index[1].contiguous())
+            return neighbor_plan(edge_index[:, perm], num_nodes, num_targets,
+                                 None if distances is None else distances[perm], boundaries,
+                                 None if edge_mask is None else edge_mask[perm], backward)
+        by_target = _Rows(order, ptr, idx, bucket)
+        by_target.split(t.long_rows, t.long_entries, s)
+        by_source, n = None, t.n_entries
+        symmetric = bool(backward and t.symmetric)
+        if symmetric:
+            by_source = by_target
+        elif backward:
+            sptr, sidx = new(num_nodes + 1), new(n + pad)
+            sbucket = new(n + pad, torch.uint8) if bucket is not None else None
+            sort_bytes = lib.dg_neighbors_sort_workspace_size(n)
+            sort_ws = new(sort_bytes, torch.uint8)
+            L.check(lib.dg_neighbors_by_source(d, n, L.ptr(idx), L.ptr(bucket), L.ptr(sptr), L.ptr(sidx),
+                                               L.ptr(sbucket), L.ptr(ws), wsb, L.ptr(sort_ws), sort_bytes, s),
+                    "neighbor_plan")
+            L.check(lib.dg_neighbors_read_totals(d, L.ptr(ws), t, s), "neighbor_plan")
+            by_source = _Rows(order, sptr, sidx, sbucket)
+            by_source.split(t.long_rows, t.long_entries, s)
+        return NeighborPlan(dev, num_nodes, num_targets, n, n_bounds + 1 if bucket is not None else 0, by_target,
+                            by_source, symmetric)
+
+
+def _rows_16(t):
+    """t [n, heads, dim] as it is if its rows are whole, start at 16 bytes and lie a multiple of
+    16 bytes apart; else a copy."""
+    step = 16 // t.element_size()
+    if t.stride(2) == 1 and (t.size(1) == 1 or t.stride(1) == t.size(2)) and t.stride(0) % step == 0 \
+            and t.stride(0) >= 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _attention_desc(q, k, v, n_nodes, n_buckets, scale):
+    d = L.AttentionDesc()
+    d.n_targets, d.n_nodes = q.size(0), n_nodes
+    d.ld_q, d.ld_k, d.ld_v = q.stride(0), k.stride(0), v.stride(0)
+    d.heads, d.kv_heads, d.dim = q.size(1), k.size(1), q.size(2)
+    d.n_buckets, d.dtype, d.scale = n_buckets, _DTYPES[q.dtype], scale
+    return d
+
+
+def _forward(q, k, v, table, plan, scale, train, want_lse):
+    lib, dev = L.lib(), q.device
+    q, k, v = _rows_16(q), _rows_16(k), _rows_16(v)
+    table = table.contiguous() if table is not None else None
+    d = _attention_desc(q, k, v, plan.num_nodes, 0 if table is None else table.size(0), scale)
+    rows = plan.by_target
+    wsb = lib.dg_attention_workspace_size(d, rows.byref, None)
+    if wsb == 0:
+        raise RuntimeError(f"neighbor_attention: {lib.dg_last_error().decode()}")
+    with torch.cuda.device(dev):
+        plan._use()
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out32 = torch.empty(q.shape, dtype=torch.float32, device=dev) if train and q.dtype != torch.float32 else None
+        norm = torch.empty((*q.shape[:2], 2), dtype=torch.float32, device=dev) if train else None
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if want_lse else None
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        L.check(lib.dg_attention_forward(d, rows.byref, L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(table), L.ptr(out),
+                                         L.ptr(out32), L.ptr(norm), L.ptr(lse), L.ptr(ws), wsb, L.stream_of(dev)),
+                "neighbor_attention")
+    return out, lse, out32, norm
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, plan, scale, want_lse):
+        out, lse, out32, norm = _forward(q, k, v, table, plan, scale, True, want_lse)
+        ctx.save_for_backward(q, k, v, table, out if out32 is None else out32, norm)
+        ctx.plan, ctx.scale = plan, scale
+        if lse is not None:
+            ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _grad_lse):
+        q, k, v, table, out32, norm = ctx.saved_tensors
+        plan, lib, dev = ctx.plan, L.lib(), q.device
+        _check(plan.by_source is not None, "neighbor_attention: the plan was made with backward=False")
+        q, k, v, grad = _rows_16(q), _rows_16(k), _rows_16(v), _rows_16(grad)
+        table = table.contiguous() if table is not None else None
+        d = _attention_desc(q, k, v, plan.num_nodes, 0 if table is None else table.size(0), ctx.scale)
+        d.ld_g = grad.stride(0)
+        to, fro = plan.by_target.byref, plan.by_source.byref
+        wsb = lib.dg_attention_workspace_size(d, to, fro)
+        if wsb == 0:
+            raise RuntimeError(f"neighbor_attention: {lib.dg_last_error().decode()}")
+        with torch.cuda.device(dev):
+            plan._use()
+            new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
+            dq, dk, dv = new(q), new(k), new(v)
+            dtable = new(table) if table is not None else None
+            ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+            L.check(lib.dg_attention_backward(d, to, fro, L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(table), L.ptr(out32),
+                                              L.ptr(norm), L.ptr(grad), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(dtable),
+                                              L.ptr(ws), wsb, L.stream_of(dev)), "neighbor_attention")
+        return dq, dk, dv, dtable, None, None, None
+
+
+def neighbor_attention(q, k, v, plan, bias_table=None, scale=None, return_lse=False):
+    """Attention of every target over the sources of its edges.
+
+      logit[e, h] = scale <q[t, h], k[s, h // (heads // kv_heads)]> + bias_table[bucket(e), h]
+      out[t, h]   = sum_e softmax_e(logit)[e, h] v[s, h // (heads // kv_heads)]
+
+    q [num_targets, heads, dim], k and v [num_nodes, kv_heads, dim], float32 or bfloat16; heads a
+    multiple of kv_heads, dim a multiple of 8 up to 256; any strides (rows that are whole and
+    start at 16 bytes are read in place).  bias_table [plan.num_buckets, heads], at most 4096
+    entries, used in float32; an entry of -inf takes its edges out for that head, whatever q, k
+    and v hold there.  scale defaults to dim ** -0.5.  A target without edges gives zeros (and a
+    log-sum of -inf).  Returns out like q, and with return_lse also the natural log-sums
+    [num_targets, heads] in float32 (not differentiable).
+
+    Differentiable in q, k, v and bias_table (once).  All sums are float32, in a fixed order:
+    results repeat bit for bit.
+    """
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
+        _check(t.dim() == 3, f"{name} must have shape [nodes, heads, dim], got {_shape(t)}")
+        _check(t.device == plan.device, f"{name} must be on the plan's device {plan.device}, got {t.device}")
+        _check(t.dtype in _DTYPES, f"{name} must be float32 or bfloat16, got {t.dtype}")
+        _check(t.dtype == q.dtype, f"q, k and v must have one dtype, got {q.dtype} and {t.dtype}")
+        _check(t.size(2) == q.size(2), f"q, k and v must have one head width, got {q.size(2)} and {t.size(2)}")
+    _check(q.size(0) == plan.num_targets, f"q must have {plan.num_targets} rows, got {q.size(0)}")
+    _check(k.size(0) == plan.num_nodes and v.shape == k.shape,
+           f"k and v must have {plan.num_nodes} rows and one shape, got {_shape(k)} and {_shape(v)}")
+    heads, kv, dim = q.size(1), k.size(1), q.size(2)
+    _check(heads >= 1 and kv >= 1 and heads % kv == 0, f"heads ({heads}) must be a multiple of kv_heads ({kv})")
+    _check(8 <= dim <= 256 and dim % 8 == 0, f"the head width must be a multiple of 8, 8 to 256, got {dim}")
+    if bias_table is not None:
+        _check(plan.num_buckets > 0, "bias_table needs a plan with distances")
+        _check(bias_table.device == plan.device and bias_table.is_floating_point()
+               and tuple(bias_table.shape) == (plan.num_buckets, heads),
+               f"bias_table must be floating [{plan.num_buckets}, {heads}] on {plan.device}, got {_shape(bias_table)}")
+        _check(bias_table.numel() <= 4096, f"bias_table must hold at most 4096 entries, got {bias_table.numel()}")
+        bias_table = bias_table.float()
+    scale = float(dim ** -0.5 if scale is None else scale)
+    _check(math.isfinite(scale), f"scale must be finite, got {scale}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table)):
+        out, lse = _Attention.apply(q, k, v, bias_table, plan, scale, return_lse)
+    else:
+        out, lse, _, _ = _forward(q, k, v, bias_table, plan, scale, False, return_lse)
+    return (out, lse) if return_lse else out

@@ -42,13 +42,14 @@ typedef enum {
     DG_ERR_CAPACITY = 5   /* edge capacity smaller than the edge count */
 } dg_status;
 
-typedef enum { DG_F32 = 0, DG_F64 = 1, DG_I64 = 2, DG_I32 = 3 } dg_dtype;
+typedef enum { DG_F32 = 0, DG_F64 = 1, DG_I64 = 2, DG_I32 = 3, DG_BF16 = 4 } dg_dtype;
 
 /* Status flag bits of dg_graph_read_totals(). */
 #define DG_FLAG_RANGE 1
 #define DG_FLAG_NONFINITE 2
 #define DG_FLAG_CAPACITY 4
 #define DG_FLAG_TARGET 8
+#define DG_FLAG_UNGROUPED 16
 
 /* Description of one radius-graph build.
  * Mirrors the arguments of radius_graph_pbc_ex (dynamis_state/src/csrc/graph/
@@ -345,6 +346,126 @@ dg_status dg_halo_read_totals(const void* workspace, int64_t* total_send, int64_
 dg_status dg_halo_write(const dg_halo_desc* desc, const void* pid, int64_t* send_local_indices,
                         int64_t* recv_ghost_indices, int64_t* recv_atom_global, void* workspace,
                         size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------ operators on a built graph
+ * What a model runs on an edge list, layer after layer: attention of every target over the
+ * sources of its edges, and linear maps whose weights go by group (structure, species,
+ * expert).  No counterpart in the reference, whose force models bring their own layers. */
+
+/* Index lists of a graph, made once per edge list and read by every attention call.
+ *   edge_src / edge_dst  int64 [n_edges], edge_dst in [0, n_targets), edge_src in [0, n_nodes);
+ *                        every target's edges in one run, as the builders here write them
+ *   mask                 uint8 [n_edges] or NULL: edges at 0 are left out
+ *   dist                 [n_edges] of dist_dtype, with boundaries [n_boundaries] (ascending, of
+ *                        the same type): an entry's bucket is the number of boundaries <= dist
+ * Rows sit in slots: nodes in the order of their runs, then the nodes without one.
+ *   order  out int32 [n_nodes]      node of a slot
+ *   ptr    out int32 [n_nodes + 1]  a slot's entries
+ *   idx    out int32 [n_edges + DG_NEIGHBOR_PAD]  sources (by target) or targets (by source)
+ *   bucket out uint8 [n_edges + DG_NEIGHBOR_PAD] or NULL
+ * dg_neighbors_by_target (asynchronous; by_source != 0: prepares dg_neighbors_by_source), then
+ * dg_neighbors_read_totals (synchronous: DG_ERR_RANGE for an index out of range).  With
+ * `symmetric` set, the lists by source are the lists by target; otherwise
+ * dg_neighbors_by_source (same workspace, n_entries and outputs of the first call; another
+ * dg_neighbors_read_totals then gives `longest`, `long_rows` and `long_entries` of its rows).
+ * `grouped` == 0: some target's edges were apart; the lists are unusable (sort the edges by
+ * target first). */
+#define DG_NEIGHBOR_PAD 64
+#define DG_NEIGHBOR_SPLIT 512 /* rows with more entries are worked on in parts */
+typedef struct dg_neighbor_desc {
+    int64_t n_edges;   /* < 2^31 - 256 */
+    int64_t n_nodes;
+    int64_t n_targets; /* targets are the nodes [0, n_targets) */
+    int32_t n_boundaries; /* <= 127 */
+    int32_t dist_dtype;   /* DG_F32 / DG_F64 */
+} dg_neighbor_desc;
+
+typedef struct dg_neighbor_totals {
+    int64_t n_entries;    /* edges kept */
+    int64_t longest;      /* entries of the longest row */
+    int64_t long_rows;    /* rows above DG_NEIGHBOR_SPLIT, and their entries */
+    int64_t long_entries;
+    int32_t grouped;
+    int32_t symmetric;
+} dg_neighbor_totals;
+
+/* One direction's lists, as the attention reads them.  Rows above DG_NEIGHBOR_SPLIT entries
+ * are worked on in items of `chunk` entries (dg_neighbors_parts); n_items == 0: by one wave. */
+typedef struct dg_neighbor_lists {
+    int64_t n_rows;  /* n_nodes */
+    int64_t n_items; /* length of item_slot (an upper bound of the items) */
+    const int32_t* order;
+    const int32_t* ptr;
+    const int32_t* idx;
+    const uint8_t* bucket;     /* or NULL */
+    const int32_t* item_slot;  /* [n_items] */
+    const int32_t* item_first; /* [n_rows + 1] */
+    int32_t chunk;
+    int32_t pad_;
+} dg_neighbor_lists;
+
+size_t dg_neighbors_workspace_size(const dg_neighbor_desc* desc);
+dg_status dg_neighbors_by_target(const dg_neighbor_desc* desc, const int64_t* edge_src,
+                                 const int64_t* edge_dst, const uint8_t* mask, const void* dist,
+                                 const void* boundaries, int32_t* order, int32_t* ptr, int32_t* idx,
+                                 uint8_t* bucket, int32_t by_source, void* workspace,
+                                 size_t workspace_bytes, hipStream_t stream);
+dg_status dg_neighbors_read_totals(const dg_neighbor_desc* desc, const void* workspace,
+                                   dg_neighbor_totals* totals, hipStream_t stream);
+size_t dg_neighbors_sort_workspace_size(int64_t n_entries);
+dg_status dg_neighbors_by_source(const dg_neighbor_desc* desc, int64_t n_entries, const int32_t* idx,
+                                 const uint8_t* bucket, int32_t* source_ptr, int32_t* source_idx,
+                                 uint8_t* source_bucket, void* workspace, size_t workspace_bytes,
+                                 void* sort_workspace, size_t sort_workspace_bytes,
+                                 hipStream_t stream);
+/* The items of rows above DG_NEIGHBOR_SPLIT entries: item_first int32 [n_rows + 1], item_slot
+ * int32 [max_items] with max_items >= long_entries / chunk + long_rows. */
+size_t dg_neighbors_parts_workspace_size(int64_t n_rows);
+dg_status dg_neighbors_parts(const int32_t* ptr, int64_t n_rows, int32_t chunk, int64_t max_items,
+                             int32_t* item_first, int32_t* item_slot, void* workspace,
+                             size_t workspace_bytes, hipStream_t stream);
+
+/* Attention over the lists:
+ *   logit[e,h] = scale <q[t,h], k[j, h / (heads / kv_heads)]> + table[bucket(e), h]
+ *   out[t,h]   = sum_e softmax_e(logit)[e,h] v[j, ...],  lse[t,h] = log sum_e exp(logit[e,h])
+ * over the entries e = (t <- j) of t's row.  A row without entries (or with -inf logits only)
+ * gives zeros and lse = -inf.  An entry of -inf in the table takes its edges out for that
+ * head, whatever q, k and v hold there.
+ *   q [n_targets, heads, dim], k, v [n_nodes, kv_heads, dim] of dtype (DG_F32 / DG_BF16), rows
+ *   ld_* elements apart, aligned to 16 bytes as their rows are; dim a multiple of 8, 8 .. 256
+ *   table  float32 [n_buckets, heads], n_buckets <= 128, n_buckets * heads <= 4096
+ *   out    [n_targets, heads, dim] of dtype;  out32 the same in float32 before its rounding
+ *          and norm float32 [n_targets, heads, 2] (the maximum of a row's base-2 logits and one
+ *          over the sum of their powers): what the backward pass takes, or NULL
+ *   lse    float32 [n_targets, heads], natural, or NULL
+ * Backward: dq, dk, dv of dtype and contiguous, dtable float32.  Sums are float32 and in a
+ * fixed order: results repeat bit for bit.  The workspace of
+ * dg_attention_workspace_size(desc, by_target, by_source or NULL for the forward pass) bytes. */
+typedef struct dg_attention_desc {
+    int64_t n_targets;
+    int64_t n_nodes;
+    int64_t ld_q, ld_k, ld_v;
+    int64_t ld_g; /* of grad_out (backward) */
+    int32_t heads;
+    int32_t kv_heads;
+    int32_t dim;
+    int32_t n_buckets; /* 0: no table */
+    int32_t dtype;
+    float scale;
+} dg_attention_desc;
+
+size_t dg_attention_workspace_size(const dg_attention_desc* desc, const dg_neighbor_lists* by_target,
+                                   const dg_neighbor_lists* by_source);
+dg_status dg_attention_forward(const dg_attention_desc* desc, const dg_neighbor_lists* by_target,
+                               const void* q, const void* k, const void* v, const float* table,
+                               void* out, float* out32, float* norm, float* lse, void* workspace,
+                               size_t workspace_bytes, hipStream_t stream);
+dg_status dg_attention_backward(const dg_attention_desc* desc, const dg_neighbor_lists* by_target,
+                                const dg_neighbor_lists* by_source, const void* q, const void* k,
+                                const void* v, const float* table, const float* out32,
+                                const float* norm, const void* grad_out, void* dq, void* dk, void* dv,
+                                float* dtable, void* workspace, size_t workspace_bytes,
+                                hipStream_t stream);
 
 /* Message of the last failure on this thread ("" if none). */
 const char* dg_last_error(void);
