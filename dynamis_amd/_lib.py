@@ -124,6 +124,19 @@ class AttentionDesc(ctypes.Structure):
     ]
 
 
+class GroupedDesc(ctypes.Structure):
+    """dg_grouped_desc."""
+
+    _fields_ = [
+        ("n_rows", ctypes.c_int64),
+        ("n_groups", ctypes.c_int64),
+        ("k", ctypes.c_int32),
+        ("n", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("pad_", ctypes.c_int32),
+    ]
+
+
 _lib = None
 
 _p = ctypes.c_void_p
@@ -143,6 +156,7 @@ def lib():
     L = ctypes.CDLL(LIB_PATH)
     D = ctypes.POINTER(GraphDesc)
     ND, NL, AD = ctypes.POINTER(NeighborDesc), ctypes.POINTER(NeighborLists), ctypes.POINTER(AttentionDesc)
+    GD = ctypes.POINTER(GroupedDesc)
     sig = {
         "dg_graph_workspace_size": (_sz, [D]),
         "dg_graph_count": (_i32, [D, _p, _p, _p, _sz, _p, _p]),
@@ -190,6 +204,9 @@ def lib():
         "dg_attention_workspace_size": (_sz, [AD, NL, NL]),
         "dg_attention_forward": (_i32, [AD, NL] + [_p] * 9 + [_sz, _p]),
         "dg_attention_backward": (_i32, [AD, NL, NL] + [_p] * 12 + [_sz, _p]),
+        "dg_grouped_forward": (_i32, [GD, _p, _p, _p, _p, _p, _p]),
+        "dg_grouped_workspace_size": (_sz, [GD]),
+        "dg_grouped_backward": (_i32, [GD] + [_p] * 8 + [_sz, _p]),
         "dg_last_error": (ctypes.c_char_p, []),
         "dg_version": (ctypes.c_char_p, []),
     }

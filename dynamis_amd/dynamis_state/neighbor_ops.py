@@ -287,3 +287,81 @@ def neighbor_attention(q, k, v, plan, bias_table=None, scale=None, return_lse=Fa
     else:
         out, lse, _, _ = _forward(q, k, v, bias_table, plan, scale, False, return_lse)
     return (out, lse) if return_lse else out
+
+
+def _grouped_desc(x, weight):
+    return L.GroupedDesc(x.size(0), weight.size(0), weight.size(2), weight.size(1), _DTYPES[x.dtype], 0)
+
+
+def _grouped_forward(x, weight, sizes, bias):
+    dev = x.device
+    with torch.cuda.device(dev):
+        y = torch.empty((x.size(0), weight.size(1)), dtype=x.dtype, device=dev)
+        L.check(L.lib().dg_grouped_forward(_grouped_desc(x, weight), L.ptr(x), L.ptr(weight), L.ptr(sizes), L.ptr(bias),
+                                           L.ptr(y), L.stream_of(dev)), "grouped_linear")
+    return y
+
+
+class _Grouped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, sizes, bias):
+        ctx.save_for_backward(x, weight, sizes)
+        return _grouped_forward(x, weight, sizes, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, sizes = ctx.saved_tensors
+        need_x, need_w, _, need_b = ctx.needs_input_grad
+        lib, dev, grad = L.lib(), x.device, grad.contiguous()
+        d = _grouped_desc(x, weight)
+        with torch.cuda.device(dev):
+            dx = torch.empty_like(x) if need_x else None
+            dw = torch.empty_like(weight) if need_w or need_b else None
+            db = torch.empty(weight.shape[:2], dtype=x.dtype, device=dev) if need_b else None
+            wsb = lib.dg_grouped_workspace_size(d) if dw is not None else 0
+            ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+            L.check(lib.dg_grouped_backward(d, L.ptr(x), L.ptr(weight), L.ptr(sizes), L.ptr(grad), L.ptr(dx), L.ptr(dw),
+                                            L.ptr(db), L.ptr(ws), wsb, L.stream_of(dev)), "grouped_linear")
+        return dx, dw if need_w else None, None, db
+
+
+def grouped_linear(x, weight, sizes, bias=None):
+    """Linear maps by group over ragged rows: y[i] = weight[g(i)] @ x[i] + bias[g(i)].
+
+    x [rows, k], weight [groups, n, k] (torch.nn.Linear's layout for each group), bias
+    [groups, n]; float32 or bfloat16, one type.  sizes [groups] int64: the first sizes[0] rows are
+    group 0's, the next sizes[1] group 1's and so on -- ``num_neighbors_image`` for rows per edge
+    of a batch, its ``natoms`` for rows per atom.  On the device (no synchronisation) rows behind
+    the last group give zeros and sizes are not checked otherwise; on the host, or as a list, they
+    have to be non-negative and to add up to the rows.  Groups may be empty.
+
+    Differentiable in x, weight and bias (once).  Sums are float32, in a fixed order: results
+    repeat bit for bit.
+    """
+    _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a CUDA tensor")
+    _check(x.dim() == 2, f"x must have shape [rows, k], got {_shape(x)}")
+    _check(x.dtype in _DTYPES, f"x must be float32 or bfloat16, got {x.dtype}")
+    _check(isinstance(weight, torch.Tensor) and weight.device == x.device, f"weight must be on {x.device}")
+    _check(weight.dim() == 3 and weight.size(2) == x.size(1),
+           f"weight must have shape [groups, n, {x.size(1)}], got {_shape(weight)}")
+    _check(weight.dtype == x.dtype, f"weight must be {x.dtype}, got {weight.dtype}")
+    groups = weight.size(0)
+    _check(1 <= groups <= 1 << 20, f"weight must hold 1 to 2^20 groups, got {groups}")
+    _check(1 <= x.size(1) <= 1 << 20 and 1 <= weight.size(1) <= 1 << 20, "the widths must be 1 to 2^20")
+    sizes = torch.as_tensor(sizes)
+    _check(sizes.dim() == 1 and sizes.size(0) == groups and sizes.dtype == torch.int64,
+           f"sizes must be int64 [{groups}], got {sizes.dtype} {_shape(sizes)}")
+    if not sizes.is_cuda:
+        _check(bool((sizes >= 0).all()) and int(sizes.sum()) == x.size(0),
+               f"sizes must be non-negative and add up to {x.size(0)} rows")
+    _check(not sizes.is_cuda or sizes.device == x.device, f"sizes must be on {x.device}")
+    sizes = sizes.to(x.device).contiguous()
+    if bias is not None:
+        _check(bias.device == x.device and bias.dtype == x.dtype and tuple(bias.shape) == tuple(weight.shape[:2]),
+               f"bias must be {x.dtype} [{groups}, {weight.size(1)}] on {x.device}, got {bias.dtype} {_shape(bias)}")
+        bias = bias.contiguous()
+    x, weight = x.contiguous(), weight.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _Grouped.apply(x, weight, sizes, bias)
+    return _grouped_forward(x, weight, sizes, bias)

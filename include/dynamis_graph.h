@@ -467,6 +467,33 @@ dg_status dg_attention_backward(const dg_attention_desc* desc, const dg_neighbor
                                 float* dtable, void* workspace, size_t workspace_bytes,
                                 hipStream_t stream);
 
+/* Linear maps by group: rows of a group follow each other, the first sizes[0] rows are group
+ * 0's and so on.
+ *   y[i] = weight[g(i)] x[i] + bias[g(i)]
+ *   x [n_rows, k], weight [n_groups, n, k], bias [n_groups, n] or NULL, y [n_rows, n], all of
+ *   dtype (DG_F32 / DG_BF16) and contiguous, aligned to their type alone; sizes device int64
+ *   [n_groups].  Rows behind the last group give zeros; a size below 0 counts as 0, one that
+ *   reaches past n_rows ends there.
+ * Backward: dx like x or NULL, dweight like weight or NULL, dbias like bias or NULL (with
+ * dweight only); workspace of dg_grouped_workspace_size bytes for dweight.  Sums are float32
+ * and in a fixed order: results repeat bit for bit. */
+typedef struct dg_grouped_desc {
+    int64_t n_rows;
+    int64_t n_groups; /* 1 .. 2^20 */
+    int32_t k;        /* width of x */
+    int32_t n;        /* width of y */
+    int32_t dtype;
+    int32_t pad_;
+} dg_grouped_desc;
+
+dg_status dg_grouped_forward(const dg_grouped_desc* desc, const void* x, const void* weight,
+                             const int64_t* sizes, const void* bias, void* y, hipStream_t stream);
+size_t dg_grouped_workspace_size(const dg_grouped_desc* desc);
+dg_status dg_grouped_backward(const dg_grouped_desc* desc, const void* x, const void* weight,
+                              const int64_t* sizes, const void* grad_y, void* dx, void* dweight,
+                              void* dbias, void* workspace, size_t workspace_bytes,
+                              hipStream_t stream);
+
 /* Message of the last failure on this thread ("" if none). */
 const char* dg_last_error(void);
 
