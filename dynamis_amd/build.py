@@ -16,7 +16,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdynamis_graph.so")
 SOURCES = ["dg_graph.hip", "dg_sfc.hip", "dg_halo.hip", "dg_batch.hip", "dg_neighbors.hip",
-           "dg_attention.hip", "dg_grouped.hip"]
+           "dg_attention.hip", "dg_attention_mfma.hip", "dg_grouped.hip"]
 ARCH = os.environ.get("DG_OFFLOAD_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -21,6 +21,7 @@
 
 #include "../../include/dynamis_graph.h"
 #include "dg_attention.hpp"
+#include "dg_attention_mfma.hpp"
 
 namespace {
 
@@ -83,11 +84,11 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(AttnArgs a)
     const bool wide = part * 4 < a.dim;     // (the last lanes of a head whose width is no power of two idle)
     const int ch = wide ? part * 4 : 0;
     const float scale2 = a.scale * kLog2e;
-    const Walk w = walk_of((a.L.n_items + a.L.n_rows) * m.groups, kWaves);
+    const Walk w = walk_of(a.L, kWaves);
     for (int64_t u = w.at; u < w.end; u += w.step) {
-        const Piece p = piece_of(a.L, u / m.groups, a.n_targets);
+        const Piece p = piece_of(a.L, w, u);
         if (p.node < 0) continue;
-        const int h_raw = (int)(u % m.groups) * m.per_wave + hl;
+        const int h_raw = (int)blockIdx.y * m.per_wave + hl;
         const bool mine = hl < m.per_wave && h_raw < a.heads;
         const int h = mine ? h_raw : 0;
         const int64_t kch = (int64_t)(h / a.per) * a.dim + ch;
@@ -176,11 +177,9 @@ __global__ __launch_bounds__(256) void forward_join_kernel(AttnArgs a, int slice
 {
     const int64_t item = blockIdx.x / slices;
     const int slice = (int)(blockIdx.x % slices);
-    if (item >= a.L.item_first[a.L.n_rows]) return;
-    const int slot = a.L.item_slot[item];
+    const int slot = a.L.items[item].w, node = a.L.items[item].z;
     const int first = a.L.item_first[slot], n = a.L.item_first[slot + 1] - first;
-    const int node = a.L.order[slot];
-    if (item != first || node >= a.n_targets) return;
+    if (node < 0 || item != first) return;
     __shared__ float s_acc[16][16][4], s_m[16][16], s_l[16][16];
     const int x = threadIdx.x % 16, y = threadIdx.x / 16;
     const int wide = a.heads * a.dim, ch = slice * 64 + x * 4;
@@ -238,11 +237,11 @@ __global__ __launch_bounds__(64 * kWaves) void backward_q_kernel(AttnArgs a)
         for (int i = threadIdx.x; i < kWaves * span * cells; i += blockDim.x) s_dtab[i] = 0;
     __syncthreads();
     float* my_dtab = s_dtab + ((threadIdx.x / 64) * span + es) * cells;
-    const Walk w = walk_of((a.L.n_items + a.L.n_rows) * m.groups, kWaves);
+    const Walk w = walk_of(a.L, kWaves);
     for (int64_t u = w.at; u < w.end; u += w.step) {
-        const Piece p = piece_of(a.L, u / m.groups, a.n_targets);
+        const Piece p = piece_of(a.L, w, u);
         if (p.node < 0) continue;
-        const int h_raw = (int)(u % m.groups) * m.per_wave + hl;
+        const int h_raw = (int)blockIdx.y * m.per_wave + hl;
         const bool mine = hl < m.per_wave && h_raw < a.heads;
         const int h = mine ? h_raw : 0;
         const int64_t kch = (int64_t)(h / a.per) * a.dim + ch;
@@ -313,7 +312,7 @@ __global__ __launch_bounds__(64 * kWaves) void backward_q_kernel(AttnArgs a)
     for (int i = threadIdx.x; i < cells; i += blockDim.x) {
         float x = 0;
         for (int c = 0; c < kWaves * span; ++c) x += s_dtab[c * cells + i];
-        a.dtab[(int64_t)blockIdx.x * cells + i] = x;
+        a.dtab[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * cells + i] = x;
     }
 }
 
@@ -331,11 +330,11 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kv_kernel(AttnArgs a)
     const int ch = wide ? part * 4 : 0;
     const float scale2 = a.scale * kLog2e;
     constexpr int kTwo = 2;
-    const Walk w = walk_of((a.L.n_items + a.L.n_rows) * m.groups, kWaves);
+    const Walk w = walk_of(a.L, kWaves);
     for (int64_t u = w.at; u < w.end; u += w.step) {
-        const Piece p = piece_of(a.L, u / m.groups, a.n_nodes);
+        const Piece p = piece_of(a.L, w, u);
         if (p.node < 0) continue;
-        const int c_raw = (int)(u % m.groups) * m.per_wave + hl;
+        const int c_raw = (int)blockIdx.y * m.per_wave + hl;
         const bool mine = hl < m.per_wave && c_raw < a.kv_heads;
         const int c = mine ? c_raw : 0;
         float k[4], v[4], dk[4] = {0, 0, 0, 0}, dv[4] = {0, 0, 0, 0};
@@ -414,15 +413,13 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kv_kernel(AttnArgs a)
 // The sum of the parts of one long row, as forward_join_kernel lays it out.
 template <typename T>
 __global__ __launch_bounds__(256) void sum_join_kernel(Lists L, const float* __restrict__ part, int wide, int slices,
-                                                       int64_t n_nodes, float factor, T* __restrict__ out)
+                                                       float factor, T* __restrict__ out)
 {
     const int64_t item = blockIdx.x / slices;
     const int slice = (int)(blockIdx.x % slices);
-    if (item >= L.item_first[L.n_rows]) return;
-    const int slot = L.item_slot[item];
+    const int slot = L.items[item].w, node = L.items[item].z;
     const int first = L.item_first[slot], n = L.item_first[slot + 1] - first;
-    const int node = L.order[slot];
-    if (item != first || node >= n_nodes) return;
+    if (node < 0 || item != first) return;
     __shared__ float s_acc[16][16][4];
     const int x = threadIdx.x % 16, y = threadIdx.x / 16;
     const int ch = slice * 64 + x * 4;
@@ -468,13 +465,13 @@ int lanes_per_head(int dim)
     return l;
 }
 
-// Workgroups of a launch over `units` waves of work: enough to fill every CU's waves, no more
-// than there is work; the kernels walk what is left over.
-unsigned groups_for(int64_t units, int per_cu)
+// A wave for each row (or part) of each group of heads, up to what fills every CU; the kernels
+// walk what is left over.
+dim3 grid_of(const Lists& L, int head_groups, int per_cu)
 {
-    const int64_t most = 256 * (int64_t)per_cu;
-    const int64_t need = (units + kWaves - 1) / kWaves;
-    return (unsigned)std::max<int64_t>(1, std::min(most, need));
+    const int64_t most = std::max(1, 256 * per_cu / head_groups);
+    const int64_t need = (L.n_items + L.n_rows + kWaves - 1) / kWaves;
+    return dim3((unsigned)std::max<int64_t>(1, std::min(most, need)), (unsigned)head_groups);
 }
 
 constexpr int kGroupsPerCu = 6;
@@ -491,7 +488,7 @@ Layout layout(const dg_attention_desc* d, const dg_neighbor_lists* t, const dg_n
     const size_t q = (size_t)d->heads * d->dim, kv = (size_t)d->kv_heads * d->dim;
     const size_t ti = (size_t)t->n_items, si = s ? (size_t)s->n_items : 0;
     L.o_stats = take(s ? 16 * (size_t)d->n_targets * d->heads : 0);
-    L.o_dtab = take(s ? 4 * (size_t)256 * kGroupsPerCu * d->n_buckets * d->heads : 0);
+    L.o_dtab = take(s ? 4 * (size_t)std::max({256 * kGroupsPerCu, kMfmaTableParts, d->heads}) * d->n_buckets * d->heads : 0);
     L.o_m = take(s ? 0 : 4 * ti * d->heads);
     L.o_l = take(s ? 0 : 4 * ti * d->heads);
     L.o_acc = take(4 * std::max(ti * q, si * kv));
@@ -527,23 +524,22 @@ dg_status check_lists(const dg_attention_desc* d, const dg_neighbor_lists* l)
     if (l->n_rows != d->n_nodes) return fail(DG_ERR_INVALID, "the lists are of another number of nodes");
     if (l->n_rows > 0 && (!l->order || !l->ptr || !l->idx)) return fail(DG_ERR_INVALID, "lists are NULL");
     if (d->n_buckets > 0 && !l->bucket) return fail(DG_ERR_INVALID, "a table, but the lists hold no buckets");
-    if (l->n_items < 0 || (l->n_items > 0 && (!l->item_slot || !l->item_first || l->chunk < 1)))
+    if (l->n_items < 0 || (l->n_items > 0 && (!l->items || !l->item_first)))
         return fail(DG_ERR_INVALID, "the parts of long rows are NULL");
     return DG_OK;
 }
 
-Lists lists_of(const dg_neighbor_lists* l)
+Lists lists_of(const dg_neighbor_lists* l, int64_t rows)
 {
     Lists r;
-    r.n_rows = l->n_rows;
+    r.n_rows = rows;
     r.n_items = l->n_items;
     r.order = l->order;
     r.ptr = l->ptr;
     r.idx = l->idx;
     r.bucket = l->bucket;
-    r.item_slot = l->item_slot;
+    r.items = (const int4*)l->items;
     r.item_first = l->item_first;
-    r.chunk = l->chunk;
     return r;
 }
 
@@ -584,9 +580,13 @@ struct Width {
 };
 
 // f(Width<LPH>) for the head width
-template <typename F>
+template <typename T, typename F>
 void by_width(int dim, F&& f)
 {
+    if constexpr (sizeof(T) == 2) {  // (heads of up to kMfmaDim channels go to the matrix units)
+        f(Width<64>{});
+        return;
+    }
     switch (lanes_per_head(dim)) {
     case 2: f(Width<2>{}); break;
     case 4: f(Width<4>{}); break;
@@ -600,12 +600,16 @@ void by_width(int dim, F&& f)
 template <typename T>
 void run_forward(const AttnArgs& a, hipStream_t s)
 {
-    const size_t lds = 4 * (size_t)a.n_buckets * a.heads;
-    by_width(a.dim, [&](auto w) {
-        constexpr int LPH = decltype(w)::lph;
-        const int64_t units = (a.L.n_items + a.L.n_rows) * lanes_of<LPH>(a.heads).groups;
-        hipLaunchKernelGGL((forward_kernel<T, LPH>), dim3(groups_for(units, kGroupsPerCu)), dim3(64 * kWaves), lds, s, a);
-    });
+    if (sizeof(T) == 2 && a.dim <= kMfmaDim) {
+        forward_mfma(a, s);
+    } else {
+        const size_t lds = 4 * (size_t)a.n_buckets * a.heads;
+        by_width<T>(a.dim, [&](auto w) {
+            constexpr int LPH = decltype(w)::lph;
+            hipLaunchKernelGGL((forward_kernel<T, LPH>), grid_of(a.L, lanes_of<LPH>(a.heads).groups, kGroupsPerCu),
+                               dim3(64 * kWaves), lds, s, a);
+        });
+    }
     if (a.L.n_items > 0) {
         const int slices = (a.heads * a.dim + 63) / 64;
         hipLaunchKernelGGL(forward_join_kernel<T>, dim3((unsigned)(a.L.n_items * slices)), dim3(256), 0, s, a, slices);
@@ -615,40 +619,48 @@ void run_forward(const AttnArgs& a, hipStream_t s)
 template <typename T>
 void run_backward(AttnArgs a, const Lists& by_target, const Lists& by_source, float* dtable, hipStream_t s)
 {
+    const bool matrix = sizeof(T) == 2 && a.dim <= kMfmaDim;
     const size_t cells = (size_t)a.n_buckets * a.heads;
     a.L = by_target;
     unsigned groups = 1;
-    by_width(a.dim, [&](auto w) {
-        constexpr int LPH = decltype(w)::lph;
-        const Lanes m = lanes_of<LPH>(a.heads);
-        const int span = 64 / (LPH * m.slots);
-        const int64_t units = (a.L.n_items + a.L.n_rows) * m.groups;
-        groups = groups_for(units, kGroupsPerCu);
-        const size_t lds = 4 * cells * (1 + (a.dtab ? kWaves * span : 0));
-        hipLaunchKernelGGL((backward_q_kernel<T, LPH>), dim3(groups), dim3(64 * kWaves), lds, s, a);
-    });
+    if (matrix) {
+        groups = backward_q_mfma(a, s);
+    } else {
+        by_width<T>(a.dim, [&](auto w) {
+            constexpr int LPH = decltype(w)::lph;
+            const Lanes m = lanes_of<LPH>(a.heads);
+            const int span = 64 / (LPH * m.slots);
+            const dim3 grid = grid_of(a.L, m.groups, kGroupsPerCu);
+            groups = grid.x * grid.y;
+            const size_t lds = 4 * cells * (1 + (a.dtab ? kWaves * span : 0));
+            hipLaunchKernelGGL((backward_q_kernel<T, LPH>), grid, dim3(64 * kWaves), lds, s, a);
+        });
+    }
     if (a.dtab)
         hipLaunchKernelGGL(table_join_kernel, dim3(nblk((int64_t)cells, 16)), dim3(1024), 0, s, (const float*)a.dtab,
                            (int)groups, (int)cells, dtable);
     if (a.L.n_items > 0) {
         const int wide = a.heads * a.dim, slices = (wide + 63) / 64;
         hipLaunchKernelGGL(sum_join_kernel<T>, dim3((unsigned)(a.L.n_items * slices)), dim3(256), 0, s, a.L,
-                           (const float*)a.part_acc, wide, slices, a.n_targets, a.scale, (T*)a.dq);
+                           (const float*)a.part_acc, wide, slices, a.scale, (T*)a.dq);
     }
     a.L = by_source;
-    by_width(a.dim, [&](auto w) {
-        constexpr int LPH = decltype(w)::lph;
-        const int64_t units = (a.L.n_items + a.L.n_rows) * lanes_of<LPH>(a.kv_heads).groups;
-        hipLaunchKernelGGL((backward_kv_kernel<T, LPH>), dim3(groups_for(units, kGroupsPerCu)), dim3(64 * kWaves),
-                           4 * cells, s, a);
-    });
+    if (matrix) {
+        backward_kv_mfma(a, s);
+    } else {
+        by_width<T>(a.dim, [&](auto w) {
+            constexpr int LPH = decltype(w)::lph;
+            hipLaunchKernelGGL((backward_kv_kernel<T, LPH>), grid_of(a.L, lanes_of<LPH>(a.kv_heads).groups, kGroupsPerCu),
+                               dim3(64 * kWaves), 4 * cells, s, a);
+        });
+    }
     if (a.L.n_items > 0) {
         const int wide = a.kv_heads * a.dim, slices = (wide + 63) / 64;
         const unsigned grid = (unsigned)(a.L.n_items * slices);
         hipLaunchKernelGGL(sum_join_kernel<T>, dim3(grid), dim3(256), 0, s, a.L, (const float*)a.part_acc, wide, slices,
-                           a.n_nodes, a.scale, (T*)a.dk);
+                           a.scale, (T*)a.dk);
         hipLaunchKernelGGL(sum_join_kernel<T>, dim3(grid), dim3(256), 0, s, a.L, (const float*)a.part_acc2, wide, slices,
-                           a.n_nodes, 1.0f, (T*)a.dv);
+                           1.0f, (T*)a.dv);
     }
 }
 
@@ -680,7 +692,7 @@ dg_status dg_attention_forward(const dg_attention_desc* d, const dg_neighbor_lis
         return fail(DG_ERR_INVALID, "tensors must be aligned to 16 bytes");
     char* w = (char*)ws;
     AttnArgs a = args_of(d, q, k, v, table);
-    a.L = lists_of(by_target);
+    a.L = lists_of(by_target, d->n_targets);
     a.out = out;
     a.out32 = out32;
     a.norm = (float2*)norm;
@@ -723,8 +735,9 @@ dg_status dg_attention_backward(const dg_attention_desc* d, const dg_neighbor_li
     a.dtab = a.table ? (float*)(w + L.o_dtab) : nullptr;
     a.part_acc = (float*)(w + L.o_acc);
     a.part_acc2 = (float*)(w + L.o_acc2);
-    if (d->dtype == DG_BF16) run_backward<__bf16>(a, lists_of(by_target), lists_of(by_source), dtable, s);
-    else run_backward<float>(a, lists_of(by_target), lists_of(by_source), dtable, s);
+    const Lists to = lists_of(by_target, d->n_targets), fro = lists_of(by_source, d->n_nodes);
+    if (d->dtype == DG_BF16) run_backward<__bf16>(a, to, fro, dtable, s);
+    else run_backward<float>(a, to, fro, dtable, s);
     return launched("dg_attention_backward");
 }
 

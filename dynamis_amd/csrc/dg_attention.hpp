@@ -35,14 +35,13 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 
 // The lists of one direction (dg_neighbor_lists, see the C header).
 struct Lists {
-    int64_t n_rows, n_items;
+    int64_t n_rows, n_items;  // rows: of the pass (the targets' are the first ones)
     const int32_t* order;
     const int32_t* ptr;
     const int32_t* idx;
     const uint8_t* bucket;
-    const int32_t* item_slot;
+    const int4* items;
     const int32_t* item_first;
-    int chunk;
 };
 
 struct AttnArgs {
@@ -82,25 +81,48 @@ struct Piece {
     int64_t item;  // >= 0: the item's partial result, else the row's own
 };
 
-__device__ __forceinline__ Piece piece_of(const Lists& L, int64_t unit, int64_t n_nodes)
+// Units of an XCD's waves (workgroups go to the XCDs in turn): its share of the parts of long
+// rows, then of the rows, so that its waves read neighbouring rows through one L2.
+struct Walk {
+    int64_t at, end, step;               // this wave's units
+    int64_t items, item0, row0;          // the XCD's parts, its first one, its first row
+    __device__ __forceinline__ bool is_item(int64_t u) const { return u < items; }
+    __device__ __forceinline__ int64_t item(int64_t u) const { return item0 + u; }
+    __device__ __forceinline__ int64_t slot(int64_t u) const { return row0 + (u - items); }
+};
+__device__ __forceinline__ Walk walk_of(const Lists& L, int waves_per_group)
 {
-    Piece p{0, 0, -1, -1};
-    if (unit < L.n_items) {  // the parts of long rows come first
-        if (unit >= L.item_first[L.n_rows]) return p;
-        const int slot = L.item_slot[unit];
-        const int begin = L.ptr[slot], end = L.ptr[slot + 1];
-        p.begin = begin + (int)(unit - L.item_first[slot]) * L.chunk;
-        p.end = min(p.begin + L.chunk, end);
-        p.node = L.order[slot];
-        p.item = unit;
+    const int xcds = min((int)gridDim.x, kXcds);
+    const int x = blockIdx.x % xcds, j = blockIdx.x / xcds;
+    const int64_t groups = ((int)gridDim.x - x + xcds - 1) / xcds;  // of this XCD
+    Walk w;
+    w.item0 = L.n_items * x / xcds;
+    w.items = L.n_items * (x + 1) / xcds - w.item0;
+    w.row0 = L.n_rows * x / xcds;
+    w.end = w.items + L.n_rows * (x + 1) / xcds - w.row0;
+    w.step = groups * waves_per_group;
+    w.at = (int64_t)j * waves_per_group + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    return w;
+}
+
+__device__ __forceinline__ Piece piece_of(const Lists& L, const Walk& w, int64_t u)
+{
+    Piece p;
+    if (w.is_item(u)) {
+        p.item = w.item(u);
+        const int4 i = L.items[p.item];
+        p.begin = i.x;
+        p.end = i.y;
+        p.node = i.z;
     } else {
-        const int64_t slot = unit - L.n_items;
+        const int64_t slot = w.slot(u);
         p.begin = L.ptr[slot];
         p.end = L.ptr[slot + 1];
         p.node = L.order[slot];
+        p.item = -1;
         if (L.n_items && p.end - p.begin > DG_NEIGHBOR_SPLIT) p.node = -1;
     }
-    if (p.node >= n_nodes) p.node = -1;
+    if (p.node < 0) p.end = p.begin;
     return p;
 }
 
@@ -170,24 +192,6 @@ __device__ __forceinline__ void store4<__bf16>(__bf16* p, const float (&x)[4])
     bf16x4 y;
     for (int i = 0; i < 4; ++i) y[i] = (__bf16)x[i];
     *(bf16x4*)p = y;
-}
-
-// Units [lo, hi) of this workgroup's XCD (workgroups go to the XCDs in turn: neighbouring
-// rows then share an L2), the wave's first unit and its step.
-struct Walk {
-    int64_t at, end, step;
-};
-__device__ __forceinline__ Walk walk_of(int64_t units, int waves_per_group)
-{
-    const int xcds = min((int)gridDim.x, kXcds);
-    const int x = blockIdx.x % xcds, j = blockIdx.x / xcds;
-    const int64_t groups = ((int)gridDim.x - x + xcds - 1) / xcds;  // of this XCD
-    Walk w;
-    const int64_t lo = units * x / xcds;
-    w.end = units * (x + 1) / xcds;
-    w.step = groups * waves_per_group;
-    w.at = lo + (int64_t)j * waves_per_group + threadIdx.x / 64;
-    return w;
 }
 
 }  // namespace dg

@@ -4,7 +4,8 @@
 // mask, distances and bucket boundaries, two compressed lists come out: for every target the
 // sources of its edges (the forward pass and the gradient of q), for every source its targets
 // (the gradients of k and v), each entry with its distance bucket.  Rows sit in slots: a
-// node's slot is the place of its run in the edge list, nodes without a run follow by number.
+// node's slot is the place of its run in the edge list, nodes without a run follow by number (so
+// the targets, being the first nodes, hold the first slots).
 // Slots keep the builder's space-filling order, so rows that run at the same time read
 // neighbouring atoms whatever the caller's numbering is.
 //
@@ -326,12 +327,17 @@ __global__ void parts_kernel(const int32_t* __restrict__ ptr, int64_t n, int spl
     parts[i] = len > split ? (len + chunk - 1) / chunk : 0;
 }
 
-__global__ void items_kernel(const int32_t* __restrict__ first, int64_t n, int64_t max_items,
-                             int32_t* __restrict__ item_slot)
+__global__ void items_kernel(const int32_t* __restrict__ first, const int32_t* __restrict__ ptr,
+                             const int32_t* __restrict__ order, int64_t n, int chunk, int64_t max_items,
+                             int4* __restrict__ item)
 {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < max_items && i >= first[n]) item[i] = make_int4(0, 0, -1, 0);  // (the bound is not reached)
     if (i >= n) return;
-    for (int64_t k = first[i]; k < first[i + 1] && k < max_items; ++k) item_slot[k] = (int32_t)i;
+    for (int64_t k = first[i]; k < first[i + 1] && k < max_items; ++k) {
+        const int at = ptr[i] + (int)(k - first[i]) * chunk;
+        item[k] = make_int4(at, min(at + chunk, ptr[i + 1]), order[i], (int)i);
+    }
 }
 
 struct Layout {
@@ -539,12 +545,13 @@ size_t dg_neighbors_parts_workspace_size(int64_t n_rows)
     return al(4 * (size_t)(n_rows + 1)) + al(4 * (size_t)(n_rows / kScanTile + 2));
 }
 
-dg_status dg_neighbors_parts(const int32_t* ptr, int64_t n_rows, int32_t chunk, int64_t max_items,
-                             int32_t* item_first, int32_t* item_slot, void* ws, size_t ws_bytes, hipStream_t s)
+dg_status dg_neighbors_parts(const int32_t* order, const int32_t* ptr, int64_t n_rows, int32_t chunk,
+                             int64_t max_items, int32_t* item_first, int32_t* items, void* ws, size_t ws_bytes,
+                             hipStream_t s)
 {
     if (n_rows < 1 || n_rows > kMaxEdges || chunk < 1 || max_items < 1)
         return fail(DG_ERR_INVALID, "n_rows, chunk and max_items must be positive");
-    if (!ptr || !item_first || !item_slot) return fail(DG_ERR_INVALID, "inputs or outputs are NULL");
+    if (!order || !ptr || !item_first || !items) return fail(DG_ERR_INVALID, "inputs or outputs are NULL");
     if (!ws || ws_bytes < dg_neighbors_parts_workspace_size(n_rows))
         return fail(DG_ERR_WORKSPACE, "workspace too small");
     int* parts = (int*)ws;
@@ -552,8 +559,8 @@ dg_status dg_neighbors_parts(const int32_t* ptr, int64_t n_rows, int32_t chunk, 
     hipLaunchKernelGGL(parts_kernel, dim3(nblk(n_rows)), dim3(256), 0, s, ptr, n_rows, DG_NEIGHBOR_SPLIT, (int)chunk,
                        parts);
     excl_scan<int, int>(parts, n_rows, item_first, part, s);
-    hipLaunchKernelGGL(items_kernel, dim3(nblk(n_rows)), dim3(256), 0, s, (const int32_t*)item_first, n_rows, max_items,
-                       item_slot);
+    hipLaunchKernelGGL(items_kernel, dim3(nblk(std::max(n_rows, max_items))), dim3(256), 0, s, (const int32_t*)item_first,
+                       ptr, order, n_rows, (int)chunk, max_items, (int4*)items);
     return launched("dg_neighbors_parts");
 }
 

@@ -30,7 +30,7 @@ class _Rows:
 
     def __init__(self, order, ptr, idx, bucket):
         self.order, self.ptr, self.idx, self.bucket = order, ptr, idx, bucket
-        self.item_slot = self.item_first = None
+        self.items = self.item_first = None
         c = self.c = L.NeighborLists()
         c.n_rows = order.numel()
         c.order, c.ptr, c.idx = order.data_ptr(), ptr.data_ptr(), idx.data_ptr()
@@ -45,16 +45,16 @@ class _Rows:
         lib, dev, c = L.lib(), self.ptr.device, self.c
         c.chunk = min(2048, max(128, -(-long_entries // 4096 + 31) // 32 * 32))
         c.n_items = long_entries // c.chunk + long_rows
-        self.item_slot = torch.empty(c.n_items, dtype=torch.int32, device=dev)
+        self.items = torch.empty((c.n_items, 4), dtype=torch.int32, device=dev)
         self.item_first = torch.empty(c.n_rows + 1, dtype=torch.int32, device=dev)
-        c.item_slot, c.item_first = self.item_slot.data_ptr(), self.item_first.data_ptr()
+        c.items, c.item_first = self.items.data_ptr(), self.item_first.data_ptr()
         wsb = lib.dg_neighbors_parts_workspace_size(c.n_rows)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-        L.check(lib.dg_neighbors_parts(L.ptr(self.ptr), c.n_rows, c.chunk, c.n_items, L.ptr(self.item_first),
-                                       L.ptr(self.item_slot), L.ptr(ws), wsb, stream), "neighbor_plan")
+        L.check(lib.dg_neighbors_parts(L.ptr(self.order), L.ptr(self.ptr), c.n_rows, c.chunk, c.n_items,
+                                       L.ptr(self.item_first), L.ptr(self.items), L.ptr(ws), wsb, stream), "neighbor_plan")
 
     def tensors(self):
-        return [t for t in (self.order, self.ptr, self.idx, self.bucket, self.item_slot, self.item_first)
+        return [t for t in (self.order, self.ptr, self.idx, self.bucket, self.items, self.item_first)
                 if t is not None]
 
 

@@ -358,7 +358,8 @@ dg_status dg_halo_write(const dg_halo_desc* desc, const void* pid, int64_t* send
  *   mask                 uint8 [n_edges] or NULL: edges at 0 are left out
  *   dist                 [n_edges] of dist_dtype, with boundaries [n_boundaries] (ascending, of
  *                        the same type): an entry's bucket is the number of boundaries <= dist
- * Rows sit in slots: nodes in the order of their runs, then the nodes without one.
+ * Rows sit in slots: nodes in the order of their runs, then the nodes without one by number; the
+ * slots [0, n_targets) so are those of the targets.
  *   order  out int32 [n_nodes]      node of a slot
  *   ptr    out int32 [n_nodes + 1]  a slot's entries
  *   idx    out int32 [n_edges + DG_NEIGHBOR_PAD]  sources (by target) or targets (by source)
@@ -393,12 +394,12 @@ typedef struct dg_neighbor_totals {
  * are worked on in items of `chunk` entries (dg_neighbors_parts); n_items == 0: by one wave. */
 typedef struct dg_neighbor_lists {
     int64_t n_rows;  /* n_nodes */
-    int64_t n_items; /* length of item_slot (an upper bound of the items) */
+    int64_t n_items; /* length of items (an upper bound of their number) */
     const int32_t* order;
     const int32_t* ptr;
     const int32_t* idx;
     const uint8_t* bucket;     /* or NULL */
-    const int32_t* item_slot;  /* [n_items] */
+    const int32_t* items;      /* [n_items, 4]: first entry, end, node (-1: none), slot */
     const int32_t* item_first; /* [n_rows + 1] */
     int32_t chunk;
     int32_t pad_;
@@ -418,11 +419,11 @@ dg_status dg_neighbors_by_source(const dg_neighbor_desc* desc, int64_t n_entries
                                  uint8_t* source_bucket, void* workspace, size_t workspace_bytes,
                                  void* sort_workspace, size_t sort_workspace_bytes,
                                  hipStream_t stream);
-/* The items of rows above DG_NEIGHBOR_SPLIT entries: item_first int32 [n_rows + 1], item_slot
- * int32 [max_items] with max_items >= long_entries / chunk + long_rows. */
+/* The items of rows above DG_NEIGHBOR_SPLIT entries: item_first int32 [n_rows + 1], items int32
+ * [max_items, 4], aligned to 16 bytes, with max_items >= long_entries / chunk + long_rows. */
 size_t dg_neighbors_parts_workspace_size(int64_t n_rows);
-dg_status dg_neighbors_parts(const int32_t* ptr, int64_t n_rows, int32_t chunk, int64_t max_items,
-                             int32_t* item_first, int32_t* item_slot, void* workspace,
+dg_status dg_neighbors_parts(const int32_t* order, const int32_t* ptr, int64_t n_rows, int32_t chunk,
+                             int64_t max_items, int32_t* item_first, int32_t* items, void* workspace,
                              size_t workspace_bytes, hipStream_t stream);
 
 /* Attention over the lists:
