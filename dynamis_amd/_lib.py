@@ -228,5 +228,30 @@ def stream_of(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(device: torch.device) -> int:
+    """The current stream of the device as an integer (a tenth of stream_of's host time)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class on_device:
+    """torch.cuda.device for the device, without its host time where it is the current one."""
+
+    def __init__(self, device):
+        self.ctx = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+
+
+def addr(t):
+    """A tensor's address for a void* argument (None: NULL)."""
+    return None if t is None else t.data_ptr()
+
+
 def ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)

@@ -684,7 +684,7 @@ dg_status dg_attention_forward(const dg_attention_desc* d, const dg_neighbor_lis
     if (st == DG_OK) st = check_lists(d, by_target);
     if (st != DG_OK) return st;
     const Layout L = layout(d, by_target, nullptr);
-    if (!ws || ws_bytes < L.total) return fail(DG_ERR_WORKSPACE, "workspace too small");
+    if (by_target->n_items > 0 && (!ws || ws_bytes < L.total)) return fail(DG_ERR_WORKSPACE, "workspace too small");
     if (d->n_targets == 0) return DG_OK;
     if (!q || !k || !v || !out || (d->n_buckets > 0 && !table))
         return fail(DG_ERR_INVALID, "inputs or outputs are NULL");

@@ -650,7 +650,13 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(NT)) void forward_mfma_kernel
 }
 
 // ---------------------------------------------------------------- backward, by target
-constexpr int waves_of_q(int NT) { return NT == 2 ? 3 : 4; }
+#ifndef WQ2
+#define WQ2 2
+#define WQ1 3
+#define WK2 2
+#define WK1 3
+#endif
+constexpr int waves_of_q(int NT) { return NT == 2 ? WQ2 : WQ1; }
 
 // delta = <g, out> of a column's head: eight channels a lane, whose sums the head's lanes add up.
 __device__ __forceinline__ float delta_of(const AttnArgs& a, const HeadGroups& hg, const Piece& p, const Lane& l, float* s_x)
@@ -864,7 +870,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_q(NT)) void backward_q_mfma_k
 }
 
 // ---------------------------------------------------------------- backward, by source
-constexpr int waves_of_kv(int NT) { return NT == 2 ? 2 : 3; }
+constexpr int waves_of_kv(int NT) { return NT == 2 ? WK2 : WK1; }
 
 __device__ __forceinline__ Lane lane_of_kv(const AttnArgs& a, const KvGroups& kg, int pass)
 {

@@ -69,13 +69,12 @@ class NeighborPlan:
         self.num_nodes, self.num_targets = num_nodes, num_targets
         self.num_edges, self.num_buckets = num_edges, num_buckets
         self.by_target, self.by_source, self.symmetric = by_target, by_source, symmetric
-        self._stream = torch.cuda.current_stream(device)
+        self._stream = L.raw_stream(device)
 
-    def _use(self):
-        """Keeps the lists' memory from being handed out again while the current stream reads it."""
-        s = torch.cuda.current_stream(self.device)
-        if s != self._stream:
-            self.record_stream(s)
+    def _use(self, stream):
+        """Keeps the lists' memory from being handed out again while another stream reads it."""
+        if stream != self._stream:
+            self.record_stream(torch.cuda.current_stream(self.device))
 
     def record_stream(self, stream):
         for rows in {id(r): r for r in (self.by_target, self.by_source) if r is not None}.values():
@@ -169,41 +168,48 @@ def neighbor_plan(edge_index, num_nodes, num_targets=None, distances=None, bound
 def _rows_16(t):
     """t [n, heads, dim] as it is if its rows are whole, start at 16 bytes and lie a multiple of
     16 bytes apart; else a copy."""
+    row, head, one = t.stride()
     step = 16 // t.element_size()
-    if t.stride(2) == 1 and (t.size(1) == 1 or t.stride(1) == t.size(2)) and t.stride(0) % step == 0 \
-            and t.stride(0) >= 0 and t.data_ptr() % 16 == 0:
+    if one == 1 and (t.size(1) == 1 or head == t.size(2)) and row % step == 0 and row >= 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _attention_desc(q, k, v, n_nodes, n_buckets, scale):
-    d = L.AttentionDesc()
-    d.n_targets, d.n_nodes = q.size(0), n_nodes
-    d.ld_q, d.ld_k, d.ld_v = q.stride(0), k.stride(0), v.stride(0)
-    d.heads, d.kv_heads, d.dim = q.size(1), k.size(1), q.size(2)
-    d.n_buckets, d.dtype, d.scale = n_buckets, _DTYPES[q.dtype], scale
-    return d
+def _workspace(lib, d, to, fro, dev):
+    wsb = lib.dg_attention_workspace_size(d, to, fro)
+    if wsb == 0:
+        raise RuntimeError(f"neighbor_attention: {lib.dg_last_error().decode()}")
+    return torch.empty(wsb, dtype=torch.uint8, device=dev), wsb
 
 
 def _forward(q, k, v, table, plan, scale, train, want_lse):
-    lib, dev = L.lib(), q.device
+    lib, dev = L.lib(), plan.device
     q, k, v = _rows_16(q), _rows_16(k), _rows_16(v)
-    table = table.contiguous() if table is not None else None
-    d = _attention_desc(q, k, v, plan.num_nodes, 0 if table is None else table.size(0), scale)
+    if table is not None:
+        table = table.contiguous()
+    targets, heads, dim = q.shape
+    d = L.AttentionDesc(targets, plan.num_nodes, q.stride(0), k.stride(0), v.stride(0), 0, heads, k.size(1), dim,
+                        0 if table is None else table.size(0), _DTYPES[q.dtype], scale)
     rows = plan.by_target
-    wsb = lib.dg_attention_workspace_size(d, rows.byref, None)
-    if wsb == 0:
-        raise RuntimeError(f"neighbor_attention: {lib.dg_last_error().decode()}")
-    with torch.cuda.device(dev):
-        plan._use()
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        out32 = torch.empty(q.shape, dtype=torch.float32, device=dev) if train and q.dtype != torch.float32 else None
-        norm = torch.empty((*q.shape[:2], 2), dtype=torch.float32, device=dev) if train else None
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if want_lse else None
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-        L.check(lib.dg_attention_forward(d, rows.byref, L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(table), L.ptr(out),
-                                         L.ptr(out32), L.ptr(norm), L.ptr(lse), L.ptr(ws), wsb, L.stream_of(dev)),
-                "neighbor_attention")
+    with L.on_device(dev):
+        stream = L.raw_stream(dev)
+        plan._use(stream)
+        out = torch.empty((targets, heads, dim), dtype=q.dtype, device=dev)
+        out32 = norm = lse = ws = None
+        wsb = 0
+        if train:
+            norm = torch.empty((targets, heads, 2), dtype=torch.float32, device=dev)
+            if q.dtype != torch.float32:
+                out32 = torch.empty((targets, heads, dim), dtype=torch.float32, device=dev)
+        if want_lse:
+            lse = torch.empty((targets, heads), dtype=torch.float32, device=dev)
+        if rows.c.n_items:  # (partial results of long rows are all that the forward pass keeps there)
+            ws, wsb = _workspace(lib, d, rows.byref, None, dev)
+        addr = L.addr
+        status = lib.dg_attention_forward(d, rows.byref, q.data_ptr(), k.data_ptr(), v.data_ptr(), addr(table),
+                                          out.data_ptr(), addr(out32), addr(norm), addr(lse), addr(ws), wsb, stream)
+        if status:
+            L.check(status, "neighbor_attention")
     return out, lse, out32, norm
 
 
@@ -221,26 +227,74 @@ class _Attention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _grad_lse):
         q, k, v, table, out32, norm = ctx.saved_tensors
-        plan, lib, dev = ctx.plan, L.lib(), q.device
-        _check(plan.by_source is not None, "neighbor_attention: the plan was made with backward=False")
+        plan, lib = ctx.plan, L.lib()
+        dev = plan.device
+        if plan.by_source is None:
+            raise RuntimeError("neighbor_attention: the plan was made with backward=False")
         q, k, v, grad = _rows_16(q), _rows_16(k), _rows_16(v), _rows_16(grad)
-        table = table.contiguous() if table is not None else None
-        d = _attention_desc(q, k, v, plan.num_nodes, 0 if table is None else table.size(0), ctx.scale)
-        d.ld_g = grad.stride(0)
+        if table is not None:
+            table = table.contiguous()
+        targets, heads, dim = q.shape
+        d = L.AttentionDesc(targets, plan.num_nodes, q.stride(0), k.stride(0), v.stride(0), grad.stride(0), heads,
+                            k.size(1), dim, 0 if table is None else table.size(0), _DTYPES[q.dtype], ctx.scale)
         to, fro = plan.by_target.byref, plan.by_source.byref
-        wsb = lib.dg_attention_workspace_size(d, to, fro)
-        if wsb == 0:
-            raise RuntimeError(f"neighbor_attention: {lib.dg_last_error().decode()}")
-        with torch.cuda.device(dev):
-            plan._use()
-            new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
-            dq, dk, dv = new(q), new(k), new(v)
-            dtable = new(table) if table is not None else None
-            ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-            L.check(lib.dg_attention_backward(d, to, fro, L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(table), L.ptr(out32),
-                                              L.ptr(norm), L.ptr(grad), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(dtable),
-                                              L.ptr(ws), wsb, L.stream_of(dev)), "neighbor_attention")
+        with L.on_device(dev):
+            stream = L.raw_stream(dev)
+            plan._use(stream)
+            dq = torch.empty((targets, heads, dim), dtype=q.dtype, device=dev)
+            dk = torch.empty(k.shape, dtype=q.dtype, device=dev)
+            dv = torch.empty(k.shape, dtype=q.dtype, device=dev)
+            dtable = torch.empty(table.shape, dtype=torch.float32, device=dev) if table is not None else None
+            ws, wsb = _workspace(lib, d, to, fro, dev)
+            addr = L.addr
+            status = lib.dg_attention_backward(d, to, fro, q.data_ptr(), k.data_ptr(), v.data_ptr(), addr(table),
+                                               out32.data_ptr(), norm.data_ptr(), grad.data_ptr(), dq.data_ptr(),
+                                               dk.data_ptr(), dv.data_ptr(), addr(dtable), ws.data_ptr(), wsb, stream)
+            if status:
+                L.check(status, "neighbor_attention")
         return dq, dk, dv, dtable, None, None, None
+
+
+def _check_attention(q, k, v, plan, bias_table):
+    """The refusals of neighbor_attention, with their messages."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
+        _check(t.dim() == 3, f"{name} must have shape [nodes, heads, dim], got {_shape(t)}")
+        _check(t.device == plan.device, f"{name} must be on the plan's device {plan.device}, got {t.device}")
+        _check(t.dtype in _DTYPES, f"{name} must be float32 or bfloat16, got {t.dtype}")
+        _check(t.dtype == q.dtype, f"q, k and v must have one dtype, got {q.dtype} and {t.dtype}")
+        _check(t.size(2) == q.size(2), f"q, k and v must have one head width, got {q.size(2)} and {t.size(2)}")
+    _check(q.size(0) == plan.num_targets, f"q must have {plan.num_targets} rows, got {q.size(0)}")
+    _check(k.size(0) == plan.num_nodes and v.shape == k.shape,
+           f"k and v must have {plan.num_nodes} rows and one shape, got {_shape(k)} and {_shape(v)}")
+    heads, kv, dim = q.size(1), k.size(1), q.size(2)
+    _check(heads >= 1 and kv >= 1 and heads % kv == 0, f"heads ({heads}) must be a multiple of kv_heads ({kv})")
+    _check(heads <= 1024, f"at most 1024 heads, got {heads}")
+    _check(8 <= dim <= 256 and dim % 8 == 0, f"the head width must be a multiple of 8, 8 to 256, got {dim}")
+    if bias_table is not None:
+        _check(plan.num_buckets > 0, "bias_table needs a plan with distances")
+        _check(bias_table.device == plan.device and bias_table.is_floating_point()
+               and tuple(bias_table.shape) == (plan.num_buckets, heads),
+               f"bias_table must be floating [{plan.num_buckets}, {heads}] on {plan.device}, got {_shape(bias_table)}")
+        _check(bias_table.numel() <= 4096, f"bias_table must hold at most 4096 entries, got {bias_table.numel()}")
+
+
+def _attention_is_fine(q, k, v, plan, bias_table):
+    """Whether _check_attention would pass, without its messages' host time."""
+    if not (type(q) in _TENSORS and type(k) in _TENSORS and type(v) in _TENSORS and q.dim() == 3 and k.dim() == 3):
+        return False
+    (targets, heads, dim), (nodes, kv, kdim) = q.shape, k.shape
+    dtype, dev = q.dtype, plan.device
+    return (targets == plan.num_targets and nodes == plan.num_nodes and dim == kdim and v.shape == k.shape
+            and dtype in _DTYPES and k.dtype == dtype and v.dtype == dtype
+            and q.device == dev and k.device == dev and v.device == dev
+            and 1 <= heads <= 1024 and kv >= 1 and heads % kv == 0 and 8 <= dim <= 256 and dim % 8 == 0
+            and (bias_table is None
+                 or bias_table.dtype == torch.float32 and bias_table.device == dev and plan.num_buckets > 0
+                 and bias_table.shape == (plan.num_buckets, heads) and plan.num_buckets * heads <= 4096))
+
+
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
 
 
 def neighbor_attention(q, k, v, plan, bias_table=None, scale=None, return_lse=False):
@@ -260,32 +314,19 @@ def neighbor_attention(q, k, v, plan, bias_table=None, scale=None, return_lse=Fa
     Differentiable in q, k, v and bias_table (once).  All sums are float32, in a fixed order:
     results repeat bit for bit.
     """
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
-        _check(t.dim() == 3, f"{name} must have shape [nodes, heads, dim], got {_shape(t)}")
-        _check(t.device == plan.device, f"{name} must be on the plan's device {plan.device}, got {t.device}")
-        _check(t.dtype in _DTYPES, f"{name} must be float32 or bfloat16, got {t.dtype}")
-        _check(t.dtype == q.dtype, f"q, k and v must have one dtype, got {q.dtype} and {t.dtype}")
-        _check(t.size(2) == q.size(2), f"q, k and v must have one head width, got {q.size(2)} and {t.size(2)}")
-    _check(q.size(0) == plan.num_targets, f"q must have {plan.num_targets} rows, got {q.size(0)}")
-    _check(k.size(0) == plan.num_nodes and v.shape == k.shape,
-           f"k and v must have {plan.num_nodes} rows and one shape, got {_shape(k)} and {_shape(v)}")
-    heads, kv, dim = q.size(1), k.size(1), q.size(2)
-    _check(heads >= 1 and kv >= 1 and heads % kv == 0, f"heads ({heads}) must be a multiple of kv_heads ({kv})")
-    _check(8 <= dim <= 256 and dim % 8 == 0, f"the head width must be a multiple of 8, 8 to 256, got {dim}")
-    if bias_table is not None:
-        _check(plan.num_buckets > 0, "bias_table needs a plan with distances")
-        _check(bias_table.device == plan.device and bias_table.is_floating_point()
-               and tuple(bias_table.shape) == (plan.num_buckets, heads),
-               f"bias_table must be floating [{plan.num_buckets}, {heads}] on {plan.device}, got {_shape(bias_table)}")
-        _check(bias_table.numel() <= 4096, f"bias_table must hold at most 4096 entries, got {bias_table.numel()}")
-        bias_table = bias_table.float()
-    scale = float(dim ** -0.5 if scale is None else scale)
-    _check(math.isfinite(scale), f"scale must be finite, got {scale}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table)):
-        out, lse = _Attention.apply(q, k, v, bias_table, plan, scale, return_lse)
+    if not _attention_is_fine(q, k, v, plan, bias_table):
+        _check_attention(q, k, v, plan, bias_table)
+        if bias_table is not None:
+            bias_table = bias_table.float()
+    if scale is None:
+        scale = q.size(2) ** -0.5
+    elif not math.isfinite(scale):
+        raise RuntimeError(f"scale must be finite, got {scale}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or bias_table is not None and bias_table.requires_grad):
+        out, lse = _Attention.apply(q, k, v, bias_table, plan, float(scale), return_lse)
     else:
-        out, lse, _, _ = _forward(q, k, v, bias_table, plan, scale, False, return_lse)
+        out, lse, _, _ = _forward(q, k, v, bias_table, plan, float(scale), False, return_lse)
     return (out, lse) if return_lse else out
 
 
@@ -295,10 +336,12 @@ def _grouped_desc(x, weight):
 
 def _grouped_forward(x, weight, sizes, bias):
     dev = x.device
-    with torch.cuda.device(dev):
+    with L.on_device(dev):
         y = torch.empty((x.size(0), weight.size(1)), dtype=x.dtype, device=dev)
-        L.check(L.lib().dg_grouped_forward(_grouped_desc(x, weight), L.ptr(x), L.ptr(weight), L.ptr(sizes), L.ptr(bias),
-                                           L.ptr(y), L.stream_of(dev)), "grouped_linear")
+        status = L.lib().dg_grouped_forward(_grouped_desc(x, weight), x.data_ptr(), weight.data_ptr(), sizes.data_ptr(),
+                                            L.addr(bias), y.data_ptr(), L.raw_stream(dev))
+        if status:
+            L.check(status, "grouped_linear")
     return y
 
 
@@ -315,15 +358,54 @@ class _Grouped(torch.autograd.Function):
         need_x, need_w, _, need_b = ctx.needs_input_grad
         lib, dev, grad = L.lib(), x.device, grad.contiguous()
         d = _grouped_desc(x, weight)
-        with torch.cuda.device(dev):
-            dx = torch.empty_like(x) if need_x else None
-            dw = torch.empty_like(weight) if need_w or need_b else None
+        with L.on_device(dev):
+            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+            dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_w or need_b else None
             db = torch.empty(weight.shape[:2], dtype=x.dtype, device=dev) if need_b else None
             wsb = lib.dg_grouped_workspace_size(d) if dw is not None else 0
             ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-            L.check(lib.dg_grouped_backward(d, L.ptr(x), L.ptr(weight), L.ptr(sizes), L.ptr(grad), L.ptr(dx), L.ptr(dw),
-                                            L.ptr(db), L.ptr(ws), wsb, L.stream_of(dev)), "grouped_linear")
+            addr = L.addr
+            status = lib.dg_grouped_backward(d, x.data_ptr(), weight.data_ptr(), sizes.data_ptr(), grad.data_ptr(),
+                                             addr(dx), addr(dw), addr(db), addr(ws), wsb, L.raw_stream(dev))
+            if status:
+                L.check(status, "grouped_linear")
         return dx, dw if need_w else None, None, db
+
+
+def _check_grouped(x, weight, sizes, bias):
+    """The refusals of grouped_linear, with their messages."""
+    _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a CUDA tensor")
+    _check(x.dim() == 2, f"x must have shape [rows, k], got {_shape(x)}")
+    _check(x.dtype in _DTYPES, f"x must be float32 or bfloat16, got {x.dtype}")
+    _check(isinstance(weight, torch.Tensor) and weight.device == x.device, f"weight must be on {x.device}")
+    _check(weight.dim() == 3 and weight.size(2) == x.size(1),
+           f"weight must have shape [groups, n, {x.size(1)}], got {_shape(weight)}")
+    _check(weight.dtype == x.dtype, f"weight must be {x.dtype}, got {weight.dtype}")
+    groups = weight.size(0)
+    _check(1 <= groups <= 1 << 20, f"weight must hold 1 to 2^20 groups, got {groups}")
+    _check(1 <= x.size(1) <= 1 << 20 and 1 <= weight.size(1) <= 1 << 20, "the widths must be 1 to 2^20")
+    _check(sizes.dim() == 1 and sizes.size(0) == groups and sizes.dtype == torch.int64,
+           f"sizes must be int64 [{groups}], got {sizes.dtype} {_shape(sizes)}")
+    if sizes.is_cuda:
+        _check(sizes.device == x.device, f"sizes must be on {x.device}")
+    else:
+        _check(bool((sizes >= 0).all()) and int(sizes.sum()) == x.size(0),
+               f"sizes must be non-negative and add up to {x.size(0)} rows")
+    if bias is not None:
+        _check(bias.device == x.device and bias.dtype == x.dtype and tuple(bias.shape) == tuple(weight.shape[:2]),
+               f"bias must be {x.dtype} [{groups}, {weight.size(1)}] on {x.device}, got {bias.dtype} {_shape(bias)}")
+
+
+def _grouped_is_fine(x, weight, sizes, bias):
+    """Whether _check_grouped would pass for tensors on one device, without its messages' host time."""
+    if not (type(x) in _TENSORS and type(weight) in _TENSORS and x.dim() == 2 and weight.dim() == 3 and x.is_cuda):
+        return False
+    groups, n, k = weight.shape
+    dev, dtype = x.device, x.dtype
+    return (x.size(1) == k and 1 <= groups <= 1 << 20 and 1 <= k <= 1 << 20 and 1 <= n <= 1 << 20
+            and dtype in _DTYPES and weight.dtype == dtype and weight.device == dev
+            and sizes.device == dev and sizes.dtype == torch.int64 and sizes.shape == (groups,)
+            and (bias is None or bias.dtype == dtype and bias.device == dev and bias.shape == (groups, n)))
 
 
 def grouped_linear(x, weight, sizes, bias=None):
@@ -339,29 +421,14 @@ def grouped_linear(x, weight, sizes, bias=None):
     Differentiable in x, weight and bias (once).  Sums are float32, in a fixed order: results
     repeat bit for bit.
     """
-    _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a CUDA tensor")
-    _check(x.dim() == 2, f"x must have shape [rows, k], got {_shape(x)}")
-    _check(x.dtype in _DTYPES, f"x must be float32 or bfloat16, got {x.dtype}")
-    _check(isinstance(weight, torch.Tensor) and weight.device == x.device, f"weight must be on {x.device}")
-    _check(weight.dim() == 3 and weight.size(2) == x.size(1),
-           f"weight must have shape [groups, n, {x.size(1)}], got {_shape(weight)}")
-    _check(weight.dtype == x.dtype, f"weight must be {x.dtype}, got {weight.dtype}")
-    groups = weight.size(0)
-    _check(1 <= groups <= 1 << 20, f"weight must hold 1 to 2^20 groups, got {groups}")
-    _check(1 <= x.size(1) <= 1 << 20 and 1 <= weight.size(1) <= 1 << 20, "the widths must be 1 to 2^20")
-    sizes = torch.as_tensor(sizes)
-    _check(sizes.dim() == 1 and sizes.size(0) == groups and sizes.dtype == torch.int64,
-           f"sizes must be int64 [{groups}], got {sizes.dtype} {_shape(sizes)}")
-    if not sizes.is_cuda:
-        _check(bool((sizes >= 0).all()) and int(sizes.sum()) == x.size(0),
-               f"sizes must be non-negative and add up to {x.size(0)} rows")
-    _check(not sizes.is_cuda or sizes.device == x.device, f"sizes must be on {x.device}")
-    sizes = sizes.to(x.device).contiguous()
+    if not isinstance(sizes, torch.Tensor):
+        sizes = torch.as_tensor(sizes)
+    if not _grouped_is_fine(x, weight, sizes, bias):
+        _check_grouped(x, weight, sizes, bias)
+        sizes = sizes.to(x.device)
+    x, weight, sizes = x.contiguous(), weight.contiguous(), sizes.contiguous()
     if bias is not None:
-        _check(bias.device == x.device and bias.dtype == x.dtype and tuple(bias.shape) == tuple(weight.shape[:2]),
-               f"bias must be {x.dtype} [{groups}, {weight.size(1)}] on {x.device}, got {bias.dtype} {_shape(bias)}")
         bias = bias.contiguous()
-    x, weight = x.contiguous(), weight.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad):
         return _Grouped.apply(x, weight, sizes, bias)
     return _grouped_forward(x, weight, sizes, bias)

@@ -441,7 +441,8 @@ dg_status dg_neighbors_parts(const int32_t* order, const int32_t* ptr, int64_t n
  *   lse    float32 [n_targets, heads], natural, or NULL
  * Backward: dq, dk, dv of dtype and contiguous, dtable float32.  Sums are float32 and in a
  * fixed order: results repeat bit for bit.  The workspace of
- * dg_attention_workspace_size(desc, by_target, by_source or NULL for the forward pass) bytes. */
+ * dg_attention_workspace_size(desc, by_target, by_source or NULL for the forward pass) bytes; a
+ * forward pass over lists without items needs none. */
 typedef struct dg_attention_desc {
     int64_t n_targets;
     int64_t n_nodes;
