@@ -114,24 +114,25 @@ __device__ __forceinline__ int swapped(int row, int chunk) { return chunk ^ ((ro
 
 // One thread's eight 16-byte loads of a slab of an operand: `n` of its rows and `c_n` summed
 // indices from c0 are real.  TURNED: memory holds [summed][row], else [row][summed].
-template <typename T, bool TURNED>
+template <typename T, bool TURNED, int ROWS = kTile>
 struct Stage {
-    u32x4 r[8];
-    __device__ __forceinline__ void load(const T* p, int64_t ld, int n, int c0, int c_n, int t)
+    static constexpr int N = ROWS / 16, R = TURNED && N < kChunk<T> ? kChunk<T> : N;
+    static __device__ __forceinline__ void load(u32x4 (&r)[R], const T* p, int64_t ld, int n, int c0, int c_n, int t)
     {
         constexpr int C = kChunk<T>;
         if constexpr (!TURNED) {
             const int chunk = t % 8, left = c_n - (c0 + chunk * C);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < N; ++i) {
                 const int row = t / 8 + 16 * i;
                 r[i] = load_chunk(p + row * ld + c0 + chunk * C, row < n ? left : 0);
             }
         } else {
-            constexpr int across = kTile / C;
+            constexpr int across = ROWS / C;
 #pragma unroll
-            for (int b = 0; b < 8 / C; ++b) {
+            for (int b = 0; b < (N + C - 1) / C; ++b) {
                 const int id = t + 128 * b, jb = id % across, cb = id / across;
+                if (N < C && cb >= 8) break;  // (half of the threads have a block)
 #pragma unroll
                 for (int i = 0; i < C; ++i) {
                     const int c = c0 + cb * C + i;
@@ -140,21 +141,22 @@ struct Stage {
             }
         }
     }
-    __device__ __forceinline__ void store(char* lds, int t) const
+    static __device__ __forceinline__ void store(const u32x4 (&r)[R], char* lds, int t)
     {
         constexpr int C = kChunk<T>;
         if constexpr (!TURNED) {
             const int chunk = t % 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < N; ++i) {
                 const int row = t / 8 + 16 * i;
                 *(u32x4*)(lds + row * kRowBytes + swapped(row, chunk) * 16) = r[i];
             }
         } else {
-            constexpr int across = kTile / C;
+            constexpr int across = ROWS / C;
 #pragma unroll
-            for (int b = 0; b < 8 / C; ++b) {
+            for (int b = 0; b < (N + C - 1) / C; ++b) {
                 const int id = t + 128 * b, jb = id % across, cb = id / across;
+                if (N < C && cb >= 8) break;
 #pragma unroll
                 for (int j = 0; j < C; ++j) {
                     u32x4 v;
@@ -267,7 +269,9 @@ struct Place {
     int64_t group, piece;  // the piece's number in its group
     int64_t row, size;     // the group's first row, its rows
     int64_t many;          // pieces of the groups before that have more than one
+    int64_t split;         // those groups' number
 };
+constexpr int kSplitBit = 40;  // in the scan: groups above pieces (2^20 groups, 2^40 rows)
 
 // A group's rows, were there enough: a negative size is empty, none is larger than all rows.
 __device__ __forceinline__ int64_t claim(const Args& a, int64_t g)
@@ -280,16 +284,17 @@ __device__ __forceinline__ int64_t granted(const Args& a, int64_t g, int64_t row
     return min(claim(a, g), max(a.rows - row, (int64_t)0));
 }
 
-// One pass of the workgroup of 256 over the groups: all pieces and rows, and where `found`
-// holds, of (group, its first piece, its pieces), that group's place (piece: see the caller).
-template <typename F>
+// One pass of the workgroup (256 threads, or 512) over the groups: all pieces and rows, and where `found`
+// holds, of (its first piece, its pieces, split groups before), that group's place (piece: its
+// first piece).
+template <int WAVES, typename F>
 __device__ __forceinline__ void pass(const Args& a, const Cuts& c, int64_t* s_w, Place* s_p, int64_t& pieces, int64_t& rows,
                                      F&& found)
 {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     pieces = 0;
     int64_t claimed = 0, many = 0;
-    for (int64_t g0 = 0; g0 < a.groups; g0 += 256) {
+    for (int64_t g0 = 0; g0 < a.groups; g0 += 64 * WAVES) {
         const int64_t g = g0 + threadIdx.x, n = claim(a, g);
         int64_t in = n;
         for (int o = 1; o < 64; o <<= 1) {
@@ -299,12 +304,12 @@ __device__ __forceinline__ void pass(const Args& a, const Cuts& c, int64_t* s_w,
         if (lane == 63) s_w[w] = in;
         __syncthreads();
         int64_t row = claimed + in - n;
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < WAVES; ++i) {
             if (i < w) row += s_w[i];
             claimed += s_w[i];
         }
         const int64_t size = min(n, max(a.rows - row, (int64_t)0));
-        const int64_t p = g < a.groups ? c.of(size) : 0, m = p > 1 ? p : 0;
+        const int64_t p = g < a.groups ? c.of(size) : 0, m = p > 1 ? p | 1ll << kSplitBit : 0;
         int64_t ip = p, im = m;
         for (int o = 1; o < 64; o <<= 1) {
             const int64_t x = __shfl_up(ip, o, 64), z = __shfl_up(im, o, 64);
@@ -314,30 +319,32 @@ __device__ __forceinline__ void pass(const Args& a, const Cuts& c, int64_t* s_w,
             }
         }
         if (lane == 63) {
-            s_w[4 + w] = ip;
-            s_w[8 + w] = im;
+            s_w[WAVES + w] = ip;
+            s_w[2 * WAVES + w] = im;
         }
         __syncthreads();
         int64_t bp = pieces + ip - p, bm = many + im - m;
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < WAVES; ++i) {
             if (i < w) {
-                bp += s_w[4 + i];
-                bm += s_w[8 + i];
+                bp += s_w[WAVES + i];
+                bm += s_w[2 * WAVES + i];
             }
-            pieces += s_w[4 + i];
-            many += s_w[8 + i];
+            pieces += s_w[WAVES + i];
+            many += s_w[2 * WAVES + i];
         }
-        if (g < a.groups && found(g, bp, p)) *s_p = Place{g, bp, min(row, a.rows), size, bm};
+        if (g < a.groups && found(bp, p, bm >> kSplitBit))
+            *s_p = Place{g, bp, min(row, a.rows), size, bm & ((1ll << kSplitBit) - 1), bm >> kSplitBit};
     }
     __syncthreads();
     rows = min(claimed, a.rows);
 }
 
 // The place of piece `at` (there is one).
+template <int WAVES>
 __device__ __forceinline__ Place locate(const Args& a, const Cuts& c, int64_t at, int64_t* s_w, Place* s_p)
 {
     int64_t pieces, rows;
-    pass(a, c, s_w, s_p, pieces, rows, [&](int64_t, int64_t first, int64_t n) { return n > 0 && at >= first && at < first + n; });
+    pass<WAVES>(a, c, s_w, s_p, pieces, rows, [&](int64_t first, int64_t n, int64_t) { return n > 0 && at >= first && at < first + n; });
     Place p = *s_p;
     p.piece = at - p.piece;
     return p;
@@ -358,7 +365,7 @@ __device__ __forceinline__ int64_t xcd_order(int64_t b, int64_t n)
 
 // result[i, j] = sum_c a[i, c] W(j, c) (+ bias[j]), W(j, c) at weight[g][j][c], or (DX) [g][c][j].
 template <typename T, bool DX>
-__global__ __launch_bounds__(256) void rows_kernel(Args a)
+__global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
 {
     __shared__ __attribute__((aligned(16))) char s_a[kSlabBytes], s_b[kSlabBytes];
     __shared__ __attribute__((aligned(16))) char s_out[4 * kOutRows * kOutPitch<T>];
@@ -366,7 +373,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a)
     __shared__ Place s_p;
     const Cuts cuts{kTile, 0};
     int64_t tiles, covered;
-    pass(a, cuts, s_w, &s_p, tiles, covered, [](int64_t, int64_t, int64_t) { return false; });
+    pass<4>(a, cuts, s_w, &s_p, tiles, covered, [](int64_t, int64_t, int64_t) { return false; });
     const int col_tiles = (a.cols + kTile - 1) / kTile;
     const int64_t units = tiles * col_tiles, me = xcd_order(blockIdx.x, gridDim.x);
     int64_t u = units * me / gridDim.x;
@@ -374,24 +381,25 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a)
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, t = threadIdx.x % 128;
     const bool first_half = threadIdx.x < 128;
     if (u < end) {
-        Place p = locate(a, cuts, u / col_tiles, s_w, &s_p);
+        Place p = locate<4>(a, cuts, u / col_tiles, s_w, &s_p);
         int64_t group = scalar64(p.group), piece = scalar64(p.piece), row = scalar64(p.row), size = scalar64(p.size);
         const int slabs = (a.depth + kSlab<T> - 1) / kSlab<T>;
-        Stage<T, false> sa;  // (one of the two is used by a wave)
-        Stage<T, DX> sb;
+        using SA = Stage<T, false>;
+        using SB = Stage<T, DX>;
+        u32x4 r[8];
         auto fetch = [&](int64_t uu, int slab) {
             const int col = (int)(uu % col_tiles) * kTile;
             const int64_t r0 = row + piece * kTile;
             if (first_half)
-                sa.load((const T*)a.a + r0 * a.depth, a.depth,
+                SA::load(r, (const T*)a.a + r0 * a.depth, a.depth,
                         (int)max((int64_t)0, min(min(size - piece * kTile, a.rows - r0), (int64_t)kTile)), slab * kSlab<T>,
                         a.depth, t);
             else {
                 const T* wt = (const T*)a.b + group * a.cols * a.depth;
                 if constexpr (DX)
-                    sb.load(wt + col, a.cols, min(a.cols - col, kTile), slab * kSlab<T>, a.depth, t);
+                    SB::load(r, wt + col, a.cols, min(a.cols - col, kTile), slab * kSlab<T>, a.depth, t);
                 else
-                    sb.load(wt + (int64_t)col * a.depth, a.depth, min(a.cols - col, kTile), slab * kSlab<T>, a.depth, t);
+                    SB::load(r, wt + (int64_t)col * a.depth, a.depth, min(a.cols - col, kTile), slab * kSlab<T>, a.depth, t);
             }
         };
         fetch(u, 0);
@@ -402,8 +410,8 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a)
             f32x16 acc[2][2] = {};
             for (int slab = 0; slab < slabs; ++slab) {
                 __syncthreads();
-                if (first_half) sa.store(s_a, t);
-                else sb.store(s_b, t);
+                if (first_half) SA::store(r, s_a, t);
+                else SB::store(r, s_b, t);
                 __syncthreads();
                 if (slab + 1 < slabs) {
                     fetch(u, slab + 1);
@@ -434,11 +442,182 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a)
     for (int64_t i = from + blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) ((T*)a.out)[i] = (T)0.0f;
 }
 
+// The same for rows whose chunks of 16 bytes are whole, with at most 1 KB of summed indices: eight
+// waves share a panel of W in LDS, PN columns by all summed indices, made once for all of the
+// workgroup's rows of a group, and each streams strips of 32 rows through 8 KB of its own: 256
+// bytes of each row a step, the next step's loads in flight while one is multiplied, and the
+// strip's result back through the same 8 KB to whole rows.  No barrier but at a change of group.
+// Loads and stores go through buffer descriptors of the strip: what lies outside reads as zero and
+// is not written, so every step has the same instructions and the waits between them are counted.
+constexpr int kStreamWaves = 8;
+constexpr int kStripRows = 32;
+constexpr int kStreamRows = kStreamWaves * kStripRows;
+constexpr int kStepBytes = 256;
+constexpr int kOutside = 0x7ffffff0;
+
+using Buffer = __amdgpu_buffer_rsrc_t;
+__device__ __forceinline__ Buffer buffer_of(const void* p, int64_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)min(bytes, (int64_t)kOutside), 0x00020000);
+}
+
+template <typename T, bool DX, int PN>
+__global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool single)
+{
+    __shared__ __attribute__((aligned(16))) char s_panel[65536];
+    __shared__ __attribute__((aligned(16))) char s_x[kStreamWaves][kStripRows * kStepBytes];
+    __shared__ int64_t s_w[3 * kStreamWaves];
+    __shared__ Place s_p;
+    constexpr int C = kChunk<T>, kStep = kStepBytes / (int)sizeof(T), kTiles = PN / 32;
+    const Cuts cuts{kStreamRows, 0};
+    const int panels = (a.cols + PN - 1) / PN;
+    const int64_t me = xcd_order(blockIdx.x, gridDim.x), lane_of_work = me / panels, lanes_of_work = gridDim.x / panels;
+    const int col = (int)(me % panels) * PN;
+    // (with a workgroup for each tile there may be, the place of the tile comes from the same pass)
+    int64_t tiles, covered;
+    pass<kStreamWaves>(a, cuts, s_w, &s_p, tiles, covered, [&](int64_t first, int64_t n, int64_t) {
+        return single && lane_of_work >= first && lane_of_work < first + n;
+    });
+    int64_t u = single ? lane_of_work : tiles * lane_of_work / lanes_of_work;
+    const int64_t end = single ? min(u + 1, tiles) : lane_of_work < lanes_of_work ? tiles * (lane_of_work + 1) / lanes_of_work : u;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = lane & 31, half = lane >> 5, quarter = lane >> 4, chunk = lane & 15;
+    char* my_x = s_x[w];
+    if (u < end) {
+        Place p = s_p;
+        p.piece = u - p.piece;
+        if (!single) p = locate<kStreamWaves>(a, cuts, u, s_w, &s_p);
+        int64_t group = scalar64(p.group), piece = scalar64(p.piece), row = scalar64(p.row), size = scalar64(p.size);
+        const int steps = (a.depth + kStep - 1) / kStep, slabs = (a.depth + kSlab<T> - 1) / kSlab<T>;
+        const int64_t ld = (int64_t)a.depth * sizeof(T), ld_out = (int64_t)a.cols * sizeof(T);
+        auto fill_panel = [&](int64_t g) {
+            const T* wt = (const T*)a.b + g * a.cols * a.depth;
+            __syncthreads();
+            for (int s = threadIdx.x / 128; s < slabs; s += kStreamWaves / 2) {
+                using S = Stage<T, DX, PN>;
+                u32x4 st[S::R];
+                const int t = threadIdx.x % 128;
+                if constexpr (DX) S::load(st, wt + col, a.cols, min(a.cols - col, PN), s * kSlab<T>, a.depth, t);
+                else S::load(st, wt + (int64_t)col * a.depth, a.depth, min(a.cols - col, PN), s * kSlab<T>, a.depth, t);
+                S::store(st, s_panel + s * PN * kRowBytes, t);
+            }
+            __syncthreads();
+        };
+        // a lane loads a chunk of 16 bytes of each eighth row of 256: rows 4 i + quarter
+        u32x4 r[8];
+        auto fetch = [&](int64_t first_row, int n_rows, int step) {
+            const Buffer b = buffer_of((const char*)a.a + first_row * ld, n_rows * ld);
+            const int at = step * kStepBytes + chunk * 16;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                r[i] = __builtin_amdgcn_raw_buffer_load_b128(b, at < ld ? (4 * i + quarter) * (int)ld + at : kOutside, 0, 0);
+        };
+        auto rows_here = [&](int64_t r0) {  // of the wave's strip of this piece
+            return (int)max((int64_t)0, min(min(size - piece * kStreamRows - w * kStripRows, a.rows - r0), (int64_t)kStripRows));
+        };
+        int64_t r0 = row + piece * kStreamRows + w * kStripRows;
+        int n_rows = rows_here(r0);
+        fetch(r0, n_rows, 0);
+        fill_panel(group);
+        while (u < end) {
+            const int64_t my_row = r0, my_group = group;
+            const int my_rows = n_rows;
+            f32x16 acc[kTiles] = {};
+            for (int step = 0; step < steps; ++step) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int rr = 4 * i + quarter;
+                    *(u32x4*)(my_x + rr * kStepBytes + (chunk ^ (rr & 15)) * 16) = r[i];
+                }
+                if (step + 1 < steps) {
+                    fetch(r0, n_rows, step + 1);
+                } else {
+                    ++u;
+                    if (u < end) {
+                        ++piece;
+                        while (piece * kStreamRows >= size) {  // (a later group has rows: u < end)
+                            row += size;
+                            piece = 0;
+                            ++group;
+                            size = scalar64(granted(a, group, row));
+                        }
+                        r0 = row + piece * kStreamRows + w * kStripRows;
+                        n_rows = rows_here(r0);
+                        fetch(r0, n_rows, 0);
+                    }
+                }
+                const char* panel = s_panel + step * 2 * PN * kRowBytes;
+                const int inner = min(2, slabs - 2 * step);  // slabs of 128 bytes in this step
+                for (int b = 0; b < inner; ++b)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+                        const int c = 8 * b + 2 * s + half;
+                        const u32x4 v = *(const u32x4*)(my_x + x * kStepBytes + (c ^ (x & 15)) * 16);
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) {
+                            const int rr = 32 * t + x;
+                            const u32x4 y = *(const u32x4*)(panel + (b * PN + rr) * kRowBytes + swapped(rr, 2 * s + half) * 16);
+                            if constexpr (sizeof(T) == 2) {
+                                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, y),
+                                                                                 __builtin_bit_cast(bf16x8, v), acc[t], 0, 0, 0);
+                            } else {
+                                const f32x4 fy = __builtin_bit_cast(f32x4, y), fv = __builtin_bit_cast(f32x4, v);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(fy[k], fv[k], acc[t], 0, 0, 0);
+                            }
+                        }
+                    }
+            }
+            // the strip's result, 256 bytes (or the panel's) of each row at once
+            constexpr int kWide = PN * (int)sizeof(T) < kStepBytes ? PN : kStep, kPieces = PN / kWide, kChunks = kWide / C;
+            const Buffer out = buffer_of((const char*)a.out + my_row * ld_out, my_rows * ld_out);
+            const T* bias = !DX && a.bias ? (const T*)a.bias + my_group * a.cols + col : nullptr;
+#pragma unroll
+            for (int piece_at = 0; piece_at < kPieces; ++piece_at) {
+#pragma unroll
+                for (int t = 0; t < kWide / 32; ++t)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int at = 32 * t + 8 * q + 4 * half, c = piece_at * kWide + at;
+                        f32x4 v;
+                        for (int k = 0; k < 4; ++k) v[k] = acc[piece_at * (kWide / 32) + t][4 * q + k];
+                        if (bias && col + c < a.cols)
+                            for (int k = 0; k < 4; ++k) v[k] += (float)bias[c + k];  // (whole chunks: four are there)
+                        if constexpr (sizeof(T) == 4) {
+                            *(f32x4*)(my_x + x * (kWide * 4) + ((at / 4) ^ (x & (kChunks - 1))) * 16) = v;
+                        } else {
+                            __attribute__((ext_vector_type(4))) __bf16 y;
+                            for (int k = 0; k < 4; ++k) y[k] = (__bf16)v[k];
+                            *(decltype(y)*)(my_x + x * (kWide * 2) + ((at / 8) ^ (x & (kChunks - 1))) * 16 + at % 8 * 2) = y;
+                        }
+                    }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int k = 0; k < kStripRows * kChunks / 64; ++k) {
+                    const int id = k * 64 + lane, rr = id / kChunks, c = id % kChunks;
+                    const int at = (col + piece_at * kWide) * (int)sizeof(T) + c * 16;
+                    const u32x4 v = *(const u32x4*)(my_x + rr * (kWide * (int)sizeof(T)) + (c ^ (rr & (kChunks - 1))) * 16);
+                    __builtin_amdgcn_raw_buffer_store_b128(v, out, at < ld_out ? rr * (int)ld_out + at : kOutside, 0, 0);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+            if (u < end && group != my_group) fill_panel(group);
+        }
+    }
+    // rows of no group
+    const int64_t from = min(covered, a.rows) * a.cols, all = a.rows * a.cols;
+    for (int64_t i = from + blockIdx.x * (64ll * kStreamWaves) + threadIdx.x; i < all; i += gridDim.x * (64ll * kStreamWaves))
+        ((T*)a.out)[i] = (T)0.0f;
+}
+
 // dW[g][n][k] = sum_i dy[i, n] x[i, k] over an item's rows of a group, 128 x 128 of it; the
 // first column tile's workgroups sum dy itself.  Groups of one item write their result,
 // others partial sums that weight_join_kernel adds up in order.
 template <typename T>
-__global__ __launch_bounds__(256) void weight_kernel(Args a, int64_t max_items)
+__global__ __launch_bounds__(256, 2) void weight_kernel(Args a, int64_t max_items)
 {
     __shared__ __attribute__((aligned(16))) char s_a[kSlabBytes], s_b[kSlabBytes];
     __shared__ __attribute__((aligned(16))) char s_out[4 * kOutRows * kOutPitch<T>];
@@ -450,30 +629,31 @@ __global__ __launch_bounds__(256) void weight_kernel(Args a, int64_t max_items)
     const int64_t at = xcd_order(blockIdx.x, gridDim.x);
     const int64_t item = at / (n_tiles * k_tiles);
     int64_t items, covered;
-    pass(a, cuts, s_w, &s_p, items, covered, [](int64_t, int64_t, int64_t) { return false; });
+    pass<4>(a, cuts, s_w, &s_p, items, covered, [](int64_t, int64_t, int64_t) { return false; });
     if (item >= items || item >= max_items) return;
     const int tile = (int)(at % (n_tiles * k_tiles)), n0 = tile / k_tiles * kTile, k0 = tile % k_tiles * kTile;
-    const Place p = locate(a, cuts, item, s_w, &s_p);
+    const Place p = locate<4>(a, cuts, item, s_w, &s_p);
     const int64_t group = scalar64(p.group), row = scalar64(p.row), size = scalar64(p.size), piece = scalar64(p.piece);
     const int64_t r0 = row + piece * a.chunk;
     const int64_t n_rows = max((int64_t)0, min(min(size - piece * a.chunk, a.chunk), a.rows - r0));
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, t = threadIdx.x % 128;
     const bool first_half = threadIdx.x < 128;
     const bool sums = a.dbias && k0 == 0;
-    Stage<T, true> st;
+    using S = Stage<T, true>;
+    u32x4 st[S::R];
     float col_sum[8 / C][C] = {};
     auto fetch = [&](int64_t r) {
         const int left = (int)min(n_rows - r, (int64_t)kSlab<T>);
         if (first_half)
-            st.load((const T*)a.a + (r0 + r) * a.cols + n0, a.cols, min(a.cols - n0, kTile), 0, left, t);
+            S::load(st, (const T*)a.a + (r0 + r) * a.cols + n0, a.cols, min(a.cols - n0, kTile), 0, left, t);
         else
-            st.load((const T*)a.b + (r0 + r) * a.depth + k0, a.depth, min(a.depth - k0, kTile), 0, left, t);
+            S::load(st, (const T*)a.b + (r0 + r) * a.depth + k0, a.depth, min(a.depth - k0, kTile), 0, left, t);
     };
     f32x16 acc[2][2] = {};
     if (n_rows > 0) fetch(0);
     for (int64_t r = 0; r < n_rows; r += kSlab<T>) {
         __syncthreads();
-        st.store(first_half ? s_a : s_b, t);
+        S::store(st, first_half ? s_a : s_b, t);
         if (sums && first_half) {
 #pragma unroll
             for (int b = 0; b < 8 / C; ++b)
@@ -481,7 +661,7 @@ __global__ __launch_bounds__(256) void weight_kernel(Args a, int64_t max_items)
                 for (int j = 0; j < C; ++j)
 #pragma unroll
                     for (int i = 0; i < C; ++i) {
-                        const uint32_t word = st.r[b * C + i][j * (int)sizeof(T) / 4];
+                        const uint32_t word = st[b * C + i][j * (int)sizeof(T) / 4];
                         col_sum[b][j] += __builtin_bit_cast(float, sizeof(T) == 4 ? word : j % 2 ? word & 0xffff0000u : word << 16);
                     }
         }
@@ -526,50 +706,57 @@ __global__ __launch_bounds__(256) void weight_kernel(Args a, int64_t max_items)
     }
 }
 
-// Adds up the partial sums of groups of more than one item: a workgroup for a tile of a group.
+// Adds up the partial sums of groups of more than one item, in the items' order: a thread for four
+// neighbouring columns, sixteen workgroups for a tile of a split group.
+constexpr int kJoinParts = 16;
 template <typename T>
 __global__ __launch_bounds__(256) void weight_join_kernel(Args a)
 {
-    __shared__ __attribute__((aligned(16))) char s_out[4 * kOutRows * kOutPitch<T>];
     __shared__ int64_t s_w[12];
     __shared__ Place s_p;
     const int n_tiles = (a.cols + kTile - 1) / kTile, k_tiles = (a.depth + kTile - 1) / kTile;
-    const int64_t group = blockIdx.x / (n_tiles * k_tiles);
-    const int tile = (int)(blockIdx.x % (n_tiles * k_tiles)), n0 = tile / k_tiles * kTile, k0 = tile % k_tiles * kTile;
+    const int64_t unit = blockIdx.x / kJoinParts, rank = unit / (n_tiles * k_tiles);
+    const int part_of = (int)(blockIdx.x % kJoinParts);
+    const int tile = (int)(unit % (n_tiles * k_tiles)), n0 = tile / k_tiles * kTile, k0 = tile % k_tiles * kTile;
     const Cuts cuts{a.chunk, 1};
+    if (threadIdx.x == 0) s_p.group = -1;
     int64_t all_pieces, all_rows;
-    pass(a, cuts, s_w, &s_p, all_pieces, all_rows, [&](int64_t g, int64_t, int64_t) { return g == group; });
+    pass<4>(a, cuts, s_w, &s_p, all_pieces, all_rows, [&](int64_t, int64_t n, int64_t split) { return n > 1 && split == rank; });
+    const int64_t group = scalar64(s_p.group);
+    if (group < 0) return;
     const int64_t pieces = scalar64(cuts.of(s_p.size)), slot = scalar64(s_p.many);
-    if (pieces == 1) return;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    f32x16 acc[2][2] = {};
-    for (int64_t i = 0; i < pieces; ++i) {
-        const f32x4* part = (const f32x4*)a.part + (((slot + i) * n_tiles * k_tiles + tile) * 4 + w) * 1024 + lane;
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            const f32x4 v = part[q * 64];
-            for (int c = 0; c < 4; ++c) acc[q / 8][q / 4 % 2][4 * (q % 4) + c] += v[c];
-        }
-    }
-    const int c0 = k0 + (w / 2) * 64, m0 = n0 + (w % 2) * 64;
-    write_out<T>(acc, s_out + w * kOutRows * kOutPitch<T>, lane, (T*)a.out + (group * a.cols + m0) * (int64_t)a.depth + c0,
-                 a.depth, a.cols - m0, a.depth - c0, (const T*)nullptr);
-    const int n = n0 + threadIdx.x;
-    if (a.dbias && k0 == 0 && threadIdx.x < kTile && n < a.cols) {
+    // (the layout of weight_kernel's accumulators: four waves of sixteen times 64 lanes)
+    const int w = part_of / 4, q = part_of % 4 * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
+    const int64_t step = (int64_t)n_tiles * k_tiles * 4096;
+    const f32x4* part = (const f32x4*)a.part + slot * step + ((int64_t)tile * 4 + w) * 1024 + q * 64 + lane;
+    f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int64_t i = 0; i < pieces; ++i) sum += part[i * step];
+    const int i = q / 8, j = q / 4 % 2;
+    const int n = n0 + (w % 2) * 64 + 32 * j + (lane & 31), k = k0 + (w / 2) * 64 + 32 * i + 8 * (q % 4) + 4 * (lane >> 5);
+    if (n < a.cols)
+        for (int c = 0; c < 4; ++c)
+            if (k + c < a.depth) ((T*)a.out)[(group * a.cols + n) * a.depth + k + c] = (T)sum[c];
+    const int col = n0 + threadIdx.x;
+    if (a.dbias && k0 == 0 && part_of == 0 && threadIdx.x < kTile && col < a.cols) {
         float x = 0;
-        for (int64_t i = 0; i < pieces; ++i) x += a.part_bias[(slot + i) * a.cols + n];
-        ((T*)a.dbias)[group * a.cols + n] = (T)x;
+#pragma unroll 4
+        for (int64_t i2 = 0; i2 < pieces; ++i2) x += a.part_bias[(slot + i2) * a.cols + col];
+        ((T*)a.dbias)[group * a.cols + col] = (T)x;
     }
 }
 
 // ---------------------------------------------------------------- host
-// Rows of an item of dW: about four workgroups for every CU over all tiles, and no shorter than
-// 256 (a partial sum costs as much memory traffic as some hundred rows).
+// Rows of an item of dW.  Where the groups' tiles alone give every CU some workgroups, items of four
+// times a group's mean rows: hardly a group is split.  Else as many items as make four workgroups
+// for every CU, and no shorter than 128 rows (a partial sum is as much memory traffic as some
+// hundred rows are).
 int64_t rows_of_item(const dg_grouped_desc* d)
 {
     const int64_t tiles = (int64_t)((d->n + kTile - 1) / kTile) * ((d->k + kTile - 1) / kTile);
-    const int64_t c = (d->n_rows * tiles + 1023) / 1024;
-    return std::max<int64_t>(256, (c + 63) / 64 * 64);
+    const int64_t mean = d->n_rows / d->n_groups + 1, each = 1024 / (d->n_groups * tiles);
+    const int64_t c = each <= 1 ? 4 * mean : mean / each;
+    return std::max<int64_t>(128, (c + 63) / 64 * 64);
 }
 
 struct Layout {
@@ -607,11 +794,37 @@ dg_status launched(const char* what)
     return DG_OK;
 }
 
+// Workgroups of the streaming kernel: one a CU (its LDS), for each panel a share of the row tiles.
+// Narrower panels where wide ones would leave most CUs without work.
+constexpr int kCus = 256;
+int64_t stream_tiles(const Args& a) { return a.rows / kStreamRows + std::min(a.groups, a.rows) + 1; }
+
+template <typename T, bool DX, int PN>
+void run_stream(const Args& a, hipStream_t s)
+{
+    const int64_t panels = (a.cols + PN - 1) / PN, tiles = stream_tiles(a);
+    const int64_t lanes = std::max<int64_t>(1, std::min<int64_t>(tiles, kCus / panels));
+    hipLaunchKernelGGL((stream_kernel<T, DX, PN>), dim3((unsigned)(panels * lanes)), dim3(64 * kStreamWaves), 0, s, a,
+                       lanes == tiles);
+}
+
 template <typename T, bool DX>
 void run_rows(const Args& a, hipStream_t s)
 {
+    // Whole chunks and a panel that fits: the streaming kernel.
+    const int64_t bytes = a.depth * (int64_t)sizeof(T);
+    const bool whole = bytes % 16 == 0 && a.cols % kChunk<T> == 0 && ((uintptr_t)a.a & 15) == 0 &&
+                       ((uintptr_t)a.out & 15) == 0 && a.cols * (int64_t)sizeof(T) <= 1 << 24;
+    if (whole && bytes <= 1024) {
+        const int64_t work = stream_tiles(a) * ((a.cols + 127) / 128);  // workgroups with panels of 128
+        if (work <= kCus / 4) run_stream<T, DX, 32>(a, s);
+        else if (bytes > 512 || work <= kCus / 2) run_stream<T, DX, 64>(a, s);
+        else run_stream<T, DX, 128>(a, s);
+        return;
+    }
+
     const int64_t tiles = (a.rows / kTile + std::min(a.groups, a.rows) + 1) * ((a.cols + kTile - 1) / kTile);
-    unsigned grid = (unsigned)std::min<int64_t>(tiles, 256 * 3);
+    unsigned grid = (unsigned)std::min<int64_t>(tiles, 256 * 2);
     if (grid > kXcds) grid = (grid + kXcds - 1) / kXcds * kXcds;
     hipLaunchKernelGGL((rows_kernel<T, DX>), dim3(grid), dim3(256), 0, s, a);
 }
@@ -624,8 +837,9 @@ void run_weight(const Args& a, hipStream_t s)
     int64_t grid = items * tiles;
     if (grid > kXcds) grid = (grid + kXcds - 1) / kXcds * kXcds;
     hipLaunchKernelGGL(weight_kernel<T>, dim3((unsigned)grid), dim3(256), 0, s, a, items);
-    if (a.rows > a.chunk)
-        hipLaunchKernelGGL(weight_join_kernel<T>, dim3((unsigned)(a.groups * tiles)), dim3(256), 0, s, a);
+    const int64_t split = std::min(a.groups, a.rows / a.chunk);  // groups above an item, at most
+    if (split > 0)
+        hipLaunchKernelGGL(weight_join_kernel<T>, dim3((unsigned)(split * tiles * kJoinParts)), dim3(256), 0, s, a);
 }
 
 }  // namespace
