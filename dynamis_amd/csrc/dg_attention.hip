@@ -619,7 +619,8 @@ void run_forward(const AttnArgs& a, hipStream_t s)
 template <typename T>
 void run_backward(AttnArgs a, const Lists& by_target, const Lists& by_source, float* dtable, hipStream_t s)
 {
-    const bool matrix = sizeof(T) == 2 && a.dim <= kMfmaDim;
+    // (the matrix kernels' rows without entries read some target's row: there has to be one)
+    const bool matrix = sizeof(T) == 2 && a.dim <= kMfmaDim && a.n_targets > 0;
     const size_t cells = (size_t)a.n_buckets * a.heads;
     a.L = by_target;
     unsigned groups = 1;

@@ -14,7 +14,7 @@
 // row's end.  The weighted sum so has 16 bits of the probability at no further instruction.
 //
 // The zeros of the block diagonal would spread a NaN or an infinity of one head of k over the
-// others (0 * inf): products of a step in which a logit is a NaN are formed again head by head.
+// others (0 * inf): a row whose sums end in a NaN is done again with products formed head by head.
 // Where the table holds entries of -inf, v of edges that these take out for all heads of the
 // group is zeroed; a row that meets values that are not finite and hidden from some heads only
 // is done again on the vector units.
@@ -102,11 +102,6 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ bool any_nan(f32x4 s)
-{
-    return __builtin_isunordered(s[0], s[1]) || __builtin_isunordered(s[2], s[3]);
-}
-
 // x and its value in the lane 16 (32) over, in an order of their own.
 template <int APART>
 __device__ __forceinline__ float2 with_lane(float x)
@@ -185,22 +180,32 @@ __device__ __forceinline__ Offset<FAR> row_at(int j, int64_t ld_bytes)
     else return __umul24((uint32_t)j, (uint32_t)ld_bytes);
 }
 
-// Row `p` (its channels of one tensor) as the block-diagonal operand: step s, column n.  Kept in
-// LDS, each lane its own 16 bytes a step.
-template <int NT>
-__device__ __forceinline__ void load_spread(const __bf16* p, const Lane& l, int dim, u32x4* s_x)
+// A row's channels of one tensor as the block-diagonal operand: step s, column n; kept in LDS, each
+// lane its own 16 bytes a step.  Loaded through a descriptor of the row, where what lies off the
+// diagonal is out of range and so reads as zero, without a branch.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* p, int bytes)
 {
-    const int at = anew(8 * l.g - l.base);  // channel of step 0 in the column's head
-    const __bf16* q = p + l.source * dim + at;
-    u32x4 v[2 * NT];
-#pragma unroll
-    for (int s = 0; s < 2 * NT; ++s) {
-        v[s] = u32x4{0, 0, 0, 0};
-        if (l.real && (uint32_t)(at + 32 * s) < (uint32_t)dim) v[s] = *(const u32x4*)(q + 32 * s);
-    }
-#pragma unroll
-    for (int s = 0; s < 2 * NT; ++s) s_x[64 * s] = v[s];
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
 }
+template <int NT>
+struct Spread {
+    u32x4 v[2 * NT];
+    __device__ __forceinline__ void load(const __bf16* row, int heads, const Lane& l, int dim)
+    {
+        const __amdgpu_buffer_rsrc_t b = row_buffer(row, 2 * heads * dim);
+        const int at = 8 * l.g - l.base;  // channel of step 0 in the column's head
+#pragma unroll
+        for (int s = 0; s < 2 * NT; ++s) {
+            const bool in = l.real && (uint32_t)(at + 32 * s) < (uint32_t)dim;
+            v[s] = __builtin_amdgcn_raw_buffer_load_b128(b, in ? 2 * (l.source * dim + at + 32 * s) : 0x7ffffff0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void put(u32x4* s_x) const
+    {
+#pragma unroll
+        for (int s = 0; s < 2 * NT; ++s) s_x[64 * s] = v[s];
+    }
+};
 
 // A lane's channels of an edge in memory: eight (16 bytes) where the group has 128 channels or
 // more, so that four lanes make a whole 64-byte access; the sixteen lanes of a quarter side by
@@ -273,14 +278,14 @@ __device__ __forceinline__ f32x4 products_apart(const char* s_k, const Lane& l, 
 
 // Edges 4 i .. 4 i + 3 of a lane's eight (sixteen of the step) through LDS: their products with
 // the spread row.
-template <int NT>
+template <int NT, bool APART>
 __device__ __forceinline__ f32x4 products(char* s_k, const Lane& l, int dim, const u32x4* spread, const VChunk<NT> (&k)[8],
                                           int i)
 {
 #pragma unroll
     for (int x = 0; x < 4; ++x) put_edge<NT>(s_k, 4 * l.g + x, l, k[4 * i + x]);
-    const f32x4 c = products_at_once<NT>(s_k, l, spread);
-    return __any(any_nan(c)) ? products_apart<NT>(s_k, l, dim, spread) : c;
+    if constexpr (APART) return products_apart<NT>(s_k, l, dim, spread);
+    return products_at_once<NT>(s_k, l, spread);
 }
 
 // The channels of each of a lane's eight edges -> for channel i of them, the eight edges.
@@ -462,27 +467,20 @@ __device__ __forceinline__ uint32_t bucket_of(const Block<FAR>& b)
     return FAR ? b.bucket : b.node >> 24;
 }
 
-// A row's sums of both parts: f(x, ch) for each chunk of eight channels that the lane holds, ch its
-// first channel in its head.  A lane of the first eight columns takes the lower half of its sixteen
-// (or eight times four) channels, its twin the upper.
+// A row's sums of both parts: f(x, ch) for each chunk of eight channels that a lane holds of its
+// column's head, ch its first channel there.  The lanes of the first eight columns add their twins'.
 template <int NT, typename F>
 __device__ __forceinline__ void each_chunk(const Lane& l, int dim, const f32x4 (&acc)[kV<NT>], F&& f)
 {
     constexpr int VW = kV<NT>;
-    const bool low = l.n >= 8;
-    const int first = anew(4 * VW * l.g + (low ? 2 * VW : 0) - l.base);
+    const int first = anew(4 * VW * l.g - l.base);
 #pragma unroll
-    for (int k = 0; k < VW / 4; ++k) {
-        // chunk k of the lower half, and of the upper
+    for (int k = 0; k < VW / 2; ++k) {
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float lo = add_twin(VW == 8 ? acc[i][k] : acc[i % 4][i / 4]);
-            const float hi = add_twin(VW == 8 ? acc[i][2 + k] : acc[i % 4][2 + i / 4]);
-            x[i] = low ? hi : lo;
-        }
+        for (int i = 0; i < 8; ++i) x[i] = add_twin(VW == 8 ? acc[i][k] : acc[i % 4][2 * k + i / 4]);
         const int ch = first + 8 * k;
-        if (l.real && (uint32_t)ch < (uint32_t)dim) f(x, ch);
+        if (l.real && l.n < 8 && (uint32_t)ch < (uint32_t)dim) f(x, ch);
     }
 }
 
@@ -505,7 +503,7 @@ __device__ __forceinline__ void finish_row(const AttnArgs& a, const Piece& p, co
 {
     sum = column_sum(sum);
     const int64_t row = (int64_t)p.node * a.heads + l.head;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(sum);
     each_chunk<NT>(l, a.dim, acc, [&](float (&x)[8], int ch) {
         if (p.item >= 0) {
             store8(a.part_acc + (p.item * a.heads + l.head) * a.dim + ch, x);
@@ -565,7 +563,11 @@ __device__ __forceinline__ void logits(const AttnArgs& a, const Lane& l, const S
     }
 }
 
-constexpr int waves_of(int NT) { return NT == 2 ? 3 : 4; }  // a SIMD
+#ifndef WF2
+#define WF2 3
+#define WF1 4
+#endif
+constexpr int waves_of(int NT) { return NT == 2 ? WF2 : WF1; }  // a SIMD
 
 template <int NT, bool BUCKETS, bool FAR>
 __global__ __launch_bounds__(64 * kWaves, waves_of(NT)) void forward_mfma_kernel(AttnArgs a, HeadGroups hg)
@@ -588,62 +590,86 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(NT)) void forward_mfma_kernel
     // The entries of the next step, and the bounds of the row after the next, are under way while
     // a step is worked on: they come from memory for the first time.  Every step issues the same
     // loads in the same order (the tail's lanes load the last edge again), so that the waits
-    // between them can be counted.
+    // between them can be counted.  A row without entries has a step too, whose sums are dropped.
+    // The next row's q is under way while a row's result is stored.
     Piece p = piece_from(a.L, w, w.at, bounds_at(a.L, w, w.at));
     Piece next = piece_from(a.L, w, w.at + w.step, bounds_at(a.L, w, w.at + w.step));
     Block<FAR> block = block_at<BUCKETS, FAR>(a.L, p.begin, p.end);
+    Spread<NT> q;
+    q.load((const __bf16*)a.q + max(p.node, 0) * a.ldq, a.heads, l, a.dim);
+    q.put(my_q);
     for (int64_t u = w.at; u < w.end; u += w.step) {
         Bounds later;
-        if (p.node >= 0) load_spread<NT>((const __bf16*)a.q + p.node * a.ldq, l, a.dim, my_q);
-        f32x4 acc[kV<NT>] = {};
-        float m = -INFINITY, sum = 0;
-        bool redo = false;
-        for (int e0 = p.begin; e0 < p.end; e0 += 32) {
-            const int n = p.end - e0;
-            const Step<FAR> st = step_of<BUCKETS, FAR>(block, l);
-            VChunk<NT> k[8], v[8];
+        f32x4 acc[kV<NT>];
+        float m, sum;
+        bool redo;
+        auto row = [&](auto apart) {
+            constexpr bool APART = decltype(apart)::value;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) k[x] = load_edge<NT, FAR>(kb, st.edge[x].node, a.ldk, lane_at);
+            for (int i = 0; i < kV<NT>; ++i) acc[i] = f32x4{0, 0, 0, 0};
+            m = -INFINITY;
+            sum = 0;
+            redo = false;
+            int e0 = p.begin;
+            do {
+                const int n = p.end - e0;
+                const Step<FAR> st = step_of<BUCKETS, FAR>(block, l);
+                VChunk<NT> k[8], v[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] = load_edge<NT, FAR>(vb, st.edge[x].node, a.ldv, lane_at);
-            __builtin_amdgcn_sched_barrier(0);  // (all in flight before the first is waited for)
-            block = block_at<BUCKETS, FAR>(a.L, n > 32 ? e0 + 32 : next.begin, n > 32 ? p.end : next.end);
-            later = bounds_at(a.L, w, u + 2 * w.step);
-            __builtin_amdgcn_sched_barrier(0);
-            const f32x4 qk[2] = {products<NT>(my_k, l, a.dim, my_q, k, 0), products<NT>(my_k, l, a.dim, my_q, k, 1)};
-            float s[8];
-            logits<BUCKETS>(a, l, st, qk, n, scale2, takes_out, s_tab, s);
-            const float top = column_max(fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
-                                               fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))));
-            if (__any(top > m + kSlack)) {
-                const float to = fmaxf(m, top);
-                const float shrink = to == -INFINITY ? 1.0f : exp2_fast(m - to);
-                m = to;
-                sum *= shrink;
+                for (int x = 0; x < 8; ++x) k[x] = load_edge<NT, FAR>(kb, st.edge[x].node, a.ldk, lane_at);
 #pragma unroll
-                for (int i = 0; i < kV<NT>; ++i) acc[i] *= shrink;
-            }
-            const float base = m == -INFINITY ? 0.0f : m;
-            float pr[8];
+                for (int x = 0; x < 8; ++x) v[x] = load_edge<NT, FAR>(vb, st.edge[x].node, a.ldv, lane_at);
+                __builtin_amdgcn_sched_barrier(0);  // (all in flight before the first is waited for)
+                block = block_at<BUCKETS, FAR>(a.L, n > 32 ? e0 + 32 : next.begin, n > 32 ? p.end : next.end);
+                later = bounds_at(a.L, w, u + 2 * w.step);
+                __builtin_amdgcn_sched_barrier(0);
+                const f32x4 qk[2] = {products<NT, APART>(my_k, l, a.dim, my_q, k, 0), products<NT, APART>(my_k, l, a.dim, my_q, k, 1)};
+                float s[8];
+                logits<BUCKETS>(a, l, st, qk, n, scale2, takes_out, s_tab, s);
+                const float top = column_max(fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                                                   fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))));
+                if (e0 == p.begin) {
+                    m = top;
+                } else if (__any(top > m + kSlack)) {
+                    const float to = fmaxf(m, top);
+                    const float shrink = to == -INFINITY ? 1.0f : exp2_fast(m - to);
+                    m = to;
+                    sum *= shrink;
 #pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                pr[x] = exp2_fast(s[x] - base);
-                sum += pr[x];
-            }
-            const bf16x8 weight = two_parts(pr, l.n >= 8 ? -1.0f : 0.0f);
-            if (BUCKETS && takes_out) {
-                keep_branch();
-                redo |= hide<NT>(l, s, v);
-            }
+                    for (int i = 0; i < kV<NT>; ++i) acc[i] *= shrink;
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                float pr[8];
 #pragma unroll
-            for (int i = 0; i < kV<NT>; ++i) acc[i] = mfma(turned(v, i), weight, acc[i]);
+                for (int x = 0; x < 8; ++x) {
+                    pr[x] = exp2_fast(s[x] - base);
+                    sum += pr[x];
+                }
+                const bf16x8 weight = two_parts(pr, l.n >= 8 ? -1.0f : 0.0f);
+                if (BUCKETS && takes_out) {
+                    keep_branch();
+                    redo |= hide<NT>(l, s, v);
+                }
+#pragma unroll
+                for (int i = 0; i < kV<NT>; ++i) acc[i] = mfma(turned(v, i), weight, acc[i]);
+                e0 += 32;
+            } while (e0 < p.end);
+        };
+        row(std::false_type{});
+        if (__any(isnan(sum))) {
+            keep_branch();
+            block = block_at<BUCKETS, FAR>(a.L, p.begin, p.end);
+            row(std::true_type{});
         }
-        if (p.begin == p.end) {  // nothing has been sent ahead
-            block = block_at<BUCKETS, FAR>(a.L, next.begin, next.end);
-            later = bounds_at(a.L, w, u + 2 * w.step);
+        q.load((const __bf16*)a.q + max(next.node, 0) * a.ldq, a.heads, l, a.dim);
+        if (p.begin == p.end) {
+            keep_branch();
+#pragma unroll
+            for (int i = 0; i < kV<NT>; ++i) acc[i] = f32x4{0, 0, 0, 0};
         }
-        if (__any(redo)) forward_apart(a, p, (int)blockIdx.y * hg.heads, hg.heads, s_tab);
+        if (__any(redo) && p.node >= 0) forward_apart(a, p, (int)blockIdx.y * hg.heads, hg.heads, s_tab);
         else if (p.node >= 0) finish_row<NT>(a, p, l, acc, m, sum);
+        q.put(my_q);
         p = next;
         next = piece_from(a.L, w, u + 2 * w.step, later);
     }
@@ -659,11 +685,11 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(NT)) void forward_mfma_kernel
 constexpr int waves_of_q(int NT) { return NT == 2 ? WQ2 : WQ1; }
 
 // delta = <g, out> of a column's head: eight channels a lane, whose sums the head's lanes add up.
-__device__ __forceinline__ float delta_of(const AttnArgs& a, const HeadGroups& hg, const Piece& p, const Lane& l, float* s_x)
+__device__ __forceinline__ float delta_of(const AttnArgs& a, const HeadGroups& hg, int node, const Lane& l, float* s_x)
 {
     const int h0 = (int)blockIdx.y * hg.heads, chunks = min(hg.heads, a.heads - h0) * a.dim / 8;
-    const __bf16* g = (const __bf16*)a.g + p.node * a.ldg + h0 * a.dim;
-    const float* o = a.out32 + ((int64_t)p.node * a.heads + h0) * a.dim;
+    const __bf16* g = (const __bf16*)a.g + node * a.ldg + h0 * a.dim;
+    const float* o = a.out32 + ((int64_t)node * a.heads + h0) * a.dim;
     for (int c = anew(threadIdx.x & 63); c < chunks; c += 64) {
         float x[4], y[4];
         load4(g + 8 * c, x);
@@ -765,22 +791,29 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_q(NT)) void backward_q_mfma_k
         Piece p = piece_from(a.L, w, w.at, bounds_at(a.L, w, w.at));
         Piece next = piece_from(a.L, w, w.at + w.step, bounds_at(a.L, w, w.at + w.step));
         Block<FAR> block = block_at<BUCKETS, FAR>(a.L, p.begin, p.end);
+        Spread<NT> q, g;
+        float2 norm;
+        float delta;
+        auto load_row = [&](int node) {
+            q.load((const __bf16*)a.q + node * a.ldq, a.heads, l, a.dim);
+            g.load((const __bf16*)a.g + node * a.ldg, a.heads, l, a.dim);
+        };
+        auto put_row = [&](const Piece& of) {
+            const int64_t row = (int64_t)max(of.node, 0) * a.heads + l.head;
+            norm = a.norm[row];
+            delta = delta_of(a, hg, max(of.node, 0), l, (float*)my_k);
+            if (of.node >= 0 && l.real && l.g == 0 && l.n < 8) a.stats[row] = make_float4(norm.x, norm.y, delta, 0.0f);
+            q.put(my_q);
+            g.put(my_g);
+        };
+        load_row(max(p.node, 0));
+        put_row(p);
         for (int64_t u = w.at; u < w.end; u += w.step) {
             Bounds later;
-            float m = 0, inv = 0, delta = 0;
-            if (p.node >= 0) {
-                load_spread<NT>((const __bf16*)a.q + p.node * a.ldq, l, a.dim, my_q);
-                load_spread<NT>((const __bf16*)a.g + p.node * a.ldg, l, a.dim, my_g);
-                const int64_t row = (int64_t)p.node * a.heads + l.head;
-                const float2 norm = a.norm[row];
-                m = norm.x;
-                inv = norm.y;
-                delta = delta_of(a, hg, p, l, (float*)my_k);
-                if (l.real && l.g == 0 && l.n < 8) a.stats[row] = make_float4(m, inv, delta, 0.0f);
-            }
             f32x4 acc[kV<NT>] = {};
             bool redo = false;
-            for (int e0 = p.begin; e0 < p.end; e0 += 32) {
+            int e0 = p.begin;
+            do {
                 const int n = p.end - e0;
                 const Step<FAR> st = step_of<BUCKETS, FAR>(block, l);
                 VChunk<NT> k[8], v[8];
@@ -792,13 +825,29 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_q(NT)) void backward_q_mfma_k
                 block = block_at<BUCKETS, FAR>(a.L, n > 32 ? e0 + 32 : next.begin, n > 32 ? p.end : next.end);
                 later = bounds_at(a.L, w, u + 2 * w.step);
                 __builtin_amdgcn_sched_barrier(0);
-                const f32x4 qk[2] = {products<NT>(my_k, l, a.dim, my_q, k, 0), products<NT>(my_k, l, a.dim, my_q, k, 1)};
-                const f32x4 gv[2] = {products<NT>(my_k, l, a.dim, my_g, v, 0), products<NT>(my_k, l, a.dim, my_g, v, 1)};
                 float s[8], ds[8];
-                logits<BUCKETS>(a, l, st, qk, n, scale2, takes_out, s_tab, s);
+                auto slopes = [&](auto apart) {
+                    constexpr bool APART = decltype(apart)::value;
+                    const f32x4 qk[2] = {products<NT, APART>(my_k, l, a.dim, my_q, k, 0),
+                                         products<NT, APART>(my_k, l, a.dim, my_q, k, 1)};
+                    const f32x4 gv[2] = {products<NT, APART>(my_k, l, a.dim, my_g, v, 0),
+                                         products<NT, APART>(my_k, l, a.dim, my_g, v, 1)};
+                    logits<BUCKETS>(a, l, st, qk, n, scale2, takes_out, s_tab, s);
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                    ds[x] = s[x] == -INFINITY ? 0.0f : exp2_fast(s[x] - m) * inv * (gv[x / 4][x % 4] - delta);
+                    for (int x = 0; x < 8; ++x)
+                        ds[x] = s[x] == -INFINITY ? 0.0f : exp2_fast(s[x] - norm.x) * norm.y * (gv[x / 4][x % 4] - delta);
+                };
+                slopes(std::false_type{});
+                float all = 0;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) all = fmaf(0.0f, ds[x], all);
+                const bool odd = __any(all != 0.0f);  // (a NaN)
+                if (odd) {
+                    keep_branch();
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) v[x] = load_edge<NT, FAR>(vb, st.edge[x].node, a.ldv, lane_at);
+                    slopes(std::true_type{});
+                }
                 const bf16x8 weight = two_parts(ds, l.n >= 8 ? -1.0f : 0.0f);
                 if (BUCKETS && takes_out) {
                     keep_branch();
@@ -807,10 +856,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_q(NT)) void backward_q_mfma_k
 #pragma unroll
                 for (int i = 0; i < kV<NT>; ++i) acc[i] = mfma(turned(k, i), weight, acc[i]);
                 if constexpr (BUCKETS) {
-                    float all = 0;
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) all += 0.0f * ds[x];
-                    if (__any(all != 0.0f)) {  // (a NaN)
+                    if (odd) {
                         keep_branch();
                         for (int x = 0; x < 8; ++x) {
                             if (0.0f * ds[x] == 0.0f) continue;
@@ -826,12 +872,15 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_q(NT)) void backward_q_mfma_k
                             tab[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(is, ds[x], tab[t], 0, 0, 0);
                         }
                 }
-            }
+                e0 += 32;
+            } while (e0 < p.end);
+            load_row(max(next.node, 0));
             if (p.begin == p.end) {
-                block = block_at<BUCKETS, FAR>(a.L, next.begin, next.end);
-                later = bounds_at(a.L, w, u + 2 * w.step);
+                keep_branch();
+#pragma unroll
+                for (int i = 0; i < kV<NT>; ++i) acc[i] = f32x4{0, 0, 0, 0};
             }
-            if (__any(redo)) {
+            if (__any(redo) && p.node >= 0) {
                 backward_q_apart(a, p, (int)blockIdx.y * hg.heads, hg.heads, s_tab);
             } else if (p.node >= 0) {
                 each_chunk<NT>(l, a.dim, acc, [&](float (&x)[8], int ch) {
@@ -845,6 +894,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_q(NT)) void backward_q_mfma_k
                 });
             }
             p = next;
+            put_row(p);
             next = piece_from(a.L, w, u + 2 * w.step, later);
         }
     }
@@ -950,13 +1000,14 @@ struct __attribute__((aligned(4))) Stats3 {
 // dk and dv: the roles of the two sides are swapped, rows of q and g are gathered against the
 // spread k and v.  A target's (m, 1 / l, delta) come with it, by the lanes of the first eight
 // columns; their twins take over what follows from them.
-template <int NT, bool BUCKETS, bool FAR>
+// (SHARED: several q heads of a head of k, whose sums are added up in LDS.)
+template <int NT, bool BUCKETS, bool FAR, bool SHARED>
 __global__ __launch_bounds__(64 * kWaves, waves_of_kv(NT)) void backward_kv_mfma_kernel(AttnArgs a, KvGroups kg)
 {
     extern __shared__ float s_tab[];
     __shared__ u32x4 s_kk[kWaves][2 * NT * 64], s_vv[kWaves][2 * NT * 64];
     __shared__ __attribute__((aligned(16))) char s_x[kWaves][16 * kRowBytes<NT>];
-    __shared__ float s_sum[kWaves][2][64 * NT];
+    __shared__ float s_sum[SHARED ? kWaves : 1][2][SHARED ? 64 * NT : 1];
     __shared__ int s_any;
     const bool takes_out = stage_table<BUCKETS>(a, s_tab, &s_any);
     const float scale2 = a.scale * kLog2e;
@@ -966,92 +1017,146 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_kv(NT)) void backward_kv_mfma
     u32x4* my_k = s_kk[wave] + lane;
     u32x4* my_v = s_vv[wave] + lane;
     char* my_x = s_x[wave];
-    float* sum_k = s_sum[wave][0];
-    float* sum_v = s_sum[wave][1];
+    float* sum_k = s_sum[SHARED ? wave : 0][0];
+    float* sum_v = s_sum[SHARED ? wave : 0][1];
     const int k0 = (int)blockIdx.y * kg.heads, out_wide = min(kg.heads, a.kv_heads - k0) * a.dim;
+    const int out_head = 2 * lane / a.dim;
+    const Lane l0 = lane_of_kv(a, kg, 0);
+    Spread<NT> k, v;
+    auto load_row = [&](const Piece& of, const Lane& l) {
+        k.load((const __bf16*)a.k + max(of.node, 0) * a.ldk, a.kv_heads, l, a.dim);
+        v.load((const __bf16*)a.v + max(of.node, 0) * a.ldv, a.kv_heads, l, a.dim);
+    };
+    auto put_row = [&] {
+        k.put(my_k);
+        v.put(my_v);
+    };
     Piece p = piece_from(a.L, w, w.at, bounds_at(a.L, w, w.at));
     Piece next = piece_from(a.L, w, w.at + w.step, bounds_at(a.L, w, w.at + w.step));
     Block<FAR> block = block_at<BUCKETS, FAR>(a.L, p.begin, p.end);
+    if (!SHARED) {
+        load_row(p, l0);
+        put_row();
+    }
     for (int64_t u = w.at; u < w.end; u += w.step) {
         Bounds later;
         bool redo = false;
         float rk[2] = {0, 0}, rv[2] = {0, 0};  // channels 2 lane, 2 lane + 1 of the group's heads of k
-        for (int pass = 0; pass < kg.passes; ++pass) {
-            const Lane l = lane_of_kv(a, kg, pass);
+        for (int pass = 0; pass < (SHARED ? kg.passes : 1); ++pass) {
+            const Lane l = SHARED ? lane_of_kv(a, kg, pass) : l0;
             const uint32_t lane_at = lane_bytes<NT>(l);
             const char* qb = (const char*)a.q + 2 * l.kv0 * a.dim;
             const char* gb = (const char*)a.g + 2 * l.kv0 * a.dim;
-            if (p.node >= 0) {
-                load_spread<NT>((const __bf16*)a.k + p.node * a.ldk, l, a.dim, my_k);
-                load_spread<NT>((const __bf16*)a.v + p.node * a.ldv, l, a.dim, my_v);
+            if (SHARED) {
+                load_row(p, l);
+                put_row();
             }
-            f32x4 acc_k[kV<NT>] = {}, acc_v[kV<NT>] = {};
-            for (int e0 = p.begin; e0 < p.end; e0 += 32) {
-                const int n = p.end - e0;
-                const Step<FAR> st = step_of<BUCKETS, FAR>(block, l);
-                VChunk<NT> q[8], g[8];
-                Stats3 row[8];
+            f32x4 acc_k[kV<NT>], acc_v[kV<NT>];
+            float odd;
+            auto row = [&](auto apart) {
+                constexpr bool APART = decltype(apart)::value;
 #pragma unroll
-                for (int x = 0; x < 8; ++x) q[x] = load_edge<NT, FAR>(qb, st.edge[x].node, a.ldq, lane_at);
+                for (int i = 0; i < kV<NT>; ++i) acc_k[i] = acc_v[i] = f32x4{0, 0, 0, 0};
+                odd = 0;
+                int e0 = p.begin;
+                do {
+                    const int n = p.end - e0;
+                    const Step<FAR> st = step_of<BUCKETS, FAR>(block, l);
+                    VChunk<NT> q[8], g[8];
+                    Stats3 of[8];
 #pragma unroll
-                for (int x = 0; x < 8; ++x) g[x] = load_edge<NT, FAR>(gb, st.edge[x].node, a.ldg, lane_at);
-                if (l.n < 8) {
+                    for (int x = 0; x < 8; ++x) q[x] = load_edge<NT, FAR>(qb, st.edge[x].node, a.ldq, lane_at);
 #pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        row[x] = *(const Stats3*)((const char*)a.stats + (row_at<FAR>(st.edge[x].node, 16 * a.heads) + 16 * l.head));
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                const bool again = n <= 32 && pass + 1 < kg.passes;
-                block = block_at<BUCKETS, FAR>(a.L, n > 32 ? e0 + 32 : again ? p.begin : next.begin,
-                                               n > 32 || again ? p.end : next.end);
-                later = bounds_at(a.L, w, u + 2 * w.step);
-                __builtin_amdgcn_sched_barrier(0);
-                const f32x4 qk[2] = {products<NT>(my_x, l, a.dim, my_k, q, 0), products<NT>(my_x, l, a.dim, my_k, q, 1)};
-                const f32x4 gv[2] = {products<NT>(my_x, l, a.dim, my_v, g, 0), products<NT>(my_x, l, a.dim, my_v, g, 1)};
-                float s[8], pr[8], ds[8];
-                logits<BUCKETS>(a, l, st, qk, n, scale2, takes_out, s_tab, s);
+                    for (int x = 0; x < 8; ++x) g[x] = load_edge<NT, FAR>(gb, st.edge[x].node, a.ldg, lane_at);
+                    if (l.n < 8) {
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    pr[x] = s[x] == -INFINITY ? 0.0f : exp2_fast(s[x] - row[x].m) * row[x].inv;
-                    ds[x] = s[x] == -INFINITY ? 0.0f : pr[x] * (gv[x / 4][x % 4] - row[x].delta);
-                    pr[x] = twin_of(pr[x], l.n >= 8);
-                    ds[x] = twin_of(ds[x], l.n >= 8);
-                }
-                if (BUCKETS && takes_out) {
-                    keep_branch();
-                    redo |= hide<NT>(l, s, q);
-                    redo |= hide<NT>(l, s, g);
-                }
-                const bf16x8 weight = two_parts(pr, l.n >= 8 ? -1.0f : 0.0f);
-#pragma unroll
-                for (int i = 0; i < kV<NT>; ++i) acc_v[i] = mfma(turned(g, i), weight, acc_v[i]);
-                const bf16x8 change = two_parts(ds, l.n >= 8 ? -1.0f : 0.0f);
-#pragma unroll
-                for (int i = 0; i < kV<NT>; ++i) acc_k[i] = mfma(turned(q, i), change, acc_k[i]);
-            }
-            // the q heads of each head of k, through LDS
-            each_chunk<NT>(l, a.dim, acc_k, [&](float (&x)[8], int ch) { store8(sum_k + l.base + ch, x); });
-            each_chunk<NT>(l, a.dim, acc_v, [&](float (&x)[8], int ch) { store8(sum_v + l.base + ch, x); });
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if (2 * lane < out_wide) {
-                const int c = 2 * lane / a.dim, at = 2 * lane + c * (kg.shared - 1) * a.dim;
-                for (int i = 0; i < kg.shared; ++i)
-                    for (int j = 0; j < 2; ++j) {
-                        rk[j] += sum_k[at + i * a.dim + j];
-                        rv[j] += sum_v[at + i * a.dim + j];
+                        for (int x = 0; x < 8; ++x)
+                            of[x] = *(const Stats3*)((const char*)a.stats +
+                                                     (row_at<FAR>(st.edge[x].node, 16 * a.heads) + 16 * l.head));
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                    const bool again = SHARED && n <= 32 && pass + 1 < kg.passes;
+                    block = block_at<BUCKETS, FAR>(a.L, n > 32 ? e0 + 32 : again ? p.begin : next.begin,
+                                                   n > 32 || again ? p.end : next.end);
+                    later = bounds_at(a.L, w, u + 2 * w.step);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const f32x4 qk[2] = {products<NT, APART>(my_x, l, a.dim, my_k, q, 0),
+                                         products<NT, APART>(my_x, l, a.dim, my_k, q, 1)};
+                    const f32x4 gv[2] = {products<NT, APART>(my_x, l, a.dim, my_v, g, 0),
+                                         products<NT, APART>(my_x, l, a.dim, my_v, g, 1)};
+                    float s[8], pr[8], ds[8];
+                    logits<BUCKETS>(a, l, st, qk, n, scale2, takes_out, s_tab, s);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        pr[x] = s[x] == -INFINITY ? 0.0f : exp2_fast(s[x] - of[x].m) * of[x].inv;
+                        ds[x] = s[x] == -INFINITY ? 0.0f : pr[x] * (gv[x / 4][x % 4] - of[x].delta);
+                        pr[x] = twin_of(pr[x], l.n >= 8);
+                        ds[x] = twin_of(ds[x], l.n >= 8);
+                        odd = fmaf(0.0f, ds[x], odd);
+                    }
+                    if (BUCKETS && takes_out) {
+                        keep_branch();
+                        redo |= hide<NT>(l, s, q);
+                        redo |= hide<NT>(l, s, g);
+                    }
+                    const bf16x8 weight = two_parts(pr, l.n >= 8 ? -1.0f : 0.0f);
+#pragma unroll
+                    for (int i = 0; i < kV<NT>; ++i) acc_v[i] = mfma(turned(g, i), weight, acc_v[i]);
+                    const bf16x8 change = two_parts(ds, l.n >= 8 ? -1.0f : 0.0f);
+#pragma unroll
+                    for (int i = 0; i < kV<NT>; ++i) acc_k[i] = mfma(turned(q, i), change, acc_k[i]);
+                    e0 += 32;
+                } while (e0 < p.end);
+            };
+            row(std::false_type{});
+            if (__any(odd != 0.0f)) {  // (a NaN)
+                keep_branch();
+                block = block_at<BUCKETS, FAR>(a.L, p.begin, p.end);
+                row(std::true_type{});
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            if (!SHARED) load_row(next, l);
+            if (p.begin == p.end) {
+                keep_branch();
+#pragma unroll
+                for (int i = 0; i < kV<NT>; ++i) acc_k[i] = acc_v[i] = f32x4{0, 0, 0, 0};
+            }
+            if constexpr (SHARED) {
+                each_chunk<NT>(l, a.dim, acc_k, [&](float (&x)[8], int ch) { store8(sum_k + l.base + ch, x); });
+                each_chunk<NT>(l, a.dim, acc_v, [&](float (&x)[8], int ch) { store8(sum_v + l.base + ch, x); });
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                if (2 * lane < out_wide) {
+                    const int at = 2 * lane + out_head * (kg.shared - 1) * a.dim;
+                    for (int i = 0; i < kg.shared; ++i) {
+                        const float2 xk = *(const float2*)(sum_k + at + i * a.dim), xv = *(const float2*)(sum_v + at + i * a.dim);
+                        rk[0] += xk.x;
+                        rk[1] += xk.y;
+                        rv[0] += xv.x;
+                        rv[1] += xv.y;
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            } else if (p.node >= 0 && !__any(redo)) {
+                const int64_t at = ((p.item >= 0 ? p.item : (int64_t)p.node) * a.kv_heads + l.source) * a.dim;
+                each_chunk<NT>(l, a.dim, acc_k, [&](float (&x)[8], int ch) {
+                    if (p.item >= 0) {
+                        store8(a.part_acc + at + ch, x);
+                        return;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] *= a.scale;
+                    store8((__bf16*)a.dk + at + ch, x);
+                });
+                each_chunk<NT>(l, a.dim, acc_v, [&](float (&x)[8], int ch) {
+                    if (p.item >= 0) store8(a.part_acc2 + at + ch, x);
+                    else store8((__bf16*)a.dv + at + ch, x);
+                });
+            }
         }
-        if (p.begin == p.end) {
-            block = block_at<BUCKETS, FAR>(a.L, next.begin, next.end);
-            later = bounds_at(a.L, w, u + 2 * w.step);
-        }
-        if (__any(redo)) {
+        if (__any(redo) && p.node >= 0) {
             backward_kv_apart(a, p, k0, kg.heads, s_tab);
-        } else if (p.node >= 0 && 2 * lane < out_wide) {
+        } else if (SHARED && p.node >= 0 && 2 * lane < out_wide) {
             if (p.item >= 0) {
                 const int64_t at = (p.item * a.kv_heads + k0) * a.dim + 2 * lane;
                 *(float2*)(a.part_acc + at) = make_float2(rk[0], rk[1]);
@@ -1062,6 +1167,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_kv(NT)) void backward_kv_mfma
                 *(bf16x2*)((__bf16*)a.dv + at) = bf16x2{(__bf16)rv[0], (__bf16)rv[1]};
             }
         }
+        if (!SHARED) put_row();
         p = next;
         next = piece_from(a.L, w, u + 2 * w.step, later);
     }
@@ -1143,9 +1249,12 @@ void backward_kv_mfma(const AttnArgs& a, hipStream_t s)
         flag(a.table != nullptr, [&](auto buckets) {
             flag(far, [&](auto is) {
                 constexpr int NT = decltype(nt)::value;
-                hipLaunchKernelGGL((backward_kv_mfma_kernel<NT, decltype(buckets)::value, decltype(is)::value>),
-                                   grid_of(a, kg.groups, waves_of_kv(NT)), dim3(64 * kWaves),
-                                   4 * (size_t)a.n_buckets * a.heads, s, a, kg);
+                flag(a.per > 1, [&](auto shared) {
+                    hipLaunchKernelGGL((backward_kv_mfma_kernel<NT, decltype(buckets)::value, decltype(is)::value,
+                                                                decltype(shared)::value>),
+                                       grid_of(a, kg.groups, waves_of_kv(NT)), dim3(64 * kWaves),
+                                       4 * (size_t)a.n_buckets * a.heads, s, a, kg);
+                });
             });
         });
     });

@@ -326,11 +326,12 @@ def test_plan_of_float64_distances_at_the_boundaries(cuda):
     assert plan.by_target.bucket[:7].tolist() == [0, 1, 0, 2, 3, 3, 0]
 
 
-def test_nothing_to_do(cuda):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_nothing_to_do(cuda, dtype):
     for n, t in ((5, 5), (5, 0), (0, 0)):
-        print(f"\n[case] empty {n} {t}", flush=True)
+        print(f"\n[case] empty {n} {t} {dtype}", flush=True)
         plan = ds.neighbor_plan(torch.empty(2, 0, dtype=torch.long, device="cuda"), n, t)
-        q, k, v = (torch.randn(m, 4, 16, device="cuda", requires_grad=True) for m in (t, n, n))
+        q, k, v = (torch.randn(m, 4, 16, device="cuda", dtype=dtype, requires_grad=True) for m in (t, n, n))
         out, lse = ds.neighbor_attention(q, k, v, plan, return_lse=True)
         assert out.shape == q.shape and not out.any() and (lse == -torch.inf).all()
         for g in torch.autograd.grad(out, (q, k, v), torch.ones_like(out)):
