@@ -100,8 +100,8 @@ class NeighborLists(ctypes.Structure):
         ("bucket", ctypes.c_void_p),
         ("items", ctypes.c_void_p),
         ("item_first", ctypes.c_void_p),
-        ("chunk", ctypes.c_int32),
-        ("pad_", ctypes.c_int32),
+        ("long_slot", ctypes.c_void_p),
+        ("n_long", ctypes.c_int64),
     ]
 
 
@@ -200,7 +200,7 @@ def lib():
         "dg_neighbors_sort_workspace_size": (_sz, [_i64]),
         "dg_neighbors_by_source": (_i32, [ND, _i64, _p, _p, _p, _p, _p, _p, _sz, _p, _sz, _p]),
         "dg_neighbors_parts_workspace_size": (_sz, [_i64]),
-        "dg_neighbors_parts": (_i32, [_p, _p, _i64, _i32, _i64, _p, _p, _p, _sz, _p]),
+        "dg_neighbors_parts": (_i32, [_p, _p, _i64, _i32, _i64, _i64, _p, _p, _p, _p, _sz, _p]),
         "dg_attention_workspace_size": (_sz, [AD, NL, NL]),
         "dg_attention_forward": (_i32, [AD, NL] + [_p] * 9 + [_sz, _p]),
         "dg_attention_backward": (_i32, [AD, NL, NL] + [_p] * 12 + [_sz, _p]),

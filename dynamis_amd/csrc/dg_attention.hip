@@ -170,45 +170,57 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(AttnArgs a)
     }
 }
 
-// A workgroup joins the parts of one long row for 64 channels: sixteen lanes of four channels
-// times sixteen strands over the parts.  (Units whose item is not a row's first do nothing.)
-template <typename T>
-__global__ __launch_bounds__(256) void forward_join_kernel(AttnArgs a, int slices)
+// A workgroup joins the parts of one long row for 64 channels: sixteen lanes of four channels times
+// 64 strands over the parts (four to a wave), first for the maximum, then for the sums against it,
+// so that a strand's loads do not wait for each other.
+constexpr int kStrands = 64, kJoinWaves = kStrands / 4;
+
+__device__ __forceinline__ float strand_sum(float x)
 {
-    const int64_t item = blockIdx.x / slices;
-    const int slice = (int)(blockIdx.x % slices);
-    const int slot = a.L.items[item].w, node = a.L.items[item].z;
-    const int first = a.L.item_first[slot], n = a.L.item_first[slot + 1] - first;
-    if (node < 0 || item != first) return;
-    __shared__ float s_acc[16][16][4], s_m[16][16], s_l[16][16];
-    const int x = threadIdx.x % 16, y = threadIdx.x / 16;
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
+}
+
+template <typename T>
+__global__ __launch_bounds__(16 * kStrands) void forward_join_kernel(AttnArgs a, int slices)
+{
+    const int slot = a.L.long_slot[blockIdx.x / slices], slice = (int)(blockIdx.x % slices);
+    const int first = a.L.item_first[slot], n = a.L.item_first[slot + 1] - first, node = a.L.order[slot];
+    __shared__ float s_m[kJoinWaves][16], s_l[kJoinWaves][16], s_acc[kJoinWaves][4][16];
+    const int x = threadIdx.x % 16, y = threadIdx.x / 16, wave = threadIdx.x / 64;
     const int wide = a.heads * a.dim, ch = slice * 64 + x * 4;
     const int h = min(ch, wide - 4) / a.dim;
-    float mx = -INFINITY, l = 0, acc[4] = {0, 0, 0, 0};
+    float mx = -INFINITY;
+#pragma unroll 4
+    for (int i = y; i < n; i += kStrands) mx = fmaxf(mx, a.part_m[(int64_t)(first + i) * a.heads + h]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    s_m[wave][x] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kJoinWaves; ++i) mx = fmaxf(mx, s_m[i][x]);
+    const float base = mx == -INFINITY ? 0.0f : mx;
+    float l = 0, acc[4] = {0, 0, 0, 0};
     if (ch < wide)
-        for (int i = y; i < n; i += 16) {
+#pragma unroll 4
+        for (int i = y; i < n; i += kStrands) {
             const int64_t it = first + i;
-            const float m2 = a.part_m[it * a.heads + h], l2 = a.part_l[it * a.heads + h];
+            const float f = exp2_fast(a.part_m[it * a.heads + h] - base);
             float b[4];
             load4(a.part_acc + it * wide + ch, b);
-            const float top = fmaxf(mx, m2), base = top == -INFINITY ? 0.0f : top;
-            const float f1 = exp2_fast(mx - base), f2 = exp2_fast(m2 - base);
-            l = l * f1 + l2 * f2;
-            for (int c = 0; c < 4; ++c) acc[c] = acc[c] * f1 + b[c] * f2;
-            mx = top;
+            l = fmaf(a.part_l[it * a.heads + h], f, l);
+            for (int c = 0; c < 4; ++c) acc[c] = fmaf(b[c], f, acc[c]);
         }
-    s_m[y][x] = mx;
-    s_l[y][x] = l;
-    for (int c = 0; c < 4; ++c) s_acc[y][x][c] = acc[c];
+    s_l[wave][x] = strand_sum(l);
+    for (int c = 0; c < 4; ++c) s_acc[wave][c][x] = strand_sum(acc[c]);
     __syncthreads();
     if (y != 0 || ch >= wide) return;
-    for (int i = 1; i < 16; ++i) {
-        const float m2 = s_m[i][x];
-        const float top = fmaxf(mx, m2), base = top == -INFINITY ? 0.0f : top;
-        const float f1 = exp2_fast(mx - base), f2 = exp2_fast(m2 - base);
-        l = l * f1 + s_l[i][x] * f2;
-        for (int c = 0; c < 4; ++c) acc[c] = acc[c] * f1 + s_acc[i][x][c] * f2;
-        mx = top;
+    l = 0;
+    for (int c = 0; c < 4; ++c) acc[c] = 0;
+#pragma unroll
+    for (int i = 0; i < kJoinWaves; ++i) {
+        l += s_l[i][x];
+        for (int c = 0; c < 4; ++c) acc[c] += s_acc[i][c][x];
     }
     for (int c = 0; c < 4; ++c) acc[c] = l == 0.0f ? 0.0f : acc[c] / l;
     const int64_t at = (int64_t)node * wide + ch;
@@ -412,29 +424,29 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kv_kernel(AttnArgs a)
 
 // The sum of the parts of one long row, as forward_join_kernel lays it out.
 template <typename T>
-__global__ __launch_bounds__(256) void sum_join_kernel(Lists L, const float* __restrict__ part, int wide, int slices,
-                                                       float factor, T* __restrict__ out)
+__global__ __launch_bounds__(16 * kStrands) void sum_join_kernel(Lists L, const float* __restrict__ part, int wide,
+                                                                 int slices, float factor, T* __restrict__ out)
 {
-    const int64_t item = blockIdx.x / slices;
-    const int slice = (int)(blockIdx.x % slices);
-    const int slot = L.items[item].w, node = L.items[item].z;
-    const int first = L.item_first[slot], n = L.item_first[slot + 1] - first;
-    if (node < 0 || item != first) return;
-    __shared__ float s_acc[16][16][4];
-    const int x = threadIdx.x % 16, y = threadIdx.x / 16;
+    const int slot = L.long_slot[blockIdx.x / slices], slice = (int)(blockIdx.x % slices);
+    const int first = L.item_first[slot], n = L.item_first[slot + 1] - first, node = L.order[slot];
+    __shared__ float s_acc[kJoinWaves][4][16];
+    const int x = threadIdx.x % 16, y = threadIdx.x / 16, wave = threadIdx.x / 64;
     const int ch = slice * 64 + x * 4;
     float acc[4] = {0, 0, 0, 0};
     if (ch < wide)
-        for (int i = y; i < n; i += 16) {
+#pragma unroll 4
+        for (int i = y; i < n; i += kStrands) {
             float b[4];
             load4(part + (int64_t)(first + i) * wide + ch, b);
             for (int c = 0; c < 4; ++c) acc[c] += b[c];
         }
-    for (int c = 0; c < 4; ++c) s_acc[y][x][c] = acc[c];
+    for (int c = 0; c < 4; ++c) s_acc[wave][c][x] = strand_sum(acc[c]);
     __syncthreads();
     if (y != 0 || ch >= wide) return;
-    for (int i = 1; i < 16; ++i)
-        for (int c = 0; c < 4; ++c) acc[c] += s_acc[i][x][c];
+    for (int c = 0; c < 4; ++c) acc[c] = 0;
+#pragma unroll
+    for (int i = 0; i < kJoinWaves; ++i)
+        for (int c = 0; c < 4; ++c) acc[c] += s_acc[i][c][x];
     for (int c = 0; c < 4; ++c) acc[c] *= factor;
     store4(out + (int64_t)node * wide + ch, acc);
 }
@@ -524,7 +536,7 @@ dg_status check_lists(const dg_attention_desc* d, const dg_neighbor_lists* l)
     if (l->n_rows != d->n_nodes) return fail(DG_ERR_INVALID, "the lists are of another number of nodes");
     if (l->n_rows > 0 && (!l->order || !l->ptr || !l->idx)) return fail(DG_ERR_INVALID, "lists are NULL");
     if (d->n_buckets > 0 && !l->bucket) return fail(DG_ERR_INVALID, "a table, but the lists hold no buckets");
-    if (l->n_items < 0 || (l->n_items > 0 && (!l->items || !l->item_first)))
+    if (l->n_items < 0 || (l->n_items > 0 && (!l->items || !l->item_first || !l->long_slot || l->n_long < 1)))
         return fail(DG_ERR_INVALID, "the parts of long rows are NULL");
     return DG_OK;
 }
@@ -540,6 +552,8 @@ Lists lists_of(const dg_neighbor_lists* l, int64_t rows)
     r.bucket = l->bucket;
     r.items = (const int4*)l->items;
     r.item_first = l->item_first;
+    r.long_slot = l->long_slot;
+    r.n_long = l->n_long;
     return r;
 }
 
@@ -612,7 +626,8 @@ void run_forward(const AttnArgs& a, hipStream_t s)
     }
     if (a.L.n_items > 0) {
         const int slices = (a.heads * a.dim + 63) / 64;
-        hipLaunchKernelGGL(forward_join_kernel<T>, dim3((unsigned)(a.L.n_items * slices)), dim3(256), 0, s, a, slices);
+        hipLaunchKernelGGL(forward_join_kernel<T>, dim3((unsigned)(a.L.n_long * slices)), dim3(16 * kStrands), 0, s, a,
+                           slices);
     }
 }
 
@@ -642,7 +657,7 @@ void run_backward(AttnArgs a, const Lists& by_target, const Lists& by_source, fl
                            (int)groups, (int)cells, dtable);
     if (a.L.n_items > 0) {
         const int wide = a.heads * a.dim, slices = (wide + 63) / 64;
-        hipLaunchKernelGGL(sum_join_kernel<T>, dim3((unsigned)(a.L.n_items * slices)), dim3(256), 0, s, a.L,
+        hipLaunchKernelGGL(sum_join_kernel<T>, dim3((unsigned)(a.L.n_long * slices)), dim3(16 * kStrands), 0, s, a.L,
                            (const float*)a.part_acc, wide, slices, a.scale, (T*)a.dq);
     }
     a.L = by_source;
@@ -657,10 +672,10 @@ void run_backward(AttnArgs a, const Lists& by_target, const Lists& by_source, fl
     }
     if (a.L.n_items > 0) {
         const int wide = a.kv_heads * a.dim, slices = (wide + 63) / 64;
-        const unsigned grid = (unsigned)(a.L.n_items * slices);
-        hipLaunchKernelGGL(sum_join_kernel<T>, dim3(grid), dim3(256), 0, s, a.L, (const float*)a.part_acc, wide, slices,
+        const unsigned grid = (unsigned)(a.L.n_long * slices);
+        hipLaunchKernelGGL(sum_join_kernel<T>, dim3(grid), dim3(16 * kStrands), 0, s, a.L, (const float*)a.part_acc, wide, slices,
                            a.scale, (T*)a.dk);
-        hipLaunchKernelGGL(sum_join_kernel<T>, dim3(grid), dim3(256), 0, s, a.L, (const float*)a.part_acc2, wide, slices,
+        hipLaunchKernelGGL(sum_join_kernel<T>, dim3(grid), dim3(16 * kStrands), 0, s, a.L, (const float*)a.part_acc2, wide, slices,
                            1.0f, (T*)a.dv);
     }
 }

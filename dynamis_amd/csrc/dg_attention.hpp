@@ -42,6 +42,8 @@ struct Lists {
     const uint8_t* bucket;
     const int4* items;
     const int32_t* item_first;
+    const int32_t* long_slot;
+    int64_t n_long;
 };
 
 struct AttnArgs {

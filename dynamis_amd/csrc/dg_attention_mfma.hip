@@ -563,11 +563,7 @@ __device__ __forceinline__ void logits(const AttnArgs& a, const Lane& l, const S
     }
 }
 
-#ifndef WF2
-#define WF2 3
-#define WF1 4
-#endif
-constexpr int waves_of(int NT) { return NT == 2 ? WF2 : WF1; }  // a SIMD
+constexpr int waves_of(int NT) { return NT == 2 ? 3 : 4; }  // a SIMD
 
 template <int NT, bool BUCKETS, bool FAR>
 __global__ __launch_bounds__(64 * kWaves, waves_of(NT)) void forward_mfma_kernel(AttnArgs a, HeadGroups hg)
@@ -676,13 +672,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(NT)) void forward_mfma_kernel
 }
 
 // ---------------------------------------------------------------- backward, by target
-#ifndef WQ2
-#define WQ2 2
-#define WQ1 3
-#define WK2 2
-#define WK1 3
-#endif
-constexpr int waves_of_q(int NT) { return NT == 2 ? WQ2 : WQ1; }
+constexpr int waves_of_q(int NT) { return NT == 2 ? 2 : 3; }
 
 // delta = <g, out> of a column's head: eight channels a lane, whose sums the head's lanes add up.
 __device__ __forceinline__ float delta_of(const AttnArgs& a, const HeadGroups& hg, int node, const Lane& l, float* s_x)
@@ -920,7 +910,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_q(NT)) void backward_q_mfma_k
 }
 
 // ---------------------------------------------------------------- backward, by source
-constexpr int waves_of_kv(int NT) { return NT == 2 ? WK2 : WK1; }
+constexpr int waves_of_kv(int NT) { return NT == 2 ? 2 : 3; }
 
 __device__ __forceinline__ Lane lane_of_kv(const AttnArgs& a, const KvGroups& kg, int pass)
 {

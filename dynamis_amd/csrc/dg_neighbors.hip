@@ -319,12 +319,20 @@ __global__ void bounds_kernel(const int32_t* __restrict__ sorted, int64_t n, int
 }
 
 // ---------------------------------------------------------------- long rows in parts
-__global__ void parts_kernel(const int32_t* __restrict__ ptr, int64_t n, int split, int chunk, int* __restrict__ parts)
+__global__ void parts_kernel(const int32_t* __restrict__ ptr, int64_t n, int split, int chunk, int* __restrict__ parts,
+                             int* __restrict__ is_long)
 {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
     const int len = ptr[i + 1] - ptr[i];
     parts[i] = len > split ? (len + chunk - 1) / chunk : 0;
+    is_long[i] = len > split;
+}
+
+__global__ void long_kernel(const int* __restrict__ rank, int64_t n, int64_t n_long, int32_t* __restrict__ long_slot)
+{
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n && rank[i + 1] > rank[i] && rank[i] < n_long) long_slot[rank[i]] = (int32_t)i;
 }
 
 __global__ void items_kernel(const int32_t* __restrict__ first, const int32_t* __restrict__ ptr,
@@ -542,23 +550,28 @@ size_t dg_neighbors_parts_workspace_size(int64_t n_rows)
         fail(DG_ERR_INVALID, "n_rows must be in [0, 2^31 - 256]");
         return 0;
     }
-    return al(4 * (size_t)(n_rows + 1)) + al(4 * (size_t)(n_rows / kScanTile + 2));
+    return 3 * al(4 * (size_t)(n_rows + 1)) + al(4 * (size_t)(n_rows / kScanTile + 2));
 }
 
 dg_status dg_neighbors_parts(const int32_t* order, const int32_t* ptr, int64_t n_rows, int32_t chunk,
-                             int64_t max_items, int32_t* item_first, int32_t* items, void* ws, size_t ws_bytes,
-                             hipStream_t s)
+                             int64_t max_items, int64_t n_long, int32_t* item_first, int32_t* items,
+                             int32_t* long_slot, void* ws, size_t ws_bytes, hipStream_t s)
 {
-    if (n_rows < 1 || n_rows > kMaxEdges || chunk < 1 || max_items < 1)
-        return fail(DG_ERR_INVALID, "n_rows, chunk and max_items must be positive");
-    if (!order || !ptr || !item_first || !items) return fail(DG_ERR_INVALID, "inputs or outputs are NULL");
+    if (n_rows < 1 || n_rows > kMaxEdges || chunk < 1 || max_items < 1 || n_long < 1)
+        return fail(DG_ERR_INVALID, "n_rows, chunk, max_items and n_long must be positive");
+    if (!order || !ptr || !item_first || !items || !long_slot) return fail(DG_ERR_INVALID, "inputs or outputs are NULL");
     if (!ws || ws_bytes < dg_neighbors_parts_workspace_size(n_rows))
         return fail(DG_ERR_WORKSPACE, "workspace too small");
     int* parts = (int*)ws;
-    int* part = (int*)((char*)ws + al(4 * (size_t)(n_rows + 1)));
+    const size_t each = al(4 * (size_t)(n_rows + 1));
+    int* is_long = (int*)((char*)ws + each);
+    int* rank = (int*)((char*)ws + 2 * each);
+    int* part = (int*)((char*)ws + 3 * each);
     hipLaunchKernelGGL(parts_kernel, dim3(nblk(n_rows)), dim3(256), 0, s, ptr, n_rows, DG_NEIGHBOR_SPLIT, (int)chunk,
-                       parts);
+                       parts, is_long);
     excl_scan<int, int>(parts, n_rows, item_first, part, s);
+    excl_scan<int, int>(is_long, n_rows, rank, part, s);
+    hipLaunchKernelGGL(long_kernel, dim3(nblk(n_rows)), dim3(256), 0, s, (const int*)rank, n_rows, n_long, long_slot);
     hipLaunchKernelGGL(items_kernel, dim3(nblk(std::max(n_rows, max_items))), dim3(256), 0, s, (const int32_t*)item_first,
                        ptr, order, n_rows, (int)chunk, max_items, (int4*)items);
     return launched("dg_neighbors_parts");

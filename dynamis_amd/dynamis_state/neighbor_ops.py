@@ -30,7 +30,7 @@ class _Rows:
 
     def __init__(self, order, ptr, idx, bucket):
         self.order, self.ptr, self.idx, self.bucket = order, ptr, idx, bucket
-        self.items = self.item_first = None
+        self.items = self.item_first = self.long_slot = None
         c = self.c = L.NeighborLists()
         c.n_rows = order.numel()
         c.order, c.ptr, c.idx = order.data_ptr(), ptr.data_ptr(), idx.data_ptr()
@@ -38,23 +38,27 @@ class _Rows:
         self.byref = ctypes.byref(c)
 
     def split(self, long_rows, long_entries, stream):
-        """Rows above DG_NEIGHBOR_SPLIT entries in parts: as many entries as give every SIMD of
-        the card a few parts, at least 128 (a part's result costs as much as some entries)."""
+        """Rows above DG_NEIGHBOR_SPLIT entries in parts: as many as the card holds waves for two
+        groups of heads (4 rows of 100,000: 62 us with 768 parts to 4096, the join of them 7 us and
+        more the more there are), at least 128 entries (a part's result costs as much as some)."""
         if not long_rows:
             return
         lib, dev, c = L.lib(), self.ptr.device, self.c
-        c.chunk = min(2048, max(128, -(-long_entries // 4096 + 31) // 32 * 32))
-        c.n_items = long_entries // c.chunk + long_rows
-        self.items = torch.empty((c.n_items, 4), dtype=torch.int32, device=dev)
-        self.item_first = torch.empty(c.n_rows + 1, dtype=torch.int32, device=dev)
+        chunk = min(2048, max(128, (-(-long_entries // 1536) + 31) // 32 * 32))
+        c.n_items, c.n_long = long_entries // chunk + long_rows, long_rows
+        new = lambda *n: torch.empty(n, dtype=torch.int32, device=dev)  # noqa: E731
+        self.items, self.item_first, self.long_slot = new(c.n_items, 4), new(c.n_rows + 1), new(long_rows)
         c.items, c.item_first = self.items.data_ptr(), self.item_first.data_ptr()
+        c.long_slot = self.long_slot.data_ptr()
         wsb = lib.dg_neighbors_parts_workspace_size(c.n_rows)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-        L.check(lib.dg_neighbors_parts(L.ptr(self.order), L.ptr(self.ptr), c.n_rows, c.chunk, c.n_items,
-                                       L.ptr(self.item_first), L.ptr(self.items), L.ptr(ws), wsb, stream), "neighbor_plan")
+        L.check(lib.dg_neighbors_parts(L.ptr(self.order), L.ptr(self.ptr), c.n_rows, chunk, c.n_items, long_rows,
+                                       L.ptr(self.item_first), L.ptr(self.items), L.ptr(self.long_slot), L.ptr(ws), wsb,
+                                       stream), "neighbor_plan")
 
     def tensors(self):
-        return [t for t in (self.order, self.ptr, self.idx, self.bucket, self.items, self.item_first)
+        return [t for t in (self.order, self.ptr, self.idx, self.bucket, self.items, self.item_first,
+                            self.long_slot)
                 if t is not None]
 
 

@@ -391,7 +391,7 @@ typedef struct dg_neighbor_totals {
 } dg_neighbor_totals;
 
 /* One direction's lists, as the attention reads them.  Rows above DG_NEIGHBOR_SPLIT entries
- * are worked on in items of `chunk` entries (dg_neighbors_parts); n_items == 0: by one wave. */
+ * are worked on in items (dg_neighbors_parts); n_items == 0: by one wave. */
 typedef struct dg_neighbor_lists {
     int64_t n_rows;  /* n_nodes */
     int64_t n_items; /* length of items (an upper bound of their number) */
@@ -401,8 +401,8 @@ typedef struct dg_neighbor_lists {
     const uint8_t* bucket;     /* or NULL */
     const int32_t* items;      /* [n_items, 4]: first entry, end, node (-1: none), slot */
     const int32_t* item_first; /* [n_rows + 1] */
-    int32_t chunk;
-    int32_t pad_;
+    const int32_t* long_slot;  /* [n_long] slots of the rows in items */
+    int64_t n_long;
 } dg_neighbor_lists;
 
 size_t dg_neighbors_workspace_size(const dg_neighbor_desc* desc);
@@ -419,12 +419,14 @@ dg_status dg_neighbors_by_source(const dg_neighbor_desc* desc, int64_t n_entries
                                  uint8_t* source_bucket, void* workspace, size_t workspace_bytes,
                                  void* sort_workspace, size_t sort_workspace_bytes,
                                  hipStream_t stream);
-/* The items of rows above DG_NEIGHBOR_SPLIT entries: item_first int32 [n_rows + 1], items int32
- * [max_items, 4], aligned to 16 bytes, with max_items >= long_entries / chunk + long_rows. */
+/* The items of `chunk` entries of the n_long rows above DG_NEIGHBOR_SPLIT entries: item_first int32
+ * [n_rows + 1], items int32 [max_items, 4], aligned to 16 bytes, with max_items >= long_entries /
+ * chunk + n_long, long_slot int32 [n_long]. */
 size_t dg_neighbors_parts_workspace_size(int64_t n_rows);
 dg_status dg_neighbors_parts(const int32_t* order, const int32_t* ptr, int64_t n_rows, int32_t chunk,
-                             int64_t max_items, int32_t* item_first, int32_t* items, void* workspace,
-                             size_t workspace_bytes, hipStream_t stream);
+                             int64_t max_items, int64_t n_long, int32_t* item_first, int32_t* items,
+                             int32_t* long_slot, void* workspace, size_t workspace_bytes,
+                             hipStream_t stream);
 
 /* Attention over the lists:
  *   logit[e,h] = scale <q[t,h], k[j, h / (heads / kv_heads)]> + table[bucket(e), h]
