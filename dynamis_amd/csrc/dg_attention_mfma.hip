@@ -385,6 +385,18 @@ __device__ __forceinline__ bf16x8 two_parts(const float (&p)[8], float minus)
     return r;
 }
 
+// What two_parts leave out (2^-18 of a weight at most), in columns 0 .. 7.
+__device__ __forceinline__ bf16x8 third_part(const float (&p)[8], bool first)
+{
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float rest = p[i] - (float)(__bf16)p[i];
+        r[i] = (__bf16)(first ? rest - (float)(__bf16)rest : 0.0f);
+    }
+    return r;
+}
+
 // 32 entries of a row, one a lane: the node, with the bucket in the upper eight bits where nodes
 // take 24 (!FAR).  A lane past the row's end holds the row's last entry.  The lanes of a step
 // then fetch the entries that they need from each other: one access a list where loads by those
@@ -648,6 +660,12 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(NT)) void forward_mfma_kernel
                 }
 #pragma unroll
                 for (int i = 0; i < kV<NT>; ++i) acc[i] = mfma(turned(v, i), weight, acc[i]);
+                if (a.out32) {  // (the gradients take their sums <g, out> from it: all of a float's bits)
+                    keep_branch();
+                    const bf16x8 last = third_part(pr, l.n < 8);
+#pragma unroll
+                    for (int i = 0; i < kV<NT>; ++i) acc[i] = mfma(turned(v, i), last, acc[i]);
+                }
                 e0 += 32;
             } while (e0 < p.end);
         };
