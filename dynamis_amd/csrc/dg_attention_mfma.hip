@@ -11,7 +11,8 @@
 //
 // Columns 8 .. 15 repeat the heads: the first eight carry the probability rounded to bfloat16,
 // the others what the rounding left, also in bfloat16, and the two results are added at the
-// row's end.  The weighted sum so has 16 bits of the probability at no further instruction.
+// row's end.  The weighted sum so has 16 bits of the probability at no further product; the
+// forward pass adds a third part.
 //
 // The zeros of the block diagonal would spread a NaN or an infinity of one head of k over the
 // others (0 * inf): a row whose sums end in a NaN is done again with products formed head by head.
@@ -385,7 +386,10 @@ __device__ __forceinline__ bf16x8 two_parts(const float (&p)[8], float minus)
     return r;
 }
 
-// What two_parts leave out (2^-18 of a weight at most), in columns 0 .. 7.
+// What two_parts leave out, in columns 0 .. 7.  (That is 2^-18 of a weight at most; but the backward
+// pass takes <g, out> from the sums, which is summed over a bucket's edges where it cancels: with two
+// parts the table's gradient was 1.0e-6 off the 64-bit one, with three it is 2e-7.  27M edges of 8
+// heads of 16: 851 us with two, 887 us with three, 904 us with `v` turned anew for the third.)
 __device__ __forceinline__ bf16x8 third_part(const float (&p)[8], bool first)
 {
     bf16x8 r;
@@ -653,18 +657,15 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(NT)) void forward_mfma_kernel
                     pr[x] = exp2_fast(s[x] - base);
                     sum += pr[x];
                 }
-                const bf16x8 weight = two_parts(pr, l.n >= 8 ? -1.0f : 0.0f);
+                const bf16x8 weight = two_parts(pr, l.n >= 8 ? -1.0f : 0.0f), last = third_part(pr, l.n < 8);
                 if (BUCKETS && takes_out) {
                     keep_branch();
                     redo |= hide<NT>(l, s, v);
                 }
 #pragma unroll
-                for (int i = 0; i < kV<NT>; ++i) acc[i] = mfma(turned(v, i), weight, acc[i]);
-                if (a.out32) {  // (the gradients take their sums <g, out> from it: all of a float's bits)
-                    keep_branch();
-                    const bf16x8 last = third_part(pr, l.n < 8);
-#pragma unroll
-                    for (int i = 0; i < kV<NT>; ++i) acc[i] = mfma(turned(v, i), last, acc[i]);
+                for (int i = 0; i < kV<NT>; ++i) {
+                    const bf16x8 vi = turned(v, i);
+                    acc[i] = mfma(vi, last, mfma(vi, weight, acc[i]));
                 }
                 e0 += 32;
             } while (e0 < p.end);

@@ -179,6 +179,11 @@ def _rows_16(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _new_like(t):
+    """A contiguous tensor like t."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _workspace(lib, d, to, fro, dev):
     wsb = lib.dg_attention_workspace_size(d, to, fro)
     if wsb == 0:
@@ -186,24 +191,25 @@ def _workspace(lib, d, to, fro, dev):
     return torch.empty(wsb, dtype=torch.uint8, device=dev), wsb
 
 
-def _forward(q, k, v, table, plan, scale, train, want_lse):
+def _forward(q, k, v, table, plan, scale, want_lse, ctx=None):
     lib, dev = L.lib(), plan.device
     q, k, v = _rows_16(q), _rows_16(k), _rows_16(v)
     if table is not None:
         table = table.contiguous()
     targets, heads, dim = q.shape
+    dtype = q.dtype
     d = L.AttentionDesc(targets, plan.num_nodes, q.stride(0), k.stride(0), v.stride(0), 0, heads, k.size(1), dim,
-                        0 if table is None else table.size(0), _DTYPES[q.dtype], scale)
+                        0 if table is None else table.size(0), _DTYPES[dtype], scale)
     rows = plan.by_target
     with L.on_device(dev):
         stream = L.raw_stream(dev)
         plan._use(stream)
-        out = torch.empty((targets, heads, dim), dtype=q.dtype, device=dev)
+        out = torch.empty((targets, heads, dim), dtype=dtype, device=dev)
         out32 = norm = lse = ws = None
         wsb = 0
-        if train:
+        if ctx is not None:
             norm = torch.empty((targets, heads, 2), dtype=torch.float32, device=dev)
-            if q.dtype != torch.float32:
+            if dtype != torch.float32:
                 out32 = torch.empty((targets, heads, dim), dtype=torch.float32, device=dev)
         if want_lse:
             lse = torch.empty((targets, heads), dtype=torch.float32, device=dev)
@@ -214,15 +220,18 @@ def _forward(q, k, v, table, plan, scale, train, want_lse):
                                           out.data_ptr(), addr(out32), addr(norm), addr(lse), addr(ws), wsb, stream)
         if status:
             L.check(status, "neighbor_attention")
-    return out, lse, out32, norm
+    if ctx is not None:
+        # (the backward pass runs on a thread of its own, where each host instruction costs twice:
+        # it takes over what is worked out here)
+        ctx.save_for_backward(q, k, v, table, out if out32 is None else out32, norm)
+        ctx.desc, ctx.plan = d, plan
+    return out, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, plan, scale, want_lse):
-        out, lse, out32, norm = _forward(q, k, v, table, plan, scale, True, want_lse)
-        ctx.save_for_backward(q, k, v, table, out if out32 is None else out32, norm)
-        ctx.plan, ctx.scale = plan, scale
+        out, lse = _forward(q, k, v, table, plan, scale, want_lse, ctx)
         if lse is not None:
             ctx.mark_non_differentiable(lse)
         return out, lse
@@ -231,24 +240,18 @@ class _Attention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _grad_lse):
         q, k, v, table, out32, norm = ctx.saved_tensors
-        plan, lib = ctx.plan, L.lib()
+        plan, d, lib = ctx.plan, ctx.desc, L.lib()
         dev = plan.device
         if plan.by_source is None:
             raise RuntimeError("neighbor_attention: the plan was made with backward=False")
-        q, k, v, grad = _rows_16(q), _rows_16(k), _rows_16(v), _rows_16(grad)
-        if table is not None:
-            table = table.contiguous()
-        targets, heads, dim = q.shape
-        d = L.AttentionDesc(targets, plan.num_nodes, q.stride(0), k.stride(0), v.stride(0), grad.stride(0), heads,
-                            k.size(1), dim, 0 if table is None else table.size(0), _DTYPES[q.dtype], ctx.scale)
+        grad = _rows_16(grad)
+        d.ld_g = grad.stride(0)
         to, fro = plan.by_target.byref, plan.by_source.byref
         with L.on_device(dev):
             stream = L.raw_stream(dev)
             plan._use(stream)
-            dq = torch.empty((targets, heads, dim), dtype=q.dtype, device=dev)
-            dk = torch.empty(k.shape, dtype=q.dtype, device=dev)
-            dv = torch.empty(k.shape, dtype=q.dtype, device=dev)
-            dtable = torch.empty(table.shape, dtype=torch.float32, device=dev) if table is not None else None
+            dq, dk, dv = _new_like(q), _new_like(k), _new_like(v)
+            dtable = torch.empty_like(table) if table is not None else None
             ws, wsb = _workspace(lib, d, to, fro, dev)
             addr = L.addr
             status = lib.dg_attention_backward(d, to, fro, q.data_ptr(), k.data_ptr(), v.data_ptr(), addr(table),
@@ -330,7 +333,7 @@ def neighbor_attention(q, k, v, plan, bias_table=None, scale=None, return_lse=Fa
                                     or bias_table is not None and bias_table.requires_grad):
         out, lse = _Attention.apply(q, k, v, bias_table, plan, float(scale), return_lse)
     else:
-        out, lse, _, _ = _forward(q, k, v, bias_table, plan, float(scale), False, return_lse)
+        out, lse = _forward(q, k, v, bias_table, plan, float(scale), return_lse)
     return (out, lse) if return_lse else out
 
 
@@ -353,6 +356,7 @@ class _Grouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, sizes, bias):
         ctx.save_for_backward(x, weight, sizes)
+        ctx.desc = _grouped_desc(x, weight)
         return _grouped_forward(x, weight, sizes, bias)
 
     @staticmethod
@@ -361,10 +365,10 @@ class _Grouped(torch.autograd.Function):
         x, weight, sizes = ctx.saved_tensors
         need_x, need_w, _, need_b = ctx.needs_input_grad
         lib, dev, grad = L.lib(), x.device, grad.contiguous()
-        d = _grouped_desc(x, weight)
+        d = ctx.desc
         with L.on_device(dev):
-            dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-            dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_w or need_b else None
+            dx = torch.empty_like(x) if need_x else None
+            dw = torch.empty_like(weight) if need_w or need_b else None
             db = torch.empty(weight.shape[:2], dtype=x.dtype, device=dev) if need_b else None
             wsb = lib.dg_grouped_workspace_size(d) if dw is not None else 0
             ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
