@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "../../include/dynamis_graph.h"
 #include "dg_attention.hpp"
@@ -171,9 +172,8 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(AttnArgs a)
 }
 
 // A workgroup joins the parts of one long row for 64 channels: sixteen lanes of four channels times
-// 64 strands over the parts (four to a wave), first for the maximum, then for the sums against it,
+// STRANDS over the parts (four to a wave), first for the maximum, then for the sums against it,
 // so that a strand's loads do not wait for each other.
-constexpr int kStrands = 64, kJoinWaves = kStrands / 4;
 
 __device__ __forceinline__ float strand_sum(float x)
 {
@@ -181,18 +181,19 @@ __device__ __forceinline__ float strand_sum(float x)
     return x + __shfl_xor(x, 32, 64);
 }
 
-template <typename T>
-__global__ __launch_bounds__(16 * kStrands) void forward_join_kernel(AttnArgs a, int slices)
+template <typename T, int STRANDS>
+__global__ __launch_bounds__(16 * STRANDS) void forward_join_kernel(AttnArgs a, int slices)
 {
     const int slot = a.L.long_slot[blockIdx.x / slices], slice = (int)(blockIdx.x % slices);
     const int first = a.L.item_first[slot], n = a.L.item_first[slot + 1] - first, node = a.L.order[slot];
+    constexpr int kJoinWaves = STRANDS / 4;
     __shared__ float s_m[kJoinWaves][16], s_l[kJoinWaves][16], s_acc[kJoinWaves][4][16];
     const int x = threadIdx.x % 16, y = threadIdx.x / 16, wave = threadIdx.x / 64;
     const int wide = a.heads * a.dim, ch = slice * 64 + x * 4;
     const int h = min(ch, wide - 4) / a.dim;
     float mx = -INFINITY;
 #pragma unroll 4
-    for (int i = y; i < n; i += kStrands) mx = fmaxf(mx, a.part_m[(int64_t)(first + i) * a.heads + h]);
+    for (int i = y; i < n; i += STRANDS) mx = fmaxf(mx, a.part_m[(int64_t)(first + i) * a.heads + h]);
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     s_m[wave][x] = mx;
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(16 * kStrands) void forward_join_kernel(AttnArgs a,
     float l = 0, acc[4] = {0, 0, 0, 0};
     if (ch < wide)
 #pragma unroll 4
-        for (int i = y; i < n; i += kStrands) {
+        for (int i = y; i < n; i += STRANDS) {
             const int64_t it = first + i;
             const float f = exp2_fast(a.part_m[it * a.heads + h] - base);
             float b[4];
@@ -423,19 +424,20 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kv_kernel(AttnArgs a)
 }
 
 // The sum of the parts of one long row, as forward_join_kernel lays it out.
-template <typename T>
-__global__ __launch_bounds__(16 * kStrands) void sum_join_kernel(Lists L, const float* __restrict__ part, int wide,
+template <typename T, int STRANDS>
+__global__ __launch_bounds__(16 * STRANDS) void sum_join_kernel(Lists L, const float* __restrict__ part, int wide,
                                                                  int slices, float factor, T* __restrict__ out)
 {
     const int slot = L.long_slot[blockIdx.x / slices], slice = (int)(blockIdx.x % slices);
     const int first = L.item_first[slot], n = L.item_first[slot + 1] - first, node = L.order[slot];
+    constexpr int kJoinWaves = STRANDS / 4;
     __shared__ float s_acc[kJoinWaves][4][16];
     const int x = threadIdx.x % 16, y = threadIdx.x / 16, wave = threadIdx.x / 64;
     const int ch = slice * 64 + x * 4;
     float acc[4] = {0, 0, 0, 0};
     if (ch < wide)
 #pragma unroll 4
-        for (int i = y; i < n; i += kStrands) {
+        for (int i = y; i < n; i += STRANDS) {
             float b[4];
             load4(part + (int64_t)(first + i) * wide + ch, b);
             for (int c = 0; c < 4; ++c) acc[c] += b[c];
@@ -486,6 +488,7 @@ dim3 grid_of(const Lists& L, int head_groups, int per_cu)
     return dim3((unsigned)std::max<int64_t>(1, std::min(most, need)), (unsigned)head_groups);
 }
 
+// (600,000 edges of 8 heads of 32 floats: 144 us with 4, 137 us with 6, 138 us with 8)
 constexpr int kGroupsPerCu = 6;
 
 struct Layout {
@@ -611,9 +614,21 @@ void by_width(int dim, F&& f)
     }
 }
 
+// f(strands of the joins): 64 where the long rows have many parts, one wave where there are few (the
+// whole forward pass, 8 heads of 32: 4 rows of 348 parts 67 us with 64 strands, 81 us with 4; 1000
+// rows of 2 parts 152 us with 64, 125 us with 4).
+template <typename F>
+void by_parts(const Lists& L, F&& f)
+{
+    if (L.n_items > 16 * L.n_long) f(std::integral_constant<int, 64>{});
+    else f(std::integral_constant<int, 4>{});
+}
+
 template <typename T>
 void run_forward(const AttnArgs& a, hipStream_t s)
 {
+    // (bfloat16 on the matrix units: 27M edges of 8 heads of 16 take 887 us there, 2016 us here; the
+    // registers of a wave hold heads of up to kMfmaDim channels)
     if (sizeof(T) == 2 && a.dim <= kMfmaDim) {
         forward_mfma(a, s);
     } else {
@@ -626,8 +641,10 @@ void run_forward(const AttnArgs& a, hipStream_t s)
     }
     if (a.L.n_items > 0) {
         const int slices = (a.heads * a.dim + 63) / 64;
-        hipLaunchKernelGGL(forward_join_kernel<T>, dim3((unsigned)(a.L.n_long * slices)), dim3(16 * kStrands), 0, s, a,
-                           slices);
+        by_parts(a.L, [&](auto strands) {
+            hipLaunchKernelGGL((forward_join_kernel<T, strands()>), dim3((unsigned)(a.L.n_long * slices)),
+                               dim3(16 * strands()), 0, s, a, slices);
+        });
     }
 }
 
@@ -657,8 +674,11 @@ void run_backward(AttnArgs a, const Lists& by_target, const Lists& by_source, fl
                            (int)groups, (int)cells, dtable);
     if (a.L.n_items > 0) {
         const int wide = a.heads * a.dim, slices = (wide + 63) / 64;
-        hipLaunchKernelGGL(sum_join_kernel<T>, dim3((unsigned)(a.L.n_long * slices)), dim3(16 * kStrands), 0, s, a.L,
-                           (const float*)a.part_acc, wide, slices, a.scale, (T*)a.dq);
+        by_parts(a.L, [&](auto strands) {
+            hipLaunchKernelGGL((sum_join_kernel<T, strands()>), dim3((unsigned)(a.L.n_long * slices)),
+                               dim3(16 * strands()), 0, s, a.L, (const float*)a.part_acc, wide, slices, a.scale,
+                               (T*)a.dq);
+        });
     }
     a.L = by_source;
     if (matrix) {
@@ -672,11 +692,13 @@ void run_backward(AttnArgs a, const Lists& by_target, const Lists& by_source, fl
     }
     if (a.L.n_items > 0) {
         const int wide = a.kv_heads * a.dim, slices = (wide + 63) / 64;
-        const unsigned grid = (unsigned)(a.L.n_long * slices);
-        hipLaunchKernelGGL(sum_join_kernel<T>, dim3(grid), dim3(16 * kStrands), 0, s, a.L, (const float*)a.part_acc, wide, slices,
-                           a.scale, (T*)a.dk);
-        hipLaunchKernelGGL(sum_join_kernel<T>, dim3(grid), dim3(16 * kStrands), 0, s, a.L, (const float*)a.part_acc2, wide, slices,
-                           1.0f, (T*)a.dv);
+        by_parts(a.L, [&](auto strands) {
+            const dim3 grid((unsigned)(a.L.n_long * slices)), block(16 * strands());
+            hipLaunchKernelGGL((sum_join_kernel<T, strands()>), grid, block, 0, s, a.L, (const float*)a.part_acc, wide,
+                               slices, a.scale, (T*)a.dk);
+            hipLaunchKernelGGL((sum_join_kernel<T, strands()>), grid, block, 0, s, a.L, (const float*)a.part_acc2, wide,
+                               slices, 1.0f, (T*)a.dv);
+        });
     }
 }
 

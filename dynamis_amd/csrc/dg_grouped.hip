@@ -747,16 +747,24 @@ __global__ __launch_bounds__(256) void weight_join_kernel(Args a)
 }
 
 // ---------------------------------------------------------------- host
-// Rows of an item of dW.  Where the groups' tiles alone give every CU some workgroups, items of four
-// times a group's mean rows: hardly a group is split.  Else as many items as make four workgroups
-// for every CU, and no shorter than 128 rows (a partial sum is as much memory traffic as some
-// hundred rows are).
-int64_t rows_of_item(const dg_grouped_desc* d)
+// Rows of an item of dW.  Splitting a group costs the join's launch and its partial sums' traffic, as
+// much time as 512 rows of bfloat16 or 128 of float take to add up (one 128 x 128 tile, 128 groups
+// of 250 rows: 18 us whole, 26 us in items of 128 rows; 7 groups of 1400 rows of 100 by 164 floats:
+// 181 us whole, 27 us in items of 128).  Groups of fewer rows, and groups whose tiles alone give
+// every CU two workgroups (128 groups of 256 by 512: 50 us, split 85 to 107 us), are taken whole up
+// to four times their mean.  Else as many items as make two workgroups for every CU (8 groups of
+// 25,000 rows: 33 us, four workgroups 46 us), of 128 rows and more.
+template <typename T>
+int64_t item_rows(const dg_grouped_desc* d)
 {
     const int64_t tiles = (int64_t)((d->n + kTile - 1) / kTile) * ((d->k + kTile - 1) / kTile);
-    const int64_t mean = d->n_rows / d->n_groups + 1, each = 1024 / (d->n_groups * tiles);
-    const int64_t c = each <= 1 ? 4 * mean : mean / each;
+    const int64_t mean = d->n_rows / d->n_groups + 1, each = 512 / (d->n_groups * tiles);
+    const int64_t c = each <= 1 || mean <= (sizeof(T) == 2 ? 512 : 128) ? 4 * mean : mean / each;
     return std::max<int64_t>(128, (c + 63) / 64 * 64);
+}
+int64_t rows_of_item(const dg_grouped_desc* d)
+{
+    return d->dtype == DG_BF16 ? item_rows<__bf16>(d) : item_rows<float>(d);
 }
 
 struct Layout {
@@ -795,7 +803,6 @@ dg_status launched(const char* what)
 }
 
 // Workgroups of the streaming kernel: one a CU (its LDS), for each panel a share of the row tiles.
-// Narrower panels where wide ones would leave most CUs without work.
 constexpr int kCus = 256;
 int64_t stream_tiles(const Args& a) { return a.rows / kStreamRows + std::min(a.groups, a.rows) + 1; }
 
@@ -811,7 +818,11 @@ void run_stream(const Args& a, hipStream_t s)
 template <typename T, bool DX>
 void run_rows(const Args& a, hipStream_t s)
 {
-    // Whole chunks and a panel that fits: the streaming kernel.
+    // Whole chunks and a panel that fits: the streaming kernel (128 by 128 in bfloat16, 864 rows: 6.3
+    // us, the other 10.0 us; 200,000 rows: 24.5 us, 33.0 us).  Narrower panels read x more often and
+    // need less time to fill; they pay where wide ones would leave most CUs without work (128 by 128,
+    // panels of 32, 64 and 128: 864 rows 6.3, 6.8 and 8.1 us; 30,000 rows 10.6, 8.2 and 9.3 us; 60,000
+    // rows 13.9, 12.6 and 11.1 us).  Rows of more than 512 bytes leave the panel's LDS 64 columns.
     const int64_t bytes = a.depth * (int64_t)sizeof(T);
     const bool whole = bytes % 16 == 0 && a.cols % kChunk<T> == 0 && ((uintptr_t)a.a & 15) == 0 &&
                        ((uintptr_t)a.out & 15) == 0 && a.cols * (int64_t)sizeof(T) <= 1 << 24;
