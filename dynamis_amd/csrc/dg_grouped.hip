@@ -12,7 +12,7 @@
 // slab is multiplied.  The group's row count is not a multiple of a tile: rows past it are
 // zeros in LDS and are not stored.
 //
-// With widths of 64 to 512 these products are bound by memory more than by arithmetic: a row
+// In bfloat16, widths of 64 to 512 make these products bound by memory more than by arithmetic: a row
 // tile's workgroup takes all its column tiles in turn, so x is read once from HBM, and the
 // workgroups of an XCD hold neighbouring rows, whose weights then stay in its L2.
 #include <hip/hip_runtime.h>
@@ -449,6 +449,8 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
 // strip's result back through the same 8 KB to whole rows.  No barrier but at a change of group.
 // Loads and stores go through buffer descriptors of the strip: what lies outside reads as zero and
 // is not written, so every step has the same instructions and the waits between them are counted.
+// 2.2M rows of 128 by 128 in bfloat16: 232 us, 4.86 TB/s, what a copy reaches (4.9).  100,000 rows of
+// 256 by 256 floats: 135 us, 97 TFLOP/s of the 153 that a product of 8192 cubed reaches.
 constexpr int kStreamWaves = 8;
 constexpr int kStripRows = 32;
 constexpr int kStreamRows = kStreamWaves * kStripRows;
@@ -615,7 +617,9 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
 
 // dW[g][n][k] = sum_i dy[i, n] x[i, k] over an item's rows of a group, 128 x 128 of it; the
 // first column tile's workgroups sum dy itself.  Groups of one item write their result,
-// others partial sums that weight_join_kernel adds up in order.
+// others partial sums that weight_join_kernel adds up in order.  128 groups of 250 rows, 256 by 512:
+// 40 us, bound by the turning of both operands in registers (each is read twice to four times, from
+// L2): 83 MB in and out, 2.1 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256, 2) void weight_kernel(Args a, int64_t max_items)
 {
@@ -629,11 +633,12 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(Args a, int64_t max_item
     const int64_t at = xcd_order(blockIdx.x, gridDim.x);
     const int64_t item = at / (n_tiles * k_tiles);
     int64_t items, covered;
-    pass<4>(a, cuts, s_w, &s_p, items, covered, [](int64_t, int64_t, int64_t) { return false; });
+    pass<4>(a, cuts, s_w, &s_p, items, covered,
+            [&](int64_t first, int64_t n, int64_t) { return item >= first && item < first + n; });
     if (item >= items || item >= max_items) return;
     const int tile = (int)(at % (n_tiles * k_tiles)), n0 = tile / k_tiles * kTile, k0 = tile % k_tiles * kTile;
-    const Place p = locate<4>(a, cuts, item, s_w, &s_p);
-    const int64_t group = scalar64(p.group), row = scalar64(p.row), size = scalar64(p.size), piece = scalar64(p.piece);
+    const Place p = s_p;
+    const int64_t group = scalar64(p.group), row = scalar64(p.row), size = scalar64(p.size), piece = item - scalar64(p.piece);
     const int64_t r0 = row + piece * a.chunk;
     const int64_t n_rows = max((int64_t)0, min(min(size - piece * a.chunk, a.chunk), a.rows - r0));
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, t = threadIdx.x % 128;
@@ -707,16 +712,16 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(Args a, int64_t max_item
 }
 
 // Adds up the partial sums of groups of more than one item, in the items' order: a thread for four
-// neighbouring columns, sixteen workgroups for a tile of a split group.
+// neighbouring columns a time, `parts` workgroups (a divisor of sixteen) for a tile of a split group.
 constexpr int kJoinParts = 16;
 template <typename T>
-__global__ __launch_bounds__(256) void weight_join_kernel(Args a)
+__global__ __launch_bounds__(256) void weight_join_kernel(Args a, int parts)
 {
     __shared__ int64_t s_w[12];
     __shared__ Place s_p;
     const int n_tiles = (a.cols + kTile - 1) / kTile, k_tiles = (a.depth + kTile - 1) / kTile;
-    const int64_t unit = blockIdx.x / kJoinParts, rank = unit / (n_tiles * k_tiles);
-    const int part_of = (int)(blockIdx.x % kJoinParts);
+    const int64_t unit = blockIdx.x / parts, rank = unit / (n_tiles * k_tiles);
+    const int first_part = (int)(blockIdx.x % parts);
     const int tile = (int)(unit % (n_tiles * k_tiles)), n0 = tile / k_tiles * kTile, k0 = tile % k_tiles * kTile;
     const Cuts cuts{a.chunk, 1};
     if (threadIdx.x == 0) s_p.group = -1;
@@ -726,19 +731,23 @@ __global__ __launch_bounds__(256) void weight_join_kernel(Args a)
     if (group < 0) return;
     const int64_t pieces = scalar64(cuts.of(s_p.size)), slot = scalar64(s_p.many);
     // (the layout of weight_kernel's accumulators: four waves of sixteen times 64 lanes)
-    const int w = part_of / 4, q = part_of % 4 * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63;
     const int64_t step = (int64_t)n_tiles * k_tiles * 4096;
-    const f32x4* part = (const f32x4*)a.part + slot * step + ((int64_t)tile * 4 + w) * 1024 + q * 64 + lane;
-    f32x4 sum = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int64_t i = 0; i < pieces; ++i) sum += part[i * step];
-    const int i = q / 8, j = q / 4 % 2;
-    const int n = n0 + (w % 2) * 64 + 32 * j + (lane & 31), k = k0 + (w / 2) * 64 + 32 * i + 8 * (q % 4) + 4 * (lane >> 5);
-    if (n < a.cols)
-        for (int c = 0; c < 4; ++c)
-            if (k + c < a.depth) ((T*)a.out)[(group * a.cols + n) * a.depth + k + c] = (T)sum[c];
+    for (int part_of = first_part; part_of < kJoinParts; part_of += parts) {
+        const int w = part_of / 4, q = part_of % 4 * 4 + threadIdx.x / 64;
+        const f32x4* part = (const f32x4*)a.part + slot * step + ((int64_t)tile * 4 + w) * 1024 + q * 64 + lane;
+        f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 8
+        for (int64_t i = 0; i < pieces; ++i) sum += part[i * step];
+        const int i = q / 8, j = q / 4 % 2;
+        const int n = n0 + (w % 2) * 64 + 32 * j + (lane & 31);
+        const int k = k0 + (w / 2) * 64 + 32 * i + 8 * (q % 4) + 4 * (lane >> 5);
+        if (n < a.cols)
+            for (int c = 0; c < 4; ++c)
+                if (k + c < a.depth) ((T*)a.out)[(group * a.cols + n) * a.depth + k + c] = (T)sum[c];
+    }
     const int col = n0 + threadIdx.x;
-    if (a.dbias && k0 == 0 && part_of == 0 && threadIdx.x < kTile && col < a.cols) {
+    if (a.dbias && k0 == 0 && first_part == 0 && threadIdx.x < kTile && col < a.cols) {
         float x = 0;
 #pragma unroll 4
         for (int64_t i2 = 0; i2 < pieces; ++i2) x += a.part_bias[(slot + i2) * a.cols + col];
@@ -749,11 +758,11 @@ __global__ __launch_bounds__(256) void weight_join_kernel(Args a)
 // ---------------------------------------------------------------- host
 // Rows of an item of dW.  Splitting a group costs the join's launch and its partial sums' traffic, as
 // much time as 512 rows of bfloat16 or 128 of float take to add up (one 128 x 128 tile, 128 groups
-// of 250 rows: 18 us whole, 26 us in items of 128 rows; 7 groups of 1400 rows of 100 by 164 floats:
-// 181 us whole, 27 us in items of 128).  Groups of fewer rows, and groups whose tiles alone give
-// every CU two workgroups (128 groups of 256 by 512: 50 us, split 85 to 107 us), are taken whole up
+// of 250 rows: 17 us whole, 25 us in items of 128 rows; 7 groups of 1400 rows of 100 by 164 floats:
+// 182 us whole, 27 us in items of 128).  Groups of fewer rows, and groups whose tiles alone give
+// every CU two workgroups (128 groups of 256 by 512: 41 us, split 71 to 102 us), are taken whole up
 // to four times their mean.  Else as many items as make two workgroups for every CU (8 groups of
-// 25,000 rows: 33 us, four workgroups 46 us), of 128 rows and more.
+// 25,000 rows: 32 us, four workgroups 41 us, whole 538 us), of 128 rows and more.
 template <typename T>
 int64_t item_rows(const dg_grouped_desc* d)
 {
@@ -849,8 +858,12 @@ void run_weight(const Args& a, hipStream_t s)
     if (grid > kXcds) grid = (grid + kXcds - 1) / kXcds * kXcds;
     hipLaunchKernelGGL(weight_kernel<T>, dim3((unsigned)grid), dim3(256), 0, s, a, items);
     const int64_t split = std::min(a.groups, a.rows / a.chunk);  // groups above an item, at most
-    if (split > 0)
-        hipLaunchKernelGGL(weight_join_kernel<T>, dim3((unsigned)(split * tiles * kJoinParts)), dim3(256), 0, s, a);
+    if (split > 0) {
+        // (most of a large number find no group: one round of workgroups, each with more to do)
+        int parts = kJoinParts;
+        while (parts > 1 && split * tiles * parts > 4 * kCus) parts /= 2;
+        hipLaunchKernelGGL(weight_join_kernel<T>, dim3((unsigned)(split * tiles * parts)), dim3(256), 0, s, a, parts);
+    }
 }
 
 }  // namespace
