@@ -278,11 +278,6 @@ __device__ __forceinline__ int64_t claim(const Args& a, int64_t g)
 {
     return g < a.groups ? min(max(a.sizes[g], (int64_t)0), a.rows) : 0;
 }
-// ... and those it has, its first row given: the rows end where they end.
-__device__ __forceinline__ int64_t granted(const Args& a, int64_t g, int64_t row)
-{
-    return min(claim(a, g), max(a.rows - row, (int64_t)0));
-}
 
 // One pass of the workgroup (256 threads, or 512) over the groups: all pieces and rows, and where `found`
 // holds, of (its first piece, its pieces, split groups before), that group's place (piece: its
@@ -356,6 +351,22 @@ __device__ __forceinline__ int64_t scalar64(int64_t x)
     return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
+// The first group after `group` that claims rows (there is one), its first row given; `size`: its rows.
+// 64 groups a load: a run of empty ones costs little.
+__device__ __forceinline__ int64_t next_group(const Args& a, int64_t group, int64_t row, int64_t& size)
+{
+    for (++group; group < a.groups; group += 64) {
+        const int64_t n = claim(a, group + (threadIdx.x & 63));
+        const unsigned long long some = __ballot(n > 0);
+        if (!some) continue;
+        const int first = __builtin_ctzll(some);
+        size = min(scalar64(__shfl(n, first, 64)), max(a.rows - row, (int64_t)0));
+        return group + first;
+    }
+    size = 0x7fffffffffffffffll;  // (not reached: ends the caller's search)
+    return a.groups - 1;
+}
+
 // This workgroup's place in an order in which an XCD's workgroups are neighbours.
 __device__ __forceinline__ int64_t xcd_order(int64_t b, int64_t n)
 {
@@ -423,8 +434,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
                             while (piece * kTile >= size) {  // (a later group has rows: u < end)
                                 row += size;
                                 piece = 0;
-                                ++group;
-                                size = scalar64(granted(a, group, row));
+                                group = next_group(a, group, row, size);
                             }
                         }
                         fetch(u, 0);
@@ -540,8 +550,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                         while (piece * kStreamRows >= size) {  // (a later group has rows: u < end)
                             row += size;
                             piece = 0;
-                            ++group;
-                            size = scalar64(granted(a, group, row));
+                            group = next_group(a, group, row, size);
                         }
                         r0 = row + piece * kStreamRows + w * kStripRows;
                         n_rows = rows_here(r0);
