@@ -22,7 +22,6 @@ from .. import _lib as L
 from .dynamis_state_impl import _check, _shape, sfc_order
 
 _DTYPES = {torch.float32: L.DG_F32, torch.bfloat16: L.DG_BF16}
-_NULL = ctypes.c_void_p(0)
 
 
 class _Rows:
@@ -57,9 +56,8 @@ class _Rows:
                                        stream), "neighbor_plan")
 
     def tensors(self):
-        return [t for t in (self.order, self.ptr, self.idx, self.bucket, self.items, self.item_first,
-                            self.long_slot)
-                if t is not None]
+        lists = self.order, self.ptr, self.idx, self.bucket, self.items, self.item_first, self.long_slot
+        return [t for t in lists if t is not None]
 
 
 class NeighborPlan:
