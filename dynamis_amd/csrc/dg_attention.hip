@@ -191,6 +191,7 @@ template <typename T, int STRANDS>
 __global__ __launch_bounds__(16 * STRANDS) void forward_join_kernel(AttnArgs a, int slices)
 {
     const int slot = a.L.long_slot[blockIdx.x / slices], slice = (int)(blockIdx.x % slices);
+    if (slot < 0) return;  // (fewer long rows than said)
     const int first = a.L.item_first[slot], n = a.L.item_first[slot + 1] - first, node = a.L.order[slot];
     constexpr int kJoinWaves = STRANDS / 4;
     __shared__ float s_m[kJoinWaves][16], s_l[kJoinWaves][16], s_acc[kJoinWaves][4][16];
@@ -435,6 +436,7 @@ __global__ __launch_bounds__(16 * STRANDS) void sum_join_kernel(Lists L, const f
                                                                  int slices, float factor, T* __restrict__ out)
 {
     const int slot = L.long_slot[blockIdx.x / slices], slice = (int)(blockIdx.x % slices);
+    if (slot < 0) return;
     const int first = L.item_first[slot], n = L.item_first[slot + 1] - first, node = L.order[slot];
     constexpr int kJoinWaves = STRANDS / 4;
     __shared__ float s_acc[kJoinWaves][4][16];

@@ -333,6 +333,7 @@ __global__ void long_kernel(const int* __restrict__ rank, int64_t n, int64_t n_l
 {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i < n && rank[i + 1] > rank[i] && rank[i] < n_long) long_slot[rank[i]] = (int32_t)i;
+    if (i < n_long && i >= rank[n]) long_slot[i] = -1;
 }
 
 __global__ void items_kernel(const int32_t* __restrict__ first, const int32_t* __restrict__ ptr,
@@ -571,7 +572,8 @@ dg_status dg_neighbors_parts(const int32_t* order, const int32_t* ptr, int64_t n
                        parts, is_long);
     excl_scan<int, int>(parts, n_rows, item_first, part, s);
     excl_scan<int, int>(is_long, n_rows, rank, part, s);
-    hipLaunchKernelGGL(long_kernel, dim3(nblk(n_rows)), dim3(256), 0, s, (const int*)rank, n_rows, n_long, long_slot);
+    hipLaunchKernelGGL(long_kernel, dim3(nblk(std::max(n_rows, n_long))), dim3(256), 0, s, (const int*)rank, n_rows, n_long,
+                       long_slot);
     hipLaunchKernelGGL(items_kernel, dim3(nblk(std::max(n_rows, max_items))), dim3(256), 0, s, (const int32_t*)item_first,
                        ptr, order, n_rows, (int)chunk, max_items, (int4*)items);
     return launched("dg_neighbors_parts");

@@ -424,7 +424,7 @@ dg_status dg_neighbors_by_source(const dg_neighbor_desc* desc, int64_t n_entries
                                  hipStream_t stream);
 /* The items of `chunk` entries of the n_long rows above DG_NEIGHBOR_SPLIT entries: item_first int32
  * [n_rows + 1], items int32 [max_items, 4], aligned to 16 bytes, with max_items >= long_entries /
- * chunk + n_long, long_slot int32 [n_long]. */
+ * chunk + n_long, long_slot int32 [n_long] (-1 where there are fewer long rows). */
 size_t dg_neighbors_parts_workspace_size(int64_t n_rows);
 dg_status dg_neighbors_parts(const int32_t* order, const int32_t* ptr, int64_t n_rows, int32_t chunk,
                              int64_t max_items, int64_t n_long, int32_t* item_first, int32_t* items,
