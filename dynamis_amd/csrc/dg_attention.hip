@@ -15,9 +15,9 @@
 //
 // Bound by the vector units' instructions (a logit of 32 channels is four multiply-adds and three
 // exchanges a lane, of which half the lanes' work is the reduction's) next to the gathered rows:
-// 670,000 edges of 4 heads of 32 floats take 33 us, 20 TB/s of rows out of the caches.  Few rows are
-// bound by the wait for a row's loads in turn: 864 rows of 86 edges take 24 us forward, 28 us by
-// target and 23 us by source.
+// 670,000 edges of 4 heads of 32 floats take 29 us, 24 TB/s of rows out of the caches.  Few rows are
+// bound by the wait for a row's loads in turn: 864 rows of 86 edges take 18 us forward, 21 us by
+// target and 20 us by source.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -77,7 +77,24 @@ __device__ __forceinline__ bool stage_table(const AttnArgs& a, float* s_tab)
     return s_any != 0;
 }
 
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 4;  // (600,000 edges of 8 heads of 32 floats: 140 us, eight edges a step 148 us)
+
+// The entries of a lane's next edges, under way while the ones before are worked on: of few rows a
+// wave else waits twice for each of its steps, for the entries and for the rows that they name.
+// (1000 rows of 60 edges, 8 heads of 32 floats: 34 us, without 47 us; 100,000 rows: 1697 and 1644 us.)
+template <int N>
+struct Entries {
+    int node[N], bucket[N];
+    __device__ __forceinline__ void load(const AttnArgs& a, const Piece& p, int e0, int span)
+    {
+#pragma unroll
+        for (int r = 0; r < N; ++r) {
+            const int at = max(min(e0 + r * span, p.end - 1), 0);  // (an empty row reads some entry)
+            node[r] = a.L.idx[at];
+            bucket[r] = a.table ? (int)a.L.bucket[at] : 0;
+        }
+    }
+};
 
 template <typename T, int LPH>
 __global__ __launch_bounds__(64 * kWaves) void forward_kernel(AttnArgs a)
@@ -104,18 +121,19 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(AttnArgs a)
         if (!wide)
             for (int i = 0; i < 4; ++i) q[i] = 0;
         float mx = -INFINITY, l = 0;
+        Entries<kUnroll> entry;
+        entry.load(a, p, p.begin + es, span);
         for (int e0 = p.begin; e0 < p.end; e0 += kUnroll * span) {
             float k[kUnroll][4], v[kUnroll][4], s[kUnroll];
 #pragma unroll
             for (int r = 0; r < kUnroll; ++r) {
-                const int e = e0 + r * span + es;
-                const int at = min(e, p.end - 1);
-                const int64_t j = a.L.idx[at];
+                const int64_t j = entry.node[r];
                 load4((const T*)a.k + j * a.ldk + kch, k[r]);
                 load4((const T*)a.v + j * a.ldv + kch, v[r]);
-                s[r] = e < p.end ? 0.0f : -INFINITY;
-                if (a.table) s[r] += s_tab[(int)a.L.bucket[at] * a.heads + h];
+                s[r] = e0 + r * span + es < p.end ? 0.0f : -INFINITY;
+                if (a.table) s[r] += s_tab[entry.bucket[r] * a.heads + h];
             }
+            entry.load(a, p, e0 + kUnroll * span + es, span);
             float top = mx;
 #pragma unroll
             for (int r = 0; r < kUnroll; ++r) {
@@ -278,23 +296,21 @@ __global__ __launch_bounds__(64 * kWaves) void backward_q_kernel(AttnArgs a)
         const float2 norm = a.norm[(int64_t)p.node * a.heads + h];
         if (part == 0 && es == 0 && mine)
             a.stats[(int64_t)p.node * a.heads + h] = make_float4(norm.x, norm.y, delta, 0.0f);
+        Entries<kUnroll> entry;
+        entry.load(a, p, p.begin + es, span);
         for (int e0 = p.begin; e0 < p.end; e0 += kUnroll * span) {
             float k[kUnroll][4], v[kUnroll][4], s[kUnroll];
             int b[kUnroll];
 #pragma unroll
             for (int r = 0; r < kUnroll; ++r) {
-                const int e = e0 + r * span + es;
-                const int at = min(e, p.end - 1);
-                const int64_t j = a.L.idx[at];
+                const int64_t j = entry.node[r];
                 load4((const T*)a.k + j * a.ldk + kch, k[r]);
                 load4((const T*)a.v + j * a.ldv + kch, v[r]);
-                s[r] = e < p.end ? 0.0f : -INFINITY;
-                b[r] = 0;
-                if (a.table) {
-                    b[r] = (int)a.L.bucket[at] * a.heads + h;
-                    s[r] += s_tab[b[r]];
-                }
+                s[r] = e0 + r * span + es < p.end ? 0.0f : -INFINITY;
+                b[r] = entry.bucket[r] * a.heads + h;
+                if (a.table) s[r] += s_tab[b[r]];
             }
+            entry.load(a, p, e0 + kUnroll * span + es, span);
 #pragma unroll
             for (int r = 0; r < kUnroll; ++r) {
                 if (!wide)
@@ -362,18 +378,19 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kv_kernel(AttnArgs a)
         load4((const T*)a.v + p.node * a.ldv + (int64_t)c * a.dim + ch, v);
         if (!wide)
             for (int i = 0; i < 4; ++i) k[i] = v[i] = 0;
+        Entries<kTwo> entry;
+        entry.load(a, p, p.begin + es, span);
         for (int e0 = p.begin; e0 < p.end; e0 += kTwo * span) {
             int64_t t[kTwo];
             int b[kTwo];
             bool in[kTwo];
 #pragma unroll
             for (int r = 0; r < kTwo; ++r) {
-                const int e = e0 + r * span + es;
-                const int at = min(e, p.end - 1);
-                t[r] = a.L.idx[at];
-                b[r] = a.table ? (int)a.L.bucket[at] * a.heads : 0;
-                in[r] = e < p.end;
+                t[r] = entry.node[r];
+                b[r] = entry.bucket[r] * a.heads;
+                in[r] = e0 + r * span + es < p.end;
             }
+            entry.load(a, p, e0 + kTwo * span + es, span);
             for (int x = 0; x < a.per; ++x) {
                 const int h = c * a.per + x;
                 float q[kTwo][4], g[kTwo][4], s[kTwo];
