@@ -431,7 +431,7 @@ dg_status dg_neighbors_by_target(const dg_neighbor_desc* d, const int64_t* src, 
     const Layout L = layout(d->n_edges, d->n_nodes);
     if (!ws || ws_bytes < L.total) return fail(DG_ERR_WORKSPACE, "workspace too small");
     if (!ptr || !idx || (d->n_nodes > 0 && !order) || (d->n_edges > 0 && (!src || !dst)) ||
-        (bucket && !dist) || (dist && d->n_boundaries > 0 && !boundaries))
+        (bucket && d->n_edges > 0 && !dist) || (dist && d->n_boundaries > 0 && !boundaries))
         return fail(DG_ERR_INVALID, "inputs or outputs are NULL");
     char* w = (char*)ws;
     Args a = {};

@@ -1,0 +1,37 @@
+"""The operators on a built graph at the ends of their ranges, on the GPU: lists without edges,
+infinities, derivatives that they do not have, what two backward passes share."""
+import numpy as np
+import pytest
+import torch
+
+from dynamis_amd import dynamis_state as ds
+
+pytestmark = pytest.mark.gpu
+TYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+
+
+def _leave_nans(sizes):
+    """Freed memory of these many floats holds NaN, so that a result which is not written shows."""
+    for n in sizes:
+        del [torch.full((n,), float("nan"), device="cuda") for _ in range(16)][:]
+
+
+# ---------------------------------------------------------------- no edges
+
+
+@TYPES
+@pytest.mark.parametrize("nodes,targets,edges", [(5, 5, 0), (5, 0, 0), (5, 5, 40)], ids=str)
+def test_no_edges_with_a_table(cuda, nodes, targets, edges, dtype):
+    """An edge list without edges, or one whose mask leaves none: zeros everywhere."""
+    print(f"\n[case] no edges {nodes} {targets} {edges} {dtype}", flush=True)
+    ei = torch.randint(0, max(targets, 1), (2, edges), device="cuda")
+    plan = ds.neighbor_plan(ei, nodes, targets, distances=torch.rand(edges, device="cuda") * 4,
+                            boundaries=[1.0, 2.0, 3.0], edge_mask=torch.zeros(edges, dtype=torch.bool, device="cuda"))
+    assert plan.num_edges == 0 and plan.num_buckets == 4
+    q, k, v = (torch.randn(m, 4, 16, device="cuda", dtype=dtype, requires_grad=True) for m in (targets, nodes, nodes))
+    table = torch.randn(4, 4, device="cuda", requires_grad=True)
+    out, lse = ds.neighbor_attention(q, k, v, plan, table, return_lse=True)
+    assert out.shape == q.shape and not out.any() and (lse == -torch.inf).all()
+    _leave_nans([16, 128, 512])
+    for g, of in zip(torch.autograd.grad(out, (q, k, v, table), torch.ones_like(out)), (q, k, v, table)):
+        assert g.shape == of.shape and not g.any()
