@@ -779,7 +779,14 @@ dg_status dg_attention_backward(const dg_attention_desc* d, const dg_neighbor_li
     if (st != DG_OK) return st;
     const Layout L = layout(d, by_target, by_source);
     if (!ws || ws_bytes < L.total) return fail(DG_ERR_WORKSPACE, "workspace too small");
-    if (d->n_nodes == 0) return DG_OK;
+    if (d->n_nodes == 0) {  // (no terms: the table's gradient is zeros, the others are empty)
+        const int cells = d->n_buckets * d->heads;
+        if (cells == 0) return DG_OK;
+        if (!dtable) return fail(DG_ERR_INVALID, "inputs or outputs are NULL");
+        hipLaunchKernelGGL(table_join_kernel, dim3(nblk(cells, 16)), dim3(1024), 0, s, (const float*)nullptr, 0, cells,
+                           dtable);
+        return launched("dg_attention_backward");
+    }
     if (!k || !v || !dk || !dv || (d->n_targets > 0 && (!q || !out32 || !norm || !grad_out || !dq)) ||
         (d->n_buckets > 0 && (!table || !dtable)))
         return fail(DG_ERR_INVALID, "inputs or outputs are NULL");

@@ -35,3 +35,15 @@ def test_no_edges_with_a_table(cuda, nodes, targets, edges, dtype):
     _leave_nans([16, 128, 512])
     for g, of in zip(torch.autograd.grad(out, (q, k, v, table), torch.ones_like(out)), (q, k, v, table)):
         assert g.shape == of.shape and not g.any()
+
+
+@TYPES
+def test_the_tables_gradient_of_no_nodes(cuda, dtype):
+    print(f"\n[case] no nodes {dtype}", flush=True)
+    plan = ds.neighbor_plan(torch.empty(2, 0, dtype=torch.long, device="cuda"), 0,
+                            distances=torch.empty(0, device="cuda"), boundaries=[1.0, 2.0, 3.0])
+    q, k, v = (torch.empty(0, 4, 16, device="cuda", dtype=dtype, requires_grad=True) for _ in range(3))
+    table = torch.randn(4, 4, device="cuda", requires_grad=True)
+    out = ds.neighbor_attention(q, k, v, plan, table)
+    _leave_nans([16, 128])
+    assert not torch.autograd.grad(out, table, torch.ones_like(out))[0].any()
