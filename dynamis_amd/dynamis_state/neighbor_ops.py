@@ -17,6 +17,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib as L
 from .dynamis_state_impl import _check, _shape, sfc_order
@@ -260,6 +261,14 @@ class _Attention(torch.autograd.Function):
         return dq, dk, dv, dtable, None, None, None
 
 
+def _refuse_tangents(name, *tensors):
+    """Called at a level of forward-mode differentiation, where a tensor may carry a tangent without
+    requiring a gradient: a result without one would be a derivative of zero."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
 def _check_attention(q, k, v, plan, bias_table):
     """The refusals of neighbor_attention, with their messages."""
     for name, t in (("q", q), ("k", k), ("v", v)):
@@ -316,9 +325,12 @@ def neighbor_attention(q, k, v, plan, bias_table=None, scale=None, return_lse=Fa
     log-sum of -inf).  Returns out like q, and with return_lse also the natural log-sums
     [num_targets, heads] in float32 (not differentiable).
 
-    Differentiable in q, k, v and bias_table (once).  All sums are float32, in a fixed order:
+    Differentiable in q, k, v and bias_table (once, in reverse: a tensor with a forward-mode tangent
+    is refused).  All sums are float32, in a fixed order:
     results repeat bit for bit.
     """
+    if forward_ad._current_level >= 0:  # (unpack_dual itself takes half a microsecond a tensor)
+        _refuse_tangents("neighbor_attention", q, k, v, bias_table)
     if not _attention_is_fine(q, k, v, plan, bias_table):
         _check_attention(q, k, v, plan, bias_table)
         if bias_table is not None:
@@ -424,9 +436,12 @@ def grouped_linear(x, weight, sizes, bias=None):
     the last group give zeros and sizes are not checked otherwise; on the host, or as a list, they
     have to be non-negative and to add up to the rows.  Groups may be empty.
 
-    Differentiable in x, weight and bias (once).  Sums are float32, in a fixed order: results
+    Differentiable in x, weight and bias (once, in reverse: a tensor with a forward-mode tangent is
+    refused).  Sums are float32, in a fixed order: results
     repeat bit for bit.
     """
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("grouped_linear", x, weight, bias)
     if not isinstance(sizes, torch.Tensor):
         sizes = torch.as_tensor(sizes)
     if not _grouped_is_fine(x, weight, sizes, bias):

@@ -3,6 +3,7 @@ infinities, derivatives that they do not have, what two backward passes share.""
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from dynamis_amd import dynamis_state as ds
 
@@ -47,3 +48,38 @@ def test_the_tables_gradient_of_no_nodes(cuda, dtype):
     out = ds.neighbor_attention(q, k, v, plan, table)
     _leave_nans([16, 128])
     assert not torch.autograd.grad(out, table, torch.ones_like(out))[0].any()
+
+
+# ---------------------------------------------------------------- derivatives that there are not
+
+
+@pytest.mark.parametrize("of", ["q", "k", "v", "table"])
+def test_attention_refuses_tangents(cuda, of):
+    """Forward-mode derivatives are refused, not dropped."""
+    print(f"\n[case] tangent of {of}", flush=True)
+    ei = torch.tensor([[0, 1, 2], [0, 0, 1]], device="cuda")
+    plan = ds.neighbor_plan(ei, 4, 2, distances=torch.ones(3, device="cuda"), boundaries=[1.0])
+    t = {"q": torch.randn(2, 2, 8, device="cuda"), "k": torch.randn(4, 2, 8, device="cuda"),
+         "v": torch.randn(4, 2, 8, device="cuda"), "table": torch.randn(2, 2, device="cuda")}
+    want = ds.neighbor_attention(t["q"], t["k"], t["v"], plan, t["table"])
+    with forward_ad.dual_level():
+        # (tensors without a tangent may be used at a level)
+        assert torch.equal(ds.neighbor_attention(t["q"], t["k"], t["v"], plan, t["table"]), want)
+        t[of] = forward_ad.make_dual(t[of], torch.ones_like(t[of]))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                ds.neighbor_attention(t["q"], t["k"], t["v"], plan, t["table"])
+
+
+@pytest.mark.parametrize("of", ["x", "weight", "bias"])
+def test_grouped_refuses_tangents(cuda, of):
+    print(f"\n[case] tangent of {of}", flush=True)
+    t = {"x": torch.randn(7, 8, device="cuda"), "weight": torch.randn(2, 4, 8, device="cuda"),
+         "bias": torch.randn(2, 4, device="cuda")}
+    want = ds.grouped_linear(t["x"], t["weight"], [3, 4], t["bias"])
+    with forward_ad.dual_level():
+        assert torch.equal(ds.grouped_linear(t["x"], t["weight"], [3, 4], t["bias"]), want)
+        t[of] = forward_ad.make_dual(t[of], torch.ones_like(t[of]))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                ds.grouped_linear(t["x"], t["weight"], [3, 4], t["bias"])
