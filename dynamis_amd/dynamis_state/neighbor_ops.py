@@ -239,11 +239,13 @@ class _Attention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _grad_lse):
         q, k, v, table, out32, norm = ctx.saved_tensors
-        plan, d, lib = ctx.plan, ctx.desc, L.lib()
+        plan, lib = ctx.plan, L.lib()
         dev = plan.device
         if plan.by_source is None:
             raise RuntimeError("neighbor_attention: the plan was made with backward=False")
         grad = _rows_16(grad)
+        # (its own: another backward pass of the same graph may be under way with another stride)
+        d = L.AttentionDesc.from_buffer_copy(ctx.desc)
         d.ld_g = grad.stride(0)
         to, fro = plan.by_target.byref, plan.by_source.byref
         with L.on_device(dev):

@@ -5,6 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from dynamis_amd import _lib
 from dynamis_amd import dynamis_state as ds
 
 pytestmark = pytest.mark.gpu
@@ -83,3 +84,31 @@ def test_grouped_refuses_tangents(cuda, of):
         for grad in (True, False):
             with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
                 ds.grouped_linear(t["x"], t["weight"], [3, 4], t["bias"])
+
+
+# ---------------------------------------------------------------- backward passes side by side
+
+
+def test_backward_passes_share_no_descriptor(cuda, monkeypatch):
+    """Two backward passes of a retained graph may run at the same time: what one hands to the
+    library is not written by the other."""
+    print("\n[case] descriptors", flush=True)
+    plan = ds.neighbor_plan(torch.tensor([[0, 1, 2], [0, 0, 1]], device="cuda"), 4)
+    q, k, v = (torch.randn(4, 2, 8, device="cuda", requires_grad=True) for _ in range(3))
+    out = ds.neighbor_attention(q, k, v, plan)
+    seen, lib = [], _lib.lib()
+
+    class Spy:
+        def __getattr__(self, name):
+            return getattr(lib, name)
+
+        def dg_attention_backward(self, desc, *args):
+            seen.append((desc, desc.ld_g))
+            return lib.dg_attention_backward(desc, *args)
+
+    monkeypatch.setattr(_lib, "lib", lambda: Spy())
+    wide = torch.randn(4, 64, device="cuda")
+    for grad in (wide[:, :16].unflatten(1, (2, 8)), wide[:, :16].contiguous().unflatten(1, (2, 8))):
+        torch.autograd.grad(out, (q, k, v), grad, retain_graph=True)
+    assert [ld for _, ld in seen] == [64, 16]
+    assert [d.ld_g for d, _ in seen] == [64, 16]
