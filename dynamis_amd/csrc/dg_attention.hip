@@ -125,6 +125,7 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(AttnArgs a)
         entry.load(a, p, p.begin + es, span);
         for (int e0 = p.begin; e0 < p.end; e0 += kUnroll * span) {
             float k[kUnroll][4], v[kUnroll][4], s[kUnroll];
+            bool there[kUnroll];
 #pragma unroll
             for (int r = 0; r < kUnroll; ++r) {
                 const int64_t j = entry.node[r];
@@ -132,7 +133,10 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(AttnArgs a)
                 load4((const T*)a.v + j * a.ldv + kch, v[r]);
                 s[r] = e0 + r * span + es < p.end ? 0.0f : -INFINITY;
                 if (a.table) s[r] += s_tab[entry.bucket[r] * a.heads + h];
+                there[r] = s[r] != -INFINITY;
             }
+            // (lanes past the row's end hold its last edge: a weight of zero must not meet an infinity)
+            const bool hides = takes_out || p.end - e0 < kUnroll * span;
             entry.load(a, p, e0 + kUnroll * span + es, span);
             float top = mx;
 #pragma unroll
@@ -145,7 +149,7 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(AttnArgs a)
                 d = fmaf(q[3], k[r][3], d);
                 d = sum_lanes<LPH>(d);
                 // an edge that is not there stays at -inf whatever its product is
-                s[r] = s[r] == -INFINITY ? s[r] : fmaf(d, scale2, s[r]);
+                s[r] = there[r] ? fmaf(d, scale2, s[r]) : s[r];
                 top = fmaxf(top, s[r]);
             }
             const float base = top == -INFINITY ? 0.0f : top;
@@ -156,7 +160,7 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(AttnArgs a)
 #pragma unroll
             for (int r = 0; r < kUnroll; ++r) {
                 const float pr = exp2_fast(s[r] - base);
-                if (takes_out && s[r] == -INFINITY)
+                if (hides && !there[r])
                     for (int i = 0; i < 4; ++i) v[r][i] = 0;
                 l += pr;
 #pragma unroll

@@ -7,6 +7,7 @@ from torch.autograd import forward_ad
 
 from dynamis_amd import _lib
 from dynamis_amd import dynamis_state as ds
+from oracle import operators as oracle
 
 pytestmark = pytest.mark.gpu
 TYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
@@ -112,3 +113,82 @@ def test_backward_passes_share_no_descriptor(cuda, monkeypatch):
         torch.autograd.grad(out, (q, k, v), grad, retain_graph=True)
     assert [ld for _, ld in seen] == [64, 16]
     assert [d.ld_g for d, _ in seen] == [64, 16]
+
+
+FLOATS = pytest.mark.parametrize("dtype", [torch.float32], ids=["f32"])
+
+
+# ---------------------------------------------------------------- infinities that are there to see
+
+
+def _infinite_case(heads, kv, dim, dtype, table, seed=0):
+    """Rows of 1 to 70 edges whose sources are all different; returns also, for some rows, an edge
+    in the row's middle and its last one."""
+    rng = np.random.default_rng(seed)
+    deg = np.concatenate([[1, 2, 31, 32, 33, 600, 5], rng.integers(1, 71, 30)])
+    n = 700
+    dst = np.repeat(rng.permutation(len(deg)), deg)
+    src = np.concatenate([rng.permutation(n)[:d] for d in deg])
+    g = torch.Generator().manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, generator=g).to(dtype)  # noqa: E731
+    c = {"q": rand(len(deg), heads, dim), "k": rand(n, kv, dim), "v": rand(n, kv, dim), "grad": rand(len(deg), heads, dim),
+         "table": None}
+    bucket = rng.integers(0, 6, len(src))
+    if table:
+        c["table"] = torch.randn(8, heads, generator=g)
+        if table == "unused":
+            c["table"][7] = -float("inf")  # no edge is in it
+        if table == "used":
+            c["table"][5] = -float("inf")
+    end = np.cumsum(deg)
+    at = np.concatenate([end[[1, 2, 5, 8]] - 1, (end - deg // 2 - 1)[[3, 5, 9]]])
+    return c, src, dst, bucket, at
+
+
+def _infinite_plan(c, src, dst, bucket):
+    """(buckets by distances)"""
+    return ds.neighbor_plan(torch.as_tensor(np.stack([src, dst])).cuda(), len(c["k"]), len(c["q"]),
+                            distances=torch.as_tensor(bucket + 0.5).cuda(), boundaries=np.arange(1.0, 8.0))
+
+
+def _same_kind(name, got, want):
+    """NaN where the definition has NaN, the same infinities, all else finite."""
+    got = got.detach().double().cpu().numpy()
+    for what, f in (("NaN", np.isnan), ("+inf", np.isposinf), ("-inf", np.isneginf)):
+        a, b = f(got), f(want)
+        assert (a == b).all(), f"{name}: {what} at {a.sum()} places, {b.sum()} are right, {(a & b).sum()} in both"
+
+
+LAYOUTS = pytest.mark.parametrize("layout", [(8, 8, 16), (4, 4, 16), (8, 2, 32), (6, 3, 24), (8, 1, 128), (1, 1, 8), (2, 2, 256)],
+                                  ids=str)
+
+
+@FLOATS
+@LAYOUTS
+@pytest.mark.parametrize("table", [None, "plain", "unused", "used"])
+def test_infinities_in_v_show_as_the_definition_has_them(cuda, layout, dtype, table):
+    """An infinity times a probability above zero is an infinity, whichever edge of a row holds it and
+    whatever the table's other entries are; two of opposite signs make a NaN.  The gradients have
+    their NaN and infinities where the formulas have them."""
+    print(f"\n[case] inf in v {layout} {dtype} {table}", flush=True)
+    c, src, dst, bucket, at = _infinite_case(*layout, dtype, table)
+    heads, kv, dim = layout
+    for i, e in enumerate(at):
+        c["v"][src[e], i % kv, i % dim] = (1 if i % 2 else -1) * float("inf")
+    c["v"][src[at[3]], 0, :] = float("nan")
+    plan = _infinite_plan(c, src, dst, bucket)
+    leaves = [c[x].cuda().requires_grad_(True) for x in ("q", "k", "v", "table") if c[x] is not None]
+    out = ds.neighbor_attention(*leaves[:3], plan, leaves[3] if table else None)
+    grads = torch.autograd.grad(out, leaves, c["grad"].cuda())
+    f = {x: None if c[x] is None else c[x].double().numpy() for x in c}
+    args = (f["q"], f["k"], f["v"], src, dst)
+    with np.errstate(invalid="ignore"):
+        want = oracle.attention(*args, bucket, f["table"])["out"]
+        gwant = oracle.attention_grads(*args, f["grad"], bucket, f["table"])[0]
+    assert np.isinf(want).any() and np.isnan(want).any() and np.isinf(gwant["dk"]).any()
+    _same_kind("out", out, want)
+    finite = np.isfinite(want)
+    tol = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -14  # (results of order one; finiteness is what is tested)
+    assert np.abs(out.detach().double().cpu().numpy() - want)[finite].max() < tol * max(1, np.abs(want[finite]).max())
+    for name, g in zip(("dq", "dk", "dv", "dtable"), grads):
+        _same_kind(name, g, gwant[name])
