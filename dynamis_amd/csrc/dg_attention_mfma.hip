@@ -15,7 +15,9 @@
 // forward pass adds a third part.
 //
 // The zeros of the block diagonal would spread a NaN or an infinity of one head of k over the
-// others (0 * inf): a row whose sums end in a NaN is done again with products formed head by head.
+// others (0 * inf), and a weight's parts, some of them zero or negative, make a NaN of an infinity in
+// v: a row whose sums are not finite is done again with products formed head by head, and with v's
+// infinities taken apart from its numbers.
 // Where the table holds entries of -inf, v of edges that these take out for all heads of the
 // group is zeroed; a row that meets values that are not finite and hidden from some heads only
 // is done again on the vector units.
@@ -300,6 +302,20 @@ __device__ __forceinline__ bf16x8 turned(const C (&v)[8], int i)
     return __builtin_bit_cast(bf16x8, r);
 }
 
+// Those of eight values that are infinite, the others as zeros (or, FINITE, the other way round).
+template <bool FINITE>
+__device__ __forceinline__ bf16x8 only(bf16x8 v)
+{
+    const u32x4 u = __builtin_bit_cast(u32x4, v);
+    u32x4 r;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+        const uint32_t mask = ((u[d] & 0x7fffu) == 0x7f80u ? 0xffffu : 0) | ((u[d] & 0x7fff0000u) == 0x7f800000u ? 0xffff0000u : 0);
+        r[d] = u[d] & (FINITE ? ~mask : mask);
+    }
+    return __builtin_bit_cast(bf16x8, r);
+}
+
 // Whether any of the values is a NaN or an infinity.
 template <typename C>
 __device__ __forceinline__ bool unbounded(C v)
@@ -386,6 +402,15 @@ __device__ __forceinline__ bf16x8 two_parts(const float (&p)[8], float minus)
     return r;
 }
 
+// One where a weight is not zero: what an infinity is to be multiplied with (and a NaN, as the weights are).
+__device__ __forceinline__ bf16x8 above_zero(const float (&p)[8])
+{
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (__bf16)(p[i] > 0.0f ? 1.0f : p[i]);
+    return r;
+}
+
 // What two_parts leave out, in columns 0 .. 7.  (That is 2^-18 of a weight at most; but the backward
 // pass takes <g, out> from the sums, which is summed over a bucket's edges where it cancels: with two
 // parts the table's gradient was 1.0e-6 off the 64-bit one, with three it is 2e-7.  27M edges of 8
@@ -399,6 +424,18 @@ __device__ __forceinline__ bf16x8 third_part(const float (&p)[8], bool first)
         r[i] = (__bf16)(first ? rest - (float)(__bf16)rest : 0.0f);
     }
     return r;
+}
+
+// Whether all sums of a lane are numbers.
+template <int NT>
+__device__ __forceinline__ bool finite(const f32x4 (&acc)[kV<NT>])
+{
+    float x = 0;
+#pragma unroll
+    for (int i = 0; i < kV<NT>; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x = fmaf(0.0f, acc[i][r], x);
+    return x == 0.0f;
 }
 
 // 32 entries of a row, one a lane: the node, with the bucket in the upper eight bits where nodes
@@ -667,16 +704,29 @@ __global__ __launch_bounds__(64 * kWaves, waves_of(NT)) void forward_mfma_kernel
                     keep_branch();
                     redo |= hide<NT>(l, s, v);
                 }
+                if constexpr (APART) {  // (lanes past the row's end hold its last edge)
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        if (edge_of(l, x) >= n) v[x] = VChunk<NT>{};
+                }
 #pragma unroll
                 for (int i = 0; i < kV<NT>; ++i) {
                     const bf16x8 vi = turned(v, i);
-                    acc[i] = mfma(vi, last, mfma(vi, weight, acc[i]));
+                    if constexpr (APART) {  // an infinity meets a weight that is whole
+                        const bf16x8 finite = only<true>(vi);
+                        acc[i] = mfma(finite, last, mfma(finite, weight, acc[i]));
+                        acc[i] = mfma(only<false>(vi), above_zero(pr), acc[i]);
+                    } else {
+                        acc[i] = mfma(vi, last, mfma(vi, weight, acc[i]));
+                    }
                 }
                 e0 += 32;
             } while (e0 < p.end);
         };
         row(std::false_type{});
-        if (__any(isnan(sum))) {
+        // (said to be rare: else what this branch needs spills registers of the loop, 962 us against 850 for
+        // 27M edges of 8 heads of 16)
+        if (__builtin_expect(__any(isnan(sum) || !finite<NT>(acc)), 0)) {
             keep_branch();
             block = block_at<BUCKETS, FAR>(a.L, p.begin, p.end);
             row(std::true_type{});

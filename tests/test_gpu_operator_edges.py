@@ -115,9 +115,6 @@ def test_backward_passes_share_no_descriptor(cuda, monkeypatch):
     assert [d.ld_g for d, _ in seen] == [64, 16]
 
 
-FLOATS = pytest.mark.parametrize("dtype", [torch.float32], ids=["f32"])
-
-
 # ---------------------------------------------------------------- infinities that are there to see
 
 
@@ -159,36 +156,57 @@ def _same_kind(name, got, want):
         assert (a == b).all(), f"{name}: {what} at {a.sum()} places, {b.sum()} are right, {(a & b).sum()} in both"
 
 
+FLOATS = pytest.mark.parametrize("dtype", [torch.float32], ids=["f32"])
 LAYOUTS = pytest.mark.parametrize("layout", [(8, 8, 16), (4, 4, 16), (8, 2, 32), (6, 3, 24), (8, 1, 128), (1, 1, 8), (2, 2, 256)],
                                   ids=str)
+TABLES = pytest.mark.parametrize("table", [None, "plain", "unused", "used"])
+
+
+def _infinite_v(layout, dtype, table):
+    """Inputs with infinities and a NaN in v, and what the kernels and the definitions make of them."""
+    c, src, dst, bucket, at = _infinite_case(*layout, dtype, table)
+    for i, e in enumerate(at):
+        c["v"][src[e], i % layout[1], i % layout[2]] = (1 if i % 2 else -1) * float("inf")
+    c["v"][src[at[3]], 0, :] = float("nan")
+    return c, src, dst, bucket, _run(c, src, dst, bucket)
+
+
+def _run(c, src, dst, bucket):
+    plan = _infinite_plan(c, src, dst, bucket)
+    leaves = [c[x].cuda().requires_grad_(True) for x in ("q", "k", "v", "table") if c[x] is not None]
+    out = ds.neighbor_attention(*leaves[:3], plan, leaves[3] if c["table"] is not None else None)
+    got = [out.detach(), *torch.autograd.grad(out, leaves, c["grad"].cuda())]
+    f = {x: None if c[x] is None else c[x].double().numpy() for x in c}
+    args = (f["q"], f["k"], f["v"], src, dst)
+    with np.errstate(invalid="ignore"):
+        want = {"out": oracle.attention(*args, bucket, f["table"])["out"],
+                **oracle.attention_grads(*args, f["grad"], bucket, f["table"])[0]}
+    return dict(zip(("out", "dq", "dk", "dv", "dtable"), got)), want
+
+
+@TYPES
+@LAYOUTS
+@TABLES
+def test_infinities_in_v_show_as_the_definition_has_them(cuda, layout, dtype, table):
+    """An infinity times a probability above zero is an infinity, whichever edge of a row holds it and
+    whatever the table's other entries are; two of opposite signs make a NaN."""
+    print(f"\n[case] inf in v {layout} {dtype} {table}", flush=True)
+    got, want = _infinite_v(layout, dtype, table)[-1]
+    assert np.isinf(want["out"]).any() and np.isnan(want["out"]).any()
+    _same_kind("out", got["out"], want["out"])
+    finite = np.isfinite(want["out"])
+    want, got = want["out"][finite], got["out"].double().cpu().numpy()[finite]
+    # (a rounding to bfloat16, or those of some hundreds of terms of order one; the kind is what is tested)
+    assert np.abs(got - want).max() < (2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -14) * max(1, np.abs(want).max())
 
 
 @FLOATS
 @LAYOUTS
-@pytest.mark.parametrize("table", [None, "plain", "unused", "used"])
-def test_infinities_in_v_show_as_the_definition_has_them(cuda, layout, dtype, table):
-    """An infinity times a probability above zero is an infinity, whichever edge of a row holds it and
-    whatever the table's other entries are; two of opposite signs make a NaN.  The gradients have
-    their NaN and infinities where the formulas have them."""
-    print(f"\n[case] inf in v {layout} {dtype} {table}", flush=True)
-    c, src, dst, bucket, at = _infinite_case(*layout, dtype, table)
-    heads, kv, dim = layout
-    for i, e in enumerate(at):
-        c["v"][src[e], i % kv, i % dim] = (1 if i % 2 else -1) * float("inf")
-    c["v"][src[at[3]], 0, :] = float("nan")
-    plan = _infinite_plan(c, src, dst, bucket)
-    leaves = [c[x].cuda().requires_grad_(True) for x in ("q", "k", "v", "table") if c[x] is not None]
-    out = ds.neighbor_attention(*leaves[:3], plan, leaves[3] if table else None)
-    grads = torch.autograd.grad(out, leaves, c["grad"].cuda())
-    f = {x: None if c[x] is None else c[x].double().numpy() for x in c}
-    args = (f["q"], f["k"], f["v"], src, dst)
-    with np.errstate(invalid="ignore"):
-        want = oracle.attention(*args, bucket, f["table"])["out"]
-        gwant = oracle.attention_grads(*args, f["grad"], bucket, f["table"])[0]
-    assert np.isinf(want).any() and np.isnan(want).any() and np.isinf(gwant["dk"]).any()
-    _same_kind("out", out, want)
-    finite = np.isfinite(want)
-    tol = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -14  # (results of order one; finiteness is what is tested)
-    assert np.abs(out.detach().double().cpu().numpy() - want)[finite].max() < tol * max(1, np.abs(want[finite]).max())
-    for name, g in zip(("dq", "dk", "dv", "dtable"), grads):
-        _same_kind(name, g, gwant[name])
+@TABLES
+def test_the_gradients_of_infinities_in_v(cuda, layout, dtype, table):
+    """The gradients have their NaN and infinities where the formulas have them."""
+    print(f"\n[case] gradients, inf in v {layout} {dtype} {table}", flush=True)
+    got, want = _infinite_v(layout, dtype, table)[-1]
+    assert np.isinf(want["dk"]).any() and np.isnan(want["dq"]).any()
+    for name in ("dq", "dk", "dv", "dtable")[:len(got) - 1]:
+        _same_kind(name, got[name], want[name])
