@@ -1173,8 +1173,36 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_kv(NT)) void backward_kv_mfma
                         redo |= hide<NT>(l, s, g);
                     }
                     const bf16x8 weight = two_parts(pr, l.n >= 8 ? -1.0f : 0.0f);
+                    if constexpr (APART) {  // infinities of g meet weights that are whole
 #pragma unroll
-                    for (int i = 0; i < kV<NT>; ++i) acc_v[i] = mfma(turned(g, i), weight, acc_v[i]);
+                        for (int x = 0; x < 8; ++x)
+                            if (edge_of(l, x) >= n) g[x] = VChunk<NT>{};
+                        const bf16x8 whole = above_zero(pr);
+#pragma unroll
+                        for (int i = 0; i < kV<NT>; ++i) {
+                            const bf16x8 gi = turned(g, i);
+                            acc_v[i] = mfma(only<true>(gi), weight, acc_v[i]);
+                            acc_v[i] = mfma(only<false>(gi), whole, acc_v[i]);
+                            __builtin_amdgcn_sched_barrier(0);  // (one at a time: few registers)
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kV<NT>; ++i) acc_v[i] = mfma(turned(g, i), weight, acc_v[i]);
+                    }
+                    if constexpr (APART) {  // those of ds have no parts
+                        bf16x8 vast;
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) {
+                            const bool is = isinf(ds[x]);
+                            vast[x] = (__bf16)(is ? ds[x] : 0.0f);
+                            ds[x] = is ? 0.0f : ds[x];
+                        }
+#pragma unroll
+                        for (int i = 0; i < kV<NT>; ++i) {
+                            acc_k[i] = mfma(turned(q, i), vast, acc_k[i]);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
                     const bf16x8 change = two_parts(ds, l.n >= 8 ? -1.0f : 0.0f);
 #pragma unroll
                     for (int i = 0; i < kV<NT>; ++i) acc_k[i] = mfma(turned(q, i), change, acc_k[i]);
@@ -1182,7 +1210,7 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_kv(NT)) void backward_kv_mfma
                 } while (e0 < p.end);
             };
             row(std::false_type{});
-            if (__any(odd != 0.0f)) {  // (a NaN)
+            if (__builtin_expect(__any(odd != 0.0f), 0)) {  // (a NaN)
                 keep_branch();
                 block = block_at<BUCKETS, FAR>(a.L, p.begin, p.end);
                 row(std::true_type{});

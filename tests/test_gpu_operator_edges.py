@@ -156,7 +156,6 @@ def _same_kind(name, got, want):
         assert (a == b).all(), f"{name}: {what} at {a.sum()} places, {b.sum()} are right, {(a & b).sum()} in both"
 
 
-FLOATS = pytest.mark.parametrize("dtype", [torch.float32], ids=["f32"])
 LAYOUTS = pytest.mark.parametrize("layout", [(8, 8, 16), (4, 4, 16), (8, 2, 32), (6, 3, 24), (8, 1, 128), (1, 1, 8), (2, 2, 256)],
                                   ids=str)
 TABLES = pytest.mark.parametrize("table", [None, "plain", "unused", "used"])
@@ -200,7 +199,7 @@ def test_infinities_in_v_show_as_the_definition_has_them(cuda, layout, dtype, ta
     assert np.abs(got - want).max() < (2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -14) * max(1, np.abs(want).max())
 
 
-@FLOATS
+@TYPES
 @LAYOUTS
 @TABLES
 def test_the_gradients_of_infinities_in_v(cuda, layout, dtype, table):
@@ -208,5 +207,19 @@ def test_the_gradients_of_infinities_in_v(cuda, layout, dtype, table):
     print(f"\n[case] gradients, inf in v {layout} {dtype} {table}", flush=True)
     got, want = _infinite_v(layout, dtype, table)[-1]
     assert np.isinf(want["dk"]).any() and np.isnan(want["dq"]).any()
+    for name in ("dq", "dk", "dv", "dtable")[:len(got) - 1]:
+        _same_kind(name, got[name], want[name])
+
+
+@TYPES
+@LAYOUTS
+@TABLES
+def test_infinities_in_the_gradient_show_as_the_formulas_have_them(cuda, layout, dtype, table):
+    print(f"\n[case] inf in the gradient {layout} {dtype} {table}", flush=True)
+    c, src, dst, bucket, at = _infinite_case(*layout, dtype, table, seed=1)
+    for i, e in enumerate(at):
+        c["grad"][dst[e], i % layout[0], i % layout[2]] = (1 if i % 2 else -1) * float("inf")
+    got, want = _run(c, src, dst, bucket)
+    assert np.isinf(want["dv"]).any()
     for name in ("dq", "dk", "dv", "dtable")[:len(got) - 1]:
         _same_kind(name, got[name], want[name])
