@@ -223,3 +223,28 @@ def test_infinities_in_the_gradient_show_as_the_formulas_have_them(cuda, layout,
     assert np.isinf(want["dv"]).any()
     for name in ("dq", "dk", "dv", "dtable")[:len(got) - 1]:
         _same_kind(name, got[name], want[name])
+
+
+# ---------------------------------------------------------------- as many workgroups as there may be
+
+
+def test_weight_gradients_of_more_than_2_to_the_32_threads(cuda):
+    """4,097 groups of 4,096 tiles of the weight's gradient, a workgroup each."""
+    groups, k, sizes = 4097, 4096 * 128, {3: 2, 4000: 1, 4096: 2}
+    print("\n[case] weights of 4.3 GB", flush=True)
+    at = torch.zeros(groups, dtype=torch.long)
+    for g, n in sizes.items():
+        at[g] = n
+    x = torch.randn(5, k, device="cuda").bfloat16()
+    w = torch.zeros(1, device="cuda", dtype=torch.bfloat16).expand(groups, 1, k).contiguous().requires_grad_(True)
+    b = torch.zeros(groups, 1, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    grad = torch.tensor([[1.0], [2.0], [-1.0], [0.5], [4.0]], device="cuda").bfloat16()
+    dw, db = torch.autograd.grad(ds.grouped_linear(x, w, at.cuda(), b), (w, b), grad)
+    f = x.double()
+    want = {3: f[0] + 2 * f[1], 4000: -f[2], 4096: 0.5 * f[3] + 4 * f[4]}
+    for g, y in want.items():
+        # (products by powers of two and one sum in 32 bits: the result's rounding to bfloat16, and what it moves)
+        assert ((dw[g, 0].double() - y).abs() <= 2.0 ** -8 * y.abs() + 2.0 ** -22 * f.abs().max() * 4).all(), g
+        dw[g] = 0
+    assert db[:, 0].nonzero()[:, 0].tolist() == [3, 4000, 4096] and db[[3, 4000, 4096], 0].tolist() == [3.0, -1.0, 4.5]
+    assert not any(part.any() for part in dw.split(512))
