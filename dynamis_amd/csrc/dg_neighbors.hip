@@ -325,7 +325,7 @@ __global__ void parts_kernel(const int32_t* __restrict__ ptr, int64_t n, int spl
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
     const int len = ptr[i + 1] - ptr[i];
-    parts[i] = len > split ? (len + chunk - 1) / chunk : 0;
+    parts[i] = len > split ? (len - 1) / chunk + 1 : 0;  // (len may be near 2^31)
     is_long[i] = len > split;
 }
 
@@ -344,8 +344,8 @@ __global__ void items_kernel(const int32_t* __restrict__ first, const int32_t* _
     if (i < max_items && i >= first[n]) item[i] = make_int4(0, 0, -1, 0);  // (the bound is not reached)
     if (i >= n) return;
     for (int64_t k = first[i]; k < first[i + 1] && k < max_items; ++k) {
-        const int at = ptr[i] + (int)(k - first[i]) * chunk;
-        item[k] = make_int4(at, min(at + chunk, ptr[i + 1]), order[i], (int)i);
+        const int at = ptr[i] + (int)(k - first[i]) * chunk;  // (below the row's end; at + chunk may pass 2^31)
+        item[k] = make_int4(at, at + min(chunk, ptr[i + 1] - at), order[i], (int)i);
     }
 }
 

@@ -248,3 +248,35 @@ def test_weight_gradients_of_more_than_2_to_the_32_threads(cuda):
         dw[g] = 0
     assert db[:, 0].nonzero()[:, 0].tolist() == [3, 4000, 4096] and db[[3, 4000, 4096], 0].tolist() == [3.0, -1.0, 4.5]
     assert not any(part.any() for part in dw.split(512))
+
+
+# ---------------------------------------------------------------- lists near 2^31 entries
+
+
+@pytest.mark.parametrize("chunk", [2048, 4096])
+def test_parts_of_a_row_that_ends_near_2_to_the_31(cuda, chunk):
+    """The parts of rows are made from the pointers alone: one row of two up to the last entry that a
+    list may hold."""
+    print(f"\n[case] parts near 2^31, {chunk}", flush=True)
+    end, start = 2 ** 31 - 256, 1000
+    ptr = torch.tensor([0, start, end], dtype=torch.int32, device="cuda")
+    order = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    parts = [-(-n // chunk) for n in (start, end - start)]
+    n_items = end // chunk + 2
+    new = lambda *n: torch.empty(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    first, items, slots = new(3), new(n_items, 4), new(2)
+    lib = _lib.lib()
+    size = lib.dg_neighbors_parts_workspace_size(2)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    _lib.check(lib.dg_neighbors_parts(_lib.ptr(order), _lib.ptr(ptr), 2, chunk, n_items, 2, _lib.ptr(first), _lib.ptr(items),
+                                      _lib.ptr(slots), _lib.ptr(ws), size, _lib.stream_of(ptr.device)), "parts")
+    assert first.tolist() == [0, parts[0], sum(parts)] and slots.tolist() == [0, 1]
+    items = items.cpu().long()
+    rest = items[sum(parts):]
+    assert (rest[:, :2] == 0).all() and (rest[:, 2] == -1).all()
+    items = items[:sum(parts)]
+    at = torch.cat([torch.arange(0, start, chunk), torch.arange(start, end, chunk)])
+    slot = torch.repeat_interleave(torch.arange(2), torch.tensor(parts))
+    assert torch.equal(items[:, 0], at)
+    assert torch.equal(items[:, 1], torch.minimum(at + chunk, torch.tensor([start, end])[slot]))
+    assert torch.equal(items[:, 2], 1 - slot) and torch.equal(items[:, 3], slot)
