@@ -29,6 +29,7 @@
 #include "../../include/dynamis_graph.h"
 #include "dg_attention.hpp"
 #include "dg_attention_mfma.hpp"
+#include "dg_grid.hpp"
 
 namespace {
 
@@ -212,7 +213,8 @@ __device__ __forceinline__ float strand_sum(float x)
 template <typename T, int STRANDS>
 __global__ __launch_bounds__(16 * STRANDS) void forward_join_kernel(AttnArgs a, int slices)
 {
-    const int slot = a.L.long_slot[blockIdx.x / slices], slice = (int)(blockIdx.x % slices);
+    const int64_t unit = workgroup(), rank = unit / slices;
+    const int slot = rank < a.L.n_long ? a.L.long_slot[rank] : -1, slice = (int)(unit % slices);
     if (slot < 0) return;  // (fewer long rows than said)
     const int first = a.L.item_first[slot], n = a.L.item_first[slot + 1] - first, node = a.L.order[slot];
     constexpr int kJoinWaves = STRANDS / 4;
@@ -456,7 +458,8 @@ template <typename T, int STRANDS>
 __global__ __launch_bounds__(16 * STRANDS) void sum_join_kernel(Lists L, const float* __restrict__ part, int wide,
                                                                  int slices, float factor, T* __restrict__ out)
 {
-    const int slot = L.long_slot[blockIdx.x / slices], slice = (int)(blockIdx.x % slices);
+    const int64_t unit = workgroup(), rank = unit / slices;
+    const int slot = rank < L.n_long ? L.long_slot[rank] : -1, slice = (int)(unit % slices);
     if (slot < 0) return;
     const int first = L.item_first[slot], n = L.item_first[slot + 1] - first, node = L.order[slot];
     constexpr int kJoinWaves = STRANDS / 4;
@@ -671,7 +674,7 @@ void run_forward(const AttnArgs& a, hipStream_t s)
     if (a.L.n_items > 0) {
         const int slices = (a.heads * a.dim + 63) / 64;
         by_parts(a.L, [&](auto strands) {
-            hipLaunchKernelGGL((forward_join_kernel<T, strands()>), dim3((unsigned)(a.L.n_long * slices)),
+            hipLaunchKernelGGL((forward_join_kernel<T, strands()>), workgroups(a.L.n_long * slices),
                                dim3(16 * strands()), 0, s, a, slices);
         });
     }
@@ -704,7 +707,7 @@ void run_backward(AttnArgs a, const Lists& by_target, const Lists& by_source, fl
     if (a.L.n_items > 0) {
         const int wide = a.heads * a.dim, slices = (wide + 63) / 64;
         by_parts(a.L, [&](auto strands) {
-            hipLaunchKernelGGL((sum_join_kernel<T, strands()>), dim3((unsigned)(a.L.n_long * slices)),
+            hipLaunchKernelGGL((sum_join_kernel<T, strands()>), workgroups(a.L.n_long * slices),
                                dim3(16 * strands()), 0, s, a.L, (const float*)a.part_acc, wide, slices, a.scale,
                                (T*)a.dq);
         });
@@ -722,7 +725,7 @@ void run_backward(AttnArgs a, const Lists& by_target, const Lists& by_source, fl
     if (a.L.n_items > 0) {
         const int wide = a.kv_heads * a.dim, slices = (wide + 63) / 64;
         by_parts(a.L, [&](auto strands) {
-            const dim3 grid((unsigned)(a.L.n_long * slices)), block(16 * strands());
+            const dim3 grid = workgroups(a.L.n_long * slices), block(16 * strands());
             hipLaunchKernelGGL((sum_join_kernel<T, strands()>), grid, block, 0, s, a.L, (const float*)a.part_acc, wide,
                                slices, a.scale, (T*)a.dk);
             hipLaunchKernelGGL((sum_join_kernel<T, strands()>), grid, block, 0, s, a.L, (const float*)a.part_acc2, wide,

@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "../../include/dynamis_graph.h"
+#include "dg_grid.hpp"
 
 namespace dg {
 dg_status fail(dg_status st, const std::string& msg);  // dg_graph.hip
@@ -639,7 +640,7 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(Args a, int64_t max_item
     constexpr int C = kChunk<T>;
     const Cuts cuts{a.chunk, 1};
     const int n_tiles = (a.cols + kTile - 1) / kTile, k_tiles = (a.depth + kTile - 1) / kTile;
-    const int64_t at = xcd_order((int64_t)blockIdx.y * gridDim.x + blockIdx.x, (int64_t)gridDim.y * gridDim.x);
+    const int64_t at = xcd_order(workgroup(), (int64_t)gridDim.y * gridDim.x);
     const int64_t item = at / (n_tiles * k_tiles);
     int64_t items, covered;
     pass<4>(a, cuts, s_w, &s_p, items, covered,
@@ -865,10 +866,7 @@ void run_weight(const Args& a, hipStream_t s)
     const int64_t items = a.rows / a.chunk + a.groups;
     int64_t grid = items * tiles;
     if (grid > kXcds) grid = (grid + kXcds - 1) / kXcds * kXcds;
-    // (a launch holds less than 2^32 threads along an axis: many groups of wide, flat weights have more)
-    const int64_t across = std::min<int64_t>(grid, 1 << 20);
-    hipLaunchKernelGGL(weight_kernel<T>, dim3((unsigned)across, (unsigned)((grid + across - 1) / across)), dim3(256), 0, s, a,
-                       items);
+    hipLaunchKernelGGL(weight_kernel<T>, workgroups(grid), dim3(256), 0, s, a, items);
     const int64_t split = std::min(a.groups, a.rows / a.chunk);  // groups above an item, at most
     if (split > 0) {
         // (most of a large number find no group: one round of workgroups, each with more to do)

@@ -250,6 +250,29 @@ def test_weight_gradients_of_more_than_2_to_the_32_threads(cuda):
     assert not any(part.any() for part in dw.split(512))
 
 
+def test_joins_of_more_than_2_to_the_32_threads(cuda):
+    """Lists that say 2^26 + 2 long rows, of which the last is there: a workgroup of 64 threads each."""
+    print("\n[case] joins of 2^26 rows", flush=True)
+    n, entries, said = 700, 600, 2 ** 26 + 2
+    plan = ds.neighbor_plan(torch.stack([torch.arange(entries), torch.zeros(entries, dtype=torch.long)]).cuda(), n, 1)
+    q, k, v = (torch.randn(m, 1, 8, device="cuda", requires_grad=True) for m in (1, n, n))
+    grad = torch.randn(1, 1, 8, device="cuda")
+
+    def step():
+        out, lse = ds.neighbor_attention(q, k, v, plan, return_lse=True)
+        return [out, lse, *torch.autograd.grad(out, (q, k, v), grad)]
+
+    want = step()
+    rows = plan.by_target
+    assert rows.c.n_long == 1 and rows.c.n_items > 1
+    slots = torch.full((said,), -1, dtype=torch.int32, device="cuda")
+    slots[-1:] = rows.long_slot
+    rows.c.long_slot, rows.c.n_long = slots.data_ptr(), said
+    _leave_nans([1, 8])
+    got = step()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---------------------------------------------------------------- lists near 2^31 entries
 
 
