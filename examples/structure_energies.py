@@ -37,7 +37,7 @@ def make_batch(structures, atoms, seed=0, device="cuda"):
     natoms = torch.randint(max(2, atoms // 2), atoms + 1, (structures,), generator=g)
     pos, cells = [], []
     for n in natoms.tolist():
-        side = int(round(n ** (1 / 3) + 0.49))
+        side = next(s for s in range(1, n + 1) if s ** 3 >= n)
         a = (10.0 * n) ** (1 / 3) / side
         at = torch.randperm(side ** 3, generator=g)[:n]
         grid = torch.stack([at // (side * side), at // side % side, at % side], 1)
