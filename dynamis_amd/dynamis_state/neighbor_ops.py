@@ -107,6 +107,7 @@ def neighbor_plan(edge_index, num_nodes, num_targets=None, distances=None, bound
     _check(0 <= num_targets <= num_nodes, f"num_targets must be in [0, num_nodes], got {num_targets}")
     n_bounds = 0
     if distances is not None:
+        _check(isinstance(distances, torch.Tensor), "distances must be a tensor")
         _check(distances.device == dev and distances.dim() == 1 and distances.size(0) == E,
                f"distances must have shape [{E}] on {dev}, got {_shape(distances)} on {distances.device}")
         _check(distances.dtype in (torch.float32, torch.float64),
@@ -120,6 +121,7 @@ def neighbor_plan(edge_index, num_nodes, num_targets=None, distances=None, bound
     else:
         _check(boundaries is None, "boundaries come with distances")
     if edge_mask is not None:
+        _check(isinstance(edge_mask, torch.Tensor), "edge_mask must be a tensor")
         _check(edge_mask.device == dev and edge_mask.dtype == torch.bool and edge_mask.dim() == 1
                and edge_mask.size(0) == E, f"edge_mask must be bool [{E}] on {dev}")
         edge_mask = edge_mask.contiguous()
@@ -273,6 +275,7 @@ def _refuse_tangents(name, *tensors):
 
 def _check_attention(q, k, v, plan, bias_table):
     """The refusals of neighbor_attention, with their messages."""
+    _check(isinstance(plan, NeighborPlan), "plan must be a NeighborPlan")
     for name, t in (("q", q), ("k", k), ("v", v)):
         _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
         _check(t.dim() == 3, f"{name} must have shape [nodes, heads, dim], got {_shape(t)}")
@@ -288,6 +291,7 @@ def _check_attention(q, k, v, plan, bias_table):
     _check(heads <= 1024, f"at most 1024 heads, got {heads}")
     _check(8 <= dim <= 256 and dim % 8 == 0, f"the head width must be a multiple of 8, 8 to 256, got {dim}")
     if bias_table is not None:
+        _check(isinstance(bias_table, torch.Tensor), "bias_table must be a tensor")
         _check(plan.num_buckets > 0, "bias_table needs a plan with distances")
         _check(bias_table.device == plan.device and bias_table.is_floating_point()
                and tuple(bias_table.shape) == (plan.num_buckets, heads),
@@ -297,7 +301,8 @@ def _check_attention(q, k, v, plan, bias_table):
 
 def _attention_is_fine(q, k, v, plan, bias_table):
     """Whether _check_attention would pass, without its messages' host time."""
-    if not (type(q) in _TENSORS and type(k) in _TENSORS and type(v) in _TENSORS and q.dim() == 3 and k.dim() == 3):
+    if not (type(q) in _TENSORS and type(k) in _TENSORS and type(v) in _TENSORS and q.dim() == 3 and k.dim() == 3
+            and type(plan) is NeighborPlan and (bias_table is None or type(bias_table) in _TENSORS)):
         return False
     (targets, heads, dim), (nodes, kv, kdim) = q.shape, k.shape
     dtype, dev = q.dtype, plan.device
@@ -412,13 +417,15 @@ def _check_grouped(x, weight, sizes, bias):
         _check(bool((sizes >= 0).all()) and int(sizes.sum()) == x.size(0),
                f"sizes must be non-negative and add up to {x.size(0)} rows")
     if bias is not None:
+        _check(isinstance(bias, torch.Tensor), "bias must be a tensor")
         _check(bias.device == x.device and bias.dtype == x.dtype and tuple(bias.shape) == tuple(weight.shape[:2]),
                f"bias must be {x.dtype} [{groups}, {weight.size(1)}] on {x.device}, got {bias.dtype} {_shape(bias)}")
 
 
 def _grouped_is_fine(x, weight, sizes, bias):
     """Whether _check_grouped would pass for tensors on one device, without its messages' host time."""
-    if not (type(x) in _TENSORS and type(weight) in _TENSORS and x.dim() == 2 and weight.dim() == 3 and x.is_cuda):
+    if not (type(x) in _TENSORS and type(weight) in _TENSORS and x.dim() == 2 and weight.dim() == 3 and x.is_cuda
+            and (bias is None or type(bias) in _TENSORS)):
         return False
     groups, n, k = weight.shape
     dev, dtype = x.device, x.dtype

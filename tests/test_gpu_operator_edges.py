@@ -303,3 +303,23 @@ def test_parts_of_a_row_that_ends_near_2_to_the_31(cuda, chunk):
     assert torch.equal(items[:, 0], at)
     assert torch.equal(items[:, 1], torch.minimum(at + chunk, torch.tensor([start, end])[slot]))
     assert torch.equal(items[:, 2], 1 - slot) and torch.equal(items[:, 3], slot)
+
+
+# ---------------------------------------------------------------- arguments that are no tensors
+
+
+def test_refusals_of_what_is_no_tensor(cuda):
+    ei = torch.tensor([[0, 1, 2], [0, 0, 1]], device="cuda")
+    one = torch.ones(3, device="cuda")
+    bad = lambda match, f, *a, **k: pytest.raises(RuntimeError, f, *a, **k).match(match)  # noqa: E731
+    bad("distances must be a tensor", ds.neighbor_plan, ei, 4, distances=[1.0, 1.0, 1.0], boundaries=[1.0])
+    bad("edge_mask must be a tensor", ds.neighbor_plan, ei, 4, edge_mask=[True, True, False])
+    plan = ds.neighbor_plan(ei, 4, distances=one, boundaries=[1.0])
+    q = torch.zeros(4, 2, 8, device="cuda")
+    bad("plan must be a NeighborPlan", ds.neighbor_attention, q, q, q, None)
+    bad("plan must be a NeighborPlan", ds.neighbor_attention, q, q, q, ei)
+    bad("bias_table must be a tensor", ds.neighbor_attention, q, q, q, plan, [[0.0, 0.0], [0.0, 0.0]])
+    bad("k must be a CUDA tensor", ds.neighbor_attention, q, None, q, plan)
+    x, w = torch.zeros(3, 8, device="cuda"), torch.zeros(1, 4, 8, device="cuda")
+    bad("bias must be a tensor", ds.grouped_linear, x, w, [3], [[0.0] * 4])
+    bad("weight must be on", ds.grouped_linear, x, None, [3])
