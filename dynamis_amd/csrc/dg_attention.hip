@@ -503,6 +503,8 @@ __global__ __launch_bounds__(1024) void table_join_kernel(const float* __restric
 }
 
 // ---------------------------------------------------------------- host
+constexpr int64_t kMaxNodes = 0x7fffff00LL;  // as of the lists
+
 // Lanes of a head: a lane's four channels, rounded up to a power of two.
 int lanes_per_head(int dim)
 {
@@ -549,6 +551,7 @@ dg_status check(const dg_attention_desc* d)
     if (!d) return fail(DG_ERR_INVALID, "desc is NULL");
     if (d->dtype != DG_F32 && d->dtype != DG_BF16)
         return fail(DG_ERR_INVALID, "q, k and v must be float32 or bfloat16");
+    if (d->n_nodes < 0 || d->n_nodes > kMaxNodes) return fail(DG_ERR_INVALID, "n_nodes must be in [0, 2^31 - 256]");
     if (d->n_targets < 0 || d->n_nodes < d->n_targets)
         return fail(DG_ERR_INVALID, "n_targets must be in [0, n_nodes]");
     if (d->heads < 1 || d->kv_heads < 1 || d->heads % d->kv_heads || d->heads > 1024)
@@ -560,7 +563,8 @@ dg_status check(const dg_attention_desc* d)
     const int64_t a = d->dtype == DG_F32 ? 4 : 8;  // rows start at 16 bytes
     const int64_t ld[4] = {d->ld_q, d->ld_k, d->ld_v, d->ld_g};
     for (int64_t x : ld)
-        if (x % a || x < 0) return fail(DG_ERR_INVALID, "row strides must be multiples of 16 bytes");
+        if (x % a || x < 0 || x > (1ll << 60) / (d->n_nodes + 1))  // (offsets in bytes stay below 2^63)
+            return fail(DG_ERR_INVALID, "row strides must be multiples of 16 bytes, and all rows below 2^60 elements");
     if (!isfinite(d->scale)) return fail(DG_ERR_INVALID, "scale must be finite");
     return DG_OK;
 }
@@ -571,6 +575,8 @@ dg_status check_lists(const dg_attention_desc* d, const dg_neighbor_lists* l)
     if (l->n_rows != d->n_nodes) return fail(DG_ERR_INVALID, "the lists are of another number of nodes");
     if (l->n_rows > 0 && (!l->order || !l->ptr || !l->idx)) return fail(DG_ERR_INVALID, "lists are NULL");
     if (d->n_buckets > 0 && !l->bucket) return fail(DG_ERR_INVALID, "a table, but the lists hold no buckets");
+    if (l->n_items > kMaxNodes || l->n_long > kMaxNodes)
+        return fail(DG_ERR_INVALID, "lists hold less than 2^31 parts");
     if (l->n_items < 0 || (l->n_items > 0 && (!l->items || !l->item_first || !l->long_slot || l->n_long < 1)))
         return fail(DG_ERR_INVALID, "the parts of long rows are NULL");
     return DG_OK;
