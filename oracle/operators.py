@@ -65,8 +65,9 @@ def attention_grads(q, k, v, src, dst, grad, bucket=None, table=None, scale=None
         return np.where(there[..., None], s[..., None] * x, 0)
 
     g, m = {}, {}
-    g["dq"], m["dq"] = (_rows_sum(T, dst, terms(s, x)) * scale for s, x in ((ds, ke), (mag, np.abs(ke))))
-    g["dk"], m["dk"] = (_rows_sum(N, src, by_kv(terms(s, x))) * scale for s, x in ((ds, q[dst]), (mag, np.abs(q[dst]))))
+    g["dq"], m["dq"] = (_rows_sum(T, dst, terms(s, x)) * f for s, x, f in ((ds, ke, scale), (mag, np.abs(ke), abs(scale))))
+    g["dk"], m["dk"] = (_rows_sum(N, src, by_kv(terms(s, x))) * f
+                        for s, x, f in ((ds, q[dst], scale), (mag, np.abs(q[dst]), abs(scale))))
     g["dv"], m["dv"] = (_rows_sum(N, src, by_kv(terms(f["p"], x))) for x in (grad[dst], np.abs(grad[dst])))
     if table is not None:
         g["dtable"], m["dtable"] = (_rows_sum(len(table), bucket, s) for s in (ds, mag))
