@@ -15,7 +15,8 @@
 //
 // Bound by the vector units' instructions (a logit of 32 channels is four multiply-adds and three
 // exchanges a lane, of which half the lanes' work is the reduction's) next to the gathered rows:
-// 670,000 edges of 4 heads of 32 floats take 29 us, 24 TB/s of rows out of the caches.  Few rows are
+// 360,000 edges of 4 heads of 32 floats take 29 us, 13 TB/s of rows out of the caches, at 65 % of the
+// vector units; 26.5M edges of 8 heads of 16 1630 us, 17 TB/s.  Few rows are
 // bound by the wait for a row's loads in turn: 864 rows of 86 edges take 18 us forward, 21 us by
 // target and 20 us by source.
 #include <hip/hip_runtime.h>
@@ -665,7 +666,7 @@ void by_parts(const Lists& L, F&& f)
 template <typename T>
 void run_forward(const AttnArgs& a, hipStream_t s)
 {
-    // (bfloat16 on the matrix units: 27M edges of 8 heads of 16 take 887 us there, 2016 us here; the
+    // (bfloat16 on the matrix units: 26.5M edges of 8 heads of 16 take 840 us there, 2016 us here; the
     // registers of a wave hold heads of up to kMfmaDim channels)
     if (sizeof(T) == 2 && a.dim <= kMfmaDim) {
         forward_mfma(a, s);

@@ -620,7 +620,8 @@ __device__ __forceinline__ void logits(const AttnArgs& a, const Lane& l, const S
 // for.  (2.9M edges, 8 heads of 32: 200 us with 2, 183 with 3, 378 with 4, which spills; 4 heads of
 // 16: 75 us with 3, 70 with 4, 83 with 5.)  What bounds it there: the gathered rows, 64 bytes a clock
 // and CU into registers (80 us), the vector units' instructions (90 us), and the wait for one step's
-// rows, of which a wave has no more than one under way: 27M edges of 8 heads of 16 take 887 us.
+// rows, of which a wave has no more than one under way: 26.5M edges of 8 heads of 16 take 840 us, at 63 %
+// of the vector units' cycles and 58 % of the L1's.
 constexpr int waves_of(int NT) { return NT == 2 ? 3 : 4; }
 
 template <int NT, bool BUCKETS, bool FAR>
@@ -824,9 +825,9 @@ __device__ void backward_q_apart(const AttnArgs& a, const Piece& p, int h0, int 
 // dq, stats, and with BT > 0 the table's gradient: its sums over the edges of a bucket are products
 // with the buckets' indicators, 16 buckets by 4 edges a step in full float (one bit of each
 // indicator is set, so every term is exact), and stay in BT accumulators for all of a wave's rows.
-// What is not finite would meet the indicators' zeros: it goes to LDS by itself.  2.9M edges of 8
-// heads of 32, 32 buckets: 364 us, half of the vector units' time and a wait for rows as in the
-// forward pass; 7.3M edges of 8 heads over 2: 359 us.
+// What is not finite would meet the indicators' zeros: it goes to LDS by itself.  3.0M edges of 8
+// heads of 32, 32 buckets: 348 us, at 38 % of the vector units and 33 % of the L1's cycles, waiting for
+// rows as in the forward pass; 7.8M edges of 8 heads over 2: 341 us.
 template <int NT, int BT, bool FAR>
 __global__ __launch_bounds__(64 * kWaves, waves_of_q(NT)) void backward_q_mfma_kernel(AttnArgs a, HeadGroups hg)
 {
@@ -989,8 +990,9 @@ __global__ __launch_bounds__(64 * kWaves, waves_of_q(NT)) void backward_q_mfma_k
 
 // ---------------------------------------------------------------- backward, by source
 // Bound as the pass by target, with q's and g's rows for k's and v's and 16 bytes of statistics for
-// each edge and head: of shared heads as many rows as q has.  2.9M edges of 8 heads of 32: 362 us, at
-// 44 % of the vector units and 39 % of the cache's accesses; 7.3M edges of 8 heads over 2: 1061 us.
+// each edge and head: of shared heads as many rows as q has.  3.0M edges of 8 heads of 32: 336 us, at
+// 48 % of the vector units and 42 % of the L1's cycles; 7.8M edges of 8 heads over 2: 973 us, at 48 % and
+// 45 %.  (These times are a profile's, which are the longer ones.)
 // (waves: the whole backward pass, 8 heads of 32: 733 us with 1, 601 with 2, 1518 with 3; 4 heads of
 // 16: 233 us with 2, 222 with 3, 398 with 4)
 constexpr int waves_of_kv(int NT) { return NT == 2 ? 2 : 3; }

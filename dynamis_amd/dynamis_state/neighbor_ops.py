@@ -10,6 +10,9 @@ No counterpart in the reference, whose force models bring their own layers.  The
 those of libdynamis_graph.so (dg_neighbors_*, dg_attention_*, dg_grouped_*); there is no CPU
 path.  Everything runs on the current stream; tensors follow torch's rules for streams, and a
 plan made on one stream may be read on another once the caller has ordered the two.
+
+Distances enter by their buckets alone, so positions get no gradient through these operators: forces
+as the derivative of an energy need a term that depends on them smoothly beside it.
 """
 from __future__ import annotations
 
@@ -95,7 +98,12 @@ def neighbor_plan(edge_index, num_nodes, num_targets=None, distances=None, bound
     distances [E] with boundaries [B - 1], ascending and of the same type, put an edge into
     bucket #{boundaries <= distance} of B <= 128.  edge_mask [E] bool leaves edges out (a list
     with a skin, cut to the radius).  backward=False leaves out the lists that only gradients
-    need.  One host synchronisation; E < 2^31 - 256.
+    need.  E <= 2^31 - 256.
+
+    A plan costs as much as several calls and more (864 atoms, 74,000 edges: 115 us; 300,000 atoms, 26.5M
+    edges: 0.47 ms, and 2.2 ms with lists by source that are not those by target).  It synchronises the
+    host once; once more where the lists by source have to be sorted, which a mask or boundaries that
+    part an edge from its opposite bring about; and once more where the edges have to be sorted.
     """
     _check(isinstance(edge_index, torch.Tensor) and edge_index.is_cuda, "edge_index must be a CUDA tensor")
     _check(edge_index.dim() == 2 and edge_index.size(0) == 2,
@@ -332,8 +340,10 @@ def neighbor_attention(q, k, v, plan, bias_table=None, scale=None, return_lse=Fa
     log-sum of -inf).  Returns out like q, and with return_lse also the natural log-sums
     [num_targets, heads] in float32 (not differentiable).
 
+    What is not finite shows in the head that reads it and in no other, as the formulas have it.
+
     Differentiable in q, k, v and bias_table (once, in reverse: a tensor with a forward-mode tangent
-    is refused).  All sums are float32, in a fixed order:
+    is refused); all four gradients are formed, whichever are asked for.  All sums are float32, in a fixed order:
     results repeat bit for bit.
     """
     if forward_ad._current_level >= 0:  # (unpack_dual itself takes half a microsecond a tensor)
@@ -443,7 +453,9 @@ def grouped_linear(x, weight, sizes, bias=None):
     group 0's, the next sizes[1] group 1's and so on -- ``num_neighbors_image`` for rows per edge
     of a batch, its ``natoms`` for rows per atom.  On the device (no synchronisation) rows behind
     the last group give zeros and sizes are not checked otherwise; on the host, or as a list, they
-    have to be non-negative and to add up to the rows.  Groups may be empty.
+    have to be non-negative and to add up to the rows.  Groups may be empty.  The weight's gradient reads
+    all sizes once for each group and 128 x 128 of its weight: its time grows with the square of
+    the groups (of one such tile: 4,096 groups 0.26 ms, 65,536 groups 45 ms).
 
     Differentiable in x, weight and bias (once, in reverse: a tensor with a forward-mode tangent is
     refused).  Sums are float32, in a fixed order: results

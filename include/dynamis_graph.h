@@ -364,6 +364,7 @@ dg_status dg_halo_write(const dg_halo_desc* desc, const void* pid, int64_t* send
  *   ptr    out int32 [n_nodes + 1]  a slot's entries
  *   idx    out int32 [n_edges + DG_NEIGHBOR_PAD]  sources (by target) or targets (by source)
  *   bucket out uint8 [n_edges + DG_NEIGHBOR_PAD] or NULL
+ * The entries end in DG_NEIGHBOR_PAD zeros (a row of an empty list reads the first of them).
  * dg_neighbors_by_target (asynchronous; by_source != 0: prepares dg_neighbors_by_source), then
  * dg_neighbors_read_totals (synchronous: DG_ERR_RANGE for an index out of range).  With
  * `symmetric` set, the lists by source are the lists by target; otherwise
@@ -377,8 +378,8 @@ dg_status dg_halo_write(const dg_halo_desc* desc, const void* pid, int64_t* send
  * entries 61 and 56 us.) */
 #define DG_NEIGHBOR_SPLIT 512
 typedef struct dg_neighbor_desc {
-    int64_t n_edges;   /* < 2^31 - 256 */
-    int64_t n_nodes;
+    int64_t n_edges;   /* <= 2^31 - 256 */
+    int64_t n_nodes;   /* <= 2^31 - 256 */
     int64_t n_targets; /* targets are the nodes [0, n_targets) */
     int32_t n_boundaries; /* <= 127 */
     int32_t dist_dtype;   /* DG_F32 / DG_F64 */
@@ -439,10 +440,12 @@ dg_status dg_neighbors_parts(const int32_t* order, const int32_t* ptr, int64_t n
  * head, whatever q, k and v hold there.
  *   q [n_targets, heads, dim], k, v [n_nodes, kv_heads, dim] of dtype (DG_F32 / DG_BF16), rows
  *   ld_* elements apart, aligned to 16 bytes as their rows are; dim a multiple of 8, 8 .. 256
- *   table  float32 [n_buckets, heads], n_buckets <= 128, n_buckets * heads <= 4096
+ *   table  float32 [n_buckets, heads], n_buckets <= 128, n_buckets * heads <= 4096; the lists' buckets
+ *          have to be below n_buckets
  *   out    [n_targets, heads, dim] of dtype;  out32 the same in float32 before its rounding
- *          and norm float32 [n_targets, heads, 2] (the maximum of a row's base-2 logits and one
- *          over the sum of their powers): what the backward pass takes, or NULL
+ *          and norm float32 [n_targets, heads, 2] (a row's reference m, which is the maximum of its
+ *          base-2 logits or up to 8 below it, and one over the sum of the powers of 2 above m): what
+ *          the backward pass takes, or NULL
  *   lse    float32 [n_targets, heads], natural, or NULL
  * Backward: dq, dk, dv of dtype and contiguous, dtable float32.  Sums are float32 and in a
  * fixed order: results repeat bit for bit.  The workspace of
@@ -482,7 +485,8 @@ dg_status dg_attention_backward(const dg_attention_desc* desc, const dg_neighbor
  *   [n_groups].  Rows behind the last group give zeros; a size below 0 counts as 0, one that
  *   reaches past n_rows ends there.
  * Backward: dx like x or NULL, dweight like weight or NULL, dbias like bias or NULL (with
- * dweight only); workspace of dg_grouped_workspace_size bytes for dweight.  Sums are float32
+ * dweight only); workspace of dg_grouped_workspace_size bytes for dweight, whose time grows with the
+ * square of the groups (4,096 groups of up to 128 x 128: 0.26 ms, 65,536: 45 ms).  Sums are float32
  * and in a fixed order: results repeat bit for bit. */
 typedef struct dg_grouped_desc {
     int64_t n_rows;
