@@ -19,6 +19,7 @@
 
 #include "../../include/dynamis_graph.h"
 #include "dg_common.hpp"
+#include "dg_grid.hpp"
 #include "dg_scan.hpp"
 
 namespace dg {
@@ -185,7 +186,7 @@ __device__ __forceinline__ int64_t image_of(const int64_t* off, int64_t B, int64
 template <bool WRITE>
 __global__ __launch_bounds__(256) void batch_kernel(Args a)
 {
-    const int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 6;  // one wave per target
+    const int64_t t = (workgroup() * blockDim.x + threadIdx.x) >> 6;  // one wave per target
     const int lane = threadIdx.x & 63;
     if (t >= a.N) return;
     const Image& m = a.img[image_of(a.off, a.B, t)];
@@ -332,7 +333,7 @@ dg_status dg_batch_count(const dg_batch_desc* desc, const void* pos, const int64
                        (const int64_t*)off, (int)a.pbc[0], (int)a.pbc[1], (int)a.pbc[2], desc->radius,
                        (Image*)(w + L.o_img), a.totals);
     if (desc->n_atoms > 0) {
-        hipLaunchKernelGGL(batch_kernel<false>, dim3(nblk(64 * desc->n_atoms)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(batch_kernel<false>, workgroups((desc->n_atoms + 3) / 4), dim3(256), 0, s, a);
         excl_scan<int, int64_t>(a.cnt, desc->n_atoms, (int64_t*)(w + L.o_offs), (int64_t*)(w + L.o_part), s,
                                 a.totals);
     } else {
@@ -377,7 +378,7 @@ dg_status dg_batch_write(const dg_batch_desc* desc, const void* pos, void* ws, s
     a.capacity = capacity;
     if (desc->n_atoms > 0 && capacity > 0) {
         if (!edge_src || !edge_dst || !cell_shift) return fail(DG_ERR_INVALID, "edge outputs are NULL");
-        hipLaunchKernelGGL(batch_kernel<true>, dim3(nblk(64 * desc->n_atoms)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(batch_kernel<true>, workgroups((desc->n_atoms + 3) / 4), dim3(256), 0, s, a);
     }
     if (edges_per_image) {
         char* w = (char*)ws;
