@@ -1119,6 +1119,9 @@ dg_status dg_filter_edges_to_radius(const void* pos, int32_t pos_dtype, int64_t 
 {
     dg_status st = filter_check(pos_dtype, shift_dtype, radius, E, n_atoms);
     if (st != DG_OK) return st;
+    // (a thread an edge; a launch of 2^32 threads runs, without an error, what is left modulo 2^32)
+    if (E > 0xffffff00LL)
+        return fail(DG_ERR_INVALID, "at most 2^32 - 256 edges (dg_filter_count and dg_filter_write take more)");
     if (ws_bytes < dg_filter_workspace_size(E)) return fail(DG_ERR_WORKSPACE, "workspace too small");
     char* w = (char*)ws;
     int* flag = (int*)w;

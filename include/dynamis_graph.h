@@ -179,8 +179,8 @@ dg_status dg_graph_build_noalloc(const dg_graph_desc* desc, const void* pos,
 /* Order-preserving filter of an edge list to radius (keep iff d2 <= radius^2, canonical
  * fp64 d2).  Replaces filter_edges_to_radius (dist_graph_ops.cpp:5-35,
  * dist_graph_ops_kernels.cu:16-43,62-102).
- *   edge_src/edge_dst int64 [n_edges], cell_shift [n_edges,3] of shift_dtype (DG_F32,
- *     DG_F64, DG_I64 or DG_I32)
+ *   edge_src/edge_dst int64 [n_edges] (at most 2^32 - 256), cell_shift [n_edges,3] of
+ *     shift_dtype (DG_F32, DG_F64, DG_I64 or DG_I32)
  *   keep_idx out int64 [n_edges]: indices of kept edges, ascending
  *   n_kept   out int64 (device, one value); -1 if an edge names an atom outside
  *            [0, n_atoms) (such edges are never read through: no position is gathered)
