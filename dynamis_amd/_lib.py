@@ -137,6 +137,30 @@ class GroupedDesc(ctypes.Structure):
     ]
 
 
+class RotateDesc(ctypes.Structure):
+    """dg_rotate_desc."""
+
+    _fields_ = [
+        ("n_targets", ctypes.c_int64),
+        ("n_nodes", ctypes.c_int64),
+        ("ld_q", ctypes.c_int64),
+        ("ld_k", ctypes.c_int64),
+        ("ld_gq", ctypes.c_int64),
+        ("ld_gk", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 8),
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("pos_dtype", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
 _lib = None
 
 _p = ctypes.c_void_p
@@ -156,7 +180,7 @@ def lib():
     L = ctypes.CDLL(LIB_PATH)
     D = ctypes.POINTER(GraphDesc)
     ND, NL, AD = ctypes.POINTER(NeighborDesc), ctypes.POINTER(NeighborLists), ctypes.POINTER(AttentionDesc)
-    GD = ctypes.POINTER(GroupedDesc)
+    GD, RD = ctypes.POINTER(GroupedDesc), ctypes.POINTER(RotateDesc)
     sig = {
         "dg_graph_workspace_size": (_sz, [D]),
         "dg_graph_count": (_i32, [D, _p, _p, _p, _sz, _p, _p]),
@@ -207,6 +231,9 @@ def lib():
         "dg_grouped_forward": (_i32, [GD, _p, _p, _p, _p, _p, _p]),
         "dg_grouped_workspace_size": (_sz, [GD]),
         "dg_grouped_backward": (_i32, [GD] + [_p] * 8 + [_sz, _p]),
+        "dg_rotate_forward": (_i32, [RD] + [_p] * 9),
+        "dg_rotate_workspace_size": (_sz, [RD]),
+        "dg_rotate_backward": (_i32, [RD] + [_p] * 14 + [_sz, _p]),
         "dg_last_error": (ctypes.c_char_p, []),
         "dg_version": (ctypes.c_char_p, []),
     }

@@ -1,0 +1,578 @@
+// dg_rotate.hip -- heads of queries and keys, normalised and rotated by their atoms' positions:
+// forward and backward.
+//
+//   n[c]     = x[c] / sqrt(mean_c x[c]^2 + eps) * w[c]              (or n = x)
+//   theta[j] = position[i, axis(j)] * frequency[j]                  pair j = channels (j, j + P) or (2j, 2j + 1)
+//   y_a = n_a cos - n_b sin,   y_b = n_a sin + n_b cos              channels from 2 P on: y = n
+//
+//   g' = the gradient of y turned back by theta;  xhat = x / rms;  t = g' w
+//   dx = (t - xhat mean(t xhat)) / rms,   dw = sum g' xhat,
+//   dtheta[j] = sum_heads n_a g'_b - n_b g'_a,   dposition[i, a] = sum_{j of axis a} frequency[j] dtheta[j]
+//
+// Every element is read and written once, with some twenty operations: bound by memory.  A lane
+// holds 16 bytes of a head, a power of two of lanes the head, and a group of lanes all heads of one
+// atom, as many at once as there are lanes; waves share nothing, so there is no barrier.  The
+// angles' sines are made once for an atom and serve all of its heads from LDS.  An angle is
+// worked out in turns in 64 bits and brought into half a turn before it is rounded: positions are
+// as far away as they like.  Where pairs lie P channels apart a channel's partner, at any P,
+// comes through LDS, in 32 bits.  All sums have one owner and one order.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <initializer_list>
+#include <string>
+
+#include "../../include/dynamis_graph.h"
+#include "dg_grid.hpp"
+
+namespace dg {
+dg_status fail(dg_status st, const std::string& msg);  // dg_graph.hip
+}
+
+namespace {
+
+using namespace dg;
+
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+
+constexpr int kWaves = 4;
+constexpr int kMaxAxes = 8;
+constexpr int kMaxBlocks = 1024;  // of the backward pass: its partial sums of the weights' gradients
+
+template <typename T>
+constexpr int kC = 16 / (int)sizeof(T);  // channels of a lane
+
+struct Args {
+    const void *q, *k, *pos, *gq, *gk, *qw, *kw;
+    const float* freq;
+    void *oq, *ok;    // results, or (backward) dq and dk
+    void* dpos;
+    float* part;      // [blocks, 2, dim] sums of dw
+    int64_t targets, nodes, ldq, ldk, ldgq, ldgk;
+    int heads, kv, dim, pairs, axes, pos_dtype;
+    int norm, w_own;  // w_own: the weights are of the heads' type (else float)
+    float eps;
+    int per, at_once;  // lanes of a head; heads at once (powers of two, their product up to 64)
+    int ends[kMaxAxes];  // pairs up to and with an axis
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(u32x4 r, float (&v)[kC<T>])
+{
+    if constexpr (sizeof(T) == 4) {
+        const f32x4 f = __builtin_bit_cast(f32x4, r);
+        for (int i = 0; i < 4; ++i) v[i] = f[i];
+    } else {
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __builtin_bit_cast(float, r[i] << 16);
+            v[2 * i + 1] = __builtin_bit_cast(float, r[i] & 0xffff0000u);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ u32x4 pack(const float (&v)[kC<T>])
+{
+    u32x4 r;
+    if constexpr (sizeof(T) == 4) {
+        for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, v[i]);
+    } else {
+        using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+        for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)v[2 * i], (__bf16)v[2 * i + 1]});
+    }
+    return r;
+}
+
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Sum over `n` neighbouring lanes (a power of two, the same for the wave), in each of them.
+__device__ __forceinline__ float sum_lanes(float x, int n)
+{
+    auto add = [&](float y) { x += y; };
+#define DPP(ctrl) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), ctrl, 0xf, 0xf, true))
+    if (n > 1) add(DPP(0xb1));   // lanes 1 0 3 2
+    if (n > 2) add(DPP(0x4e));   // 2 3 0 1
+    if (n > 4) add(DPP(0x141));  // mirrored in halves of a row of 16
+    if (n > 8) add(DPP(0x140));  // in the row
+#undef DPP
+    if (n > 16) add(__shfl_xor(x, 16, 64));
+    if (n > 32) add(__shfl_xor(x, 32, 64));
+    return x;
+}
+
+__device__ __forceinline__ double position(const Args& a, int64_t i)
+{
+    return a.pos_dtype == DG_F32   ? (double)((const float*)a.pos)[i]
+           : a.pos_dtype == DG_F64 ? ((const double*)a.pos)[i]
+                                   : (double)((const int64_t*)a.pos)[i];
+}
+
+__device__ __forceinline__ int axis_of(const Args& a, int j)
+{
+    int x = 0;
+    for (int i = 0; i + 1 < a.axes; ++i) x += j >= a.ends[i];
+    return x;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_weight(const Args& a, const void* w, int c0, float (&v)[kC<T>])
+{
+    for (int i = 0; i < kC<T>; ++i)
+        v[i] = !w || c0 >= a.dim ? 1.0f : a.w_own ? (float)((const T*)w)[c0 + i] : ((const float*)w)[c0 + i];
+}
+
+// LDS of a wave: its atoms' cosines and sines (tokens * P <= 32 C of them, whatever the head), and a
+// word for each channel in flight.  One word in nine is spare, so that lanes eight apart do not meet.
+template <typename T>
+struct Shared {
+    float2 turn[32 * kC<T>];
+    float row[64 * kC<T> + 64 * kC<T> / 8];
+};
+__device__ __forceinline__ int spread(int i) { return i + (i >> 3); }
+
+// The turns of the wave's atoms first .. first + count (some may not exist).
+template <typename T>
+__device__ __forceinline__ void make_turns(const Args& a, int64_t first, int count, int lane, Shared<T>& s)
+{
+    constexpr double kInverse = 0.15915494309189533577;  // 1 / (2 pi)
+    for (int i = lane; i < count * a.pairs; i += 64) {
+        const int t = i / a.pairs, j = i - t * a.pairs;
+        const int64_t node = first + t;
+        if (node >= a.nodes) break;  // (what was there turns zeros, which nobody stores or adds up)
+        const double turns = position(a, node * a.axes + axis_of(a, j)) * ((double)a.freq[j] * kInverse);
+        float sine, cosine;
+        sincospif(2.0f * (float)(turns - rint(turns)), &sine, &cosine);
+        s.turn[i] = make_float2(cosine, sine);
+    }
+    wave_sync();
+}
+
+// Where a lane works: chunk `c0` of head `slot` (plus a multiple of at_once) of the wave's atom `t`.
+struct Seat {
+    int c0, slot, t, base;  // base: of the head's channels in Shared::row
+};
+template <typename T>
+__device__ __forceinline__ Seat seat(const Args& a, int lane)
+{
+    const int group = a.per * a.at_once;
+    Seat s;
+    s.c0 = (lane & (a.per - 1)) * kC<T>;
+    s.slot = (lane & (group - 1)) / a.per;
+    s.t = lane / group;
+    s.base = (lane & ~(a.per - 1)) * kC<T>;
+    return s;
+}
+
+// y = the lane's channels v turned by the angles (BACK: by their opposites); with HALVES through LDS,
+// where `other` receives the partners.
+template <typename T, bool HALVES, bool BACK>
+__device__ __forceinline__ void turn(const Args& a, const Seat& at, const float2* turns, Shared<T>& s, const float (&v)[kC<T>],
+                                     float (&y)[kC<T>])
+{
+    constexpr int C = kC<T>;
+    if constexpr (HALVES) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) s.row[spread(at.base + at.c0 + i)] = v[i];
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int c = at.c0 + i;
+            const bool second = c >= a.pairs;
+            y[i] = v[i];
+            if (c < 2 * a.pairs) {
+                const float other = s.row[spread(at.base + c + (second ? -a.pairs : a.pairs))];
+                const float2 z = turns[second ? c - a.pairs : c];
+                y[i] = fmaf(v[i], z.x, second != BACK ? other * z.y : -(other * z.y));
+            }
+        }
+        wave_sync();
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; i += 2) {
+            const int c = at.c0 + i;
+            y[i] = v[i];
+            y[i + 1] = v[i + 1];
+            if (c < 2 * a.pairs) {
+                const float2 z = turns[c / 2];
+                const float sine = BACK ? -z.y : z.y;
+                y[i] = fmaf(v[i], z.x, -(v[i + 1] * sine));
+                y[i + 1] = fmaf(v[i + 1], z.x, v[i] * sine);
+            }
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float inverse_rms(const Args& a, const float (&x)[kC<T>])
+{
+    float ss = 0;
+    for (int i = 0; i < kC<T>; ++i) ss = fmaf(x[i], x[i], ss);
+    return 1.0f / sqrtf(sum_lanes(ss, a.per) / (float)a.dim + a.eps);
+}
+
+template <typename T, bool HALVES>
+__global__ __launch_bounds__(64 * kWaves) void forward_kernel(Args a, int64_t tokens_end)
+{
+    __shared__ Shared<T> shared[kWaves];
+    constexpr int C = kC<T>;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    Shared<T>& s = shared[w];
+    const Seat at = seat<T>(a, lane);
+    const int count = 64 / (a.per * a.at_once);
+    float qw[C], kw[C];
+    load_weight<T>(a, a.qw, at.c0, qw);
+    load_weight<T>(a, a.kw, at.c0, kw);
+    for (int64_t first = (workgroup() * kWaves + w) * count; first < tokens_end;
+         first += (int64_t)gridDim.x * gridDim.y * kWaves * count) {
+        const int64_t node = first + at.t;
+        const bool chunk = at.c0 < a.dim;
+        auto load = [&](int step) {
+            u32x4 r = {0, 0, 0, 0};
+            const int q_steps = (a.heads + a.at_once - 1) / a.at_once;
+            const bool is_q = step < q_steps;
+            const int head = (is_q ? step : step - q_steps) * a.at_once + at.slot;
+            if (chunk && node < (is_q ? a.targets : a.nodes) && head < (is_q ? a.heads : a.kv))
+                r = *(const u32x4*)((const T*)(is_q ? a.q : a.k) + node * (is_q ? a.ldq : a.ldk) + head * a.dim + at.c0);
+            return r;
+        };
+        const int q_steps = (a.heads + a.at_once - 1) / a.at_once, steps = q_steps + (a.kv + a.at_once - 1) / a.at_once;
+        u32x4 next = load(0);
+        make_turns(a, first, count, lane, s);
+        const float2* turns = s.turn + at.t * a.pairs;
+        for (int step = 0; step < steps; ++step) {
+            float x[C], y[C];
+            unpack<T>(next, x);
+            if (step + 1 < steps) next = load(step + 1);
+            const bool is_q = step < q_steps;
+            if (a.norm) {
+                const float r = inverse_rms<T>(a, x);
+                for (int i = 0; i < C; ++i) x[i] = x[i] * r * (is_q ? qw[i] : kw[i]);
+            }
+            turn<T, HALVES, false>(a, at, turns, s, x, y);
+            const int heads = is_q ? a.heads : a.kv, head = (is_q ? step : step - q_steps) * a.at_once + at.slot;
+            if (chunk && node < (is_q ? a.targets : a.nodes) && head < heads)
+                *(u32x4*)((T*)(is_q ? a.oq : a.ok) + (node * heads + head) * a.dim + at.c0) = pack<T>(y);
+        }
+        wave_sync();
+    }
+}
+
+template <typename T, bool HALVES>
+__global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
+{
+    __shared__ Shared<T> shared[kWaves];
+    __shared__ float s_sum[64 * kWaves * kC<T>];
+    constexpr int C = kC<T>;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    Shared<T>& s = shared[w];
+    const Seat at = seat<T>(a, lane);
+    const int group = a.per * a.at_once, count = 64 / group;
+    const bool chunk = at.c0 < a.dim;
+    float sum_q[C] = {}, sum_k[C] = {};
+    const int q_steps = (a.heads + a.at_once - 1) / a.at_once, steps = q_steps + (a.kv + a.at_once - 1) / a.at_once;
+    for (int64_t first = ((int64_t)blockIdx.x * kWaves + w) * count; first < a.nodes;
+         first += (int64_t)gridDim.x * kWaves * count) {
+        const int64_t node = first + at.t;
+        auto load = [&](int step, u32x4& x, u32x4& g) {
+            x = g = u32x4{0, 0, 0, 0};
+            const bool is_q = step < q_steps;
+            const int head = (is_q ? step : step - q_steps) * a.at_once + at.slot;
+            if (chunk && node < (is_q ? a.targets : a.nodes) && head < (is_q ? a.heads : a.kv)) {
+                const int64_t in = head * a.dim + at.c0;
+                x = *(const u32x4*)((const T*)(is_q ? a.q : a.k) + node * (is_q ? a.ldq : a.ldk) + in);
+                g = *(const u32x4*)((const T*)(is_q ? a.gq : a.gk) + node * (is_q ? a.ldgq : a.ldgk) + in);
+            }
+        };
+        u32x4 next_x, next_g;
+        load(0, next_x, next_g);
+        make_turns(a, first, count, lane, s);
+        const float2* turns = s.turn + at.t * a.pairs;
+        float dtheta[C] = {};  // of the pairs whose first channel the lane holds
+        for (int step = 0; step < steps; ++step) {
+            float x[C], g[C], back[C], n[C];
+            unpack<T>(next_x, x);
+            unpack<T>(next_g, g);
+            if (step + 1 < steps) load(step + 1, next_x, next_g);
+            const bool is_q = step < q_steps;
+            const int heads = is_q ? a.heads : a.kv, head = (is_q ? step : step - q_steps) * a.at_once + at.slot;
+            // (a lane without a head adds nothing: an angle or a scale that is not finite would make a NaN of its zeros)
+            const bool live = chunk && node < (is_q ? a.targets : a.nodes) && head < heads;
+            turn<T, HALVES, true>(a, at, turns, s, g, back);
+            float r = 1.0f, wt[C];
+            load_weight<T>(a, is_q ? a.qw : a.kw, at.c0, wt);
+            if (a.norm) {
+                r = inverse_rms<T>(a, x);
+                for (int i = 0; i < C; ++i) x[i] *= r;
+            }
+            for (int i = 0; i < C; ++i) n[i] = x[i] * wt[i];
+            if (a.dpos) {
+                if constexpr (HALVES) {
+                    // (the partner of `back`, turned back in its turn, from the partner of n)
+                    for (int i = 0; i < C; ++i) s.row[spread(at.base + at.c0 + i)] = n[i];
+                    wave_sync();
+                    float other[C];
+                    for (int i = 0; i < C; ++i) other[i] = at.c0 + i < a.pairs ? s.row[spread(at.base + at.c0 + i + a.pairs)] : 0.0f;
+                    wave_sync();
+                    for (int i = 0; i < C; ++i) s.row[spread(at.base + at.c0 + i)] = back[i];
+                    wave_sync();
+                    for (int i = 0; i < C; ++i)
+                        if (live && at.c0 + i < a.pairs)
+                            dtheta[i] += n[i] * s.row[spread(at.base + at.c0 + i + a.pairs)] - other[i] * back[i];
+                    wave_sync();
+                } else {
+                    for (int i = 0; i < C; i += 2)
+                        if (live && at.c0 + i < 2 * a.pairs) dtheta[i] += n[i] * back[i + 1] - n[i + 1] * back[i];
+                }
+            }
+            if (a.norm) {
+                float dot = 0;
+                for (int i = 0; i < C; ++i) {
+                    const float term = live ? back[i] * x[i] : 0.0f;
+                    if (is_q) sum_q[i] += term;
+                    else sum_k[i] += term;
+                    back[i] *= wt[i];
+                    dot = fmaf(back[i], x[i], dot);
+                }
+                dot = sum_lanes(dot, a.per) / (float)a.dim;
+                for (int i = 0; i < C; ++i) back[i] = r * (back[i] - x[i] * dot);
+            }
+            if (live) *(u32x4*)((T*)(is_q ? a.oq : a.ok) + (node * heads + head) * a.dim + at.c0) = pack<T>(back);
+        }
+        if (a.dpos) {
+            for (int axis = 0; axis < a.axes; ++axis) {
+                double sum = 0;
+                for (int i = 0; i < C; i += HALVES ? 1 : 2) {
+                    const int j = HALVES ? at.c0 + i : (at.c0 + i) / 2;
+                    if (j < a.ends[axis] && (axis == 0 || j >= a.ends[axis - 1])) sum += (double)a.freq[j] * (double)dtheta[i];
+                }
+                for (int o = 1; o < group; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                if ((lane & (group - 1)) == 0 && node < a.nodes) {
+                    if (a.pos_dtype == DG_F64) ((double*)a.dpos)[node * a.axes + axis] = sum;
+                    else ((float*)a.dpos)[node * a.axes + axis] = (float)sum;
+                }
+            }
+        }
+        wave_sync();
+    }
+    if (!a.part) return;
+    // the workgroup's sums of each channel, in the lanes' order
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+        for (int i = 0; i < C; ++i) s_sum[threadIdx.x * C + i] = which ? sum_k[i] : sum_q[i];
+        __syncthreads();
+        if ((int)threadIdx.x < a.dim) {
+            const int c = threadIdx.x;
+            float x = 0;
+            for (int l = c / C; l < 64 * kWaves; l += a.per) x += s_sum[l * C + c % C];
+            a.part[((int64_t)blockIdx.x * 2 + which) * a.dim + c] = x;
+        }
+    }
+}
+
+// dw: the workgroups' sums of 64 channels, sixteen strands of them in turn.
+template <typename T>
+__global__ __launch_bounds__(1024) void join_kernel(const float* part, int blocks, int dim, void* dqw, void* dkw, int w_own)
+{
+    __shared__ float s[16][64];
+    const int lane = threadIdx.x & 63, strand = threadIdx.x >> 6, which = blockIdx.y, c = blockIdx.x * 64 + lane;
+    float x = 0;
+    if (c < dim)
+#pragma unroll 8
+        for (int b = strand; b < blocks; b += 16) x += part[((int64_t)b * 2 + which) * dim + c];
+    s[strand][lane] = x;
+    __syncthreads();
+    void* out = which ? dkw : dqw;
+    if (strand || c >= dim || !out) return;
+    x = 0;
+    for (int i = 0; i < 16; ++i) x += s[i][lane];
+    if (w_own) ((T*)out)[c] = (T)x;
+    else ((float*)out)[c] = x;
+}
+
+// ---------------------------------------------------------------- host
+dg_status check(const dg_rotate_desc* d)
+{
+    if (!d) return fail(DG_ERR_INVALID, "desc is NULL");
+    if (d->dtype != DG_F32 && d->dtype != DG_BF16) return fail(DG_ERR_INVALID, "q and k must be float32 or bfloat16");
+    if (d->weight_dtype != DG_F32 && d->weight_dtype != d->dtype)
+        return fail(DG_ERR_INVALID, "the weights must be float32 or of q's type");
+    if (d->pos_dtype != DG_F32 && d->pos_dtype != DG_F64 && d->pos_dtype != DG_I64)
+        return fail(DG_ERR_INVALID, "positions must be float32, float64 or int64");
+    if (d->n_nodes < 0 || d->n_nodes > (1ll << 40) || d->n_targets < 0 || d->n_targets > d->n_nodes)
+        return fail(DG_ERR_INVALID, "nodes must be in [0, 2^40] and targets among them");
+    if (d->heads < 1 || d->heads > 1024 || d->kv_heads < 1 || d->kv_heads > 1024)
+        return fail(DG_ERR_INVALID, "heads must be in [1, 1024]");
+    if (d->dim < 8 || d->dim > 256 || d->dim % 8) return fail(DG_ERR_INVALID, "dim must be a multiple of 8 in [8, 256]");
+    if (d->axes < 1 || d->axes > kMaxAxes) return fail(DG_ERR_INVALID, "axes must be in [1, 8]");
+    int64_t pairs = 0;
+    for (int i = 0; i < d->axes; ++i) {
+        if (d->sections[i] < 0) return fail(DG_ERR_INVALID, "sections must not be negative");
+        pairs += d->sections[i];
+    }
+    if (pairs < 1 || pairs > d->dim / 2) return fail(DG_ERR_INVALID, "sections must add up to 1 to dim / 2 pairs");
+    if (d->norm && !(d->eps >= 0.0f && d->eps <= 3e38f)) return fail(DG_ERR_INVALID, "eps must be finite and not negative");
+    const int64_t most = 1ll << 40;
+    for (int64_t ld : {d->ld_q, d->ld_k, d->ld_gq, d->ld_gk}) {
+        if (ld < 0 || ld > most || ld % (d->dtype == DG_F32 ? 4 : 8))
+            return fail(DG_ERR_INVALID, "rows must lie a multiple of 16 bytes apart");
+        if (d->n_nodes > 0 && ld > (1ll << 60) / d->n_nodes) return fail(DG_ERR_INVALID, "rows reach past 2^60 elements");
+    }
+    return DG_OK;
+}
+
+int power_of_two(int x)
+{
+    int p = 1;
+    while (p < x) p *= 2;
+    return p;
+}
+
+Args make_args(const dg_rotate_desc* d)
+{
+    Args a = {};
+    a.targets = d->n_targets;
+    a.nodes = d->n_nodes;
+    a.ldq = d->ld_q;
+    a.ldk = d->ld_k;
+    a.ldgq = d->ld_gq;
+    a.ldgk = d->ld_gk;
+    a.heads = d->heads;
+    a.kv = d->kv_heads;
+    a.dim = d->dim;
+    a.axes = d->axes;
+    a.pos_dtype = d->pos_dtype;
+    a.norm = d->norm != 0;
+    a.w_own = d->weight_dtype == d->dtype && d->dtype != DG_F32;
+    a.eps = d->eps;
+    for (int i = 0; i < d->axes; ++i) {
+        a.pairs += d->sections[i];
+        a.ends[i] = a.pairs;
+    }
+    const int c = d->dtype == DG_F32 ? 4 : 8;
+    a.per = power_of_two(d->dim / c);
+    a.at_once = std::min(64 / a.per, power_of_two(std::max(d->heads, d->kv_heads)));
+    return a;
+}
+
+// Atoms of a workgroup's pass.
+int64_t pass_of(const Args& a) { return kWaves * (64 / (a.per * a.at_once)); }
+
+int64_t blocks_of(const Args& a)
+{
+    return std::max<int64_t>(1, std::min<int64_t>((a.nodes + pass_of(a) - 1) / pass_of(a), kMaxBlocks));
+}
+
+bool misaligned(std::initializer_list<const void*> p)
+{
+    for (const void* x : p)
+        if ((uintptr_t)x & 15) return true;
+    return false;
+}
+
+dg_status launched(const char* what)
+{
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(DG_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+    return DG_OK;
+}
+
+template <typename T>
+void run_forward(const Args& a, bool interleaved, hipStream_t s)
+{
+    const dim3 grid = workgroups((a.nodes + pass_of(a) - 1) / pass_of(a));
+    if (interleaved) hipLaunchKernelGGL((forward_kernel<T, false>), grid, dim3(64 * kWaves), 0, s, a, a.nodes);
+    else hipLaunchKernelGGL((forward_kernel<T, true>), grid, dim3(64 * kWaves), 0, s, a, a.nodes);
+}
+
+template <typename T>
+void run_backward(const Args& a, bool interleaved, void* dqw, void* dkw, hipStream_t s)
+{
+    const int64_t blocks = a.nodes ? blocks_of(a) : 0;
+    if (blocks) {
+        const dim3 grid((unsigned)blocks);
+        if (interleaved) hipLaunchKernelGGL((backward_kernel<T, false>), grid, dim3(64 * kWaves), 0, s, a);
+        else hipLaunchKernelGGL((backward_kernel<T, true>), grid, dim3(64 * kWaves), 0, s, a);
+    }
+    if (a.part)
+        hipLaunchKernelGGL(join_kernel<T>, dim3((a.dim + 63) / 64, 2), dim3(1024), 0, s, a.part, (int)blocks, a.dim, dqw, dkw,
+                           a.w_own);
+}
+
+}  // namespace
+
+extern "C" {
+
+dg_status dg_rotate_forward(const dg_rotate_desc* d, const void* q, const void* k, const void* positions,
+                            const float* frequencies, const void* q_weight, const void* k_weight, void* q_out, void* k_out,
+                            hipStream_t s)
+{
+    dg_status st = check(d);
+    if (st != DG_OK) return st;
+    if (d->n_nodes == 0) return DG_OK;
+    if ((d->n_targets > 0 && (!q || !q_out)) || !k || !positions || !frequencies || !k_out)
+        return fail(DG_ERR_INVALID, "inputs or outputs are NULL");
+    if (misaligned({q, k, q_out, k_out})) return fail(DG_ERR_INVALID, "q, k and the results must be aligned to 16 bytes");
+    if (!d->norm && (q_weight || k_weight)) return fail(DG_ERR_INVALID, "weights come with norm");
+    Args a = make_args(d);
+    a.q = q;
+    a.k = k;
+    a.pos = positions;
+    a.freq = frequencies;
+    a.qw = q_weight;
+    a.kw = k_weight;
+    a.oq = q_out;
+    a.ok = k_out;
+    if (d->dtype == DG_BF16) run_forward<__bf16>(a, d->interleaved != 0, s);
+    else run_forward<float>(a, d->interleaved != 0, s);
+    return launched("dg_rotate_forward");
+}
+
+size_t dg_rotate_workspace_size(const dg_rotate_desc* d)
+{
+    if (check(d) != DG_OK) return 0;
+    const Args a = make_args(d);
+    return (size_t)blocks_of(a) * 2 * a.dim * sizeof(float);
+}
+
+dg_status dg_rotate_backward(const dg_rotate_desc* d, const void* q, const void* k, const void* positions,
+                             const float* frequencies, const void* q_weight, const void* k_weight, const void* grad_q,
+                             const void* grad_k, void* dq, void* dk, void* dpositions, void* dq_weight, void* dk_weight,
+                             void* ws, size_t ws_bytes, hipStream_t s)
+{
+    dg_status st = check(d);
+    if (st != DG_OK) return st;
+    if (d->n_nodes > 0 && ((d->n_targets > 0 && (!q || !grad_q || !dq)) || !k || !positions || !frequencies || !grad_k || !dk))
+        return fail(DG_ERR_INVALID, "inputs or outputs are NULL");
+    if (misaligned({q, k, grad_q, grad_k, dq, dk}))
+        return fail(DG_ERR_INVALID, "q, k, their gradients and the results must be aligned to 16 bytes");
+    if (!d->norm && (q_weight || k_weight || dq_weight || dk_weight)) return fail(DG_ERR_INVALID, "weights come with norm");
+    if ((dq_weight && !q_weight) || (dk_weight && !k_weight)) return fail(DG_ERR_INVALID, "a weight's gradient comes with it");
+    if (dpositions && d->pos_dtype == DG_I64) return fail(DG_ERR_INVALID, "whole positions have no gradient");
+    Args a = make_args(d);
+    a.q = q;
+    a.k = k;
+    a.pos = positions;
+    a.freq = frequencies;
+    a.qw = q_weight;
+    a.kw = k_weight;
+    a.gq = grad_q;
+    a.gk = grad_k;
+    a.oq = dq;
+    a.ok = dk;
+    a.dpos = dpositions;
+    if (dq_weight || dk_weight) {
+        if (!ws || ws_bytes < dg_rotate_workspace_size(d)) return fail(DG_ERR_WORKSPACE, "workspace too small");
+        a.part = (float*)ws;
+    }
+    if (d->dtype == DG_BF16) run_backward<__bf16>(a, d->interleaved != 0, dq_weight, dk_weight, s);
+    else run_backward<float>(a, d->interleaved != 0, dq_weight, dk_weight, s);
+    return launched("dg_rotate_backward");
+}
+
+}  // extern "C"

@@ -505,6 +505,46 @@ dg_status dg_grouped_backward(const dg_grouped_desc* desc, const void* x, const 
                               void* dbias, void* workspace, size_t workspace_bytes,
                               hipStream_t stream);
 
+/* Heads of queries and keys, normalised one by one and rotated by their nodes' positions:
+ *   n[c] = x[c] / sqrt(mean_c x[c]^2 + eps) * weight[c]     (norm != 0; else n = x)
+ *   theta[j] = positions[i, axis of j] * frequencies[j], the pairs j < P = sum of sections, the
+ *              first sections[0] of them on axis 0 and so on
+ *   y_a = n_a cos(theta) - n_b sin(theta), y_b = n_a sin(theta) + n_b cos(theta) for the channels
+ *              (a, b) = (j, j + P), or (2j, 2j + 1) (interleaved != 0); y = n from channel 2 P on
+ *   q [n_targets, heads, dim], k [n_nodes, kv_heads, dim] of dtype (DG_F32 / DG_BF16), rows ld_*
+ *   elements apart (0: one row for all), they and their rows aligned to 16 bytes; dim a multiple of
+ *   8, 8 .. 256.  Row i of q and of k belongs to node i.  positions [n_nodes, axes] of pos_dtype
+ *   (DG_F32, DG_F64, DG_I64), angles worked out in 64 bits; frequencies float32 [P], radians for a
+ *   unit of the position; q_weight, k_weight [dim] of weight_dtype (DG_F32 or dtype) or NULL (ones).
+ *   q_out, k_out contiguous, of dtype, rounded once.
+ * Backward: dq, dk contiguous, of dtype; dpositions like positions or NULL; dq_weight, dk_weight like
+ * the weights or NULL, for which the workspace of dg_rotate_workspace_size bytes is needed.  Sums are
+ * float32 (those of dpositions float64 over the pairs) and in a fixed order: results repeat bit for
+ * bit.  Both enqueue work only. */
+typedef struct dg_rotate_desc {
+    int64_t n_targets;
+    int64_t n_nodes;
+    int64_t ld_q, ld_k;
+    int64_t ld_gq, ld_gk; /* of the gradients (backward) */
+    int32_t heads, kv_heads;
+    int32_t dim;
+    int32_t axes;         /* 1 .. 8 */
+    int32_t sections[8];
+    int32_t dtype, weight_dtype, pos_dtype;
+    int32_t norm, interleaved;
+    float eps;
+} dg_rotate_desc;
+
+dg_status dg_rotate_forward(const dg_rotate_desc* desc, const void* q, const void* k, const void* positions,
+                            const float* frequencies, const void* q_weight, const void* k_weight,
+                            void* q_out, void* k_out, hipStream_t stream);
+size_t dg_rotate_workspace_size(const dg_rotate_desc* desc);
+dg_status dg_rotate_backward(const dg_rotate_desc* desc, const void* q, const void* k, const void* positions,
+                             const float* frequencies, const void* q_weight, const void* k_weight,
+                             const void* grad_q, const void* grad_k, void* dq, void* dk, void* dpositions,
+                             void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes,
+                             hipStream_t stream);
+
 /* Message of the last failure on this thread ("" if none). */
 const char* dg_last_error(void);
 
