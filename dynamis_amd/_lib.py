@@ -161,6 +161,38 @@ class RotateDesc(ctypes.Structure):
     ]
 
 
+class RouteDesc(ctypes.Structure):
+    """dg_route_desc."""
+
+    _fields_ = [
+        ("n_rows", ctypes.c_int64),
+        ("ld", ctypes.c_int64),
+        ("n_experts", ctypes.c_int32),
+        ("k", ctypes.c_int32),
+        ("groups", ctypes.c_int32),
+        ("top_groups", ctypes.c_int32),
+        ("group_best", ctypes.c_int32),
+        ("sigmoid", ctypes.c_int32),
+        ("renormalize", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("pad_", ctypes.c_int32),
+    ]
+
+
+class ExchangeDesc(ctypes.Structure):
+    """dg_exchange_desc."""
+
+    _fields_ = [
+        ("n_rows", ctypes.c_int64),
+        ("ld", ctypes.c_int64),
+        ("k", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("pad_", ctypes.c_int32),
+    ]
+
+
 _lib = None
 
 _p = ctypes.c_void_p
@@ -181,6 +213,7 @@ def lib():
     D = ctypes.POINTER(GraphDesc)
     ND, NL, AD = ctypes.POINTER(NeighborDesc), ctypes.POINTER(NeighborLists), ctypes.POINTER(AttentionDesc)
     GD, RD = ctypes.POINTER(GroupedDesc), ctypes.POINTER(RotateDesc)
+    UD, XD = ctypes.POINTER(RouteDesc), ctypes.POINTER(ExchangeDesc)
     sig = {
         "dg_graph_workspace_size": (_sz, [D]),
         "dg_graph_count": (_i32, [D, _p, _p, _p, _sz, _p, _p]),
@@ -234,6 +267,12 @@ def lib():
         "dg_rotate_forward": (_i32, [RD] + [_p] * 9),
         "dg_rotate_workspace_size": (_sz, [RD]),
         "dg_rotate_backward": (_i32, [RD] + [_p] * 14 + [_sz, _p]),
+        "dg_route_workspace_size": (_sz, [UD]),
+        "dg_route_forward": (_i32, [UD] + [_p] * 7 + [_sz, _p]),
+        "dg_route_backward": (_i32, [UD] + [_p] * 5),
+        "dg_exchange_dispatch": (_i32, [XD] + [_p] * 4),
+        "dg_exchange_combine": (_i32, [XD] + [_p] * 6),
+        "dg_exchange_combine_backward": (_i32, [XD] + [_p] * 7),
         "dg_last_error": (ctypes.c_char_p, []),
         "dg_version": (ctypes.c_char_p, []),
     }

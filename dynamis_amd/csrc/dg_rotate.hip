@@ -26,6 +26,7 @@
 
 #include "../../include/dynamis_graph.h"
 #include "dg_grid.hpp"
+#include "dg_lanes.hpp"
 
 namespace dg {
 dg_status fail(dg_status st, const std::string& msg);  // dg_graph.hip
@@ -83,27 +84,6 @@ __device__ __forceinline__ u32x4 pack(const float (&v)[kC<T>])
         for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)v[2 * i], (__bf16)v[2 * i + 1]});
     }
     return r;
-}
-
-__device__ __forceinline__ void wave_sync()
-{
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
-// Sum over `n` neighbouring lanes (a power of two, the same for the wave), in each of them.
-__device__ __forceinline__ float sum_lanes(float x, int n)
-{
-    auto add = [&](float y) { x += y; };
-#define DPP(ctrl) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), ctrl, 0xf, 0xf, true))
-    if (n > 1) add(DPP(0xb1));   // lanes 1 0 3 2
-    if (n > 2) add(DPP(0x4e));   // 2 3 0 1
-    if (n > 4) add(DPP(0x141));  // mirrored in halves of a row of 16
-    if (n > 8) add(DPP(0x140));  // in the row
-#undef DPP
-    if (n > 16) add(__shfl_xor(x, 16, 64));
-    if (n > 32) add(__shfl_xor(x, 32, 64));
-    return x;
 }
 
 __device__ __forceinline__ double position(const Args& a, int64_t i)
@@ -351,7 +331,7 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
                     const int j = HALVES ? at.c0 + i : (at.c0 + i) / 2;
                     if (j < a.ends[axis] && (axis == 0 || j >= a.ends[axis - 1])) sum += (double)a.freq[j] * (double)dtheta[i];
                 }
-                for (int o = 1; o < group; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                sum = sum_lanes(sum, group);
                 if ((lane & (group - 1)) == 0 && node < a.nodes) {
                     if (a.pos_dtype == DG_F64) ((double*)a.dpos)[node * a.axes + axis] = sum;
                     else ((float*)a.dpos)[node * a.axes + axis] = (float)sum;
@@ -424,13 +404,6 @@ dg_status check(const dg_rotate_desc* d)
         if (d->n_nodes > 0 && ld > (1ll << 60) / d->n_nodes) return fail(DG_ERR_INVALID, "rows reach past 2^60 elements");
     }
     return DG_OK;
-}
-
-int power_of_two(int x)
-{
-    int p = 1;
-    while (p < x) p *= 2;
-    return p;
 }
 
 Args make_args(const dg_rotate_desc* d)

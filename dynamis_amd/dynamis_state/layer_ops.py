@@ -3,9 +3,13 @@ normalised and rotated by the atoms' positions, rows routed to experts, taken in
 back.
 
     q, k = rotate_heads(q, k, positions, frequencies)     # before neighbor_attention
+    routing = route_rows(grouped_linear(x, router, natoms), k=2)
+    rows = dispatch_rows(x, routing)                      # in the experts' order
+    rows = grouped_linear(rows, weight, routing.sizes)    # a weight for each expert
+    x = combine_rows(rows, routing, residual=x)
 
-No counterpart in the reference.  The kernels are those of libdynamis_graph.so (dg_rotate_*); there
-is no CPU path.  Everything runs on the current stream without synchronising the host and can be
+No counterpart in the reference.  The kernels are those of libdynamis_graph.so (dg_rotate_*, dg_route_*,
+dg_exchange_*); there is no CPU path.  Everything runs on the current stream without synchronising the host and can be
 captured in a HIP graph; tensors follow torch's rules for streams.
 """
 from __future__ import annotations
@@ -188,3 +192,220 @@ def rotate_heads(q, k, positions, frequencies, sections=None, q_weight=None, k_w
                                     or k_weight is not None and k_weight.requires_grad):
         return _Rotate.apply(q, k, positions, frequencies, q_weight, k_weight, *how)
     return _rotate_forward(q, k, positions, frequencies, q_weight, k_weight, *how)[3:]
+
+
+class Routing:
+    """Which experts a batch's rows go to (see ``route_rows``).
+
+    rows, num_experts, k;  weights [rows, k] float32;  experts [rows, k] int32 (-1: none);
+    sizes [num_experts] int64, the rows of each expert, as ``grouped_linear`` takes them;
+    places [rows, k] int32, where a choice lies in the experts' order (of a choice of none, -1 minus
+    its place behind the last)."""
+
+    def __init__(self, num_experts, weights, experts, sizes, places):
+        (self.rows, self.k), self.num_experts = experts.shape, num_experts
+        self.weights, self.experts, self.sizes, self.places = weights, experts, sizes, places
+
+
+def _route_forward(logits, bias, d):
+    lib, dev = L.lib(), logits.device
+    rows, k = logits.size(0), d.k
+    with L.on_device(dev):
+        weights = torch.empty((rows, k), dtype=torch.float32, device=dev)
+        experts = torch.empty((rows, k), dtype=torch.int32, device=dev)
+        places = torch.empty((rows, k), dtype=torch.int32, device=dev)
+        sizes = torch.empty(d.n_experts, dtype=torch.int64, device=dev)
+        wsb = lib.dg_route_workspace_size(d)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        status = lib.dg_route_forward(d, logits.data_ptr(), L.addr(bias), weights.data_ptr(), experts.data_ptr(),
+                                      sizes.data_ptr(), places.data_ptr(), ws.data_ptr(), wsb, L.raw_stream(dev))
+        if status:
+            L.check(status, "route_rows")
+    return weights, experts, sizes, places
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, d):
+        weights, experts, sizes, places = _route_forward(logits, bias, d)
+        ctx.save_for_backward(logits, experts)
+        ctx.desc = d
+        ctx.mark_non_differentiable(experts, sizes, places)
+        return weights, experts, sizes, places
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, *_):
+        logits, experts = ctx.saved_tensors
+        dev, grad = logits.device, grad.contiguous()
+        with L.on_device(dev):
+            dlogits = _new_like(logits)
+            status = L.lib().dg_route_backward(ctx.desc, logits.data_ptr(), experts.data_ptr(), grad.data_ptr(),
+                                               dlogits.data_ptr(), L.raw_stream(dev))
+            if status:
+                L.check(status, "route_rows")
+        return dlogits, None, None
+
+
+def _whole_rows(t):
+    """t [rows, width] as it is if its rows are whole; else a copy."""
+    return t if (t.stride(1) == 1 or t.size(1) == 1) and 0 <= t.stride(0) <= 1 << 31 else t.contiguous()
+
+
+def route_rows(logits, k, scoring="softmax", bias=None, groups=1, top_groups=1, group_best=1, renormalize=True, scale=1.0):
+    """The k experts of each row by its logits, their weights, and the experts' order of the rows.
+
+      s       = softmax(logits) or sigmoid(logits)
+      v       = logits where there is neither a bias nor group_best=2, else s + bias, in 64 bits
+      experts = the k largest v, NaN above all and the first of equals
+      weights = scale s[experts], with renormalize divided by their sum over the row
+
+    logits [rows, experts], float32 or bfloat16, 1 to 1024 experts; k up to 64; scoring "softmax" or
+    "sigmoid".  bias [experts], used in float32, moves the choice alone and never the weights (it
+    keeps the experts balanced).  groups > 1 parts the experts into as many neighbouring groups, each
+    worth the sum of its group_best (1 or 2) largest v; experts are chosen from the top_groups worthiest groups.
+
+    An expert whose logit or bias is -inf is never chosen.  Where fewer than k are left (a row of
+    padding, all -inf), the rest of the row's choices is -1 with weight 0, and takes no place among
+    the experts' rows.  rows * k has to be below 2^31.
+
+    Returns a Routing.  Nothing synchronises the host.  Its weights are differentiable in the logits (once, in
+    reverse; the choice has no gradient, nor has the bias).  Results repeat bit for bit.
+    """
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("route_rows", logits, bias)
+    _check(isinstance(logits, torch.Tensor) and logits.is_cuda, "logits must be a CUDA tensor")
+    _check(logits.dim() == 2, f"logits must have shape [rows, experts], got {_shape(logits)}")
+    _check(logits.dtype in _DTYPES, f"logits must be float32 or bfloat16, got {logits.dtype}")
+    rows, experts = logits.shape
+    k, groups, top_groups, group_best = int(k), int(groups), int(top_groups), int(group_best)
+    _check(1 <= experts <= 1024, f"there must be 1 to 1024 experts, got {experts}")
+    _check(1 <= k <= min(64, experts), f"k must be 1 to {min(64, experts)}, got {k}")
+    _check(rows * k < 1 << 31, f"rows times k must be below 2^31, got {rows} times {k}")
+    _check(scoring in ("softmax", "sigmoid"), f'scoring must be "softmax" or "sigmoid", got {scoring!r}')
+    _check(1 <= groups <= 64 and experts % groups == 0, f"groups must be 1 to 64 and divide the {experts} experts, got {groups}")
+    _check(1 <= top_groups <= groups, f"top_groups must be 1 to {groups}, got {top_groups}")
+    _check(group_best in (1, 2), f"group_best must be 1 or 2, got {group_best}")
+    _check(-3e38 <= scale <= 3e38, f"scale must be finite, got {scale}")
+    if bias is not None:
+        _check(isinstance(bias, torch.Tensor) and bias.device == logits.device and bias.is_floating_point()
+               and tuple(bias.shape) == (experts,), f"bias must be floating [{experts}] on {logits.device}")
+        bias = bias.detach().float().contiguous()
+    logits = _whole_rows(logits)
+    d = L.RouteDesc(rows, logits.stride(0), experts, k, groups, top_groups, group_best, scoring == "sigmoid",
+                    bool(renormalize), _DTYPES[logits.dtype], scale, 0)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return Routing(experts, *_Route.apply(logits, bias, d))
+    return Routing(experts, *_route_forward(logits, bias, d))
+
+
+def _dispatch(x, places):
+    dev = x.device
+    rows, k = places.shape
+    with L.on_device(dev):
+        out = torch.empty((rows * k, x.size(1)), dtype=x.dtype, device=dev)
+        d = L.ExchangeDesc(rows, x.stride(0), k, x.size(1), _DTYPES[x.dtype], 0)
+        status = L.lib().dg_exchange_dispatch(d, x.data_ptr(), places.data_ptr(), out.data_ptr(), L.raw_stream(dev))
+        if status:
+            L.check(status, "dispatch_rows")
+    return out
+
+
+def _combine(y, places, weights, residual, name):
+    dev = y.device
+    rows, k = places.shape
+    with L.on_device(dev):
+        out = torch.empty((rows, y.size(1)), dtype=y.dtype, device=dev)
+        d = L.ExchangeDesc(rows, 0 if residual is None else residual.stride(0), k, y.size(1), _DTYPES[y.dtype], 0)
+        status = L.lib().dg_exchange_combine(d, y.data_ptr(), places.data_ptr(), L.addr(weights), L.addr(residual),
+                                             out.data_ptr(), L.raw_stream(dev))
+        if status:
+            L.check(status, name)
+    return out
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, places):
+        ctx.save_for_backward(places)
+        return _dispatch(x, places)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _combine(grad.contiguous(), ctx.saved_tensors[0], None, None, "dispatch_rows"), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, residual, places):
+        ctx.save_for_backward(y, weights, places)
+        return _combine(y, places, weights, residual, "combine_rows")
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        y, weights, places = ctx.saved_tensors
+        need_y, need_w, need_r, _ = ctx.needs_input_grad
+        dev, rows_of = y.device, _whole_rows(grad)
+        rows, k = places.shape
+        with L.on_device(dev):
+            dy = torch.empty_like(y) if need_y else None
+            dw = torch.empty_like(weights) if need_w else None
+            d = L.ExchangeDesc(rows, rows_of.stride(0), k, y.size(1), _DTYPES[y.dtype], 0)
+            status = L.lib().dg_exchange_combine_backward(d, y.data_ptr(), places.data_ptr(), weights.data_ptr(),
+                                                          rows_of.data_ptr(), L.addr(dy), L.addr(dw), L.raw_stream(dev))
+            if status:
+                L.check(status, "combine_rows")
+        return dy, dw, grad if need_r else None, None
+
+
+def _check_rows(name, t, routing, rows):
+    _check(isinstance(routing, Routing), "routing must be a Routing")
+    _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
+    _check(t.dim() == 2 and t.size(0) == rows, f"{name} must have shape [{rows}, width], got {_shape(t)}")
+    _check(t.dtype in _DTYPES, f"{name} must be float32 or bfloat16, got {t.dtype}")
+    _check(t.device == routing.places.device, f"{name} must be on {routing.places.device}, got {t.device}")
+    _check(1 <= t.size(1) <= 1 << 20, f"the width must be 1 to 2^20, got {t.size(1)}")
+
+
+def dispatch_rows(x, routing):
+    """Rows in the order of the experts that they are routed to: x[i] at each of routing.places[i].
+
+    x [rows, width], float32 or bfloat16.  Returns [rows * k, width]: the first routing.sizes[0] rows are
+    expert 0's, in the order of x, and so on, as ``grouped_linear`` takes them with routing.sizes; rows
+    behind the last expert's (choices of none) are zeros.  Differentiable in x (once, in reverse): the
+    gradient is the sum over a row's choices, in 32 bits and in their order.
+    """
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("dispatch_rows", x)
+    _check(isinstance(routing, Routing), "routing must be a Routing")
+    _check_rows("x", x, routing, routing.rows)
+    x = _whole_rows(x)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Dispatch.apply(x, routing.places)
+    return _dispatch(x, routing.places)
+
+
+def combine_rows(y, routing, residual=None):
+    """The experts' results back: out[i] = residual[i] + sum_j routing.weights[i, j] y[routing.places[i, j]].
+
+    y [rows * k, width], in the order of ``dispatch_rows``, and residual [rows, width] (or None) of its
+    type, float32 or bfloat16.  Choices of none add nothing, whatever y holds behind the last
+    expert's rows.  Sums are 32 bits, in the choices' order, and rounded once.  Differentiable in y, the
+    routing's weights (and so in the router's logits) and the residual, once, in reverse.
+    """
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("combine_rows", y, residual)
+    _check(isinstance(routing, Routing), "routing must be a Routing")
+    _check_rows("y", y, routing, routing.rows * routing.k)
+    if residual is not None:
+        _check_rows("residual", residual, routing, routing.rows)
+        _check(residual.dtype == y.dtype and residual.size(1) == y.size(1),
+               f"residual must be {y.dtype} [{routing.rows}, {y.size(1)}], got {residual.dtype} {_shape(residual)}")
+        residual = _whole_rows(residual)
+    y, weights = y.contiguous(), routing.weights
+    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad
+                                    or residual is not None and residual.requires_grad):
+        return _Combine.apply(y, weights, residual, routing.places)
+    return _combine(y, routing.places, weights, residual, "combine_rows")

@@ -545,6 +545,70 @@ dg_status dg_rotate_backward(const dg_rotate_desc* desc, const void* q, const vo
                              void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes,
                              hipStream_t stream);
 
+/* Rows routed to experts by their logits x:
+ *   s = softmax(x), or 1 / (1 + exp(-x)) (sigmoid != 0)
+ *   v = x where bias is NULL and (groups == 1 or group_best == 1), else s + bias (0), in 64 bits;
+ *       an expert whose logit or bias is -inf is never chosen
+ *   groups > 1: n_experts / groups neighbouring experts each; a group is worth the sum of its group_best (1, 2)
+ *       largest v; only the experts of the top_groups worthiest are chosen from
+ *   experts[i] = the k largest v in falling order (NaN above all; of equals the lowest first), -1
+ *       where none is left
+ *   weights[i, j] = scale s[experts[i, j]], renormalize != 0: divided by the sum of the row's chosen s;
+ *       0 for a choice of none
+ *   sizes[e]     = rows that chose e
+ *   places[i, j] = place of the choice in the order by (expert, i), experts without their choices of
+ *       none, which follow: a choice of none has -1 - place
+ *   logits [n_rows, n_experts] of dtype (DG_F32 / DG_BF16), rows ld elements apart; bias float32
+ *   [n_experts] or NULL; weights float32, experts, places int32 [n_rows, k]; sizes int64 [n_experts]
+ * Backward: grad_logits of dtype, contiguous, from the experts of the forward pass (the choice itself
+ * has no gradient, nor has the bias).  Both enqueue work only; results repeat bit for bit. */
+typedef struct dg_route_desc {
+    int64_t n_rows;    /* n_rows * k < 2^31 */
+    int64_t ld;
+    int32_t n_experts; /* 1 .. 1024 */
+    int32_t k;         /* 1 .. min(64, n_experts) */
+    int32_t groups;    /* 1 .. 64, a divisor of n_experts */
+    int32_t top_groups;
+    int32_t group_best;
+    int32_t sigmoid, renormalize;
+    int32_t dtype;
+    float scale;
+    int32_t pad_;
+} dg_route_desc;
+
+size_t dg_route_workspace_size(const dg_route_desc* desc);
+dg_status dg_route_forward(const dg_route_desc* desc, const void* logits, const float* bias, float* weights,
+                           int32_t* experts, int64_t* sizes, int32_t* places, void* workspace,
+                           size_t workspace_bytes, hipStream_t stream);
+dg_status dg_route_backward(const dg_route_desc* desc, const void* logits, const int32_t* experts,
+                            const float* grad_weights, void* grad_logits, hipStream_t stream);
+
+/* Rows into the experts' order and back, by the places of dg_route_forward (a permutation of
+ * [0, n_rows * k); it is not checked):
+ *   dispatch  out[places[i, j]] = x[i]; zeros in the rows of choices of none
+ *   combine   out[i] = residual[i] + sum_j weights[i, j] y[places[i, j]] over the choices that are not
+ *             of none; weights NULL: ones (so the gradient of a dispatch), residual NULL: zeros
+ *   combine_backward  dy[places[i, j]] = weights[i, j] grad[i] (zeros in rows of choices of none),
+ *             dweights[i, j] = <grad[i], y[places[i, j]]> (0); either may be NULL
+ *   x, residual, grad [n_rows, width] of dtype, rows ld elements apart; the others contiguous, those in
+ *   the experts' order [n_rows * k, width]; weights, dweights float32 [n_rows, k] */
+typedef struct dg_exchange_desc {
+    int64_t n_rows; /* n_rows * k < 2^31 */
+    int64_t ld;
+    int32_t k;      /* 1 .. 64 */
+    int32_t width;
+    int32_t dtype;
+    int32_t pad_;
+} dg_exchange_desc;
+
+dg_status dg_exchange_dispatch(const dg_exchange_desc* desc, const void* x, const int32_t* places, void* out,
+                               hipStream_t stream);
+dg_status dg_exchange_combine(const dg_exchange_desc* desc, const void* y, const int32_t* places,
+                              const float* weights, const void* residual, void* out, hipStream_t stream);
+dg_status dg_exchange_combine_backward(const dg_exchange_desc* desc, const void* y, const int32_t* places,
+                                       const float* weights, const void* grad, void* dy, float* dweights,
+                                       hipStream_t stream);
+
 /* Message of the last failure on this thread ("" if none). */
 const char* dg_last_error(void);
 
