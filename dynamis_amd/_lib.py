@@ -18,6 +18,7 @@ LIB_PATH = os.environ.get("DYNAMIS_GRAPH_LIB") or os.path.join(_HERE, "libdynami
 
 DG_F32, DG_F64, DG_I64, DG_I32, DG_BF16 = 0, 1, 2, 3, 4
 DG_NEIGHBOR_PAD = 64
+DG_ACT_NONE, DG_ACT_SILU, DG_ACT_GELU = range(3)
 DG_OK, DG_ERR_INVALID, DG_ERR_WORKSPACE, DG_ERR_HIP, DG_ERR_RANGE, DG_ERR_CAPACITY = range(6)
 
 
@@ -264,6 +265,8 @@ def lib():
         "dg_grouped_forward": (_i32, [GD, _p, _p, _p, _p, _p, _p]),
         "dg_grouped_workspace_size": (_sz, [GD]),
         "dg_grouped_backward": (_i32, [GD] + [_p] * 8 + [_sz, _p]),
+        "dg_grouped_apply": (_i32, [GD, _i32] + [_p] * 7),
+        "dg_grouped_apply_backward": (_i32, [GD, _i32] + [_p] * 7),
         "dg_rotate_forward": (_i32, [RD] + [_p] * 9),
         "dg_rotate_workspace_size": (_sz, [RD]),
         "dg_rotate_backward": (_i32, [RD] + [_p] * 14 + [_sz, _p]),

@@ -2,6 +2,8 @@
 //
 //   y[i] = W[g(i)] x[i] + b[g(i)]        rows of a group follow each other
 //   dx[i] = W[g(i)]^T dy[i]   dW[g] = sum_{i in g} dy[i] x[i]^T   db[g] = sum_{i in g} dy[i]
+// and with an activation f and a residual r, in the epilogue of the same product (z is y above)
+//   y[i] = f(z[i]) + r[i]     dz[i] = dy[i] f'(z[i]), which takes dy's place above     dr = dy
 //
 // Tiles of 128 x 128 on the matrix units, 32 x 32 a step, sums in 32 bits.  Both operands pass
 // through LDS in rows of 128 bytes along the summed index (64 bfloat16 or 32 float), in chunks
@@ -36,6 +38,7 @@ using namespace dg;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
+using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 inline size_t al(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -56,6 +59,8 @@ struct Args {
     const void* b;  // weights [groups, ...]; x (dW)
     const void* bias;
     void* out;
+    const void* aux;  // of out's layout: the residual, or dy (dz)
+    int act;
     const int64_t* sizes;
     int64_t rows, groups;
     int cols, depth;  // of the result and of the sum (dW: the result is [cols = N, K = depth])
@@ -209,15 +214,44 @@ __device__ __forceinline__ void multiply(const char* rows, const char* cols, int
     }
 }
 
+// What becomes of a result: nothing, f(z) + r, or dy f'(z).
+enum { kPlain, kApply, kSlope };
+
+// f(z) (SLOPE: its derivative).  The normal distribution's share below z comes from erfc, which keeps its
+// digits far below zero where 1 + erf has lost them.
+template <bool SLOPE>
+__device__ __forceinline__ float activation(int act, float z)
+{
+    if (act == DG_ACT_SILU) {
+        const float e = expf(-z), s = 1.0f / (1.0f + e);
+        if constexpr (!SLOPE) return z * s;
+        // (1 - s as s e where that is finite)
+        return s * fmaf(z, z > -80.0f ? s * e : 1.0f, 1.0f);
+    }
+    if (act == DG_ACT_GELU) {
+        const float share = 0.5f * erfcf(-0.70710678f * z);
+        if constexpr (!SLOPE) return z * share;
+        return fmaf(z * 0.39894228f, expf(-0.5f * z * z), share);
+    }
+    return SLOPE ? 1.0f : z;
+}
+template <int EPI>
+__device__ __forceinline__ float finish(int act, float z, float aux)
+{
+    if constexpr (EPI == kApply) return activation<false>(act, z) + aux;
+    if constexpr (EPI == kSlope) return activation<true>(act, z) * aux;
+    return z;
+}
+
 // A wave's 64 x 64 of the result to memory: in the accumulators a lane holds four neighbouring
 // columns of one row, which LDS turns into whole chunks of rows.  `s` is the wave's own.
 constexpr int kOutRows = 32;
 template <typename T>
 constexpr int kOutPitch = 64 * (int)sizeof(T) + 16;
 
-template <typename T>
+template <typename T, int EPI = kPlain>
 __device__ __forceinline__ void write_out(const f32x16 (&acc)[2][2], char* s, int lane, T* out, int64_t ld, int n_rows,
-                                          int n_cols, const T* bias)
+                                          int n_cols, const T* bias, const T* aux = nullptr, int act = 0)
 {
     const int x = lane & 31, half = lane >> 5;
     constexpr int chunks = 64 / kChunk<T>;
@@ -232,6 +266,10 @@ __device__ __forceinline__ void write_out(const f32x16 (&acc)[2][2], char* s, in
                 for (int c = 0; c < 4; ++c) {
                     v[c] = acc[i][j][4 * q + c];
                     if (bias && col + c < n_cols) v[c] += (float)bias[col + c];
+                    if constexpr (EPI != kPlain) {
+                        const bool there = aux && col + c < n_cols && 32 * j + x < n_rows;
+                        v[c] = finish<EPI>(act, v[c], there ? (float)aux[(int64_t)(32 * j + x) * ld + col + c] : 0.0f);
+                    }
                 }
                 if constexpr (sizeof(T) == 4) {
                     *(f32x4*)(s + x * kOutPitch<T> + col * 4) = v;
@@ -376,7 +414,7 @@ __device__ __forceinline__ int64_t xcd_order(int64_t b, int64_t n)
 }
 
 // result[i, j] = sum_c a[i, c] W(j, c) (+ bias[j]), W(j, c) at weight[g][j][c], or (DX) [g][c][j].
-template <typename T, bool DX>
+template <typename T, bool DX, int EPI>
 __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
 {
     __shared__ __attribute__((aligned(16))) char s_a[kSlabBytes], s_b[kSlabBytes];
@@ -444,13 +482,16 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
                 multiply<T>(s_b, s_a, (w / 2) * 64, (w % 2) * 64, lane, acc);
             }
             const int c0 = col + (w / 2) * 64, r0 = (w % 2) * 64;
-            write_out<T>(acc, s_out + w * kOutRows * kOutPitch<T>, lane, (T*)a.out + (my_row + r0) * a.cols + c0, a.cols,
-                         n_rows - r0, a.cols - c0, !DX && a.bias ? (const T*)a.bias + my_group * a.cols + c0 : nullptr);
+            const int64_t at = (my_row + r0) * a.cols + c0;
+            write_out<T, EPI>(acc, s_out + w * kOutRows * kOutPitch<T>, lane, (T*)a.out + at, a.cols, n_rows - r0, a.cols - c0,
+                              !DX && a.bias ? (const T*)a.bias + my_group * a.cols + c0 : nullptr,
+                              EPI != kPlain && a.aux ? (const T*)a.aux + at : nullptr, a.act);
         }
     }
     // rows of no group
     const int64_t from = min(covered, a.rows) * a.cols, all = a.rows * a.cols;
-    for (int64_t i = from + blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) ((T*)a.out)[i] = (T)0.0f;
+    for (int64_t i = from + blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll)
+        ((T*)a.out)[i] = EPI == kApply && a.aux ? ((const T*)a.aux)[i] : (T)0.0f;
 }
 
 // The same for rows whose chunks of 16 bytes are whole, with at most 1 KB of summed indices: eight
@@ -474,7 +515,7 @@ __device__ __forceinline__ Buffer buffer_of(const void* p, int64_t bytes)
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)min(bytes, (int64_t)kOutside), 0x00020000);
 }
 
-template <typename T, bool DX, int PN>
+template <typename T, bool DX, int PN, int EPI>
 __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool single)
 {
     __shared__ __attribute__((aligned(16))) char s_panel[65536];
@@ -536,12 +577,28 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
             const int64_t my_row = r0, my_group = group;
             const int my_rows = n_rows;
             f32x16 acc[kTiles] = {};
+            // (what the epilogue reads, as the accumulators lie: four neighbouring columns of a row)
+            using Four = typename std::conditional<sizeof(T) == 4, u32x4, u32x2>::type;
+            Four aux[EPI == kPlain ? 1 : kTiles][4] = {};
             for (int step = 0; step < steps; ++step) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int rr = 4 * i + quarter;
                     *(u32x4*)(my_x + rr * kStepBytes + (chunk ^ (rr & 15)) * 16) = r[i];
                 }
+                if constexpr (EPI != kPlain)
+                    if (a.aux && step + 1 == steps) {  // (ahead of the next strip's rows)
+                        const Buffer b = buffer_of((const char*)a.aux + my_row * ld_out, my_rows * ld_out);
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const int c = col + 32 * t + 8 * q + 4 * half;
+                                const int at = c < a.cols ? x * (int)ld_out + c * (int)sizeof(T) : kOutside;
+                                if constexpr (sizeof(T) == 4) aux[t][q] = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
+                                else aux[t][q] = __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0);
+                            }
+                    }
                 if (step + 1 < steps) {
                     fetch(r0, n_rows, step + 1);
                 } else {
@@ -596,6 +653,15 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                         for (int k = 0; k < 4; ++k) v[k] = acc[piece_at * (kWide / 32) + t][4 * q + k];
                         if (bias && col + c < a.cols)
                             for (int k = 0; k < 4; ++k) v[k] += (float)bias[c + k];  // (whole chunks: four are there)
+                        if constexpr (EPI != kPlain) {
+                            const Four z = aux[piece_at * (kWide / 32) + t][q];
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t word = z[k * (int)sizeof(T) / 4];
+                                v[k] = finish<EPI>(a.act, v[k], __builtin_bit_cast(float, sizeof(T) == 4 ? word
+                                                                                          : k % 2      ? word & 0xffff0000u
+                                                                                                       : word << 16));
+                            }
+                        }
                         if constexpr (sizeof(T) == 4) {
                             *(f32x4*)(my_x + x * (kWide * 4) + ((at / 4) ^ (x & (kChunks - 1))) * 16) = v;
                         } else {
@@ -622,7 +688,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
     // rows of no group
     const int64_t from = min(covered, a.rows) * a.cols, all = a.rows * a.cols;
     for (int64_t i = from + blockIdx.x * (64ll * kStreamWaves) + threadIdx.x; i < all; i += gridDim.x * (64ll * kStreamWaves))
-        ((T*)a.out)[i] = (T)0.0f;
+        ((T*)a.out)[i] = EPI == kApply && a.aux ? ((const T*)a.aux)[i] : (T)0.0f;
 }
 
 // dW[g][n][k] = sum_i dy[i, n] x[i, k] over an item's rows of a group, 128 x 128 of it; the
@@ -825,16 +891,16 @@ dg_status launched(const char* what)
 constexpr int kCus = 256;
 int64_t stream_tiles(const Args& a) { return a.rows / kStreamRows + std::min(a.groups, a.rows) + 1; }
 
-template <typename T, bool DX, int PN>
+template <typename T, bool DX, int PN, int EPI>
 void run_stream(const Args& a, hipStream_t s)
 {
     const int64_t panels = (a.cols + PN - 1) / PN, tiles = stream_tiles(a);
     const int64_t lanes = std::max<int64_t>(1, std::min<int64_t>(tiles, kCus / panels));
-    hipLaunchKernelGGL((stream_kernel<T, DX, PN>), dim3((unsigned)(panels * lanes)), dim3(64 * kStreamWaves), 0, s, a,
+    hipLaunchKernelGGL((stream_kernel<T, DX, PN, EPI>), dim3((unsigned)(panels * lanes)), dim3(64 * kStreamWaves), 0, s, a,
                        lanes == tiles);
 }
 
-template <typename T, bool DX>
+template <typename T, bool DX, int EPI = kPlain>
 void run_rows(const Args& a, hipStream_t s)
 {
     // Whole chunks and a panel that fits: the streaming kernel (128 by 128 in bfloat16, 864 rows: 6.3
@@ -844,19 +910,19 @@ void run_rows(const Args& a, hipStream_t s)
     // rows 13.9, 12.6 and 11.1 us).  Rows of more than 512 bytes leave the panel's LDS 64 columns.
     const int64_t bytes = a.depth * (int64_t)sizeof(T);
     const bool whole = bytes % 16 == 0 && a.cols % kChunk<T> == 0 && ((uintptr_t)a.a & 15) == 0 &&
-                       ((uintptr_t)a.out & 15) == 0 && a.cols * (int64_t)sizeof(T) <= 1 << 24;
+                       ((uintptr_t)a.out & 15) == 0 && ((uintptr_t)a.aux & 15) == 0 && a.cols * (int64_t)sizeof(T) <= 1 << 24;
     if (whole && bytes <= 1024) {
         const int64_t work = stream_tiles(a) * ((a.cols + 127) / 128);  // workgroups with panels of 128
-        if (work <= kCus / 4) run_stream<T, DX, 32>(a, s);
-        else if (bytes > 512 || work <= kCus / 2) run_stream<T, DX, 64>(a, s);
-        else run_stream<T, DX, 128>(a, s);
+        if (work <= kCus / 4) run_stream<T, DX, 32, EPI>(a, s);
+        else if (bytes > 512 || work <= kCus / 2) run_stream<T, DX, 64, EPI>(a, s);
+        else run_stream<T, DX, 128, EPI>(a, s);
         return;
     }
 
     const int64_t tiles = (a.rows / kTile + std::min(a.groups, a.rows) + 1) * ((a.cols + kTile - 1) / kTile);
     unsigned grid = (unsigned)std::min<int64_t>(tiles, 256 * 2);
     if (grid > kXcds) grid = (grid + kXcds - 1) / kXcds * kXcds;
-    hipLaunchKernelGGL((rows_kernel<T, DX>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((rows_kernel<T, DX, EPI>), dim3(grid), dim3(256), 0, s, a);
 }
 
 template <typename T>
@@ -900,6 +966,48 @@ dg_status dg_grouped_forward(const dg_grouped_desc* d, const void* x, const void
     if (d->dtype == DG_BF16) run_rows<__bf16, false>(a, s);
     else run_rows<float, false>(a, s);
     return launched("dg_grouped_forward");
+}
+
+static dg_status apply(const dg_grouped_desc* d, int32_t act, bool slope, const void* x, const void* weight, const int64_t* sizes,
+                       const void* bias, const void* aux, void* out, hipStream_t s)
+{
+    dg_status st = check(d);
+    if (st != DG_OK) return st;
+    if (act != DG_ACT_NONE && act != DG_ACT_SILU && act != DG_ACT_GELU) return fail(DG_ERR_INVALID, "unknown activation");
+    if (d->n_rows == 0) return DG_OK;
+    if (!x || !weight || !sizes || !out || (slope && !aux)) return fail(DG_ERR_INVALID, "inputs or outputs are NULL");
+    Args a = {};
+    a.a = x;
+    a.b = weight;
+    a.bias = bias;
+    a.aux = aux;
+    a.act = act;
+    a.out = out;
+    a.sizes = sizes;
+    a.rows = d->n_rows;
+    a.groups = d->n_groups;
+    a.cols = d->n;
+    a.depth = d->k;
+    if (d->dtype == DG_BF16) {
+        if (slope) run_rows<__bf16, false, kSlope>(a, s);
+        else run_rows<__bf16, false, kApply>(a, s);
+    } else {
+        if (slope) run_rows<float, false, kSlope>(a, s);
+        else run_rows<float, false, kApply>(a, s);
+    }
+    return launched("dg_grouped_apply");
+}
+
+dg_status dg_grouped_apply(const dg_grouped_desc* d, int32_t act, const void* x, const void* weight, const int64_t* sizes,
+                           const void* bias, const void* residual, void* y, hipStream_t s)
+{
+    return apply(d, act, false, x, weight, sizes, bias, residual, y, s);
+}
+
+dg_status dg_grouped_apply_backward(const dg_grouped_desc* d, int32_t act, const void* x, const void* weight,
+                                    const int64_t* sizes, const void* bias, const void* grad_y, void* dz, hipStream_t s)
+{
+    return apply(d, act, true, x, weight, sizes, bias, grad_y, dz, s);
 }
 
 size_t dg_grouped_workspace_size(const dg_grouped_desc* d)

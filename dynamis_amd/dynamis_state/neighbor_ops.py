@@ -368,12 +368,20 @@ def _grouped_desc(x, weight):
     return L.GroupedDesc(x.size(0), weight.size(0), weight.size(2), weight.size(1), _DTYPES[x.dtype], 0)
 
 
-def _grouped_forward(x, weight, sizes, bias):
-    dev = x.device
+_ACTIVATIONS = {None: L.DG_ACT_NONE, "silu": L.DG_ACT_SILU, "gelu": L.DG_ACT_GELU}
+
+
+def _grouped_forward(x, weight, sizes, bias, act=L.DG_ACT_NONE, residual=None):
+    dev, lib = x.device, L.lib()
     with L.on_device(dev):
         y = torch.empty((x.size(0), weight.size(1)), dtype=x.dtype, device=dev)
-        status = L.lib().dg_grouped_forward(_grouped_desc(x, weight), x.data_ptr(), weight.data_ptr(), sizes.data_ptr(),
-                                            L.addr(bias), y.data_ptr(), L.raw_stream(dev))
+        d = _grouped_desc(x, weight)
+        if act == L.DG_ACT_NONE and residual is None:
+            status = lib.dg_grouped_forward(d, x.data_ptr(), weight.data_ptr(), sizes.data_ptr(), L.addr(bias), y.data_ptr(),
+                                            L.raw_stream(dev))
+        else:
+            status = lib.dg_grouped_apply(d, act, x.data_ptr(), weight.data_ptr(), sizes.data_ptr(), L.addr(bias),
+                                          L.addr(residual), y.data_ptr(), L.raw_stream(dev))
         if status:
             L.check(status, "grouped_linear")
     return y
@@ -381,19 +389,30 @@ def _grouped_forward(x, weight, sizes, bias):
 
 class _Grouped(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, sizes, bias):
-        ctx.save_for_backward(x, weight, sizes)
-        ctx.desc = _grouped_desc(x, weight)
-        return _grouped_forward(x, weight, sizes, bias)
+    def forward(ctx, x, weight, sizes, bias, act=L.DG_ACT_NONE, residual=None):
+        # (with an activation the backward pass makes z again: fewer bytes than keeping it)
+        ctx.save_for_backward(x, weight, sizes, bias if act != L.DG_ACT_NONE else None)
+        ctx.desc, ctx.act = _grouped_desc(x, weight), act
+        return _grouped_forward(x, weight, sizes, bias, act, residual)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, sizes = ctx.saved_tensors
-        need_x, need_w, _, need_b = ctx.needs_input_grad
+        x, weight, sizes, bias = ctx.saved_tensors
+        need_x, need_w, _, need_b, _, need_r = ctx.needs_input_grad
+        dresidual = grad if need_r else None
+        if not (need_x or need_w or need_b):
+            return None, None, None, None, None, dresidual
         lib, dev, grad = L.lib(), x.device, grad.contiguous()
         d = ctx.desc
         with L.on_device(dev):
+            if ctx.act != L.DG_ACT_NONE:
+                dz = torch.empty_like(grad)
+                status = lib.dg_grouped_apply_backward(d, ctx.act, x.data_ptr(), weight.data_ptr(), sizes.data_ptr(),
+                                                       L.addr(bias), grad.data_ptr(), dz.data_ptr(), L.raw_stream(dev))
+                if status:
+                    L.check(status, "grouped_linear")
+                grad = dz
             dx = torch.empty_like(x) if need_x else None
             dw = torch.empty_like(weight) if need_w or need_b else None
             db = torch.empty(weight.shape[:2], dtype=x.dtype, device=dev) if need_b else None
@@ -404,10 +423,10 @@ class _Grouped(torch.autograd.Function):
                                              addr(dx), addr(dw), addr(db), addr(ws), wsb, L.raw_stream(dev))
             if status:
                 L.check(status, "grouped_linear")
-        return dx, dw if need_w else None, None, db
+        return dx, dw if need_w else None, None, db, None, dresidual
 
 
-def _check_grouped(x, weight, sizes, bias):
+def _check_grouped(x, weight, sizes, bias, residual):
     """The refusals of grouped_linear, with their messages."""
     _check(isinstance(x, torch.Tensor) and x.is_cuda, "x must be a CUDA tensor")
     _check(x.dim() == 2, f"x must have shape [rows, k], got {_shape(x)}")
@@ -430,23 +449,31 @@ def _check_grouped(x, weight, sizes, bias):
         _check(isinstance(bias, torch.Tensor), "bias must be a tensor")
         _check(bias.device == x.device and bias.dtype == x.dtype and tuple(bias.shape) == tuple(weight.shape[:2]),
                f"bias must be {x.dtype} [{groups}, {weight.size(1)}] on {x.device}, got {bias.dtype} {_shape(bias)}")
+    if residual is not None:
+        _check(isinstance(residual, torch.Tensor), "residual must be a tensor")
+        _check(residual.device == x.device and residual.dtype == x.dtype
+               and tuple(residual.shape) == (x.size(0), weight.size(1)),
+               f"residual must be {x.dtype} [{x.size(0)}, {weight.size(1)}] on {x.device}, "
+               f"got {residual.dtype} {_shape(residual)}")
 
 
-def _grouped_is_fine(x, weight, sizes, bias):
+def _grouped_is_fine(x, weight, sizes, bias, residual):
     """Whether _check_grouped would pass for tensors on one device, without its messages' host time."""
     if not (type(x) in _TENSORS and type(weight) in _TENSORS and x.dim() == 2 and weight.dim() == 3 and x.is_cuda
-            and (bias is None or type(bias) in _TENSORS)):
+            and (bias is None or type(bias) in _TENSORS) and (residual is None or type(residual) in _TENSORS)):
         return False
     groups, n, k = weight.shape
     dev, dtype = x.device, x.dtype
     return (x.size(1) == k and 1 <= groups <= 1 << 20 and 1 <= k <= 1 << 20 and 1 <= n <= 1 << 20
             and dtype in _DTYPES and weight.dtype == dtype and weight.device == dev
             and sizes.device == dev and sizes.dtype == torch.int64 and sizes.shape == (groups,)
-            and (bias is None or bias.dtype == dtype and bias.device == dev and bias.shape == (groups, n)))
+            and (bias is None or bias.dtype == dtype and bias.device == dev and bias.shape == (groups, n))
+            and (residual is None
+                 or residual.dtype == dtype and residual.device == dev and residual.shape == (x.size(0), n)))
 
 
-def grouped_linear(x, weight, sizes, bias=None):
-    """Linear maps by group over ragged rows: y[i] = weight[g(i)] @ x[i] + bias[g(i)].
+def grouped_linear(x, weight, sizes, bias=None, activation=None, residual=None):
+    """Linear maps by group over ragged rows: y[i] = f(weight[g(i)] @ x[i] + bias[g(i)]) + residual[i].
 
     x [rows, k], weight [groups, n, k] (torch.nn.Linear's layout for each group), bias
     [groups, n]; float32 or bfloat16, one type.  sizes [groups] int64: the first sizes[0] rows are
@@ -457,20 +484,31 @@ def grouped_linear(x, weight, sizes, bias=None):
     all sizes once for each group and 128 x 128 of its weight: its time grows with the square of
     the groups (of one such tile: 4,096 groups 0.26 ms, 65,536 groups 45 ms).
 
-    Differentiable in x, weight and bias (once, in reverse: a tensor with a forward-mode tangent is
+    activation f: None, "silu" (z / (1 + exp(-z))) or "gelu" (z times the normal distribution's share below z,
+    by its error function); residual [rows, n] of x's type.  Both are taken in 32 bits on the way to
+    memory, and y is rounded once.  Rows behind the last group give their residual.  The backward pass with an
+    activation makes z again from x and the weights, and rounds its gradient to x's type before the other products.
+
+    Differentiable in x, weight, bias and residual (once, in reverse: a tensor with a forward-mode tangent is
     refused).  Sums are float32, in a fixed order: results
     repeat bit for bit.
     """
     if forward_ad._current_level >= 0:
-        _refuse_tangents("grouped_linear", x, weight, bias)
+        _refuse_tangents("grouped_linear", x, weight, bias, residual)
+    if not (activation is None or isinstance(activation, str) and activation in _ACTIVATIONS):
+        raise RuntimeError(f'activation must be None, "silu" or "gelu", got {activation!r}')
+    act = _ACTIVATIONS[activation]
     if not isinstance(sizes, torch.Tensor):
         sizes = torch.as_tensor(sizes)
-    if not _grouped_is_fine(x, weight, sizes, bias):
-        _check_grouped(x, weight, sizes, bias)
+    if not _grouped_is_fine(x, weight, sizes, bias, residual):
+        _check_grouped(x, weight, sizes, bias, residual)
         sizes = sizes.to(x.device)
     x, weight, sizes = x.contiguous(), weight.contiguous(), sizes.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad):
-        return _Grouped.apply(x, weight, sizes, bias)
-    return _grouped_forward(x, weight, sizes, bias)
+    if residual is not None:
+        residual = residual.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad
+                                    or residual is not None and residual.requires_grad):
+        return _Grouped.apply(x, weight, sizes, bias, act, residual)
+    return _grouped_forward(x, weight, sizes, bias, act, residual)

@@ -505,6 +505,22 @@ dg_status dg_grouped_backward(const dg_grouped_desc* desc, const void* x, const 
                               void* dbias, void* workspace, size_t workspace_bytes,
                               hipStream_t stream);
 
+/* The same with an activation f and a residual in the product's epilogue, z being y above:
+ *   y[i] = f(z[i]) + residual[i]       residual like y or NULL (zeros)
+ *   dz[i] = grad_y[i] f'(z[i])         z made again from x and the weights
+ * DG_ACT_SILU: z / (1 + exp(-z)); DG_ACT_GELU: z times the normal distribution's share below z.  Rows behind
+ * the last group give their residual; their dz is zero.  dz, rounded to dtype, is the grad_y of
+ * dg_grouped_backward for the other gradients; that of the residual is grad_y itself. */
+#define DG_ACT_NONE 0
+#define DG_ACT_SILU 1
+#define DG_ACT_GELU 2
+dg_status dg_grouped_apply(const dg_grouped_desc* desc, int32_t activation, const void* x, const void* weight,
+                           const int64_t* sizes, const void* bias, const void* residual, void* y,
+                           hipStream_t stream);
+dg_status dg_grouped_apply_backward(const dg_grouped_desc* desc, int32_t activation, const void* x,
+                                    const void* weight, const int64_t* sizes, const void* bias,
+                                    const void* grad_y, void* dz, hipStream_t stream);
+
 /* Heads of queries and keys, normalised one by one and rotated by their nodes' positions:
  *   n[c] = x[c] / sqrt(mean_c x[c]^2 + eps) * weight[c]     (norm != 0; else n = x)
  *   theta[j] = positions[i, axis of j] * frequencies[j], the pairs j < P = sum of sections, the
