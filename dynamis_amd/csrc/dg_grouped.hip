@@ -26,6 +26,7 @@
 
 #include "../../include/dynamis_graph.h"
 #include "dg_grid.hpp"
+#include "dg_lanes.hpp"
 
 namespace dg {
 dg_status fail(dg_status st, const std::string& msg);  // dg_graph.hip
@@ -217,21 +218,34 @@ __device__ __forceinline__ void multiply(const char* rows, const char* cols, int
 // What becomes of a result: nothing, f(z) + r, or dy f'(z).
 enum { kPlain, kApply, kSlope };
 
-// f(z) (SLOPE: its derivative).  The normal distribution's share below z comes from erfc, which keeps its
-// digits far below zero where 1 + erf has lost them.
+// f(z) (SLOPE: its derivative), in some ten to thirty instructions, which the library's functions would take
+// twice.  silu: from exp(-|z|), which neither overflows nor loses 1 - s.  gelu: the normal distribution's share
+// beyond |z| is exp(-z^2 / 2) t Q(t) with t = 1 / (1 + 0.318 |z|), so that it keeps its digits far out; Q is a
+// least-maximum fit of degree 9 to it in relative error (0.55 2^-24, 5.1 2^-24 as evaluated).
 template <bool SLOPE>
 __device__ __forceinline__ float activation(int act, float z)
 {
     if (act == DG_ACT_SILU) {
-        const float e = expf(-z), s = 1.0f / (1.0f + e);
+        const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
+        const float s = z < 0.0f ? e * r : r;
         if constexpr (!SLOPE) return z * s;
-        // (1 - s as s e where that is finite)
-        return s * fmaf(z, z > -80.0f ? s * e : 1.0f, 1.0f);
+        return s * fmaf(z, z < 0.0f ? r : e * r, 1.0f);
     }
     if (act == DG_ACT_GELU) {
-        const float share = 0.5f * erfcf(-0.70710678f * z);
+        const float e = __builtin_amdgcn_exp2f(-0.72134752f * (z * z)), t = __builtin_amdgcn_rcpf(fmaf(0.318f, fabsf(z), 1.0f));
+        float q = -0.020624028518795967f;
+        q = fmaf(q, t, 0.09520687907934189f);
+        q = fmaf(q, t, -0.15045107901096344f);
+        q = fmaf(q, t, 0.07162534445524216f);
+        q = fmaf(q, t, -0.011254116892814636f);
+        q = fmaf(q, t, 0.06007798761129379f);
+        q = fmaf(q, t, 0.08761146664619446f);
+        q = fmaf(q, t, 0.11408133804798126f);
+        q = fmaf(q, t, 0.1268625557422638f);
+        q = fmaf(q, t, 0.12686364352703094f);
+        const float beyond = e * (t * q), share = z < 0.0f ? beyond : 1.0f - beyond;
         if constexpr (!SLOPE) return z * share;
-        return fmaf(z * 0.39894228f, expf(-0.5f * z * z), share);
+        return fmaf(z * e, 0.39894228f, share);
     }
     return SLOPE ? 1.0f : z;
 }
@@ -577,28 +591,12 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
             const int64_t my_row = r0, my_group = group;
             const int my_rows = n_rows;
             f32x16 acc[kTiles] = {};
-            // (what the epilogue reads, as the accumulators lie: four neighbouring columns of a row)
-            using Four = typename std::conditional<sizeof(T) == 4, u32x4, u32x2>::type;
-            Four aux[EPI == kPlain ? 1 : kTiles][4] = {};
             for (int step = 0; step < steps; ++step) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int rr = 4 * i + quarter;
                     *(u32x4*)(my_x + rr * kStepBytes + (chunk ^ (rr & 15)) * 16) = r[i];
                 }
-                if constexpr (EPI != kPlain)
-                    if (a.aux && step + 1 == steps) {  // (ahead of the next strip's rows)
-                        const Buffer b = buffer_of((const char*)a.aux + my_row * ld_out, my_rows * ld_out);
-#pragma unroll
-                        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const int c = col + 32 * t + 8 * q + 4 * half;
-                                const int at = c < a.cols ? x * (int)ld_out + c * (int)sizeof(T) : kOutside;
-                                if constexpr (sizeof(T) == 4) aux[t][q] = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
-                                else aux[t][q] = __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0);
-                            }
-                    }
                 if (step + 1 < steps) {
                     fetch(r0, n_rows, step + 1);
                 } else {
@@ -638,49 +636,99 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                         }
                     }
             }
-            // the strip's result, 256 bytes (or the panel's) of each row at once
-            constexpr int kWide = PN * (int)sizeof(T) < kStepBytes ? PN : kStep, kPieces = PN / kWide, kChunks = kWide / C;
-            const Buffer out = buffer_of((const char*)a.out + my_row * ld_out, my_rows * ld_out);
-            const T* bias = !DX && a.bias ? (const T*)a.bias + my_group * a.cols + col : nullptr;
+            if constexpr (EPI == kPlain) {
+                // the strip's result, 256 bytes (or the panel's) of each row at once
+                constexpr int kWide = PN * (int)sizeof(T) < kStepBytes ? PN : kStep, kPieces = PN / kWide, kChunks = kWide / C;
+                const Buffer out = buffer_of((const char*)a.out + my_row * ld_out, my_rows * ld_out);
+                const T* bias = !DX && a.bias ? (const T*)a.bias + my_group * a.cols + col : nullptr;
 #pragma unroll
-            for (int piece_at = 0; piece_at < kPieces; ++piece_at) {
+                for (int piece_at = 0; piece_at < kPieces; ++piece_at) {
 #pragma unroll
-                for (int t = 0; t < kWide / 32; ++t)
+                    for (int t = 0; t < kWide / 32; ++t)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int at = 32 * t + 8 * q + 4 * half, c = piece_at * kWide + at;
-                        f32x4 v;
-                        for (int k = 0; k < 4; ++k) v[k] = acc[piece_at * (kWide / 32) + t][4 * q + k];
-                        if (bias && col + c < a.cols)
-                            for (int k = 0; k < 4; ++k) v[k] += (float)bias[c + k];  // (whole chunks: four are there)
-                        if constexpr (EPI != kPlain) {
-                            const Four z = aux[piece_at * (kWide / 32) + t][q];
-                            for (int k = 0; k < 4; ++k) {
-                                const uint32_t word = z[k * (int)sizeof(T) / 4];
-                                v[k] = finish<EPI>(a.act, v[k], __builtin_bit_cast(float, sizeof(T) == 4 ? word
-                                                                                          : k % 2      ? word & 0xffff0000u
-                                                                                                       : word << 16));
+                        for (int q = 0; q < 4; ++q) {
+                            const int at = 32 * t + 8 * q + 4 * half, c = piece_at * kWide + at;
+                            f32x4 v;
+                            for (int k = 0; k < 4; ++k) v[k] = acc[piece_at * (kWide / 32) + t][4 * q + k];
+                            if (bias && col + c < a.cols)
+                                for (int k = 0; k < 4; ++k) v[k] += (float)bias[c + k];  // (whole chunks: four are there)
+                            if constexpr (sizeof(T) == 4) {
+                                *(f32x4*)(my_x + x * (kWide * 4) + ((at / 4) ^ (x & (kChunks - 1))) * 16) = v;
+                            } else {
+                                __attribute__((ext_vector_type(4))) __bf16 y;
+                                for (int k = 0; k < 4; ++k) y[k] = (__bf16)v[k];
+                                *(decltype(y)*)(my_x + x * (kWide * 2) + ((at / 8) ^ (x & (kChunks - 1))) * 16 + at % 8 * 2) = y;
                             }
                         }
-                        if constexpr (sizeof(T) == 4) {
-                            *(f32x4*)(my_x + x * (kWide * 4) + ((at / 4) ^ (x & (kChunks - 1))) * 16) = v;
-                        } else {
-                            __attribute__((ext_vector_type(4))) __bf16 y;
-                            for (int k = 0; k < 4; ++k) y[k] = (__bf16)v[k];
-                            *(decltype(y)*)(my_x + x * (kWide * 2) + ((at / 8) ^ (x & (kChunks - 1))) * 16 + at % 8 * 2) = y;
-                        }
-                    }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int k = 0; k < kStripRows * kChunks / 64; ++k) {
-                    const int id = k * 64 + lane, rr = id / kChunks, c = id % kChunks;
-                    const int at = (col + piece_at * kWide) * (int)sizeof(T) + c * 16;
-                    const u32x4 v = *(const u32x4*)(my_x + rr * (kWide * (int)sizeof(T)) + (c ^ (rr & (kChunks - 1))) * 16);
-                    __builtin_amdgcn_raw_buffer_store_b128(v, out, at < ld_out ? rr * (int)ld_out + at : kOutside, 0, 0);
+                    for (int k = 0; k < kStripRows * kChunks / 64; ++k) {
+                        const int id = k * 64 + lane, rr = id / kChunks, c = id % kChunks;
+                        const int at = (col + piece_at * kWide) * (int)sizeof(T) + c * 16;
+                        const u32x4 v = *(const u32x4*)(my_x + rr * (kWide * (int)sizeof(T)) + (c ^ (rr & (kChunks - 1))) * 16);
+                        __builtin_amdgcn_raw_buffer_store_b128(v, out, at < ld_out ? rr * (int)ld_out + at : kOutside, 0, 0);
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
                 }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+            } else {
+                // In 32 bits through the same 8 KB, 64 columns of each row at once, so that a lane has
+                // whole chunks of rows, the same columns in each of them: bias, residual (or dy) and
+                // activation there, and one rounding.  The chunks of `aux` are under way meanwhile.
+                constexpr int kWide = PN < 64 ? PN : 64, kPieces = PN / kWide, kChunks = kWide / C, kEach = kStripRows * kChunks / 64;
+                const Buffer out = buffer_of((const char*)a.out + my_row * ld_out, my_rows * ld_out);
+                const Buffer in = buffer_of((const char*)a.aux + my_row * ld_out, a.aux ? my_rows * ld_out : 0);
+                const int c = lane % kChunks, r_first = lane / kChunks;
+#pragma unroll
+                for (int piece_at = 0; piece_at < kPieces; ++piece_at) {
+                    const int first = col + piece_at * kWide + c * C;  // the lane's first column
+                    const int at = first < a.cols ? first * (int)sizeof(T) : kOutside;
+                    u32x4 aux[kEach];
+#pragma unroll
+                    for (int k = 0; k < kEach; ++k)
+                        aux[k] = __builtin_amdgcn_raw_buffer_load_b128(in, at == kOutside ? at : (r_first + k * (64 / kChunks)) * (int)ld_out + at, 0, 0);
+                    float b[C] = {};
+                    if (a.bias && first < a.cols) {
+                        const T* p = (const T*)a.bias + my_group * a.cols + first;
+                        for (int i = 0; i < C; ++i) b[i] = (float)p[i];
+                    }
+#pragma unroll
+                    for (int t = 0; t < kWide / 32; ++t)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            f32x4 v;
+                            for (int k = 0; k < 4; ++k) v[k] = acc[piece_at * (kWide / 32) + t][4 * q + k];
+                            *(f32x4*)(my_x + x * (kWide * 4) + ((8 * t + 2 * q + half) ^ (x & (kWide / 4 - 1))) * 16) = v;
+                        }
+                    wave_sync();
+#pragma unroll
+                    for (int k = 0; k < kEach; ++k) {
+                        const int rr = r_first + k * (64 / kChunks);
+                        float v[C];
+#pragma unroll
+                        for (int h = 0; h < C / 4; ++h) {
+                            const f32x4 f = *(const f32x4*)(my_x + rr * (kWide * 4) + ((c * (C / 4) + h) ^ (rr & (kWide / 4 - 1))) * 16);
+                            for (int i = 0; i < 4; ++i) v[4 * h + i] = f[i];
+                        }
+                        u32x4 y;
+                        if constexpr (sizeof(T) == 4) {
+                            const f32x4 z = __builtin_bit_cast(f32x4, aux[k]);
+                            f32x4 f;
+                            for (int i = 0; i < 4; ++i) f[i] = finish<EPI>(a.act, v[i] + b[i], z[i]);
+                            y = __builtin_bit_cast(u32x4, f);
+                        } else {
+                            bf16x8 f;
+                            for (int i = 0; i < 8; ++i) {
+                                const uint32_t word = aux[k][i / 2];
+                                f[i] = (__bf16)finish<EPI>(a.act, v[i] + b[i], __builtin_bit_cast(float, i % 2 ? word & 0xffff0000u : word << 16));
+                            }
+                            y = __builtin_bit_cast(u32x4, f);
+                        }
+                        __builtin_amdgcn_raw_buffer_store_b128(y, out, at == kOutside ? at : rr * (int)ld_out + at, 0, 0);
+                    }
+                    wave_sync();
+                }
             }
             if (u < end && group != my_group) fill_panel(group);
         }
