@@ -222,16 +222,16 @@ enum { kPlain, kApply, kSlope };
 // twice.  silu: from exp(-|z|), which neither overflows nor loses 1 - s.  gelu: the normal distribution's share
 // beyond |z| is exp(-z^2 / 2) t Q(t) with t = 1 / (1 + 0.318 |z|), so that it keeps its digits far out; Q is a
 // least-maximum fit of degree 9 to it in relative error (0.55 2^-24, 5.1 2^-24 as evaluated).
-template <bool SLOPE>
-__device__ __forceinline__ float activation(int act, float z)
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float activation(float z)
 {
-    if (act == DG_ACT_SILU) {
+    if constexpr (ACT == DG_ACT_SILU) {
         const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
         const float s = z < 0.0f ? e * r : r;
         if constexpr (!SLOPE) return z * s;
         return s * fmaf(z, z < 0.0f ? r : e * r, 1.0f);
     }
-    if (act == DG_ACT_GELU) {
+    if constexpr (ACT == DG_ACT_GELU) {
         const float e = __builtin_amdgcn_exp2f(-0.72134752f * (z * z)), t = __builtin_amdgcn_rcpf(fmaf(0.318f, fabsf(z), 1.0f));
         float q = -0.020624028518795967f;
         q = fmaf(q, t, 0.09520687907934189f);
@@ -249,12 +249,18 @@ __device__ __forceinline__ float activation(int act, float z)
     }
     return SLOPE ? 1.0f : z;
 }
-template <int EPI>
-__device__ __forceinline__ float finish(int act, float z, float aux)
+// N results at once (the branch is the same for the whole grid, and the N chains overlap).
+template <int EPI, int ACT, int N>
+__device__ __forceinline__ void finish_as(float (&z)[N], const float (&aux)[N])
 {
-    if constexpr (EPI == kApply) return activation<false>(act, z) + aux;
-    if constexpr (EPI == kSlope) return activation<true>(act, z) * aux;
-    return z;
+    for (int i = 0; i < N; ++i) z[i] = EPI == kApply ? activation<ACT, false>(z[i]) + aux[i] : activation<ACT, true>(z[i]) * aux[i];
+}
+template <int EPI, int N>
+__device__ __forceinline__ void finish(int act, float (&z)[N], const float (&aux)[N])
+{
+    if (act == DG_ACT_SILU) finish_as<EPI, DG_ACT_SILU>(z, aux);
+    else if (act == DG_ACT_GELU) finish_as<EPI, DG_ACT_GELU>(z, aux);
+    else finish_as<EPI, DG_ACT_NONE>(z, aux);
 }
 
 // A wave's 64 x 64 of the result to memory: in the accumulators a lane holds four neighbouring
@@ -280,10 +286,15 @@ __device__ __forceinline__ void write_out(const f32x16 (&acc)[2][2], char* s, in
                 for (int c = 0; c < 4; ++c) {
                     v[c] = acc[i][j][4 * q + c];
                     if (bias && col + c < n_cols) v[c] += (float)bias[col + c];
-                    if constexpr (EPI != kPlain) {
-                        const bool there = aux && col + c < n_cols && 32 * j + x < n_rows;
-                        v[c] = finish<EPI>(act, v[c], there ? (float)aux[(int64_t)(32 * j + x) * ld + col + c] : 0.0f);
-                    }
+                }
+                if constexpr (EPI != kPlain) {
+                    float z[4], r[4] = {};
+                    for (int c = 0; c < 4; ++c) z[c] = v[c];
+                    if (aux && 32 * j + x < n_rows)
+                        for (int c = 0; c < 4; ++c)
+                            if (col + c < n_cols) r[c] = (float)aux[(int64_t)(32 * j + x) * ld + col + c];
+                    finish<EPI>(act, z, r);
+                    for (int c = 0; c < 4; ++c) v[c] = z[c];
                 }
                 if constexpr (sizeof(T) == 4) {
                     *(f32x4*)(s + x * kOutPitch<T> + col * 4) = v;
@@ -711,18 +722,19 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                             const f32x4 f = *(const f32x4*)(my_x + rr * (kWide * 4) + ((c * (C / 4) + h) ^ (rr & (kWide / 4 - 1))) * 16);
                             for (int i = 0; i < 4; ++i) v[4 * h + i] = f[i];
                         }
+                        float r[C];
+                        for (int i = 0; i < C; ++i) {
+                            const uint32_t word = aux[k][i * (int)sizeof(T) / 4];
+                            r[i] = as_float(sizeof(T) == 4 ? word : i % 2 ? word & 0xffff0000u : word << 16);
+                            v[i] += b[i];
+                        }
+                        finish<EPI>(a.act, v, r);
                         u32x4 y;
                         if constexpr (sizeof(T) == 4) {
-                            const f32x4 z = __builtin_bit_cast(f32x4, aux[k]);
-                            f32x4 f;
-                            for (int i = 0; i < 4; ++i) f[i] = finish<EPI>(a.act, v[i] + b[i], z[i]);
-                            y = __builtin_bit_cast(u32x4, f);
+                            for (int i = 0; i < 4; ++i) y[i] = as_bits(v[i]);
                         } else {
                             bf16x8 f;
-                            for (int i = 0; i < 8; ++i) {
-                                const uint32_t word = aux[k][i / 2];
-                                f[i] = (__bf16)finish<EPI>(a.act, v[i] + b[i], __builtin_bit_cast(float, i % 2 ? word & 0xffff0000u : word << 16));
-                            }
+                            for (int i = 0; i < 8; ++i) f[i] = (__bf16)v[i];
                             y = __builtin_bit_cast(u32x4, f);
                         }
                         __builtin_amdgcn_raw_buffer_store_b128(y, out, at == kOutside ? at : rr * (int)ld_out + at, 0, 0);
