@@ -25,8 +25,9 @@ __device__ __forceinline__ void over_lanes(int n, F&& step)
     if (n > 2) step([](uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true); });   // 2 3 0 1
     if (n > 4) step([](uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xf, 0xf, true); });  // mirrored in 8
     if (n > 8) step([](uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x140, 0xf, 0xf, true); });  // in 16
-    if (n > 16) step([](uint32_t x) { return (uint32_t)__shfl_xor((int)x, 16, 64); });
-    if (n > 32) step([](uint32_t x) { return (uint32_t)__shfl_xor((int)x, 32, 64); });
+    // (the swap of a value with itself holds, in each lane, its own and the other's: what is not its own)
+    if (n > 16) step([](uint32_t x) { const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false); return r[0] ^ r[1] ^ x; });
+    if (n > 32) step([](uint32_t x) { const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false); return r[0] ^ r[1] ^ x; });
 }
 __device__ __forceinline__ float sum_lanes(float x, int n)
 {

@@ -25,7 +25,6 @@
 #include <string>
 
 #include "../../include/dynamis_graph.h"
-#include "dg_grid.hpp"
 #include "dg_lanes.hpp"
 
 namespace dg {
@@ -41,6 +40,7 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 
 constexpr int kWaves = 4;
 constexpr int kMaxAxes = 8;
+constexpr int kForwardBlocks = 2048;
 constexpr int kMaxBlocks = 1024;  // of the backward pass: its partial sums of the weights' gradients
 
 template <typename T>
@@ -57,6 +57,8 @@ struct Args {
     int norm, w_own;  // w_own: the weights are of the heads' type (else float)
     float eps;
     int per, at_once;  // lanes of a head; heads at once (powers of two, their product up to 64)
+    int count, batch;  // atoms of a wave's step; atoms whose angles it makes at once, a multiple of those
+    int steps;         // of an atom's heads
     int ends[kMaxAxes];  // pairs up to and with an axis
 };
 
@@ -100,15 +102,8 @@ __device__ __forceinline__ int axis_of(const Args& a, int j)
     return x;
 }
 
-template <typename T>
-__device__ __forceinline__ void load_weight(const Args& a, const void* w, int c0, float (&v)[kC<T>])
-{
-    for (int i = 0; i < kC<T>; ++i)
-        v[i] = !w || c0 >= a.dim ? 1.0f : a.w_own ? (float)((const T*)w)[c0 + i] : ((const float*)w)[c0 + i];
-}
-
-// LDS of a wave: its atoms' cosines and sines (tokens * P <= 32 C of them, whatever the head), and a
-// word for each channel in flight.  One word in nine is spare, so that lanes eight apart do not meet.
+// LDS of a wave: its atoms' cosines and sines (at most 32 C of them, whatever the head), and a word for each
+// channel in flight.  One word in nine is spare, so that lanes eight apart do not meet.
 template <typename T>
 struct Shared {
     float2 turn[32 * kC<T>];
@@ -116,73 +111,124 @@ struct Shared {
 };
 __device__ __forceinline__ int spread(int i) { return i + (i >> 3); }
 
-// The turns of the wave's atoms first .. first + count (some may not exist).
+// The norms' weights (ones without), [2][dim].
 template <typename T>
-__device__ __forceinline__ void make_turns(const Args& a, int64_t first, int count, int lane, Shared<T>& s)
+__device__ __forceinline__ void load_weights(const Args& a, float* s_w)
 {
-    constexpr double kInverse = 0.15915494309189533577;  // 1 / (2 pi)
-    for (int i = lane; i < count * a.pairs; i += 64) {
-        const int t = i / a.pairs, j = i - t * a.pairs;
-        const int64_t node = first + t;
-        if (node >= a.nodes) break;  // (what was there turns zeros, which nobody stores or adds up)
-        const double turns = position(a, node * a.axes + axis_of(a, j)) * ((double)a.freq[j] * kInverse);
-        float sine, cosine;
-        sincospif(2.0f * (float)(turns - rint(turns)), &sine, &cosine);
-        s.turn[i] = make_float2(cosine, sine);
+    for (int i = threadIdx.x; i < 2 * a.dim; i += 64 * kWaves) {
+        const void* w = i < a.dim ? a.qw : a.kw;
+        const int c = i < a.dim ? i : i - a.dim;
+        s_w[i] = !w ? 1.0f : a.w_own ? (float)((const T*)w)[c] : ((const float*)w)[c];
+    }
+    __syncthreads();
+}
+
+// Angles in turns.  A wave takes `batch` atoms at a time; where their pairs are no more than its lanes, a lane
+// has its pair for good, and the next batch's position under way.
+struct Angles {
+    static constexpr double kInverse = 0.15915494309189533577;  // 1 / (2 pi)
+    int t, axis;
+    double freq, next;
+};
+__device__ __forceinline__ void prefetch(const Args& a, Angles& g, int64_t first)
+{
+    g.next = g.t < a.batch && first + g.t < a.nodes ? position(a, (first + g.t) * a.axes + g.axis) : 0.0;
+}
+__device__ __forceinline__ Angles make_angles(const Args& a, int lane, int64_t first)
+{
+    Angles g;
+    g.t = lane / a.pairs;
+    const int j = lane - g.t * a.pairs;
+    g.axis = axis_of(a, j);
+    g.freq = (double)a.freq[j] * Angles::kInverse;
+    if (a.batch * a.pairs <= 64) prefetch(a, g, first);
+    return g;
+}
+__device__ __forceinline__ float2 cos_sin(double turns)
+{
+    float sine, cosine;
+    sincospif(2.0f * (float)(turns - rint(turns)), &sine, &cosine);
+    return make_float2(cosine, sine);
+}
+template <typename T>
+__device__ __forceinline__ void make_turns(const Args& a, Angles& g, int64_t first, int64_t after, int lane, Shared<T>& s)
+{
+    if (a.batch * a.pairs <= 64) {
+        const double at = g.next;
+        prefetch(a, g, after);
+        if (g.t < a.batch) s.turn[lane] = cos_sin(at * g.freq);
+    } else {
+        for (int i = lane; i < a.batch * a.pairs; i += 64) {
+            const int t = i / a.pairs, j = i - t * a.pairs;
+            const double at = first + t < a.nodes ? position(a, (first + t) * a.axes + axis_of(a, j)) : 0.0;
+            s.turn[i] = cos_sin(at * ((double)a.freq[j] * Angles::kInverse));
+        }
     }
     wave_sync();
 }
 
-// Where a lane works: chunk `c0` of head `slot` (plus a multiple of at_once) of the wave's atom `t`.
+// Where a lane works: chunk `c0` of head `slot` (plus a multiple of at_once) of atom `t` of the wave's.
+// HALVES: where each channel's partner and its angle lie (bytes from Shared::row and from the atom's turns).
+template <typename T, bool HALVES>
 struct Seat {
-    int c0, slot, t, base;  // base: of the head's channels in Shared::row
+    int c0, slot, t;
+    int row;  // of the lane's channels in Shared::row
+    uint32_t partner[HALVES ? kC<T> : 1];
+    __device__ __forceinline__ Seat(const Args& a, int lane)
+    {
+        const int group = a.per * a.at_once;
+        c0 = (lane & (a.per - 1)) * kC<T>;
+        slot = (lane & (group - 1)) / a.per;
+        t = lane / group;
+        const int base = (lane & ~(a.per - 1)) * kC<T>;
+        row = base + c0;
+        if constexpr (HALVES)
+            for (int i = 0; i < kC<T>; ++i) {
+                const int c = c0 + i, j = c < a.pairs ? c : c - a.pairs;
+                const int other = c < a.pairs ? c + a.pairs : j;
+                partner[i] = c < 2 * a.pairs ? (uint32_t)spread(base + other) * 4 | (uint32_t)j << 19 : 0;
+            }
+    }
 };
-template <typename T>
-__device__ __forceinline__ Seat seat(const Args& a, int lane)
-{
-    const int group = a.per * a.at_once;
-    Seat s;
-    s.c0 = (lane & (a.per - 1)) * kC<T>;
-    s.slot = (lane & (group - 1)) / a.per;
-    s.t = lane / group;
-    s.base = (lane & ~(a.per - 1)) * kC<T>;
-    return s;
-}
 
-// y = the lane's channels v turned by the angles (BACK: by their opposites); with HALVES through LDS,
-// where `other` receives the partners.
+// The lane's channels v turned by the angles (BACK: by their opposites), with HALVES through LDS.  BACK: `across`
+// is what a channel's n is multiplied by in the angle's gradient, g'_b for a pair's first and -g'_a for its
+// second (a lane makes its partner's g' itself, and needs not its n).
 template <typename T, bool HALVES, bool BACK>
-__device__ __forceinline__ void turn(const Args& a, const Seat& at, const float2* turns, Shared<T>& s, const float (&v)[kC<T>],
-                                     float (&y)[kC<T>])
+__device__ __forceinline__ void turn(const Args& a, const Seat<T, HALVES>& at, const float2* turns, Shared<T>& s,
+                                     const float (&v)[kC<T>], float (&y)[kC<T>], float (&across)[kC<T>])
 {
     constexpr int C = kC<T>;
     if constexpr (HALVES) {
 #pragma unroll
-        for (int i = 0; i < C; ++i) s.row[spread(at.base + at.c0 + i)] = v[i];
+        for (int i = 0; i < C; ++i) s.row[spread(at.row + i)] = v[i];
         wave_sync();
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             const int c = at.c0 + i;
-            const bool second = c >= a.pairs;
-            y[i] = v[i];
-            if (c < 2 * a.pairs) {
-                const float other = s.row[spread(at.base + c + (second ? -a.pairs : a.pairs))];
-                const float2 z = turns[second ? c - a.pairs : c];
-                y[i] = fmaf(v[i], z.x, second != BACK ? other * z.y : -(other * z.y));
+            const float other = *(const float*)((const char*)s.row + (at.partner[i] & 0xffff));
+            const float2 z = *(const float2*)((const char*)turns + (at.partner[i] >> 16));
+            const float sine = (c >= a.pairs) != BACK ? z.y : -z.y;
+            const bool turned = c < 2 * a.pairs;
+            y[i] = turned ? fmaf(v[i], z.x, other * sine) : v[i];
+            // (the partner's: its own by cos, ours by the other sine)
+            if constexpr (BACK) {
+                const float theirs = fmaf(other, z.x, -(v[i] * sine));
+                across[i] = !turned ? 0.0f : c < a.pairs ? theirs : -theirs;
             }
         }
         wave_sync();
     } else {
 #pragma unroll
         for (int i = 0; i < C; i += 2) {
-            const int c = at.c0 + i;
-            y[i] = v[i];
-            y[i + 1] = v[i + 1];
-            if (c < 2 * a.pairs) {
-                const float2 z = turns[c / 2];
-                const float sine = BACK ? -z.y : z.y;
-                y[i] = fmaf(v[i], z.x, -(v[i + 1] * sine));
-                y[i + 1] = fmaf(v[i + 1], z.x, v[i] * sine);
+            const bool turned = at.c0 + i < 2 * a.pairs;
+            const float2 z = turned ? turns[(at.c0 + i) / 2] : make_float2(1.0f, 0.0f);
+            const float sine = BACK ? -z.y : z.y;
+            y[i] = turned ? fmaf(v[i], z.x, -(v[i + 1] * sine)) : v[i];
+            y[i + 1] = turned ? fmaf(v[i + 1], z.x, v[i] * sine) : v[i + 1];
+            if constexpr (BACK) {
+                across[i] = turned ? y[i + 1] : 0.0f;
+                across[i + 1] = turned ? -y[i] : 0.0f;
             }
         }
     }
@@ -196,48 +242,63 @@ __device__ __forceinline__ float inverse_rms(const Args& a, const float (&x)[kC<
     return 1.0f / sqrtf(sum_lanes(ss, a.per) / (float)a.dim + a.eps);
 }
 
+// A lane's part in a step: `at_once` heads of q, or of k after those, of `count` of the batch's atoms.
+struct Part {
+    int64_t node;
+    int head;
+    bool is_q, live;
+};
 template <typename T, bool HALVES>
-__global__ __launch_bounds__(64 * kWaves) void forward_kernel(Args a, int64_t tokens_end)
+__device__ __forceinline__ Part part_of(const Args& a, const Seat<T, HALVES>& at, int64_t first, int step)
+{
+    const int sub = step / a.steps, q_steps = (a.heads + a.at_once - 1) / a.at_once;
+    step -= sub * a.steps;
+    Part p;
+    p.is_q = step < q_steps;
+    p.head = (p.is_q ? step : step - q_steps) * a.at_once + at.slot;
+    p.node = first + sub * a.count + at.t;
+    p.live = at.c0 < a.dim && p.node < (p.is_q ? a.targets : a.nodes) && p.head < (p.is_q ? a.heads : a.kv);
+    return p;
+}
+
+template <typename T, bool HALVES>
+__global__ __launch_bounds__(64 * kWaves) void forward_kernel(Args a)
 {
     __shared__ Shared<T> shared[kWaves];
+    __shared__ __attribute__((aligned(16))) float s_w[2 * 256];
     constexpr int C = kC<T>;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     Shared<T>& s = shared[w];
-    const Seat at = seat<T>(a, lane);
-    const int count = 64 / (a.per * a.at_once);
-    float qw[C], kw[C];
-    load_weight<T>(a, a.qw, at.c0, qw);
-    load_weight<T>(a, a.kw, at.c0, kw);
-    for (int64_t first = (workgroup() * kWaves + w) * count; first < tokens_end;
-         first += (int64_t)gridDim.x * gridDim.y * kWaves * count) {
-        const int64_t node = first + at.t;
-        const bool chunk = at.c0 < a.dim;
-        auto load = [&](int step) {
-            u32x4 r = {0, 0, 0, 0};
-            const int q_steps = (a.heads + a.at_once - 1) / a.at_once;
-            const bool is_q = step < q_steps;
-            const int head = (is_q ? step : step - q_steps) * a.at_once + at.slot;
-            if (chunk && node < (is_q ? a.targets : a.nodes) && head < (is_q ? a.heads : a.kv))
-                r = *(const u32x4*)((const T*)(is_q ? a.q : a.k) + node * (is_q ? a.ldq : a.ldk) + head * a.dim + at.c0);
-            return r;
-        };
-        const int q_steps = (a.heads + a.at_once - 1) / a.at_once, steps = q_steps + (a.kv + a.at_once - 1) / a.at_once;
-        u32x4 next = load(0);
-        make_turns(a, first, count, lane, s);
-        const float2* turns = s.turn + at.t * a.pairs;
+    load_weights<T>(a, s_w);
+    const Seat<T, HALVES> at(a, lane);
+    const int64_t stride = (int64_t)gridDim.x * kWaves * a.batch;
+    int64_t first = ((int64_t)blockIdx.x * kWaves + w) * a.batch;
+    if (first >= a.nodes) return;
+    auto load = [&](const Part& p) {
+        u32x4 r = {0, 0, 0, 0};
+        if (p.live) r = *(const u32x4*)((const T*)(p.is_q ? a.q : a.k) + p.node * (p.is_q ? a.ldq : a.ldk) + p.head * a.dim + at.c0);
+        return r;
+    };
+    const int steps = a.steps * (a.batch / a.count);
+    Part next = part_of(a, at, first, 0);
+    u32x4 next_x = load(next);
+    Angles angles = make_angles(a, lane, first);
+    for (; first < a.nodes; first += stride) {
+        make_turns(a, angles, first, first + stride, lane, s);
         for (int step = 0; step < steps; ++step) {
-            float x[C], y[C];
-            unpack<T>(next, x);
-            if (step + 1 < steps) next = load(step + 1);
-            const bool is_q = step < q_steps;
+            const Part p = next;
+            float x[C], y[C], unused[C];
+            unpack<T>(next_x, x);
+            next = step + 1 < steps ? part_of(a, at, first, step + 1) : part_of(a, at, first + stride, 0);
+            next_x = load(next);
             if (a.norm) {
                 const float r = inverse_rms<T>(a, x);
-                for (int i = 0; i < C; ++i) x[i] = x[i] * r * (is_q ? qw[i] : kw[i]);
+                const float* wt = s_w + (p.is_q ? 0 : a.dim) + (at.c0 < a.dim ? at.c0 : 0);
+                for (int i = 0; i < C; ++i) x[i] = x[i] * r * wt[i];
             }
-            turn<T, HALVES, false>(a, at, turns, s, x, y);
-            const int heads = is_q ? a.heads : a.kv, head = (is_q ? step : step - q_steps) * a.at_once + at.slot;
-            if (chunk && node < (is_q ? a.targets : a.nodes) && head < heads)
-                *(u32x4*)((T*)(is_q ? a.oq : a.ok) + (node * heads + head) * a.dim + at.c0) = pack<T>(y);
+            turn<T, HALVES, false>(a, at, s.turn + (step / a.steps * a.count + at.t) * a.pairs, s, x, y, unused);
+            if (p.live)
+                *(u32x4*)((T*)(p.is_q ? a.oq : a.ok) + (p.node * (p.is_q ? a.heads : a.kv) + p.head) * a.dim + at.c0) = pack<T>(y);
         }
         wave_sync();
     }
@@ -247,95 +308,87 @@ template <typename T, bool HALVES>
 __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
 {
     __shared__ Shared<T> shared[kWaves];
+    __shared__ __attribute__((aligned(16))) float s_w[2 * 256];
     __shared__ float s_sum[64 * kWaves * kC<T>];
     constexpr int C = kC<T>;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     Shared<T>& s = shared[w];
-    const Seat at = seat<T>(a, lane);
-    const int group = a.per * a.at_once, count = 64 / group;
-    const bool chunk = at.c0 < a.dim;
-    float sum_q[C] = {}, sum_k[C] = {};
-    const int q_steps = (a.heads + a.at_once - 1) / a.at_once, steps = q_steps + (a.kv + a.at_once - 1) / a.at_once;
-    for (int64_t first = ((int64_t)blockIdx.x * kWaves + w) * count; first < a.nodes;
-         first += (int64_t)gridDim.x * kWaves * count) {
-        const int64_t node = first + at.t;
-        auto load = [&](int step, u32x4& x, u32x4& g) {
-            x = g = u32x4{0, 0, 0, 0};
-            const bool is_q = step < q_steps;
-            const int head = (is_q ? step : step - q_steps) * a.at_once + at.slot;
-            if (chunk && node < (is_q ? a.targets : a.nodes) && head < (is_q ? a.heads : a.kv)) {
-                const int64_t in = head * a.dim + at.c0;
-                x = *(const u32x4*)((const T*)(is_q ? a.q : a.k) + node * (is_q ? a.ldq : a.ldk) + in);
-                g = *(const u32x4*)((const T*)(is_q ? a.gq : a.gk) + node * (is_q ? a.ldgq : a.ldgk) + in);
-            }
-        };
-        u32x4 next_x, next_g;
-        load(0, next_x, next_g);
-        make_turns(a, first, count, lane, s);
-        const float2* turns = s.turn + at.t * a.pairs;
-        float dtheta[C] = {};  // of the pairs whose first channel the lane holds
+    load_weights<T>(a, s_w);
+    const Seat<T, HALVES> at(a, lane);
+    const int group = a.per * a.at_once;
+    const int64_t stride = (int64_t)gridDim.x * kWaves * a.batch;
+    int64_t first = ((int64_t)blockIdx.x * kWaves + w) * a.batch;
+    auto load = [&](const Part& p, u32x4& x, u32x4& g) {
+        x = g = u32x4{0, 0, 0, 0};
+        if (p.live) {
+            const int64_t in = p.head * a.dim + at.c0;
+            x = *(const u32x4*)((const T*)(p.is_q ? a.q : a.k) + p.node * (p.is_q ? a.ldq : a.ldk) + in);
+            g = *(const u32x4*)((const T*)(p.is_q ? a.gq : a.gk) + p.node * (p.is_q ? a.ldgq : a.ldgk) + in);
+        }
+    };
+    // (the frequencies of the lane's channels, and their axes, four bits each)
+    float freq[C];
+    uint32_t axes = 0;
+    for (int i = 0; i < C; ++i) {
+        const int c = at.c0 + i, j = HALVES ? (c < a.pairs ? c : c - a.pairs) : c / 2;
+        const bool turned = c < 2 * a.pairs;
+        freq[i] = turned ? a.freq[j] : 0.0f;
+        axes |= (uint32_t)(turned ? axis_of(a, j) : 15) << 4 * i;
+    }
+    const int steps = a.steps * (a.batch / a.count);
+    float sum_q[C] = {}, sum_k[C] = {}, dtheta[C] = {};
+    Part next = part_of(a, at, first, 0);
+    u32x4 next_x, next_g;
+    load(next, next_x, next_g);
+    Angles angles = make_angles(a, lane, first);
+    for (; first < a.nodes; first += stride) {
+        make_turns(a, angles, first, first + stride, lane, s);
         for (int step = 0; step < steps; ++step) {
-            float x[C], g[C], back[C], n[C];
+            const Part p = next;
+            float x[C], g[C], back[C], across[C];
             unpack<T>(next_x, x);
             unpack<T>(next_g, g);
-            if (step + 1 < steps) load(step + 1, next_x, next_g);
-            const bool is_q = step < q_steps;
-            const int heads = is_q ? a.heads : a.kv, head = (is_q ? step : step - q_steps) * a.at_once + at.slot;
+            next = step + 1 < steps ? part_of(a, at, first, step + 1) : part_of(a, at, first + stride, 0);
+            load(next, next_x, next_g);
+            turn<T, HALVES, true>(a, at, s.turn + (step / a.steps * a.count + at.t) * a.pairs, s, g, back, across);
             // (a lane without a head adds nothing: an angle or a scale that is not finite would make a NaN of its zeros)
-            const bool live = chunk && node < (is_q ? a.targets : a.nodes) && head < heads;
-            turn<T, HALVES, true>(a, at, turns, s, g, back);
-            float r = 1.0f, wt[C];
-            load_weight<T>(a, is_q ? a.qw : a.kw, at.c0, wt);
+            const float* wt = s_w + (p.is_q ? 0 : a.dim) + (at.c0 < a.dim ? at.c0 : 0);
+            float r = 1.0f;
             if (a.norm) {
                 r = inverse_rms<T>(a, x);
                 for (int i = 0; i < C; ++i) x[i] *= r;
             }
-            for (int i = 0; i < C; ++i) n[i] = x[i] * wt[i];
-            if (a.dpos) {
-                if constexpr (HALVES) {
-                    // (the partner of `back`, turned back in its turn, from the partner of n)
-                    for (int i = 0; i < C; ++i) s.row[spread(at.base + at.c0 + i)] = n[i];
-                    wave_sync();
-                    float other[C];
-                    for (int i = 0; i < C; ++i) other[i] = at.c0 + i < a.pairs ? s.row[spread(at.base + at.c0 + i + a.pairs)] : 0.0f;
-                    wave_sync();
-                    for (int i = 0; i < C; ++i) s.row[spread(at.base + at.c0 + i)] = back[i];
-                    wave_sync();
-                    for (int i = 0; i < C; ++i)
-                        if (live && at.c0 + i < a.pairs)
-                            dtheta[i] += n[i] * s.row[spread(at.base + at.c0 + i + a.pairs)] - other[i] * back[i];
-                    wave_sync();
-                } else {
-                    for (int i = 0; i < C; i += 2)
-                        if (live && at.c0 + i < 2 * a.pairs) dtheta[i] += n[i] * back[i + 1] - n[i + 1] * back[i];
-                }
-            }
+            if (a.dpos && p.live)
+                for (int i = 0; i < C; ++i) dtheta[i] = fmaf(x[i] * wt[i], across[i], dtheta[i]);
             if (a.norm) {
+                if (a.part && p.live) {
+                    if (p.is_q)
+                        for (int i = 0; i < C; ++i) sum_q[i] = fmaf(back[i], x[i], sum_q[i]);
+                    else
+                        for (int i = 0; i < C; ++i) sum_k[i] = fmaf(back[i], x[i], sum_k[i]);
+                }
                 float dot = 0;
                 for (int i = 0; i < C; ++i) {
-                    const float term = live ? back[i] * x[i] : 0.0f;
-                    if (is_q) sum_q[i] += term;
-                    else sum_k[i] += term;
                     back[i] *= wt[i];
                     dot = fmaf(back[i], x[i], dot);
                 }
                 dot = sum_lanes(dot, a.per) / (float)a.dim;
                 for (int i = 0; i < C; ++i) back[i] = r * (back[i] - x[i] * dot);
             }
-            if (live) *(u32x4*)((T*)(is_q ? a.oq : a.ok) + (node * heads + head) * a.dim + at.c0) = pack<T>(back);
-        }
-        if (a.dpos) {
-            for (int axis = 0; axis < a.axes; ++axis) {
-                double sum = 0;
-                for (int i = 0; i < C; i += HALVES ? 1 : 2) {
-                    const int j = HALVES ? at.c0 + i : (at.c0 + i) / 2;
-                    if (j < a.ends[axis] && (axis == 0 || j >= a.ends[axis - 1])) sum += (double)a.freq[j] * (double)dtheta[i];
+            if (p.live)
+                *(u32x4*)((T*)(p.is_q ? a.oq : a.ok) + (p.node * (p.is_q ? a.heads : a.kv) + p.head) * a.dim + at.c0) = pack<T>(back);
+            if (a.dpos && (step + 1) % a.steps == 0) {  // the atoms' last heads
+                for (int i = 0; i < C; ++i) dtheta[i] *= freq[i];
+                for (int axis = 0; axis < a.axes; ++axis) {
+                    float sum = 0;
+                    for (int i = 0; i < C; ++i) sum += (axes >> 4 * i & 15) == (uint32_t)axis ? dtheta[i] : 0.0f;
+                    sum = sum_lanes(sum, group);
+                    if ((lane & (group - 1)) == 0 && p.node < a.nodes) {
+                        if (a.pos_dtype == DG_F64) ((double*)a.dpos)[p.node * a.axes + axis] = sum;
+                        else ((float*)a.dpos)[p.node * a.axes + axis] = sum;
+                    }
                 }
-                sum = sum_lanes(sum, group);
-                if ((lane & (group - 1)) == 0 && node < a.nodes) {
-                    if (a.pos_dtype == DG_F64) ((double*)a.dpos)[node * a.axes + axis] = sum;
-                    else ((float*)a.dpos)[node * a.axes + axis] = (float)sum;
-                }
+                for (int i = 0; i < C; ++i) dtheta[i] = 0.0f;
             }
         }
         wave_sync();
@@ -430,15 +483,19 @@ Args make_args(const dg_rotate_desc* d)
     const int c = d->dtype == DG_F32 ? 4 : 8;
     a.per = power_of_two(d->dim / c);
     a.at_once = std::min(64 / a.per, power_of_two(std::max(d->heads, d->kv_heads)));
+    a.count = 64 / (a.per * a.at_once);
+    a.batch = a.count * std::max(1, 64 / (a.count * a.pairs));
+    // (few atoms: rather a wave for each step's)
+    while (a.batch > a.count && a.nodes < (int64_t)a.batch * kWaves * kMaxBlocks) a.batch -= a.count;
+    a.steps = (d->heads + a.at_once - 1) / a.at_once + (d->kv_heads + a.at_once - 1) / a.at_once;
     return a;
 }
 
-// Atoms of a workgroup's pass.
-int64_t pass_of(const Args& a) { return kWaves * (64 / (a.per * a.at_once)); }
-
-int64_t blocks_of(const Args& a)
+// Workgroups: as many as are resident, a wave then takes its atoms batch after batch.
+int64_t blocks_of(const Args& a, int most)
 {
-    return std::max<int64_t>(1, std::min<int64_t>((a.nodes + pass_of(a) - 1) / pass_of(a), kMaxBlocks));
+    const int64_t pass = (int64_t)kWaves * a.batch;
+    return std::max<int64_t>(1, std::min<int64_t>((a.nodes + pass - 1) / pass, most));
 }
 
 bool misaligned(std::initializer_list<const void*> p)
@@ -458,15 +515,15 @@ dg_status launched(const char* what)
 template <typename T>
 void run_forward(const Args& a, bool interleaved, hipStream_t s)
 {
-    const dim3 grid = workgroups((a.nodes + pass_of(a) - 1) / pass_of(a));
-    if (interleaved) hipLaunchKernelGGL((forward_kernel<T, false>), grid, dim3(64 * kWaves), 0, s, a, a.nodes);
-    else hipLaunchKernelGGL((forward_kernel<T, true>), grid, dim3(64 * kWaves), 0, s, a, a.nodes);
+    const dim3 grid((unsigned)blocks_of(a, kForwardBlocks));
+    if (interleaved) hipLaunchKernelGGL((forward_kernel<T, false>), grid, dim3(64 * kWaves), 0, s, a);
+    else hipLaunchKernelGGL((forward_kernel<T, true>), grid, dim3(64 * kWaves), 0, s, a);
 }
 
 template <typename T>
 void run_backward(const Args& a, bool interleaved, void* dqw, void* dkw, hipStream_t s)
 {
-    const int64_t blocks = a.nodes ? blocks_of(a) : 0;
+    const int64_t blocks = a.nodes ? blocks_of(a, kMaxBlocks) : 0;
     if (blocks) {
         const dim3 grid((unsigned)blocks);
         if (interleaved) hipLaunchKernelGGL((backward_kernel<T, false>), grid, dim3(64 * kWaves), 0, s, a);
@@ -510,7 +567,7 @@ size_t dg_rotate_workspace_size(const dg_rotate_desc* d)
 {
     if (check(d) != DG_OK) return 0;
     const Args a = make_args(d);
-    return (size_t)blocks_of(a) * 2 * a.dim * sizeof(float);
+    return (size_t)blocks_of(a, kMaxBlocks) * 2 * a.dim * sizeof(float);
 }
 
 dg_status dg_rotate_backward(const dg_rotate_desc* d, const void* q, const void* k, const void* positions,

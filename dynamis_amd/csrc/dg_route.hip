@@ -2,8 +2,8 @@
 //
 //   s = softmax(x) or 1 / (1 + exp(-x)) of a row's logits x, one an expert
 //   v = x (no bias), or s + bias: what is chosen by.  A logit or a bias of -inf is never chosen
-//   groups: neighbouring experts; a group's worth is the sum of its best one or two s (+ bias) (best
-//           one without a bias: x); only the experts of the top_groups worthiest are chosen from
+//   groups: neighbouring experts; a group's worth is its largest v, or the sum of its two largest s (+ bias);
+//           only the experts of the top_groups worthiest are chosen from
 //   experts[i] = the k largest v, NaN above all, ties to the lowest index;  -1 where none is left
 //   weights[i, j] = scale s[chosen] (/ sum over the chosen s)
 //   sizes[e] = rows that chose e;  places[i, j] = place of the choice in the order by expert, then row
@@ -11,8 +11,8 @@
 //   dx[j] = scale p_j (g_j [chosen] - sum_chosen g p) (softmax), scale g_j s_j (1 - s_j) (sigmoid)
 //
 // A power of two of lanes, W, holds a row, V neighbouring experts each; k rounds take the largest left
-// out, each a maximum over the lanes and a ballot for its first holder.  Sums s + bias are compared in
-// 64 bits, so that what a rounding of 32 would merge or swap is chosen as the definition has it.
+// out, each a maximum over the lanes and a ballot for its first holder.  Sums of scores are compared as 64
+// bits have them, so that what a rounding of 32 would merge or swap is chosen as the definition has it.
 // The places are a stable counting sort in three launches: each workgroup's counts of its rows' choices, a
 // scan of them for each expert, and the ranks within a workgroup by matching lanes; nothing depends
 // on the order of atomics (counts alone are added up by them).
@@ -114,41 +114,56 @@ __device__ __forceinline__ void load_logits(const Args& a, int64_t row, int e0, 
     }
 }
 
-// A row's choices: k rounds of the largest key, first holder first, into `picks` (-1: none left).
-template <int V, typename K>
-__device__ __forceinline__ void choose(const Args& a, K (&key)[V], int lane, int e0, int* picks)
+// A row's choices: k rounds of the largest key, first holder first, into `picks` (-1: none left) with what
+// the key's low half stands for (the logit, where the keys are those of logits).  A key beyond them shows
+// whether two that follow each other are nearer than `apart`.
+struct Pick {
+    int e;
+    float x;
+};
+template <int V, bool CLOSE, typename K>
+__device__ __forceinline__ bool choose(const Args& a, K (&key)[V], int lane, int e0, Pick* picks, float apart)
 {
     const int first = lane & ~(a.lanes - 1);
     const uint64_t mine = a.lanes == 64 ? ~0ull : ((1ull << a.lanes) - 1) << first;
-    for (int j = 0; j < a.k; ++j) {
+    bool close = false;
+    K before = 0;
+    for (int j = 0; j < a.k + CLOSE; ++j) {
         K best = key[0];
 #pragma unroll
         for (int i = 1; i < V; ++i) best = max(best, key[i]);
         const K top = max_lanes(best, a.lanes);
+        if constexpr (CLOSE) {
+            // (a NaN is near everything)
+            close = close || (j > 0 && top && !((float)(number_of(before) - number_of(top)) > apart));
+            before = top;
+            if (j == a.k) break;
+        }
         const uint64_t holders = __ballot(best == top) & mine;
         if (lane == __builtin_ctzll(holders)) {
             int at = V - 1;
 #pragma unroll
-            for (int i = V - 2; i >= 0; --i)
-                if (key[i] == top) at = i;
+            for (int i = V - 2; i >= 0; --i) at = key[i] == top ? i : at;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i == at) key[i] = 0;
-            picks[j] = top ? e0 + at : -1;
+            for (int i = 0; i < V; ++i) key[i] = i == at ? 0 : key[i];
+            picks[j] = Pick{top ? e0 + at : -1, number_of((uint32_t)top)};
         }
     }
+    return close;
 }
 
-// Keys of experts outside the row's worthiest groups become nothing.
+// Which groups of a row are the worthiest, as a mask.  `worth`: the keys that a group's worth sums, 0 for
+// what is never chosen.  near: whether one more and one less lie nearer than `apart`.
 template <int V, typename K>
-__device__ __forceinline__ void keep_groups(const Args& a, K (&key)[V], int lane, int e0, K* s_key, K* s_worth)
+__device__ __forceinline__ uint64_t worthiest(const Args& a, const K (&worth)[V], int lane, int e0, K* s_key, K* s_worth,
+                                              float apart, bool& near)
 {
     const int l = lane & (a.lanes - 1), per = a.n / a.groups;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        if (e0 + i < a.n) s_key[e0 + i] = key[i];
+        if (e0 + i < a.n) s_key[e0 + i] = worth[i];
     wave_sync();
-    K worth = 0;
+    K mine = 0;
     if (l < a.groups) {
         K best = 0, second = 0;
         for (int i = l * per; i < (l + 1) * per; ++i) {
@@ -156,37 +171,73 @@ __device__ __forceinline__ void keep_groups(const Args& a, K (&key)[V], int lane
             second = max(second, min(best, x));
             best = max(best, x);
         }
-        worth = a.group_best == 2 && second ? key_of(number_of(best) + number_of(second)) : best;
-        s_worth[l] = worth;
+        mine = a.group_best == 2 && second ? key_of(number_of(best) + number_of(second)) : best;
+        s_worth[l] = mine;
     }
     wave_sync();
     int rank = 0;
+    near = false;
     if (l < a.groups)
         for (int g = 0; g < a.groups; ++g) {
             const K x = s_worth[g];
-            rank += x > worth || (x == worth && g < l);
+            rank += x > mine || (x == mine && g < l);
         }
-    const uint64_t kept = __ballot(l < a.groups && worth && rank < a.top_groups) >> (lane & ~(a.lanes - 1));
+    if (l < a.groups && mine)  // (two on either side of the border, nearer than `apart`: the lesser sees both)
+        for (int g = 0; g < a.groups; ++g) {
+            const K x = s_worth[g];
+            near = near || (g != l && x && !(fabsf((float)(number_of(x) - number_of(mine))) > apart));
+        }
+    wave_sync();
+    return __ballot(l < a.groups && mine && rank < a.top_groups) >> (lane & ~(a.lanes - 1));
+}
+template <int V, typename K>
+__device__ __forceinline__ void keep(const Args& a, uint64_t groups, int e0, K (&key)[V])
+{
+    const int per = a.n / a.groups;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        if (!(e0 + i < a.n && (kept >> ((e0 + i) / per) & 1))) key[i] = 0;
-    wave_sync();
+        if (!(e0 + i < a.n && (groups >> ((e0 + i) / per) & 1))) key[i] = 0;
 }
 
-// WIDE: what is chosen by, or a group's worth, is a score (+ bias), in 64 bits.
-template <typename T, int V, bool WIDE>
+// s of a row's logits, in 32 bits (each within 32 2^-24) or 64.
+template <int V, typename F>
+__device__ __forceinline__ void scores(const Args& a, const float (&x)[V], float top, F (&s)[V])
+{
+    F sum = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if constexpr (sizeof(F) == 8) {
+            s[i] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[i])) : exp((double)x[i] - (double)top);
+        } else {
+            const float e = __builtin_amdgcn_exp2f(1.44269504f * (a.sigmoid ? -fabsf(x[i]) : x[i] - top));
+            const float r = __builtin_amdgcn_rcpf(1.0f + e);
+            s[i] = !a.sigmoid ? e : x[i] < 0.0f ? e * r : r;
+        }
+        sum += s[i];
+    }
+    if (!a.sigmoid) {
+        sum = sum_lanes(sum, a.lanes);
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] /= sum;
+    }
+}
+
+// SCORED: a bias, or groups worth a sum of scores.  What is chosen by is then worked out in 32 bits, and
+// where two values that a choice or a group hangs on lie nearer than the rounding, or are no
+// numbers, the wave's rows are done again in 64 (a row in some hundred to thousand).
+template <typename T, int V, bool SCORED>
 __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
 {
-    using K = typename std::conditional<WIDE, uint64_t, uint32_t>::type;
+    using K = typename std::conditional<SCORED, uint64_t, uint32_t>::type;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     uint32_t* s_count = (uint32_t*)smem;  // [n + 1]
     const int lane = threadIdx.x & 63, in_block = threadIdx.x / a.lanes, at_once = kThreads / a.lanes;
     const int l = lane & (a.lanes - 1), e0 = l * V;
-    int* picks = (int*)(s_count + ((a.n + 4) & ~3)) + in_block * a.k;
+    Pick* s_picks = (Pick*)(s_count + ((a.n + 4) & ~3));
+    Pick* picks = s_picks + in_block * a.k;
     // (with groups: a row's keys, and its groups' worths)
-    char* rest = (char*)((int*)(s_count + ((a.n + 4) & ~3)) + ((at_once * a.k + 3) & ~3));
-    K* s_key = (K*)rest + in_block * a.n;
-    K* s_worth = (K*)rest + at_once * a.n + in_block * a.groups;
+    K* s_key = (K*)(s_picks + ((at_once * a.k + 1) & ~1)) + in_block * a.n;
+    K* s_worth = (K*)(s_picks + ((at_once * a.k + 1) & ~1)) + at_once * a.n + in_block * a.groups;
     const int64_t block = workgroup();
     if (block >= a.blocks) return;
     for (int i = threadIdx.x; i <= a.n; i += kThreads) s_count[i] = 0;
@@ -194,7 +245,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
     const int64_t r0 = block * a.block_rows, r1 = min(r0 + a.block_rows, a.rows);
     float bias[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) bias[i] = a.bias && e0 + i < a.n ? a.bias[e0 + i] : 0.0f;
+    for (int i = 0; i < V; ++i) bias[i] = SCORED && a.bias && e0 + i < a.n ? a.bias[e0 + i] : 0.0f;
     for (int64_t base = r0; base < r1; base += at_once) {
         const int64_t row = base + in_block;
         const bool live = row < r1;
@@ -202,59 +253,69 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
         load_logits<T, V>(a, row, e0, live, x);
         // the row's maximum and sum, where a weight or a choice needs them
         float top = -INFINITY, total = 1.0f;
-        const bool softmax_all = !a.sigmoid && (WIDE || !a.renormalize);
+        const bool softmax_all = !a.sigmoid && (SCORED || !a.renormalize);
         if (softmax_all) {
 #pragma unroll
             for (int i = 0; i < V; ++i) top = x[i] > top ? x[i] : top;  // (a NaN makes the sum one)
             over_lanes(a.lanes, [&](auto&& other) { top = fmaxf(top, as_float(other(as_bits(top)))); });
             if (top == -INFINITY) top = 0.0f;
         }
-        K key[V];
-        if constexpr (WIDE) {
-            double v[V];
-            if (a.sigmoid) {
+        if (!a.sigmoid && !a.renormalize) {
+            float sum = 0;
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = 1.0 / (1.0 + exp(-(double)x[i]));
-            } else {
-                double sum = 0;
+            for (int i = 0; i < V; ++i) sum += expf(x[i] - top);
+            total = sum_lanes(sum, a.lanes);
+        }
+        uint32_t plain[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    v[i] = exp((double)x[i] - (double)top);
-                    sum += v[i];
-                }
-                sum = sum_lanes(sum, a.lanes);
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[i] /= sum;
-                total = (float)sum;
-            }
+        for (int i = 0; i < V; ++i) plain[i] = x[i] == -INFINITY || bias[i] == -INFINITY || e0 + i >= a.n ? 0 : key_of(x[i]);
+        if constexpr (SCORED) {
+            float v[V], most = 0.0f;
+            uint32_t key[V], worth[V];
+            scores<V>(a, x, top, v);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                if (a.bias) v[i] += (double)bias[i];
-                key[i] = x[i] == -INFINITY || bias[i] == -INFINITY || e0 + i >= a.n ? 0 : key_of(v[i]);
+                v[i] += bias[i];
+                worth[i] = plain[i] ? key_of(v[i]) : 0;
+                most = plain[i] ? fmaxf(most, fabsf(v[i])) : most;
+                key[i] = a.bias ? worth[i] : plain[i];
             }
-            if (a.groups > 1) keep_groups<V, K>(a, key, lane, e0, s_key, s_worth);
+            over_lanes(a.lanes, [&](auto&& other) { most = fmaxf(most, as_float(other(as_bits(most)))); });
+            const float apart = 8e-6f * (1.0f + most);  // (twice 32 2^-24, and twice that for a sum of two)
+            bool near = false;
+            if (a.groups > 1) keep<V>(a, worthiest<V>(a, worth, lane, e0, (uint32_t*)s_key, (uint32_t*)s_worth, apart, near), e0, key);
+            // (without a bias the keys are the logits, and exact)
+            const bool close = a.bias ? choose<V, true>(a, key, lane, e0, picks, apart)
+                                      : choose<V, false>(a, key, lane, e0, picks, 0.0f);
+            if (__any(live && (near || close))) {
+                double d[V];
+                uint64_t wide[V], sum_of[V];
+                scores<V>(a, x, top, d);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    d[i] += (double)bias[i];
+                    sum_of[i] = plain[i] ? key_of(d[i]) : 0;
+                    wide[i] = a.bias ? sum_of[i] : plain[i];
+                }
+                if (a.groups > 1) keep<V>(a, worthiest<V>(a, sum_of, lane, e0, s_key, s_worth, 0.0f, near), e0, wide);
+                choose<V, false>(a, wide, lane, e0, picks, 0.0f);
+            }
         } else {
-            if (softmax_all) {
-                float sum = 0;
-#pragma unroll
-                for (int i = 0; i < V; ++i) sum += expf(x[i] - top);
-                total = sum_lanes(sum, a.lanes);
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) key[i] = x[i] == -INFINITY || e0 + i >= a.n ? 0 : key_of(x[i]);
-            if (a.groups > 1) keep_groups<V, K>(a, key, lane, e0, s_key, s_worth);
+            bool near;
+            if (a.groups > 1) keep<V>(a, worthiest<V>(a, plain, lane, e0, s_key, s_worth, 0.0f, near), e0, plain);
+            choose<V, false>(a, plain, lane, e0, picks, 0.0f);
         }
-        choose<V, K>(a, key, lane, e0, picks);
         wave_sync();
         // a lane for each choice
         const bool mine = live && l < a.k;
-        const int e = l < a.k ? picks[l] : -1;
-        const float c = mine && e >= 0 ? logit<T>(a, row, e) : -INFINITY;
+        const Pick pick = l < a.k ? picks[l] : Pick{-1, 0.0f};
+        const int e = pick.e;
+        const float c = !mine || e < 0 ? -INFINITY : SCORED && a.bias ? logit<T>(a, row, e) : pick.x;
         float w = 0.0f;
         if (a.renormalize) {
             // (relative to the largest chosen: a sum that vanishes in 32 bits has no ratio.  Far below
             // zero a sigmoid is exp(x) to 32 bits.)
-            float m = l < a.k && e >= 0 ? c : -INFINITY;
+            float m = c;
             over_lanes(a.lanes, [&](auto&& other) {
                 const float y = as_float(other(as_bits(m)));
                 m = y > m || y != y ? y : m;
@@ -483,7 +544,12 @@ void share(const dg_route_desc* d, int* lanes, int* each)
 }
 
 // Rows of a workgroup.
-int64_t rows_of_block(const dg_route_desc* d) { return d->n_rows <= 16384 ? 64 : 256; }
+int64_t rows_of_block(const dg_route_desc* d)
+{
+    int64_t n = 32;
+    while (n < 256 && n * 2048 < d->n_rows) n *= 2;
+    return n;
+}
 
 struct Layout {
     int64_t blocks;
@@ -527,7 +593,7 @@ void run_route(const Args& a, hipStream_t s)
 {
     const bool wide = a.bias || (a.groups > 1 && a.group_best == 2);
     const int at_once = kThreads / a.lanes;
-    size_t lds = 4 * (size_t)((a.n + 4) & ~3) + 4 * (size_t)((at_once * a.k + 3) & ~3);
+    size_t lds = 4 * (size_t)((a.n + 4) & ~3) + 8 * (size_t)((at_once * a.k + 1) & ~1);
     if (a.groups > 1) lds += (wide ? 8 : 4) * (size_t)at_once * (a.n + a.groups);
     const dim3 grid = workgroups(a.blocks);
     if (wide) hipLaunchKernelGGL((route_kernel<T, V, true>), grid, dim3(kThreads), lds, s, a);

@@ -231,11 +231,14 @@ class _Route(torch.autograd.Function):
         ctx.save_for_backward(logits, experts)
         ctx.desc = d
         ctx.mark_non_differentiable(experts, sizes, places)
+        ctx.set_materialize_grads(False)  # (zeros for the outputs without one are three launches)
         return weights, experts, sizes, places
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, *_):
+        if grad is None:
+            return None, None, None
         logits, experts = ctx.saved_tensors
         dev, grad = logits.device, grad.contiguous()
         with L.on_device(dev):
@@ -256,14 +259,15 @@ def route_rows(logits, k, scoring="softmax", bias=None, groups=1, top_groups=1, 
     """The k experts of each row by its logits, their weights, and the experts' order of the rows.
 
       s       = softmax(logits) or sigmoid(logits)
-      v       = logits where there is neither a bias nor group_best=2, else s + bias, in 64 bits
+      v       = logits, or with a bias s + bias, in 64 bits
       experts = the k largest v, NaN above all and the first of equals
       weights = scale s[experts], with renormalize divided by their sum over the row
 
     logits [rows, experts], float32 or bfloat16, 1 to 1024 experts; k up to 64; scoring "softmax" or
     "sigmoid".  bias [experts], used in float32, moves the choice alone and never the weights (it
     keeps the experts balanced).  groups > 1 parts the experts into as many neighbouring groups, each
-    worth the sum of its group_best (1 or 2) largest v; experts are chosen from the top_groups worthiest groups.
+    worth its largest v, or with group_best=2 the sum of its two largest s (+ bias); experts are chosen from the
+    top_groups worthiest groups.
 
     An expert whose logit or bias is -inf is never chosen.  Where fewer than k are left (a row of
     padding, all -inf), the rest of the row's choices is -1 with weight 0, and takes no place among

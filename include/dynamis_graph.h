@@ -535,8 +535,7 @@ dg_status dg_grouped_apply_backward(const dg_grouped_desc* desc, int32_t activat
  *   q_out, k_out contiguous, of dtype, rounded once.
  * Backward: dq, dk contiguous, of dtype; dpositions like positions or NULL; dq_weight, dk_weight like
  * the weights or NULL, for which the workspace of dg_rotate_workspace_size bytes is needed.  Sums are
- * float32 (those of dpositions float64 over the pairs) and in a fixed order: results repeat bit for
- * bit.  Both enqueue work only. */
+ * float32 and in a fixed order: results repeat bit for bit.  Both enqueue work only. */
 typedef struct dg_rotate_desc {
     int64_t n_targets;
     int64_t n_nodes;
@@ -563,10 +562,10 @@ dg_status dg_rotate_backward(const dg_rotate_desc* desc, const void* q, const vo
 
 /* Rows routed to experts by their logits x:
  *   s = softmax(x), or 1 / (1 + exp(-x)) (sigmoid != 0)
- *   v = x where bias is NULL and (groups == 1 or group_best == 1), else s + bias (0), in 64 bits;
- *       an expert whose logit or bias is -inf is never chosen
- *   groups > 1: n_experts / groups neighbouring experts each; a group is worth the sum of its group_best (1, 2)
- *       largest v; only the experts of the top_groups worthiest are chosen from
+ *   v = x, or with a bias s + bias, in 64 bits; an expert whose logit or bias is -inf is never chosen
+ *   groups > 1: n_experts / groups neighbouring experts each; a group is worth its largest v (group_best
+ *       1) or the sum of its two largest s (+ bias), in 64 bits (2); only the experts of the top_groups
+ *       worthiest are chosen from
  *   experts[i] = the k largest v in falling order (NaN above all; of equals the lowest first), -1
  *       where none is left
  *   weights[i, j] = scale s[experts[i, j]], renormalize != 0: divided by the sum of the row's chosen s;
