@@ -40,8 +40,10 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 
 constexpr int kWaves = 4;
 constexpr int kMaxAxes = 8;
-constexpr int kForwardBlocks = 2048;
-constexpr int kMaxBlocks = 1024;  // of the backward pass: its partial sums of the weights' gradients
+// Workgroups, as many as are resident at once: each takes as many atoms as the others, so a second round would
+// leave most of the card idle (1M atoms: 404 us with 1536, 451 with 2048).
+constexpr int kForwardBlocks = 1536;
+constexpr int kMaxBlocks = 1024;
 
 template <typename T>
 constexpr int kC = 16 / (int)sizeof(T);  // channels of a lane
@@ -326,15 +328,13 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
             g = *(const u32x4*)((const T*)(p.is_q ? a.gq : a.gk) + p.node * (p.is_q ? a.ldgq : a.ldgk) + in);
         }
     };
-    // (the frequencies of the lane's channels, and their axes, four bits each)
-    float freq[C];
+    // (the lane's channels' axes, four bits each)
+    auto pair_of = [&](int i) {
+        const int c = at.c0 + i;
+        return c >= 2 * a.pairs ? 0 : HALVES ? (c < a.pairs ? c : c - a.pairs) : c / 2;
+    };
     uint32_t axes = 0;
-    for (int i = 0; i < C; ++i) {
-        const int c = at.c0 + i, j = HALVES ? (c < a.pairs ? c : c - a.pairs) : c / 2;
-        const bool turned = c < 2 * a.pairs;
-        freq[i] = turned ? a.freq[j] : 0.0f;
-        axes |= (uint32_t)(turned ? axis_of(a, j) : 15) << 4 * i;
-    }
+    for (int i = 0; i < C; ++i) axes |= (uint32_t)(at.c0 + i < 2 * a.pairs ? axis_of(a, pair_of(i)) : 15) << 4 * i;
     const int steps = a.steps * (a.batch / a.count);
     float sum_q[C] = {}, sum_k[C] = {}, dtheta[C] = {};
     Part next = part_of(a, at, first, 0);
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
             if (p.live)
                 *(u32x4*)((T*)(p.is_q ? a.oq : a.ok) + (p.node * (p.is_q ? a.heads : a.kv) + p.head) * a.dim + at.c0) = pack<T>(back);
             if (a.dpos && (step + 1) % a.steps == 0) {  // the atoms' last heads
-                for (int i = 0; i < C; ++i) dtheta[i] *= freq[i];
+                for (int i = 0; i < C; ++i) dtheta[i] *= a.freq[pair_of(i)];
                 for (int axis = 0; axis < a.axes; ++axis) {
                     float sum = 0;
                     for (int i = 0; i < C; ++i) sum += (axes >> 4 * i & 15) == (uint32_t)axis ? dtheta[i] : 0.0f;
@@ -408,22 +408,24 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
     }
 }
 
-// dw: the workgroups' sums of 64 channels, sixteen strands of them in turn.
+// dw: the workgroups' sums of 16 channels, 64 strands of them in turn.
 template <typename T>
 __global__ __launch_bounds__(1024) void join_kernel(const float* part, int blocks, int dim, void* dqw, void* dkw, int w_own)
 {
-    __shared__ float s[16][64];
-    const int lane = threadIdx.x & 63, strand = threadIdx.x >> 6, which = blockIdx.y, c = blockIdx.x * 64 + lane;
+    __shared__ float s[16][16];
+    const int strand = threadIdx.x >> 4, which = blockIdx.y, c = blockIdx.x * 16 + (threadIdx.x & 15);
     float x = 0;
     if (c < dim)
 #pragma unroll 8
-        for (int b = strand; b < blocks; b += 16) x += part[((int64_t)b * 2 + which) * dim + c];
-    s[strand][lane] = x;
+        for (int b = strand; b < blocks; b += 64) x += part[((int64_t)b * 2 + which) * dim + c];
+    x += __shfl_xor(x, 16, 64);
+    x += __shfl_xor(x, 32, 64);
+    if (threadIdx.x % 64 < 16) s[threadIdx.x >> 6][threadIdx.x & 15] = x;
     __syncthreads();
     void* out = which ? dkw : dqw;
-    if (strand || c >= dim || !out) return;
+    if (threadIdx.x >= 16 || c >= dim || !out) return;
     x = 0;
-    for (int i = 0; i < 16; ++i) x += s[i][lane];
+    for (int i = 0; i < 16; ++i) x += s[i][threadIdx.x];
     if (w_own) ((T*)out)[c] = (T)x;
     else ((float*)out)[c] = x;
 }
@@ -459,6 +461,19 @@ dg_status check(const dg_rotate_desc* d)
     return DG_OK;
 }
 
+// Heads of an atom at once: as many as there are lanes for, but fewer where that leaves lanes without a head
+// (16 and 4 heads on 8 places: a sixth of them) and there are atoms for them instead.
+int heads_at_once(const dg_rotate_desc* d, int most)
+{
+    auto places = [&](int n) { return ((d->heads + n - 1) / n + (d->kv_heads + n - 1) / n) * n; };
+    most = std::min(most, power_of_two(std::max(d->heads, d->kv_heads)));
+    int best = most;
+    if (d->n_nodes >= kMaxBlocks * kWaves * 4)
+        for (int n = most / 2; n >= 1; n /= 2)
+            if (places(n) < places(best)) best = n;
+    return best;
+}
+
 Args make_args(const dg_rotate_desc* d)
 {
     Args a = {};
@@ -482,7 +497,7 @@ Args make_args(const dg_rotate_desc* d)
     }
     const int c = d->dtype == DG_F32 ? 4 : 8;
     a.per = power_of_two(d->dim / c);
-    a.at_once = std::min(64 / a.per, power_of_two(std::max(d->heads, d->kv_heads)));
+    a.at_once = heads_at_once(d, 64 / a.per);
     a.count = 64 / (a.per * a.at_once);
     a.batch = a.count * std::max(1, 64 / (a.count * a.pairs));
     // (few atoms: rather a wave for each step's)
@@ -530,7 +545,7 @@ void run_backward(const Args& a, bool interleaved, void* dqw, void* dkw, hipStre
         else hipLaunchKernelGGL((backward_kernel<T, true>), grid, dim3(64 * kWaves), 0, s, a);
     }
     if (a.part)
-        hipLaunchKernelGGL(join_kernel<T>, dim3((a.dim + 63) / 64, 2), dim3(1024), 0, s, a.part, (int)blocks, a.dim, dqw, dkw,
+        hipLaunchKernelGGL(join_kernel<T>, dim3((a.dim + 15) / 16, 2), dim3(1024), 0, s, a.part, (int)blocks, a.dim, dqw, dkw,
                            a.w_own);
 }
 
