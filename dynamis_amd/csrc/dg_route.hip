@@ -40,6 +40,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxChoices = 64;
+constexpr int kBlockRows = 256;  // of a workgroup, at most
 
 struct Args {
     const void* logits;
@@ -50,11 +51,13 @@ struct Args {
     int32_t* places;
     uint32_t* counts;  // [experts + 1][blocks]: of each workgroup's rows, the last of choices of none
     uint32_t* totals;  // [experts + 1]
+    uint32_t* close;   // [blocks][kBlockRows / 32]: rows that are done in 64 bits
     int64_t rows, ld;
     int n, k, groups, top_groups, group_best;
     int sigmoid, renormalize;
     float scale;
-    int lanes;  // W
+    int lanes;        // W
+    int group_lanes;  // of a group, where a power of two of lanes hold it whole (else 0)
     int64_t block_rows, blocks;
     const float* grad;
     void* dlogits;
@@ -115,30 +118,23 @@ __device__ __forceinline__ void load_logits(const Args& a, int64_t row, int e0, 
 }
 
 // A row's choices: k rounds of the largest key, first holder first, into `picks` (-1: none left) with what
-// the key's low half stands for (the logit, where the keys are those of logits).  A key beyond them shows
-// whether two that follow each other are nearer than `apart`.
+// the key's low half stands for (where keys have 32 bits, the value).  Returns the largest key left.
 struct Pick {
     int e;
     float x;
 };
-template <int V, bool CLOSE, typename K>
-__device__ __forceinline__ bool choose(const Args& a, K (&key)[V], int lane, int e0, Pick* picks, float apart)
+template <int V, bool LEFT, typename K>
+__device__ __forceinline__ K choose(const Args& a, K (&key)[V], int lane, int e0, Pick* picks)
 {
     const int first = lane & ~(a.lanes - 1);
     const uint64_t mine = a.lanes == 64 ? ~0ull : ((1ull << a.lanes) - 1) << first;
-    bool close = false;
-    K before = 0;
-    for (int j = 0; j < a.k + CLOSE; ++j) {
+    for (int j = 0;; ++j) {
         K best = key[0];
 #pragma unroll
         for (int i = 1; i < V; ++i) best = max(best, key[i]);
+        if (!LEFT && j == a.k) return best;
         const K top = max_lanes(best, a.lanes);
-        if constexpr (CLOSE) {
-            // (a NaN is near everything)
-            close = close || (j > 0 && top && !((float)(number_of(before) - number_of(top)) > apart));
-            before = top;
-            if (j == a.k) break;
-        }
+        if (LEFT && j == a.k) return top;
         const uint64_t holders = __ballot(best == top) & mine;
         if (lane == __builtin_ctzll(holders)) {
             int at = V - 1;
@@ -149,14 +145,61 @@ __device__ __forceinline__ bool choose(const Args& a, K (&key)[V], int lane, int
             picks[j] = Pick{top ? e0 + at : -1, number_of((uint32_t)top)};
         }
     }
-    return close;
 }
 
-// Which groups of a row are the worthiest, as a mask.  `worth`: the keys that a group's worth sums, 0 for
-// what is never chosen.  near: whether one more and one less lie nearer than `apart`.
+// Whether a lane's experts are in one of the worthiest groups, for groups of whole lanes (a.group_lanes, a power of two, to a group).
+template <int V>
+__device__ __forceinline__ bool mine_is_worthy(const Args& a, const uint32_t (&key)[V], int lane, int e0, uint32_t* s_worth)
+{
+    uint32_t best = key[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) best = max(best, key[i]);
+    best = max_lanes(best, a.group_lanes);
+    const int own = (lane & (a.lanes - 1)) / a.group_lanes;
+    if (e0 < a.n) s_worth[own] = best;
+    wave_sync();
+    int rank = 0;
+    for (int g = 0; g < a.groups; ++g) {
+        const uint32_t x = s_worth[g];
+        rank += x > best || (x == best && g < own);
+    }
+    wave_sync();
+    return rank < a.top_groups;
+}
+// By sums in 32 bits; near: whether another group's lies nearer than `apart`.
+template <int V>
+__device__ __forceinline__ bool mine_is_worthy(const Args& a, const float (&v)[V], int lane, int e0, float* s_worth, float apart,
+                                               bool& near)
+{
+    float best = v[0], second = -INFINITY;
+#pragma unroll
+    for (int i = 1; i < V; ++i) {
+        second = __builtin_amdgcn_fmed3f(best, second, v[i]);
+        best = fmaxf(best, v[i]);
+    }
+    over_lanes(a.group_lanes, [&](auto&& other) {
+        const float b = as_float(other(as_bits(best))), t = as_float(other(as_bits(second)));
+        second = fmaxf(fminf(best, b), fmaxf(second, t));
+        best = fmaxf(best, b);
+    });
+    const float worth = a.group_best == 2 && second > -INFINITY ? best + second : best;
+    if (e0 < a.n) s_worth[(lane & (a.lanes - 1)) / a.group_lanes] = worth;
+    wave_sync();
+    int rank = 0, around = 0;
+    for (int g = 0; g < a.groups; ++g) {
+        const float x = s_worth[g];
+        rank += x > worth;
+        around += fabsf(x - worth) <= apart;  // (its own among them)
+    }
+    wave_sync();
+    near = around > 1;
+    return rank < a.top_groups;
+}
+
+// Which groups of a row are the worthiest, as a mask, for groups of any size.  `worth`: the keys that a group's
+// worth sums, 0 for what is never chosen.
 template <int V, typename K>
-__device__ __forceinline__ uint64_t worthiest(const Args& a, const K (&worth)[V], int lane, int e0, K* s_key, K* s_worth,
-                                              float apart, bool& near)
+__device__ __forceinline__ uint64_t worthiest(const Args& a, const K (&worth)[V], int lane, int e0, K* s_key, K* s_worth)
 {
     const int l = lane & (a.lanes - 1), per = a.n / a.groups;
 #pragma unroll
@@ -176,16 +219,10 @@ __device__ __forceinline__ uint64_t worthiest(const Args& a, const K (&worth)[V]
     }
     wave_sync();
     int rank = 0;
-    near = false;
     if (l < a.groups)
         for (int g = 0; g < a.groups; ++g) {
             const K x = s_worth[g];
             rank += x > mine || (x == mine && g < l);
-        }
-    if (l < a.groups && mine)  // (two on either side of the border, nearer than `apart`: the lesser sees both)
-        for (int g = 0; g < a.groups; ++g) {
-            const K x = s_worth[g];
-            near = near || (g != l && x && !(fabsf((float)(number_of(x) - number_of(mine))) > apart));
         }
     wave_sync();
     return __ballot(l < a.groups && mine && rank < a.top_groups) >> (lane & ~(a.lanes - 1));
@@ -199,7 +236,7 @@ __device__ __forceinline__ void keep(const Args& a, uint64_t groups, int e0, K (
         if (!(e0 + i < a.n && (groups >> ((e0 + i) / per) & 1))) key[i] = 0;
 }
 
-// s of a row's logits, in 32 bits (each within 32 2^-24) or 64.
+// s of a row's logits, in 32 bits or 64.
 template <int V, typename F>
 __device__ __forceinline__ void scores(const Args& a, const float (&x)[V], float top, F (&s)[V])
 {
@@ -222,13 +259,20 @@ __device__ __forceinline__ void scores(const Args& a, const float (&x)[V], float
     }
 }
 
-// SCORED: a bias, or groups worth a sum of scores.  What is chosen by is then worked out in 32 bits, and
-// where two values that a choice or a group hangs on lie nearer than the rounding, or are no
-// numbers, the wave's rows are done again in 64 (a row in some hundred to thousand).
-template <typename T, int V, bool SCORED>
+// kLogits: the logits are what is chosen by.  kScores: a bias, or groups worth a sum of scores.  What is chosen by
+// is then worked out in 32 bits; a row where two values that a choice or a group hangs on lie nearer than the
+// rounding, or are no numbers, is left to a second launch, kWide, which takes it in 64 (one of some hundred to
+// thousand).  In one launch the wide part's registers leave the other three waves a SIMD instead of
+// seven: 300,007 rows over 64 experts 104 us, these two 63.
+enum { kLogits, kScores, kWide };
+
+template <typename T, int V, int HOW>
 __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
 {
-    using K = typename std::conditional<SCORED, uint64_t, uint32_t>::type;
+    constexpr bool SCORED = HOW != kLogits;
+    using K = typename std::conditional<HOW == kWide, uint64_t, uint32_t>::type;
+    __shared__ uint32_t s_close[kBlockRows / 32], s_rows;
+    __shared__ uint8_t s_list[kBlockRows];
     extern __shared__ __attribute__((aligned(16))) char smem[];
     uint32_t* s_count = (uint32_t*)smem;  // [n + 1]
     const int lane = threadIdx.x & 63, in_block = threadIdx.x / a.lanes, at_once = kThreads / a.lanes;
@@ -241,14 +285,24 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
     const int64_t block = workgroup();
     if (block >= a.blocks) return;
     for (int i = threadIdx.x; i <= a.n; i += kThreads) s_count[i] = 0;
+    if (threadIdx.x < kBlockRows / 32) s_close[threadIdx.x] = HOW == kWide ? a.close[block * (kBlockRows / 32) + threadIdx.x] : 0;
+    if (threadIdx.x == 0) s_rows = 0;
     __syncthreads();
-    const int64_t r0 = block * a.block_rows, r1 = min(r0 + a.block_rows, a.rows);
+    const int64_t r0 = block * a.block_rows;
+    int rows = (int)min(a.block_rows, a.rows - r0);
+    if constexpr (HOW == kWide) {  // (in any order: each is by itself)
+        if (threadIdx.x < kBlockRows && s_close[threadIdx.x / 32] >> threadIdx.x % 32 & 1) s_list[atomicAdd(&s_rows, 1u)] = threadIdx.x;
+        __syncthreads();
+        rows = (int)s_rows;
+        if (!rows) return;
+    }
     float bias[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) bias[i] = SCORED && a.bias && e0 + i < a.n ? a.bias[e0 + i] : 0.0f;
-    for (int64_t base = r0; base < r1; base += at_once) {
-        const int64_t row = base + in_block;
-        const bool live = row < r1;
+    for (int base = 0; base < rows; base += at_once) {
+        const int at = base + in_block;
+        bool live = at < rows;
+        const int64_t row = r0 + (HOW == kWide ? (live ? s_list[at] : 0) : at);
         float x[V];
         load_logits<T, V>(a, row, e0, live, x);
         // the row's maximum and sum, where a weight or a choice needs them
@@ -269,41 +323,65 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
         uint32_t plain[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) plain[i] = x[i] == -INFINITY || bias[i] == -INFINITY || e0 + i >= a.n ? 0 : key_of(x[i]);
-        if constexpr (SCORED) {
+        if constexpr (HOW == kScores) {
+            bool close = false;
             float v[V], most = 0.0f;
-            uint32_t key[V], worth[V];
+            uint32_t key[V];
             scores<V>(a, x, top, v);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                v[i] += bias[i];
-                worth[i] = plain[i] ? key_of(v[i]) : 0;
+                v[i] = plain[i] ? v[i] + bias[i] : -INFINITY;
+                close = close || v[i] != v[i];
                 most = plain[i] ? fmaxf(most, fabsf(v[i])) : most;
-                key[i] = a.bias ? worth[i] : plain[i];
+                key[i] = !a.bias || !plain[i] ? plain[i] : key_of(v[i]);
             }
             over_lanes(a.lanes, [&](auto&& other) { most = fmaxf(most, as_float(other(as_bits(most)))); });
-            const float apart = 8e-6f * (1.0f + most);  // (twice 32 2^-24, and twice that for a sum of two)
-            bool near = false;
-            if (a.groups > 1) keep<V>(a, worthiest<V>(a, worth, lane, e0, (uint32_t*)s_key, (uint32_t*)s_worth, apart, near), e0, key);
-            // (without a bias the keys are the logits, and exact)
-            const bool close = a.bias ? choose<V, true>(a, key, lane, e0, picks, apart)
-                                      : choose<V, false>(a, key, lane, e0, picks, 0.0f);
-            if (__any(live && (near || close))) {
-                double d[V];
-                uint64_t wide[V], sum_of[V];
-                scores<V>(a, x, top, d);
+            // (A sigmoid is within 6 2^-24, a softmax, whose sum has n terms, within 32 2^-24, and its sum with
+            // the bias within another 2^-24 of itself; two values, each of them a sum of two.)
+            const float apart = (a.sigmoid ? 2e-6f : 8e-6f) * (1.0f + most);
+            if (a.groups > 1) {
+                bool near = true;
+                const bool worthy = !a.group_lanes || mine_is_worthy<V>(a, v, lane, e0, (float*)s_worth, apart, near);
+                close = close || near;
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    d[i] += (double)bias[i];
-                    sum_of[i] = plain[i] ? key_of(d[i]) : 0;
-                    wide[i] = a.bias ? sum_of[i] : plain[i];
-                }
-                if (a.groups > 1) keep<V>(a, worthiest<V>(a, sum_of, lane, e0, s_key, s_worth, 0.0f, near), e0, wide);
-                choose<V, false>(a, wide, lane, e0, picks, 0.0f);
+                for (int i = 0; i < V; ++i) key[i] = worthy ? key[i] : 0;
             }
+            if (a.bias) {
+                const uint32_t left = choose<V, true>(a, key, lane, e0, picks);
+                wave_sync();
+                if (l < a.k && picks[l].e >= 0) {  // (a value and the next one; none: no matter)
+                    const bool last = l + 1 == a.k, none = last ? !left : picks[l + 1].e < 0;
+                    const float next = last ? number_of(left) : picks[l + 1].x;
+                    close = close || (!none && !(picks[l].x - next > apart));
+                }
+            } else {  // (the keys are the logits, and exact)
+                choose<V, false>(a, key, lane, e0, picks);
+            }
+            const uint64_t of_row = a.lanes == 64 ? ~0ull : ((1ull << a.lanes) - 1) << (lane & ~(a.lanes - 1));
+            if (__ballot(live && close) & of_row) {
+                live = false;
+                if (l == 0) atomicOr(&s_close[at / 32], 1u << at % 32);
+            }
+        } else if constexpr (HOW == kWide) {
+            double d[V];
+            scores<V>(a, x, top, d);
+            K key[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] = plain[i] ? key_of(d[i] + (double)bias[i]) : 0;
+            const uint64_t groups = a.groups > 1 ? worthiest<V>(a, key, lane, e0, s_key, s_worth) : ~0ull;
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] = a.bias ? key[i] : plain[i];
+            if (a.groups > 1) keep<V>(a, groups, e0, key);
+            choose<V, false>(a, key, lane, e0, picks);
         } else {
-            bool near;
-            if (a.groups > 1) keep<V>(a, worthiest<V>(a, plain, lane, e0, s_key, s_worth, 0.0f, near), e0, plain);
-            choose<V, false>(a, plain, lane, e0, picks, 0.0f);
+            if (a.groups > 1 && a.group_lanes) {
+                const bool worthy = mine_is_worthy<V>(a, plain, lane, e0, s_worth);
+#pragma unroll
+                for (int i = 0; i < V; ++i) plain[i] = worthy ? plain[i] : 0;
+            } else if (a.groups > 1) {
+                keep<V>(a, worthiest<V>(a, plain, lane, e0, s_key, s_worth), e0, plain);
+            }
+            choose<V, false>(a, plain, lane, e0, picks);
         }
         wave_sync();
         // a lane for each choice
@@ -334,7 +412,11 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
         wave_sync();
     }
     __syncthreads();
-    for (int i = threadIdx.x; i <= a.n; i += kThreads) a.counts[i * a.blocks + block] = s_count[i];
+    if (HOW == kScores && threadIdx.x < kBlockRows / 32) a.close[block * (kBlockRows / 32) + threadIdx.x] = s_close[threadIdx.x];
+    for (int i = threadIdx.x; i <= a.n; i += kThreads) {
+        uint32_t* c = a.counts + i * a.blocks + block;
+        *c = HOW == kWide ? *c + s_count[i] : s_count[i];
+    }
 }
 
 // The counts of an expert become those of the workgroups before; a workgroup for each.
@@ -539,7 +621,7 @@ dg_status check(const dg_route_desc* d)
 // Lanes of a row and experts of a lane.
 void share(const dg_route_desc* d, int* lanes, int* each)
 {
-    *lanes = std::min(64, std::max({power_of_two((d->n_experts + 3) / 4), power_of_two(d->k), power_of_two(d->groups)}));
+    *lanes = std::min(64, std::max({power_of_two((d->n_experts + 7) / 8), power_of_two(d->k), power_of_two(d->groups)}));
     *each = power_of_two((d->n_experts + *lanes - 1) / *lanes);
 }
 
@@ -547,20 +629,21 @@ void share(const dg_route_desc* d, int* lanes, int* each)
 int64_t rows_of_block(const dg_route_desc* d)
 {
     int64_t n = 32;
-    while (n < 256 && n * 2048 < d->n_rows) n *= 2;
+    while (n < kBlockRows && n * 2048 < d->n_rows) n *= 2;
     return n;
 }
 
 struct Layout {
     int64_t blocks;
-    size_t o_totals, total;
+    size_t o_totals, o_close, total;
 };
 Layout layout(const dg_route_desc* d)
 {
     Layout L;
     L.blocks = (d->n_rows + rows_of_block(d) - 1) / rows_of_block(d);
     L.o_totals = al(4 * (size_t)(L.blocks * (d->n_experts + 1)));
-    L.total = L.o_totals + al(4 * (size_t)(d->n_experts + 1));
+    L.o_close = L.o_totals + al(4 * (size_t)(d->n_experts + 1));
+    L.total = L.o_close + al((size_t)L.blocks * (kBlockRows / 8));
     return L;
 }
 
@@ -578,6 +661,8 @@ Args make_args(const dg_route_desc* d, int* each)
     a.renormalize = d->renormalize != 0;
     a.scale = d->scale;
     share(d, &a.lanes, each);
+    const int per = a.n / a.groups, whole = per / *each;
+    a.group_lanes = per % *each == 0 && whole == power_of_two(whole) ? whole : 0;
     return a;
 }
 
@@ -591,13 +676,17 @@ dg_status launched(const char* what)
 template <typename T, int V>
 void run_route(const Args& a, hipStream_t s)
 {
-    const bool wide = a.bias || (a.groups > 1 && a.group_best == 2);
+    const bool scored = a.bias || (a.groups > 1 && a.group_best == 2);
     const int at_once = kThreads / a.lanes;
-    size_t lds = 4 * (size_t)((a.n + 4) & ~3) + 8 * (size_t)((at_once * a.k + 1) & ~1);
-    if (a.groups > 1) lds += (wide ? 8 : 4) * (size_t)at_once * (a.n + a.groups);
-    const dim3 grid = workgroups(a.blocks);
-    if (wide) hipLaunchKernelGGL((route_kernel<T, V, true>), grid, dim3(kThreads), lds, s, a);
-    else hipLaunchKernelGGL((route_kernel<T, V, false>), grid, dim3(kThreads), lds, s, a);
+    const size_t lds = 4 * (size_t)((a.n + 4) & ~3) + 8 * (size_t)((at_once * a.k + 1) & ~1);
+    const size_t keys = a.groups > 1 ? (size_t)at_once * (a.n + a.groups) : 0;
+    const dim3 grid = workgroups(a.blocks), block(kThreads);
+    if (!scored) {
+        hipLaunchKernelGGL((route_kernel<T, V, kLogits>), grid, block, lds + 4 * keys, s, a);
+    } else {
+        hipLaunchKernelGGL((route_kernel<T, V, kScores>), grid, block, lds + 4 * keys, s, a);
+        hipLaunchKernelGGL((route_kernel<T, V, kWide>), grid, block, lds + 8 * keys, s, a);
+    }
 }
 
 template <typename T>
@@ -658,6 +747,7 @@ dg_status dg_route_forward(const dg_route_desc* d, const void* logits, const flo
     a.blocks = L.blocks;
     a.counts = (uint32_t*)ws;
     a.totals = (uint32_t*)((char*)ws + L.o_totals);
+    a.close = (uint32_t*)((char*)ws + L.o_close);
     if (d->n_rows > 0) {
         if (d->dtype == DG_BF16) run_route<__bf16>(a, each, s);
         else run_route<float>(a, each, s);
