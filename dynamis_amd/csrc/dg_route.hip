@@ -452,7 +452,10 @@ __global__ __launch_bounds__(1024) void scan_kernel(Args a)
 }
 
 // The places of a workgroup's choices: where its experts' choices begin, and a rank within the
-// workgroup in the choices' order (a quarter of them to a wave).
+// workgroup in the choices' order (a quarter of them to a wave).  SUMS: adds up the counts itself, which
+// saves the scan's launch (864 rows: 22.6 to 18.7 us a call) but has each workgroup read them all.
+constexpr int kFewBlocks = 32;
+template <bool SUMS>
 __global__ __launch_bounds__(kThreads) void place_kernel(Args a)
 {
     __shared__ uint32_t s_at[kWaves][kMaxExperts + 1];
@@ -474,7 +477,21 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Args a)
     uint32_t before = 0;
     for (int e0 = 0; e0 <= a.n; e0 += kThreads) {
         const int e = e0 + threadIdx.x;
-        const uint32_t x = e <= a.n ? a.totals[e] : 0;
+        uint32_t x = 0, earlier = 0;
+        if (e <= a.n) {
+            if constexpr (SUMS) {
+#pragma unroll 8
+                for (int b = 0; b < a.blocks; ++b) {
+                    const uint32_t n = a.counts[e * a.blocks + b];
+                    x += n;
+                    earlier += b < block ? n : 0;
+                }
+                if (block == 0 && e < a.n) a.sizes[e] = x;
+            } else {
+                x = a.totals[e];
+                earlier = a.counts[e * a.blocks + block];
+            }
+        }
         uint32_t in = x;
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t y = __shfl_up(in, o, 64);
@@ -488,7 +505,7 @@ __global__ __launch_bounds__(kThreads) void place_kernel(Args a)
             before += s_wave[j];
         }
         if (e <= a.n) {
-            at += a.counts[e * a.blocks + block];
+            at += earlier;
             for (int j = 0; j < kWaves; ++j) {
                 const uint32_t n = s_at[j][e];
                 s_at[j][e] = at;
@@ -752,8 +769,12 @@ dg_status dg_route_forward(const dg_route_desc* d, const void* logits, const flo
         if (d->dtype == DG_BF16) run_route<__bf16>(a, each, s);
         else run_route<float>(a, each, s);
     }
+    if (a.blocks > 0 && a.blocks <= kFewBlocks) {
+        hipLaunchKernelGGL(place_kernel<true>, dim3((unsigned)a.blocks), dim3(kThreads), 0, s, a);
+        return launched("dg_route_forward");
+    }
     hipLaunchKernelGGL(scan_kernel, dim3(a.n + 1), dim3(1024), 0, s, a);
-    if (d->n_rows > 0) hipLaunchKernelGGL(place_kernel, workgroups(a.blocks), dim3(kThreads), 0, s, a);
+    if (d->n_rows > 0) hipLaunchKernelGGL(place_kernel<false>, workgroups(a.blocks), dim3(kThreads), 0, s, a);
     return launched("dg_route_forward");
 }
 

@@ -255,6 +255,36 @@ def _whole_rows(t):
     return t if (t.stride(1) == 1 or t.size(1) == 1) and 0 <= t.stride(0) <= 1 << 31 else t.contiguous()
 
 
+def _check_route(logits, k, scoring, bias, groups, top_groups, group_best, scale):
+    """The refusals of route_rows, with their messages."""
+    _check(isinstance(logits, torch.Tensor) and logits.is_cuda, "logits must be a CUDA tensor")
+    _check(logits.dim() == 2, f"logits must have shape [rows, experts], got {_shape(logits)}")
+    _check(logits.dtype in _DTYPES, f"logits must be float32 or bfloat16, got {logits.dtype}")
+    rows, experts = logits.shape
+    _check(1 <= experts <= 1024, f"there must be 1 to 1024 experts, got {experts}")
+    _check(1 <= k <= min(64, experts), f"k must be 1 to {min(64, experts)}, got {k}")
+    _check(rows * k < 1 << 31, f"rows times k must be below 2^31, got {rows} times {k}")
+    _check(scoring in ("softmax", "sigmoid"), f'scoring must be "softmax" or "sigmoid", got {scoring!r}')
+    _check(1 <= groups <= 64 and experts % groups == 0, f"groups must be 1 to 64 and divide the {experts} experts, got {groups}")
+    _check(1 <= top_groups <= groups, f"top_groups must be 1 to {groups}, got {top_groups}")
+    _check(group_best in (1, 2), f"group_best must be 1 or 2, got {group_best}")
+    _check(-3e38 <= scale <= 3e38, f"scale must be finite, got {scale}")
+    if bias is not None:
+        _check(isinstance(bias, torch.Tensor) and bias.device == logits.device and bias.is_floating_point()
+               and tuple(bias.shape) == (experts,), f"bias must be floating [{experts}] on {logits.device}")
+
+
+def _route_is_fine(logits, k, scoring, bias, groups, top_groups, group_best, scale):
+    """Whether _check_route would pass, without its messages' host time."""
+    if not (type(logits) in _TENSORS and logits.is_cuda and logits.dim() == 2 and (bias is None or type(bias) in _TENSORS)):
+        return False
+    rows, experts = logits.shape
+    return (logits.dtype in _DTYPES and 1 <= k <= 64 and k <= experts <= 1024 and rows * k < 1 << 31
+            and (scoring == "softmax" or scoring == "sigmoid") and 1 <= groups <= 64 and experts % groups == 0
+            and 1 <= top_groups <= groups and 1 <= group_best <= 2 and -3e38 <= scale <= 3e38
+            and (bias is None or bias.device == logits.device and bias.is_floating_point() and bias.shape == (experts,)))
+
+
 def route_rows(logits, k, scoring="softmax", bias=None, groups=1, top_groups=1, group_best=1, renormalize=True, scale=1.0):
     """The k experts of each row by its logits, their weights, and the experts' order of the rows.
 
@@ -278,22 +308,11 @@ def route_rows(logits, k, scoring="softmax", bias=None, groups=1, top_groups=1, 
     """
     if forward_ad._current_level >= 0:
         _refuse_tangents("route_rows", logits, bias)
-    _check(isinstance(logits, torch.Tensor) and logits.is_cuda, "logits must be a CUDA tensor")
-    _check(logits.dim() == 2, f"logits must have shape [rows, experts], got {_shape(logits)}")
-    _check(logits.dtype in _DTYPES, f"logits must be float32 or bfloat16, got {logits.dtype}")
-    rows, experts = logits.shape
     k, groups, top_groups, group_best = int(k), int(groups), int(top_groups), int(group_best)
-    _check(1 <= experts <= 1024, f"there must be 1 to 1024 experts, got {experts}")
-    _check(1 <= k <= min(64, experts), f"k must be 1 to {min(64, experts)}, got {k}")
-    _check(rows * k < 1 << 31, f"rows times k must be below 2^31, got {rows} times {k}")
-    _check(scoring in ("softmax", "sigmoid"), f'scoring must be "softmax" or "sigmoid", got {scoring!r}')
-    _check(1 <= groups <= 64 and experts % groups == 0, f"groups must be 1 to 64 and divide the {experts} experts, got {groups}")
-    _check(1 <= top_groups <= groups, f"top_groups must be 1 to {groups}, got {top_groups}")
-    _check(group_best in (1, 2), f"group_best must be 1 or 2, got {group_best}")
-    _check(-3e38 <= scale <= 3e38, f"scale must be finite, got {scale}")
+    if not _route_is_fine(logits, k, scoring, bias, groups, top_groups, group_best, scale):
+        _check_route(logits, k, scoring, bias, groups, top_groups, group_best, scale)
+    rows, experts = logits.shape
     if bias is not None:
-        _check(isinstance(bias, torch.Tensor) and bias.device == logits.device and bias.is_floating_point()
-               and tuple(bias.shape) == (experts,), f"bias must be floating [{experts}] on {logits.device}")
         bias = bias.detach().float().contiguous()
     logits = _whole_rows(logits)
     d = L.RouteDesc(rows, logits.stride(0), experts, k, groups, top_groups, group_best, scoring == "sigmoid",
@@ -365,7 +384,10 @@ class _Combine(torch.autograd.Function):
 
 
 def _check_rows(name, t, routing, rows):
-    _check(isinstance(routing, Routing), "routing must be a Routing")
+    """The refusals of rows that go with a routing; their messages cost host time where one is due alone."""
+    if type(t) in _TENSORS and t.dim() == 2 and t.size(0) == rows and t.dtype in _DTYPES \
+            and t.device == routing.places.device and 1 <= t.size(1) <= 1 << 20:
+        return
     _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a CUDA tensor")
     _check(t.dim() == 2 and t.size(0) == rows, f"{name} must have shape [{rows}, width], got {_shape(t)}")
     _check(t.dtype in _DTYPES, f"{name} must be float32 or bfloat16, got {t.dtype}")
@@ -405,8 +427,9 @@ def combine_rows(y, routing, residual=None):
     _check_rows("y", y, routing, routing.rows * routing.k)
     if residual is not None:
         _check_rows("residual", residual, routing, routing.rows)
-        _check(residual.dtype == y.dtype and residual.size(1) == y.size(1),
-               f"residual must be {y.dtype} [{routing.rows}, {y.size(1)}], got {residual.dtype} {_shape(residual)}")
+        if residual.dtype != y.dtype or residual.size(1) != y.size(1):
+            raise RuntimeError(f"residual must be {y.dtype} [{routing.rows}, {y.size(1)}], "
+                               f"got {residual.dtype} {_shape(residual)}")
         residual = _whole_rows(residual)
     y, weights = y.contiguous(), routing.weights
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad
