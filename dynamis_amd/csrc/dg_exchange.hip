@@ -6,7 +6,8 @@
 //
 // The gradient of a dispatch is a combine without weights.  A place p < 0 is a choice of none: -1 - p
 // is its place behind the last, which gets zeros and is not read.  places is a permutation, so every
-// row of the experts' order is written by one owner; a row's sum is taken over j in order, in 32 bits.
+// row of the experts' order is written by one owner (a place past the last row is left out); a row's sum is
+// taken over j in order, in 32 bits.
 //
 // Bound by memory: rows are read and written whole, 16 bytes a lane, a power of two of lanes to a row
 // as far as its width goes (an x row is read once for all of its places; a sum's k rows are in flight
@@ -91,20 +92,28 @@ __device__ __forceinline__ int64_t my_row(const Args& a, int& c0)
     return workgroup() * (kThreads / a.lanes) + threadIdx.x / a.lanes;
 }
 
-template <typename T, bool WHOLE>
+// Where a place points to, and whether that row is of a choice; false: there is no such row.
+__device__ __forceinline__ bool place_of(const Args& a, int32_t p, int64_t& at, bool& taken)
+{
+    taken = p >= 0;
+    at = taken ? p : -1 - p;
+    return at < a.rows * a.k;
+}
+
+// (Bits as they are: W is a chunk of 16 bytes, or an element.)
+template <typename W>
 __global__ __launch_bounds__(kThreads) void dispatch_kernel(Args a)
 {
-    using Ch = Chunk<T, WHOLE>;
     int c0;
-    const int64_t row = my_row<Ch::C>(a, c0);
+    const int64_t row = my_row<1>(a, c0);
     if (row >= a.rows) return;
     const int32_t* places = a.places + row * a.k;
-    for (int c = c0; c < a.width; c += a.lanes * Ch::C) {
-        float v[Ch::C], zero[Ch::C] = {};
-        Ch::load((const T*)a.x + row * a.ld + c, v);
+    for (int c = c0; c < a.width; c += a.lanes) {
+        const W v = ((const W*)a.x)[row * a.ld + c], zero = {};
         for (int j = 0; j < a.k; ++j) {
-            const int32_t p = places[j];
-            Ch::store((T*)a.out + (int64_t)(p < 0 ? -1 - p : p) * a.width + c, p < 0 ? zero : v);
+            int64_t at;
+            bool taken;
+            if (place_of(a, places[j], at, taken)) ((W*)a.out)[at * a.width + c] = taken ? v : zero;
         }
     }
 }
@@ -124,11 +133,15 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(Args a)
             bool there[kInFlight];
 #pragma unroll
             for (int j = 0; j < kInFlight; ++j) {
-                const int32_t p = j0 + j < a.k ? places[j0 + j] : -1;
-                there[j] = p >= 0;
+                int64_t at;
+                there[j] = j0 + j < a.k;
+                if (there[j]) {
+                    bool taken;
+                    there[j] = place_of(a, places[j0 + j], at, taken) && taken;
+                }
                 w[j] = 1.0f;
                 if (there[j]) {
-                    Ch::load((const T*)a.y + (int64_t)p * a.width + c, y[j]);
+                    Ch::load((const T*)a.y + at * a.width + c, y[j]);
                     if (a.weights) w[j] = a.weights[row * a.k + j0 + j];
                 }
             }
@@ -154,14 +167,17 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(Args a)
     const int64_t row = my_row<Ch::C>(a, c0);
     const bool live = row < a.rows;  // (the wave stays whole for its sums)
     for (int j = 0; j < a.k; ++j) {
-        const int32_t p = live ? a.places[row * a.k + j] : -1;
-        const float w = live && p >= 0 ? a.weights[row * a.k + j] : 0.0f;
-        const int64_t at = (int64_t)(p < 0 ? -1 - p : p) * a.width;
+        int64_t at = 0;
+        bool taken = false;
+        const bool there = live && place_of(a, a.places[row * a.k + j], at, taken);
+        taken = taken && there;
+        const float w = taken ? a.weights[row * a.k + j] : 0.0f;
+        at *= a.width;
         float dot = 0.0f;
-        if (live)
+        if (there)
             for (int c = c0; c < a.width; c += a.lanes * Ch::C) {
                 float d[Ch::C] = {};
-                if (p >= 0) {
+                if (taken) {
                     float g[Ch::C], y[Ch::C];
                     Ch::load((const T*)a.grad + row * a.ld + c, g);
                     if (a.dweights) {
@@ -174,7 +190,7 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(Args a)
             }
         if (a.dweights) {
             dot = sum_lanes(dot, a.lanes);
-            if (live && c0 == 0) a.dweights[row * a.k + j] = p < 0 ? 0.0f : dot;
+            if (live && c0 == 0) a.dweights[row * a.k + j] = dot;
         }
     }
 }
@@ -218,14 +234,18 @@ bool whole(const dg_exchange_desc* d, std::initializer_list<const void*> p)
     return ok;
 }
 
+// Lanes of a row of chunks of c elements, and the workgroups.
+dim3 grid_of(Args& a, int c)
+{
+    a.lanes = 1;
+    while (a.lanes < 64 && a.lanes * c < a.width) a.lanes *= 2;
+    const int64_t rows = kThreads / a.lanes;
+    return workgroups((a.rows + rows - 1) / rows);
+}
 template <typename F>
 void run(const dg_exchange_desc* d, Args& a, bool whole, F&& launch)
 {
-    const int c = !whole ? 1 : d->dtype == DG_F32 ? 4 : 8;
-    a.lanes = 1;
-    while (a.lanes < 64 && a.lanes * c < d->width) a.lanes *= 2;
-    const int64_t rows = kThreads / a.lanes;
-    launch(workgroups((a.rows + rows - 1) / rows));
+    launch(grid_of(a, !whole ? 1 : d->dtype == DG_F32 ? 4 : 8));
 }
 
 }  // namespace
@@ -252,8 +272,16 @@ dg_status dg_exchange_dispatch(const dg_exchange_desc* d, const void* x, const i
     Args a = make_args(d, places);
     a.x = x;
     a.out = out;
+    const int c = d->dtype == DG_F32 ? 4 : 8;
     const bool all = whole(d, {x, out});
-    DG_LAUNCH(dispatch_kernel);
+    if (all) {
+        a.width /= c;
+        a.ld /= c;
+    }
+    const dim3 grid = grid_of(a, 1), block(kThreads);
+    if (all) hipLaunchKernelGGL(dispatch_kernel<u32x4>, grid, block, 0, s, a);
+    else if (c == 4) hipLaunchKernelGGL(dispatch_kernel<uint32_t>, grid, block, 0, s, a);
+    else hipLaunchKernelGGL(dispatch_kernel<uint16_t>, grid, block, 0, s, a);
     return launched("dg_exchange_dispatch");
 }
 

@@ -296,6 +296,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
         rows = (int)s_rows;
         if (!rows) return;
     }
+    const uint64_t of_row = a.lanes == 64 ? ~0ull : ((1ull << a.lanes) - 1) << (lane & ~(a.lanes - 1));
     float bias[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) bias[i] = SCORED && a.bias && e0 + i < a.n ? a.bias[e0 + i] : 0.0f;
@@ -323,6 +324,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
         uint32_t plain[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) plain[i] = x[i] == -INFINITY || bias[i] == -INFINITY || e0 + i >= a.n ? 0 : key_of(x[i]);
+        bool poisoned = false;  // a softmax with a NaN or an infinity: every weight is one, whichever are chosen
         if constexpr (HOW == kScores) {
             bool close = false;
             float v[V], most = 0.0f;
@@ -357,7 +359,6 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
             } else {  // (the keys are the logits, and exact)
                 choose<V, false>(a, key, lane, e0, picks);
             }
-            const uint64_t of_row = a.lanes == 64 ? ~0ull : ((1ull << a.lanes) - 1) << (lane & ~(a.lanes - 1));
             if (__ballot(live && close) & of_row) {
                 live = false;
                 if (l == 0) atomicOr(&s_close[at / 32], 1u << at % 32);
@@ -367,7 +368,11 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
             scores<V>(a, x, top, d);
             K key[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) key[i] = plain[i] ? key_of(d[i] + (double)bias[i]) : 0;
+            for (int i = 0; i < V; ++i) {
+                key[i] = plain[i] ? key_of(d[i] + (double)bias[i]) : 0;
+                poisoned = poisoned || (!a.sigmoid && d[i] != d[i]);
+            }
+            poisoned = __ballot(poisoned) & of_row;
             const uint64_t groups = a.groups > 1 ? worthiest<V>(a, key, lane, e0, s_key, s_worth) : ~0ull;
 #pragma unroll
             for (int i = 0; i < V; ++i) key[i] = a.bias ? key[i] : plain[i];
@@ -406,7 +411,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
         }
         if (mine) {
             a.experts[row * a.k + l] = e;
-            a.weights[row * a.k + l] = w * a.scale;
+            a.weights[row * a.k + l] = poisoned && e >= 0 ? NAN : w * a.scale;
             atomicAdd(&s_count[e < 0 ? a.n : e], 1u);
         }
         wave_sync();

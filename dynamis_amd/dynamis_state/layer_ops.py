@@ -421,9 +421,9 @@ def combine_rows(y, routing, residual=None):
     expert's rows.  Sums are 32 bits, in the choices' order, and rounded once.  Differentiable in y, the
     routing's weights (and so in the router's logits) and the residual, once, in reverse.
     """
-    if forward_ad._current_level >= 0:
-        _refuse_tangents("combine_rows", y, residual)
     _check(isinstance(routing, Routing), "routing must be a Routing")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("combine_rows", y, routing.weights, residual)
     _check_rows("y", y, routing, routing.rows * routing.k)
     if residual is not None:
         _check_rows("residual", residual, routing, routing.rows)
@@ -431,7 +431,9 @@ def combine_rows(y, routing, residual=None):
             raise RuntimeError(f"residual must be {y.dtype} [{routing.rows}, {y.size(1)}], "
                                f"got {residual.dtype} {_shape(residual)}")
         residual = _whole_rows(residual)
-    y, weights = y.contiguous(), routing.weights
+    y, weights = y.contiguous(), routing.weights.contiguous()
+    if weights.dtype != torch.float32 or weights.shape != routing.places.shape:
+        raise RuntimeError(f"routing.weights must be float32 {_shape(routing.places)}, got {weights.dtype} {_shape(weights)}")
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad
                                     or residual is not None and residual.requires_grad):
         return _Combine.apply(y, weights, residual, routing.places)

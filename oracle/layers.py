@@ -106,6 +106,8 @@ def route_rows(logits, k, scoring="softmax", bias=None, groups=1, top_groups=1, 
                 if np.isnan(ls).any() or np.isposinf(ls).any():
                     u = np.full(len(taken), np.nan)
                 u = u / u.sum()
+                if scoring == "softmax" and np.isnan(s).any():
+                    u = np.full(len(taken), np.nan)
             else:
                 u = s[taken]
             weights[i, :len(taken)] = scale * u
