@@ -28,14 +28,20 @@ _POSITIONS = {torch.float32: L.DG_F32, torch.float64: L.DG_F64, torch.int64: L.D
 
 
 @functools.lru_cache(maxsize=64)
-def _sections(sections):
+def _sections(sections, axes, pairs):
+    """Pairs of each axis as the kernels take them."""
+    if sections is None:
+        _check(pairs % axes == 0, f"{pairs} frequencies do not go into {axes} equal sections")
+        sections = (pairs // axes,) * axes
+    _check(len(sections) == axes and min(sections) >= 0 and sum(sections) == pairs,
+           f"sections must be {axes} numbers, not negative, that add up to {pairs}, got {sections}")
     return (ctypes.c_int32 * 8)(*sections)
 
 
 def _rotate_desc(q, k, axes, sections, weight, norm, eps, interleaved, pos_dtype):
     dtype = _DTYPES[q.dtype]
     return L.RotateDesc(q.size(0), k.size(0), q.stride(0), k.stride(0), 0, 0, q.size(1), k.size(1), q.size(2), axes,
-                        _sections(sections), dtype, dtype if weight is None else _DTYPES[weight.dtype],
+                        sections, dtype, dtype if weight is None else _DTYPES[weight.dtype],
                         _POSITIONS[pos_dtype], norm, interleaved, eps)
 
 
@@ -172,15 +178,9 @@ def rotate_heads(q, k, positions, frequencies, sections=None, q_weight=None, k_w
         if positions.dim() == 1:
             positions = positions.unsqueeze(1)
     axes, pairs = positions.size(1), frequencies.size(0)
-    if sections is None:
-        if pairs % axes:
-            raise RuntimeError(f"{pairs} frequencies do not go into {axes} equal sections")
-        sections = (pairs // axes,) * axes
-    else:
-        sections = tuple(int(n) for n in sections)
-        _check(len(sections) == axes and min(sections) >= 0 and sum(sections) == pairs,
-               f"sections must be {axes} numbers, not negative, that add up to {pairs}, got {sections}")
-    _check(not norm or 0.0 <= eps <= 3e38, f"eps must be finite and not negative, got {eps}")
+    sections = _sections(sections if sections is None else tuple(map(int, sections)), axes, pairs)
+    if norm and not 0.0 <= eps <= 3e38:
+        raise RuntimeError(f"eps must be finite and not negative, got {eps}")
     positions, frequencies = positions.contiguous(), frequencies.contiguous()
     if q_weight is not None:
         q_weight = q_weight.contiguous()
