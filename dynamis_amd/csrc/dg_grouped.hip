@@ -219,17 +219,17 @@ __device__ __forceinline__ void multiply(const char* rows, const char* cols, int
 enum { kPlain, kApply, kSlope };
 
 // f(z) (SLOPE: its derivative), in some ten to thirty instructions, which the library's functions would take
-// twice.  silu: from exp(-|z|), which neither overflows nor loses 1 - s.  gelu: the normal distribution's share
+// twice.  silu: its slope from exp(-|z|), which neither overflows nor loses 1 - s.  gelu: the normal distribution's share
 // beyond |z| is exp(-z^2 / 2) t Q(t) with t = 1 / (1 + 0.318 |z|), so that it keeps its digits far out; Q is a
 // least-maximum fit of degree 9 to it in relative error (0.55 2^-24, 5.1 2^-24 as evaluated).
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ float activation(float z)
 {
     if constexpr (ACT == DG_ACT_SILU) {
+        // (below -87 the reciprocal of what has no 32-bit inverse is 0: values beneath 1e-36 are)
+        if constexpr (!SLOPE) return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * z));
         const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
-        const float s = z < 0.0f ? e * r : r;
-        if constexpr (!SLOPE) return z * s;
-        return s * fmaf(z, z < 0.0f ? r : e * r, 1.0f);
+        return (z < 0.0f ? e * r : r) * fmaf(z, z < 0.0f ? r : e * r, 1.0f);
     }
     if constexpr (ACT == DG_ACT_GELU) {
         const float e = __builtin_amdgcn_exp2f(-0.72134752f * (z * z)), t = __builtin_amdgcn_rcpf(fmaf(0.318f, fabsf(z), 1.0f));
@@ -251,16 +251,33 @@ __device__ __forceinline__ float activation(float z)
 }
 // N results at once (the branch is the same for the whole grid, and the N chains overlap).
 template <int EPI, int ACT, int N>
-__device__ __forceinline__ void finish_as(float (&z)[N], const float (&aux)[N])
+__device__ __forceinline__ void finish_as(bool more, float (&z)[N], const float (&aux)[N])
 {
-    for (int i = 0; i < N; ++i) z[i] = EPI == kApply ? activation<ACT, false>(z[i]) + aux[i] : activation<ACT, true>(z[i]) * aux[i];
+    for (int i = 0; i < N; ++i) z[i] = activation<ACT, EPI == kSlope>(z[i]);
+    if (EPI == kSlope)
+        for (int i = 0; i < N; ++i) z[i] *= aux[i];
+    else if (more)
+        for (int i = 0; i < N; ++i) z[i] += aux[i];
 }
 template <int EPI, int N>
-__device__ __forceinline__ void finish(int act, float (&z)[N], const float (&aux)[N])
+__device__ __forceinline__ void finish(int act, bool more, float (&z)[N], const float (&aux)[N])
 {
-    if (act == DG_ACT_SILU) finish_as<EPI, DG_ACT_SILU>(z, aux);
-    else if (act == DG_ACT_GELU) finish_as<EPI, DG_ACT_GELU>(z, aux);
-    else finish_as<EPI, DG_ACT_NONE>(z, aux);
+    if (act == DG_ACT_SILU) finish_as<EPI, DG_ACT_SILU>(more, z, aux);
+    else if (act == DG_ACT_GELU) finish_as<EPI, DG_ACT_GELU>(more, z, aux);
+    else finish_as<EPI, DG_ACT_NONE>(more, z, aux);
+}
+
+// Sums that begin with their columns' bias, 64 columns from c0 on.
+template <typename T>
+__device__ __forceinline__ void begin_with(f32x16 (&acc)[2][2], const T* bias, int c0, int cols, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const int c = c0 + 32 * i + 8 * (q / 4) + 4 * (lane >> 5) + q % 4;
+            acc[i][0][q] = acc[i][1][q] = c < cols ? (float)bias[c] : 0.0f;
+        }
 }
 
 // A wave's 64 x 64 of the result to memory: in the accumulators a lane holds four neighbouring
@@ -293,7 +310,7 @@ __device__ __forceinline__ void write_out(const f32x16 (&acc)[2][2], char* s, in
                     if (aux && 32 * j + x < n_rows)
                         for (int c = 0; c < 4; ++c)
                             if (col + c < n_cols) r[c] = (float)aux[(int64_t)(32 * j + x) * ld + col + c];
-                    finish<EPI>(act, z, r);
+                    finish<EPI>(act, aux != nullptr, z, r);
                     for (int c = 0; c < 4; ++c) v[c] = z[c];
                 }
                 if constexpr (sizeof(T) == 4) {
@@ -483,6 +500,8 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
             const int n_rows = (int)max((int64_t)0, min(min(size - piece * kTile, a.rows - my_row), (int64_t)kTile));
             const int col = (int)(u % col_tiles) * kTile;
             f32x16 acc[2][2] = {};
+            if constexpr (EPI != kPlain)  // (as stream_kernel has it: the same bits)
+                if (a.bias) begin_with(acc, (const T*)a.bias + my_group * a.cols, col + (w / 2) * 64, a.cols, lane);
             for (int slab = 0; slab < slabs; ++slab) {
                 __syncthreads();
                 if (first_half) SA::store(r, s_a, t);
@@ -509,7 +528,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
             const int c0 = col + (w / 2) * 64, r0 = (w % 2) * 64;
             const int64_t at = (my_row + r0) * a.cols + c0;
             write_out<T, EPI>(acc, s_out + w * kOutRows * kOutPitch<T>, lane, (T*)a.out + at, a.cols, n_rows - r0, a.cols - c0,
-                              !DX && a.bias ? (const T*)a.bias + my_group * a.cols + c0 : nullptr,
+                              !DX && EPI == kPlain && a.bias ? (const T*)a.bias + my_group * a.cols + c0 : nullptr,
                               EPI != kPlain && a.aux ? (const T*)a.aux + at : nullptr, a.act);
         }
     }
@@ -545,6 +564,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
 {
     __shared__ __attribute__((aligned(16))) char s_panel[65536];
     __shared__ __attribute__((aligned(16))) char s_x[kStreamWaves][kStripRows * kStepBytes];
+    __shared__ __attribute__((aligned(16))) float s_bias[EPI == kPlain ? 4 : PN];
     __shared__ int64_t s_w[3 * kStreamWaves];
     __shared__ Place s_p;
     constexpr int C = kChunk<T>, kStep = kStepBytes / (int)sizeof(T), kTiles = PN / 32;
@@ -580,8 +600,20 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                 else S::load(st, wt + (int64_t)col * a.depth, a.depth, min(a.cols - col, PN), s * kSlab<T>, a.depth, t);
                 S::store(st, s_panel + s * PN * kRowBytes, t);
             }
+            if constexpr (EPI != kPlain)
+                if ((int)threadIdx.x < PN)
+                    s_bias[threadIdx.x] = a.bias && col + (int)threadIdx.x < a.cols
+                                              ? (float)((const T*)a.bias)[g * a.cols + col + threadIdx.x] : 0.0f;
             __syncthreads();
         };
+        // where a lane's operands of a slab lie: x's chunks 2 s + half of row x, the panel's of rows 32 t + x (whose
+        // swap is that of row x, and another chunk's fourth for each second t)
+        int at_x[4], at_w[2][4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            at_x[s] = x * kStepBytes + ((2 * s + half) ^ (x & 15)) * 16;
+            for (int t = 0; t < 2; ++t) at_w[t][s] = x * kRowBytes + swapped(32 * t + x, 2 * s + half) * 16;
+        }
         // a lane loads a chunk of 16 bytes of each eighth row of 256: rows 4 i + quarter
         u32x4 r[8];
         auto fetch = [&](int64_t first_row, int n_rows, int step) {
@@ -602,6 +634,14 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
             const int64_t my_row = r0, my_group = group;
             const int my_rows = n_rows;
             f32x16 acc[kTiles] = {};
+            if constexpr (EPI != kPlain)  // (the bias is what the sums begin with: no instruction of its own)
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const f32x4 f = *(const f32x4*)(s_bias + 32 * t + 8 * q + 4 * half);
+                        for (int k = 0; k < 4; ++k) acc[t][4 * q + k] = f[k];
+                    }
             for (int step = 0; step < steps; ++step) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -629,12 +669,10 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                 for (int b = 0; b < inner; ++b)
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {
-                        const int c = 8 * b + 2 * s + half;
-                        const u32x4 v = *(const u32x4*)(my_x + x * kStepBytes + (c ^ (x & 15)) * 16);
+                        const u32x4 v = *(const u32x4*)(my_x + (at_x[s] ^ b << 7));
 #pragma unroll
                         for (int t = 0; t < kTiles; ++t) {
-                            const int rr = 32 * t + x;
-                            const u32x4 y = *(const u32x4*)(panel + (b * PN + rr) * kRowBytes + swapped(rr, 2 * s + half) * 16);
+                            const u32x4 y = *(const u32x4*)(panel + b * PN * kRowBytes + at_w[t & 1][s] + 32 * t * kRowBytes);
                             if constexpr (sizeof(T) == 2) {
                                 acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, y),
                                                                                  __builtin_bit_cast(bf16x8, v), acc[t], 0, 0, 0);
@@ -685,7 +723,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                 }
             } else {
                 // In 32 bits through the same 8 KB, 64 columns of each row at once, so that a lane has
-                // whole chunks of rows, the same columns in each of them: bias, residual (or dy) and
+                // whole chunks of rows, the same columns in each of them: residual (or dy) and
                 // activation there, and one rounding.  The chunks of `aux` are under way meanwhile.
                 constexpr int kWide = PN < 64 ? PN : 64, kPieces = PN / kWide, kChunks = kWide / C, kEach = kStripRows * kChunks / 64;
                 const Buffer out = buffer_of((const char*)a.out + my_row * ld_out, my_rows * ld_out);
@@ -699,11 +737,6 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
 #pragma unroll
                     for (int k = 0; k < kEach; ++k)
                         aux[k] = __builtin_amdgcn_raw_buffer_load_b128(in, at == kOutside ? at : (r_first + k * (64 / kChunks)) * (int)ld_out + at, 0, 0);
-                    float b[C] = {};
-                    if (a.bias && first < a.cols) {
-                        const T* p = (const T*)a.bias + my_group * a.cols + first;
-                        for (int i = 0; i < C; ++i) b[i] = (float)p[i];
-                    }
 #pragma unroll
                     for (int t = 0; t < kWide / 32; ++t)
 #pragma unroll
@@ -726,9 +759,8 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                         for (int i = 0; i < C; ++i) {
                             const uint32_t word = aux[k][i * (int)sizeof(T) / 4];
                             r[i] = as_float(sizeof(T) == 4 ? word : i % 2 ? word & 0xffff0000u : word << 16);
-                            v[i] += b[i];
                         }
-                        finish<EPI>(a.act, v, r);
+                        finish<EPI>(a.act, a.aux, v, r);
                         u32x4 y;
                         if constexpr (sizeof(T) == 4) {
                             for (int i = 0; i < 4; ++i) y[i] = as_bits(v[i]);
