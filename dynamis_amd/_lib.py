@@ -287,6 +287,28 @@ def lib():
     return L
 
 
+_torch_layer = None
+_TORCH_LAYER = ("dg_last_error", "dg_rotate_forward", "dg_rotate_workspace_size", "dg_rotate_backward", "dg_route_workspace_size",
+                "dg_route_forward", "dg_route_backward", "dg_exchange_dispatch", "dg_exchange_combine",
+                "dg_exchange_combine_backward", "dg_grouped_forward", "dg_grouped_apply", "dg_grouped_apply_backward",
+                "dg_grouped_workspace_size", "dg_grouped_backward")
+
+
+def torch_layer():
+    """The compiled calls of a layer's operators (csrc/torch_layer.cpp), on the library's entry points."""
+    global _torch_layer
+    if _torch_layer is None:
+        L = lib()
+        try:
+            from . import _torch_layer as module
+        except ImportError as e:
+            raise ImportError("dynamis_amd/_torch_layer.so cannot be loaded: build it first "
+                              "(python -m dynamis_amd.build, or __graft_entry__.build())") from e
+        module.load({name: ctypes.cast(getattr(L, name), _p).value for name in _TORCH_LAYER})
+        _torch_layer = module
+    return _torch_layer
+
+
 def check(status: int, what: str) -> None:
     if status != DG_OK:
         msg = lib().dg_last_error().decode(errors="replace")

@@ -9,12 +9,11 @@ back.
     x = combine_rows(rows, routing, residual=x)
 
 No counterpart in the reference.  The kernels are those of libdynamis_graph.so (dg_rotate_*, dg_route_*,
-dg_exchange_*); there is no CPU path.  Everything runs on the current stream without synchronising the host and can be
+dg_exchange_*), called through _torch_layer.so, which holds their autograd nodes; there is no CPU path.  Everything runs on the current stream without synchronising the host and can be
 captured in a HIP graph; tensors follow torch's rules for streams.
 """
 from __future__ import annotations
 
-import ctypes
 import functools
 
 import torch
@@ -22,75 +21,20 @@ from torch.autograd import forward_ad
 
 from .. import _lib as L
 from .dynamis_state_impl import _check, _shape
-from .neighbor_ops import _DTYPES, _TENSORS, _new_like, _refuse_tangents, _rows_16
+from .neighbor_ops import _DTYPES, _TENSORS, _refuse_tangents
 
-_POSITIONS = {torch.float32: L.DG_F32, torch.float64: L.DG_F64, torch.int64: L.DG_I64}
+_POSITIONS = torch.float32, torch.float64, torch.int64
 
 
 @functools.lru_cache(maxsize=64)
 def _sections(sections, axes, pairs):
-    """Pairs of each axis as the kernels take them."""
+    """Pairs of each axis."""
     if sections is None:
         _check(pairs % axes == 0, f"{pairs} frequencies do not go into {axes} equal sections")
         sections = (pairs // axes,) * axes
     _check(len(sections) == axes and min(sections) >= 0 and sum(sections) == pairs,
            f"sections must be {axes} numbers, not negative, that add up to {pairs}, got {sections}")
-    return (ctypes.c_int32 * 8)(*sections)
-
-
-def _rotate_desc(q, k, axes, sections, weight, norm, eps, interleaved, pos_dtype):
-    dtype = _DTYPES[q.dtype]
-    return L.RotateDesc(q.size(0), k.size(0), q.stride(0), k.stride(0), 0, 0, q.size(1), k.size(1), q.size(2), axes,
-                        sections, dtype, dtype if weight is None else _DTYPES[weight.dtype],
-                        _POSITIONS[pos_dtype], norm, interleaved, eps)
-
-
-def _rotate_forward(q, k, positions, frequencies, q_weight, k_weight, sections, eps, norm, interleaved):
-    q, k, dev = _rows_16(q), _rows_16(k), q.device
-    d = _rotate_desc(q, k, positions.size(1), sections, q_weight if k_weight is None else k_weight, norm, eps, interleaved,
-                     positions.dtype)
-    with L.on_device(dev):
-        q_out, k_out = _new_like(q), _new_like(k)
-        status = L.lib().dg_rotate_forward(d, q.data_ptr(), k.data_ptr(), positions.data_ptr(), frequencies.data_ptr(),
-                                           L.addr(q_weight), L.addr(k_weight), q_out.data_ptr(), k_out.data_ptr(),
-                                           L.raw_stream(dev))
-        if status:
-            L.check(status, "rotate_heads")
-    return q, k, d, q_out, k_out
-
-
-class _Rotate(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, frequencies, q_weight, k_weight, *how):
-        q, k, ctx.desc, q_out, k_out = _rotate_forward(q, k, positions, frequencies, q_weight, k_weight, *how)
-        ctx.save_for_backward(q, k, positions, frequencies, q_weight, k_weight)
-        return q_out, k_out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_q, grad_k):
-        q, k, positions, frequencies, q_weight, k_weight = ctx.saved_tensors
-        _, _, need_positions, _, need_qw, need_kw = ctx.needs_input_grad[:6]
-        lib, dev = L.lib(), q.device
-        grad_q, grad_k = _rows_16(grad_q), _rows_16(grad_k)
-        # (its own: another backward pass of the same graph may be under way with other strides)
-        d = L.RotateDesc.from_buffer_copy(ctx.desc)
-        d.ld_gq, d.ld_gk = grad_q.stride(0), grad_k.stride(0)
-        with L.on_device(dev):
-            dq, dk = _new_like(q), _new_like(k)
-            dpos = torch.empty_like(positions) if need_positions else None
-            dqw = torch.empty_like(q_weight) if need_qw else None
-            dkw = torch.empty_like(k_weight) if need_kw else None
-            wsb = lib.dg_rotate_workspace_size(d) if need_qw or need_kw else 0
-            ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-            addr = L.addr
-            status = lib.dg_rotate_backward(d, q.data_ptr(), k.data_ptr(), positions.data_ptr(), frequencies.data_ptr(),
-                                            addr(q_weight), addr(k_weight), grad_q.data_ptr(), grad_k.data_ptr(),
-                                            dq.data_ptr(), dk.data_ptr(), addr(dpos), addr(dqw), addr(dkw), addr(ws), wsb,
-                                            L.raw_stream(dev))
-            if status:
-                L.check(status, "rotate_heads")
-        return dq, dk, dpos, None, dqw, dkw, None, None, None, None
+    return sections
 
 
 def _check_rotate(q, k, positions, frequencies, q_weight, k_weight, norm):
@@ -181,17 +125,8 @@ def rotate_heads(q, k, positions, frequencies, sections=None, q_weight=None, k_w
     sections = _sections(sections if sections is None else tuple(map(int, sections)), axes, pairs)
     if norm and not 0.0 <= eps <= 3e38:
         raise RuntimeError(f"eps must be finite and not negative, got {eps}")
-    positions, frequencies = positions.contiguous(), frequencies.contiguous()
-    if q_weight is not None:
-        q_weight = q_weight.contiguous()
-    if k_weight is not None:
-        k_weight = k_weight.contiguous()
-    how = sections, float(eps), int(bool(norm)), int(bool(interleaved))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or positions.requires_grad
-                                    or q_weight is not None and q_weight.requires_grad
-                                    or k_weight is not None and k_weight.requires_grad):
-        return _Rotate.apply(q, k, positions, frequencies, q_weight, k_weight, *how)
-    return _rotate_forward(q, k, positions, frequencies, q_weight, k_weight, *how)[3:]
+    return L.torch_layer().rotate(q, k, positions, frequencies, q_weight, k_weight, sections, eps if norm else 0.0, bool(norm),
+                                  bool(interleaved))
 
 
 class Routing:
@@ -205,54 +140,6 @@ class Routing:
     def __init__(self, num_experts, weights, experts, sizes, places):
         (self.rows, self.k), self.num_experts = experts.shape, num_experts
         self.weights, self.experts, self.sizes, self.places = weights, experts, sizes, places
-
-
-def _route_forward(logits, bias, d):
-    lib, dev = L.lib(), logits.device
-    rows, k = logits.size(0), d.k
-    with L.on_device(dev):
-        weights = torch.empty((rows, k), dtype=torch.float32, device=dev)
-        experts = torch.empty((rows, k), dtype=torch.int32, device=dev)
-        places = torch.empty((rows, k), dtype=torch.int32, device=dev)
-        sizes = torch.empty(d.n_experts, dtype=torch.int64, device=dev)
-        wsb = lib.dg_route_workspace_size(d)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-        status = lib.dg_route_forward(d, logits.data_ptr(), L.addr(bias), weights.data_ptr(), experts.data_ptr(),
-                                      sizes.data_ptr(), places.data_ptr(), ws.data_ptr(), wsb, L.raw_stream(dev))
-        if status:
-            L.check(status, "route_rows")
-    return weights, experts, sizes, places
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, d):
-        weights, experts, sizes, places = _route_forward(logits, bias, d)
-        ctx.save_for_backward(logits, experts)
-        ctx.desc = d
-        ctx.mark_non_differentiable(experts, sizes, places)
-        ctx.set_materialize_grads(False)  # (zeros for the outputs without one are three launches)
-        return weights, experts, sizes, places
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad, *_):
-        if grad is None:
-            return None, None, None
-        logits, experts = ctx.saved_tensors
-        dev, grad = logits.device, grad.contiguous()
-        with L.on_device(dev):
-            dlogits = _new_like(logits)
-            status = L.lib().dg_route_backward(ctx.desc, logits.data_ptr(), experts.data_ptr(), grad.data_ptr(),
-                                               dlogits.data_ptr(), L.raw_stream(dev))
-            if status:
-                L.check(status, "route_rows")
-        return dlogits, None, None
-
-
-def _whole_rows(t):
-    """t [rows, width] as it is if its rows are whole; else a copy."""
-    return t if (t.stride(1) == 1 or t.size(1) == 1) and 0 <= t.stride(0) <= 1 << 31 else t.contiguous()
 
 
 def _check_route(logits, k, scoring, bias, groups, top_groups, group_best, scale):
@@ -311,76 +198,8 @@ def route_rows(logits, k, scoring="softmax", bias=None, groups=1, top_groups=1, 
     k, groups, top_groups, group_best = int(k), int(groups), int(top_groups), int(group_best)
     if not _route_is_fine(logits, k, scoring, bias, groups, top_groups, group_best, scale):
         _check_route(logits, k, scoring, bias, groups, top_groups, group_best, scale)
-    rows, experts = logits.shape
-    if bias is not None:
-        bias = bias.detach().float().contiguous()
-    logits = _whole_rows(logits)
-    d = L.RouteDesc(rows, logits.stride(0), experts, k, groups, top_groups, group_best, scoring == "sigmoid",
-                    bool(renormalize), _DTYPES[logits.dtype], scale, 0)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return Routing(experts, *_Route.apply(logits, bias, d))
-    return Routing(experts, *_route_forward(logits, bias, d))
-
-
-def _dispatch(x, places):
-    dev = x.device
-    rows, k = places.shape
-    with L.on_device(dev):
-        out = torch.empty((rows * k, x.size(1)), dtype=x.dtype, device=dev)
-        d = L.ExchangeDesc(rows, x.stride(0), k, x.size(1), _DTYPES[x.dtype], 0)
-        status = L.lib().dg_exchange_dispatch(d, x.data_ptr(), places.data_ptr(), out.data_ptr(), L.raw_stream(dev))
-        if status:
-            L.check(status, "dispatch_rows")
-    return out
-
-
-def _combine(y, places, weights, residual, name):
-    dev = y.device
-    rows, k = places.shape
-    with L.on_device(dev):
-        out = torch.empty((rows, y.size(1)), dtype=y.dtype, device=dev)
-        d = L.ExchangeDesc(rows, 0 if residual is None else residual.stride(0), k, y.size(1), _DTYPES[y.dtype], 0)
-        status = L.lib().dg_exchange_combine(d, y.data_ptr(), places.data_ptr(), L.addr(weights), L.addr(residual),
-                                             out.data_ptr(), L.raw_stream(dev))
-        if status:
-            L.check(status, name)
-    return out
-
-
-class _Dispatch(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, places):
-        ctx.save_for_backward(places)
-        return _dispatch(x, places)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        return _combine(grad.contiguous(), ctx.saved_tensors[0], None, None, "dispatch_rows"), None
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, weights, residual, places):
-        ctx.save_for_backward(y, weights, places)
-        return _combine(y, places, weights, residual, "combine_rows")
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        y, weights, places = ctx.saved_tensors
-        need_y, need_w, need_r, _ = ctx.needs_input_grad
-        dev, rows_of = y.device, _whole_rows(grad)
-        rows, k = places.shape
-        with L.on_device(dev):
-            dy = torch.empty_like(y) if need_y else None
-            dw = torch.empty_like(weights) if need_w else None
-            d = L.ExchangeDesc(rows, rows_of.stride(0), k, y.size(1), _DTYPES[y.dtype], 0)
-            status = L.lib().dg_exchange_combine_backward(d, y.data_ptr(), places.data_ptr(), weights.data_ptr(),
-                                                          rows_of.data_ptr(), L.addr(dy), L.addr(dw), L.raw_stream(dev))
-            if status:
-                L.check(status, "combine_rows")
-        return dy, dw, grad if need_r else None, None
+    return Routing(logits.size(1), *L.torch_layer().route(logits, bias, k, scoring == "sigmoid", groups, top_groups, group_best,
+                                                          bool(renormalize), scale))
 
 
 def _check_rows(name, t, routing, rows):
@@ -407,10 +226,7 @@ def dispatch_rows(x, routing):
         _refuse_tangents("dispatch_rows", x)
     _check(isinstance(routing, Routing), "routing must be a Routing")
     _check_rows("x", x, routing, routing.rows)
-    x = _whole_rows(x)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Dispatch.apply(x, routing.places)
-    return _dispatch(x, routing.places)
+    return L.torch_layer().dispatch(x, routing.places)
 
 
 def combine_rows(y, routing, residual=None):
@@ -430,11 +246,7 @@ def combine_rows(y, routing, residual=None):
         if residual.dtype != y.dtype or residual.size(1) != y.size(1):
             raise RuntimeError(f"residual must be {y.dtype} [{routing.rows}, {y.size(1)}], "
                                f"got {residual.dtype} {_shape(residual)}")
-        residual = _whole_rows(residual)
-    y, weights = y.contiguous(), routing.weights.contiguous()
+    weights = routing.weights
     if weights.dtype != torch.float32 or weights.shape != routing.places.shape:
         raise RuntimeError(f"routing.weights must be float32 {_shape(routing.places)}, got {weights.dtype} {_shape(weights)}")
-    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad
-                                    or residual is not None and residual.requires_grad):
-        return _Combine.apply(y, weights, residual, routing.places)
-    return _combine(y, routing.places, weights, residual, "combine_rows")
+    return L.torch_layer().combine(y, weights, residual, routing.places)

@@ -368,20 +368,12 @@ def _grouped_desc(x, weight):
     return L.GroupedDesc(x.size(0), weight.size(0), weight.size(2), weight.size(1), _DTYPES[x.dtype], 0)
 
 
-_ACTIVATIONS = {None: L.DG_ACT_NONE, "silu": L.DG_ACT_SILU, "gelu": L.DG_ACT_GELU}
-
-
-def _grouped_forward(x, weight, sizes, bias, act=L.DG_ACT_NONE, residual=None):
-    dev, lib = x.device, L.lib()
+def _grouped_forward(x, weight, sizes, bias):
+    dev = x.device
     with L.on_device(dev):
         y = torch.empty((x.size(0), weight.size(1)), dtype=x.dtype, device=dev)
-        d = _grouped_desc(x, weight)
-        if act == L.DG_ACT_NONE and residual is None:
-            status = lib.dg_grouped_forward(d, x.data_ptr(), weight.data_ptr(), sizes.data_ptr(), L.addr(bias), y.data_ptr(),
-                                            L.raw_stream(dev))
-        else:
-            status = lib.dg_grouped_apply(d, act, x.data_ptr(), weight.data_ptr(), sizes.data_ptr(), L.addr(bias),
-                                          L.addr(residual), y.data_ptr(), L.raw_stream(dev))
+        status = L.lib().dg_grouped_forward(_grouped_desc(x, weight), x.data_ptr(), weight.data_ptr(), sizes.data_ptr(),
+                                            L.addr(bias), y.data_ptr(), L.raw_stream(dev))
         if status:
             L.check(status, "grouped_linear")
     return y
@@ -389,30 +381,19 @@ def _grouped_forward(x, weight, sizes, bias, act=L.DG_ACT_NONE, residual=None):
 
 class _Grouped(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, sizes, bias, act=L.DG_ACT_NONE, residual=None):
-        # (with an activation the backward pass makes z again: fewer bytes than keeping it)
-        ctx.save_for_backward(x, weight, sizes, bias if act != L.DG_ACT_NONE else None)
-        ctx.desc, ctx.act = _grouped_desc(x, weight), act
-        return _grouped_forward(x, weight, sizes, bias, act, residual)
+    def forward(ctx, x, weight, sizes, bias):
+        ctx.save_for_backward(x, weight, sizes)
+        ctx.desc = _grouped_desc(x, weight)
+        return _grouped_forward(x, weight, sizes, bias)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, sizes, bias = ctx.saved_tensors
-        need_x, need_w, _, need_b, _, need_r = ctx.needs_input_grad
-        dresidual = grad if need_r else None
-        if not (need_x or need_w or need_b):
-            return None, None, None, None, None, dresidual
+        x, weight, sizes = ctx.saved_tensors
+        need_x, need_w, _, need_b = ctx.needs_input_grad
         lib, dev, grad = L.lib(), x.device, grad.contiguous()
         d = ctx.desc
         with L.on_device(dev):
-            if ctx.act != L.DG_ACT_NONE:
-                dz = torch.empty_like(grad)
-                status = lib.dg_grouped_apply_backward(d, ctx.act, x.data_ptr(), weight.data_ptr(), sizes.data_ptr(),
-                                                       L.addr(bias), grad.data_ptr(), dz.data_ptr(), L.raw_stream(dev))
-                if status:
-                    L.check(status, "grouped_linear")
-                grad = dz
             dx = torch.empty_like(x) if need_x else None
             dw = torch.empty_like(weight) if need_w or need_b else None
             db = torch.empty(weight.shape[:2], dtype=x.dtype, device=dev) if need_b else None
@@ -423,7 +404,10 @@ class _Grouped(torch.autograd.Function):
                                              addr(dx), addr(dw), addr(db), addr(ws), wsb, L.raw_stream(dev))
             if status:
                 L.check(status, "grouped_linear")
-        return dx, dw if need_w else None, None, db, None, dresidual
+        return dx, dw if need_w else None, None, db
+
+
+_ACTIVATIONS = {None: L.DG_ACT_NONE, "silu": L.DG_ACT_SILU, "gelu": L.DG_ACT_GELU}
 
 
 def _check_grouped(x, weight, sizes, bias, residual):
@@ -503,12 +487,11 @@ def grouped_linear(x, weight, sizes, bias=None, activation=None, residual=None):
     if not _grouped_is_fine(x, weight, sizes, bias, residual):
         _check_grouped(x, weight, sizes, bias, residual)
         sizes = sizes.to(x.device)
+    if act != L.DG_ACT_NONE or residual is not None:
+        return L.torch_layer().grouped_apply(x, weight, sizes, bias, act, residual)
     x, weight, sizes = x.contiguous(), weight.contiguous(), sizes.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    if residual is not None:
-        residual = residual.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad
-                                    or residual is not None and residual.requires_grad):
-        return _Grouped.apply(x, weight, sizes, bias, act, residual)
-    return _grouped_forward(x, weight, sizes, bias, act, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias is not None and bias.requires_grad):
+        return _Grouped.apply(x, weight, sizes, bias)
+    return _grouped_forward(x, weight, sizes, bias)

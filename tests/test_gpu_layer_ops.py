@@ -228,3 +228,48 @@ def test_operators_run_at_once_on_two_streams(cuda):
             torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+
+
+def test_gradients_are_taken_once(cuda):
+    """A graph of the gradients may be asked for; differentiating them raises, instead of calling them constants."""
+    g = torch.Generator("cuda").manual_seed(4)
+    new = lambda *s: torch.randn(*s, device="cuda", generator=g).requires_grad_(True)  # noqa: E731
+    q, k, at, logits, x, w = new(9, 2, 16), new(9, 2, 16), new(9, 2), new(9, 4), new(9, 8), new(1, 8, 8)
+    r = ds.route_rows(logits, 2)
+    calls = {"rotate_heads": (ds.rotate_heads(q, k, at, torch.ones(4, device="cuda"))[0], q),
+             "route_rows": (r.weights, logits), "dispatch_rows": (ds.dispatch_rows(x, r), x),
+             "combine_rows": (ds.combine_rows(ds.dispatch_rows(x.detach(), r).requires_grad_(True), r, x), x),
+             "grouped_linear": (ds.grouped_linear(x, w, [9], None, "silu", x), w)}
+    for name, (out, leaf) in calls.items():
+        want, = torch.autograd.grad(out, leaf, torch.ones_like(out), retain_graph=True)
+        again, = torch.autograd.grad(out, leaf, torch.ones_like(out), create_graph=True)
+        assert torch.equal(want, again), name
+        with pytest.raises(RuntimeError, match=f"twice {name}"):
+            again.square().sum().backward()
+
+
+def test_hooks_and_anomalies(cuda):
+    """Saved tensors that a hook moves to the host and back, and the mode that looks for NaN: the same gradients."""
+    g = torch.Generator("cuda").manual_seed(5)
+    new = lambda *s: torch.randn(*s, device="cuda", generator=g).requires_grad_(True)  # noqa: E731
+    logits, x, w = new(40, 6), new(40, 16), new(6, 16, 16)
+
+    def step():
+        r = ds.route_rows(logits, 2)
+        y = ds.combine_rows(ds.grouped_linear(ds.dispatch_rows(x, r), w, r.sizes, activation="gelu"), r, x)
+        return torch.autograd.grad(y, [logits, x, w], torch.ones_like(y))
+
+    want = step()
+    with torch.autograd.graph.save_on_cpu():
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    with torch.autograd.detect_anomaly(check_nan=True):
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+def test_an_input_changed_in_place_is_noticed(cuda):
+    x = torch.randn(10, 8, device="cuda")
+    w = torch.randn(1, 8, 8, device="cuda", requires_grad=True)
+    y = ds.grouped_linear(x, w, [10], None, "silu")
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
