@@ -57,10 +57,10 @@ struct Args {
     int64_t targets, nodes, ldq, ldk, ldgq, ldgk;
     int heads, kv, dim, pairs, axes, pos_dtype;
     int norm, w_own;  // w_own: the weights are of the heads' type (else float)
-    float eps;
+    float eps, inv_dim;
     int per, at_once;  // lanes of a head; heads at once (powers of two, their product up to 64)
     int count, batch;  // atoms of a wave's step; atoms whose angles it makes at once, a multiple of those
-    int steps;         // of an atom's heads
+    int q_steps, steps;  // of an atom's heads of q, and of all
     int ends[kMaxAxes];  // pairs up to and with an axis
 };
 
@@ -241,24 +241,37 @@ __device__ __forceinline__ float inverse_rms(const Args& a, const float (&x)[kC<
 {
     float ss = 0;
     for (int i = 0; i < kC<T>; ++i) ss = fmaf(x[i], x[i], ss);
-    return 1.0f / sqrtf(sum_lanes(ss, a.per) / (float)a.dim + a.eps);
+    return __builtin_amdgcn_rsqf(fmaf(sum_lanes(ss, a.per), a.inv_dim, a.eps));
 }
 
-// A lane's part in a step: `at_once` heads of q, or of k after those, of `count` of the batch's atoms.
+// Where a wave is: a step of an atom's heads, of the `sub`-th `count` atoms of its batch at `first`.
+struct Cursor {
+    int64_t first;
+    int sub, step;
+    __device__ __forceinline__ void next(const Args& a, int64_t stride)
+    {
+        if (++step < a.steps) return;
+        step = 0;
+        sub += a.count;
+        if (sub < a.batch) return;
+        sub = 0;
+        first += stride;
+    }
+};
+
+// A lane's part in a step: `at_once` heads of q, or of k after those.
 struct Part {
     int64_t node;
     int head;
     bool is_q, live;
 };
 template <typename T, bool HALVES>
-__device__ __forceinline__ Part part_of(const Args& a, const Seat<T, HALVES>& at, int64_t first, int step)
+__device__ __forceinline__ Part part_of(const Args& a, const Seat<T, HALVES>& at, const Cursor& c)
 {
-    const int sub = step / a.steps, q_steps = (a.heads + a.at_once - 1) / a.at_once;
-    step -= sub * a.steps;
     Part p;
-    p.is_q = step < q_steps;
-    p.head = (p.is_q ? step : step - q_steps) * a.at_once + at.slot;
-    p.node = first + sub * a.count + at.t;
+    p.is_q = c.step < a.q_steps;
+    p.head = (p.is_q ? c.step : c.step - a.q_steps) * a.at_once + at.slot;
+    p.node = c.first + c.sub + at.t;
     p.live = at.c0 < a.dim && p.node < (p.is_q ? a.targets : a.nodes) && p.head < (p.is_q ? a.heads : a.kv);
     return p;
 }
@@ -269,7 +282,7 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(Args a)
     __shared__ Shared<T> shared[kWaves];
     __shared__ __attribute__((aligned(16))) float s_w[2 * 256];
     constexpr int C = kC<T>;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Shared<T>& s = shared[w];
     load_weights<T>(a, s_w);
     const Seat<T, HALVES> at(a, lane);
@@ -281,24 +294,26 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(Args a)
         if (p.live) r = *(const u32x4*)((const T*)(p.is_q ? a.q : a.k) + p.node * (p.is_q ? a.ldq : a.ldk) + p.head * a.dim + at.c0);
         return r;
     };
-    const int steps = a.steps * (a.batch / a.count);
-    Part next = part_of(a, at, first, 0);
+    Cursor cursor{first, 0, 0};
+    Part next = part_of(a, at, cursor);
     u32x4 next_x = load(next);
     Angles angles = make_angles(a, lane, first);
     for (; first < a.nodes; first += stride) {
         make_turns(a, angles, first, first + stride, lane, s);
-        for (int step = 0; step < steps; ++step) {
+        while (cursor.first == first) {
+            const float2* turns = s.turn + (cursor.sub + at.t) * a.pairs;
             const Part p = next;
             float x[C], y[C], unused[C];
             unpack<T>(next_x, x);
-            next = step + 1 < steps ? part_of(a, at, first, step + 1) : part_of(a, at, first + stride, 0);
+            cursor.next(a, stride);
+            next = part_of(a, at, cursor);
             next_x = load(next);
             if (a.norm) {
                 const float r = inverse_rms<T>(a, x);
                 const float* wt = s_w + (p.is_q ? 0 : a.dim) + (at.c0 < a.dim ? at.c0 : 0);
                 for (int i = 0; i < C; ++i) x[i] = x[i] * r * wt[i];
             }
-            turn<T, HALVES, false>(a, at, s.turn + (step / a.steps * a.count + at.t) * a.pairs, s, x, y, unused);
+            turn<T, HALVES, false>(a, at, turns, s, x, y, unused);
             if (p.live)
                 *(u32x4*)((T*)(p.is_q ? a.oq : a.ok) + (p.node * (p.is_q ? a.heads : a.kv) + p.head) * a.dim + at.c0) = pack<T>(y);
         }
@@ -313,7 +328,7 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
     __shared__ __attribute__((aligned(16))) float s_w[2 * 256];
     __shared__ float s_sum[64 * kWaves * kC<T>];
     constexpr int C = kC<T>;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Shared<T>& s = shared[w];
     load_weights<T>(a, s_w);
     const Seat<T, HALVES> at(a, lane);
@@ -335,22 +350,25 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
     };
     uint32_t axes = 0;
     for (int i = 0; i < C; ++i) axes |= (uint32_t)(at.c0 + i < 2 * a.pairs ? axis_of(a, pair_of(i)) : 15) << 4 * i;
-    const int steps = a.steps * (a.batch / a.count);
     float sum_q[C] = {}, sum_k[C] = {}, dtheta[C] = {};
-    Part next = part_of(a, at, first, 0);
+    Cursor cursor{first, 0, 0};
+    Part next = part_of(a, at, cursor);
     u32x4 next_x, next_g;
     load(next, next_x, next_g);
     Angles angles = make_angles(a, lane, first);
     for (; first < a.nodes; first += stride) {
         make_turns(a, angles, first, first + stride, lane, s);
-        for (int step = 0; step < steps; ++step) {
+        while (cursor.first == first) {
+            const float2* turns = s.turn + (cursor.sub + at.t) * a.pairs;
+            const bool last = cursor.step + 1 == a.steps;  // of the atoms' heads
             const Part p = next;
             float x[C], g[C], back[C], across[C];
             unpack<T>(next_x, x);
             unpack<T>(next_g, g);
-            next = step + 1 < steps ? part_of(a, at, first, step + 1) : part_of(a, at, first + stride, 0);
+            cursor.next(a, stride);
+            next = part_of(a, at, cursor);
             load(next, next_x, next_g);
-            turn<T, HALVES, true>(a, at, s.turn + (step / a.steps * a.count + at.t) * a.pairs, s, g, back, across);
+            turn<T, HALVES, true>(a, at, turns, s, g, back, across);
             // (a lane without a head adds nothing: an angle or a scale that is not finite would make a NaN of its zeros)
             const float* wt = s_w + (p.is_q ? 0 : a.dim) + (at.c0 < a.dim ? at.c0 : 0);
             float r = 1.0f;
@@ -372,12 +390,12 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
                     back[i] *= wt[i];
                     dot = fmaf(back[i], x[i], dot);
                 }
-                dot = sum_lanes(dot, a.per) / (float)a.dim;
+                dot = sum_lanes(dot, a.per) * a.inv_dim;
                 for (int i = 0; i < C; ++i) back[i] = r * (back[i] - x[i] * dot);
             }
             if (p.live)
                 *(u32x4*)((T*)(p.is_q ? a.oq : a.ok) + (p.node * (p.is_q ? a.heads : a.kv) + p.head) * a.dim + at.c0) = pack<T>(back);
-            if (a.dpos && (step + 1) % a.steps == 0) {  // the atoms' last heads
+            if (a.dpos && last) {
                 for (int i = 0; i < C; ++i) dtheta[i] *= a.freq[pair_of(i)];
                 for (int axis = 0; axis < a.axes; ++axis) {
                     float sum = 0;
@@ -486,6 +504,7 @@ Args make_args(const dg_rotate_desc* d)
     a.heads = d->heads;
     a.kv = d->kv_heads;
     a.dim = d->dim;
+    a.inv_dim = 1.0f / (float)d->dim;
     a.axes = d->axes;
     a.pos_dtype = d->pos_dtype;
     a.norm = d->norm != 0;
@@ -502,7 +521,8 @@ Args make_args(const dg_rotate_desc* d)
     a.batch = a.count * std::max(1, 64 / (a.count * a.pairs));
     // (few atoms: rather a wave for each step's)
     while (a.batch > a.count && a.nodes < (int64_t)a.batch * kWaves * kMaxBlocks) a.batch -= a.count;
-    a.steps = (d->heads + a.at_once - 1) / a.at_once + (d->kv_heads + a.at_once - 1) / a.at_once;
+    a.q_steps = (d->heads + a.at_once - 1) / a.at_once;
+    a.steps = a.q_steps + (d->kv_heads + a.at_once - 1) / a.at_once;
     return a;
 }
 
