@@ -40,10 +40,12 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 
 constexpr int kWaves = 4;
 constexpr int kMaxAxes = 8;
-// Workgroups, as many as are resident at once: each takes as many atoms as the others, so a second round would
-// leave most of the card idle (1M atoms: 404 us with 1536, 451 with 2048).
+// Workgroups, as many as are resident at once by their registers: each takes as many atoms as the others, so a
+// second round would leave most of the card idle (1M atoms forward: 404 us with 1536, 451 with 2048; backward of
+// 32,000 in bfloat16, three waves a SIMD: 73 us with 768, 89 with 1024).
 constexpr int kForwardBlocks = 1536;
 constexpr int kMaxBlocks = 1024;
+inline int backward_blocks(int32_t dtype) { return dtype == DG_BF16 ? 768 : kMaxBlocks; }
 
 template <typename T>
 constexpr int kC = 16 / (int)sizeof(T);  // channels of a lane
@@ -558,7 +560,7 @@ void run_forward(const Args& a, bool interleaved, hipStream_t s)
 template <typename T>
 void run_backward(const Args& a, bool interleaved, void* dqw, void* dkw, hipStream_t s)
 {
-    const int64_t blocks = a.nodes ? blocks_of(a, kMaxBlocks) : 0;
+    const int64_t blocks = a.nodes ? blocks_of(a, backward_blocks(sizeof(T) == 2 ? DG_BF16 : DG_F32)) : 0;
     if (blocks) {
         const dim3 grid((unsigned)blocks);
         if (interleaved) hipLaunchKernelGGL((backward_kernel<T, false>), grid, dim3(64 * kWaves), 0, s, a);
@@ -602,7 +604,7 @@ size_t dg_rotate_workspace_size(const dg_rotate_desc* d)
 {
     if (check(d) != DG_OK) return 0;
     const Args a = make_args(d);
-    return (size_t)blocks_of(a, kMaxBlocks) * 2 * a.dim * sizeof(float);
+    return (size_t)blocks_of(a, backward_blocks(d->dtype)) * 2 * a.dim * sizeof(float);
 }
 
 dg_status dg_rotate_backward(const dg_rotate_desc* d, const void* q, const void* k, const void* positions,
