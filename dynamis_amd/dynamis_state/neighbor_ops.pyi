@@ -27,4 +27,5 @@ def neighbor_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: 
                        bias_table: torch.Tensor | None = None, scale: float | None = None, *,
                        return_lse: typing.Literal[True]) -> tuple[torch.Tensor, torch.Tensor]: ...
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, sizes: torch.Tensor | typing.Sequence[int],
-                   bias: torch.Tensor | None = None) -> torch.Tensor: ...
+                   bias: torch.Tensor | None = None, activation: typing.Literal["silu", "gelu"] | None = None,
+                   residual: torch.Tensor | None = None) -> torch.Tensor: ...
