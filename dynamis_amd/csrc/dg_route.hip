@@ -145,8 +145,8 @@ __device__ __forceinline__ void choose(const Args& a, K (&key)[V], int lane, int
 
 // Keys whose low bits may go hold their place among the lane's in them (the first the largest), in falling order:
 // then a round looks at each lane's first alone, and the winner's others move up.  The low bits may go where they say
-// nothing (a bfloat16's), or no more than `apart` allows for.  8 experts a lane, 6 rounds: a third of the
-// instructions of rounds that look through all (300,007 rows over 64 experts: 70 us then).
+// nothing (a bfloat16's), or no more than `apart` allows for.  (300,007 rows over 64 experts, 8 a lane, 6 rounds: 64
+// us, 70 where each round looks through all.)
 template <int V>
 __device__ __forceinline__ void sort_packed(uint32_t (&key)[V])
 {
@@ -279,13 +279,66 @@ __device__ __forceinline__ uint64_t worthiest(const Args& a, const K (&worth)[V]
     wave_sync();
     return __ballot(l < a.groups && mine && rank < a.top_groups) >> (lane & ~(a.lanes - 1));
 }
-template <int V, typename K>
-__device__ __forceinline__ void keep(const Args& a, uint64_t groups, int e0, K (&key)[V])
+// The same by sums in 32 bits; near: whether the lane's group and another lie nearer than `apart`.
+template <int V>
+__device__ __forceinline__ uint64_t worthiest(const Args& a, const float (&v)[V], int lane, int e0, float* s_value, float* s_worth,
+                                              float apart, bool& near)
 {
-    const int per = a.n / a.groups;
+    const int l = lane & (a.lanes - 1), per = a.n / a.groups;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        if (!(e0 + i < a.n && (groups >> ((e0 + i) / per) & 1))) key[i] = 0;
+        if (e0 + i < a.n) s_value[e0 + i] = v[i];
+    wave_sync();
+    float worth = -INFINITY;
+    if (l < a.groups) {
+        float best = -INFINITY, second = -INFINITY;
+        for (int i = l * per; i < (l + 1) * per; ++i) {
+            const float x = s_value[i];
+            second = __builtin_amdgcn_fmed3f(best, second, x);
+            best = fmaxf(best, x);
+        }
+        worth = a.group_best == 2 && second > -INFINITY ? best + second : best;
+        s_worth[l] = worth;
+    }
+    wave_sync();
+    int rank = 0, around = 0;
+    if (l < a.groups)
+        for (int g = 0; g < a.groups; ++g) {
+            const float x = s_worth[g];
+            rank += x > worth;
+            around += fabsf(x - worth) <= apart;  // (its own among them)
+        }
+    wave_sync();
+    near = around > 1;
+    return __ballot(l < a.groups && rank < a.top_groups) >> (lane & ~(a.lanes - 1));
+}
+
+// The groups of a lane's experts, a byte each.
+template <int V>
+struct Groups {
+    uint32_t of[(V + 3) / 4] = {};
+    __device__ __forceinline__ Groups(const Args& a, int e0)
+    {
+        const int per = a.n / a.groups;
+        if (a.groups > 1)
+            for (int i = 0; i < V; ++i) of[i / 4] |= (uint32_t)(min(e0 + i, a.n - 1) / per) << 8 * (i % 4);
+    }
+    template <typename K>
+    __device__ __forceinline__ void keep(uint64_t groups, K (&key)[V]) const
+    {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (!(groups >> (of[i / 4] >> 8 * (i % 4) & 255) & 1)) key[i] = 0;
+    }
+};
+
+// exp, from that of 2: its argument's rounding is |x| 2^-24 of it.  The sigmoid from exp(-|x|), which overflows
+// nowhere (where it is 0, at -103 and below, so is the sigmoid in 32 bits).
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(1.44269504f * x); }
+__device__ __forceinline__ float sigmoid(float x)
+{
+    const float e = exp_of(-fabsf(x)), r = __builtin_amdgcn_rcpf(1.0f + e);
+    return x < 0.0f ? e * r : r;
 }
 
 // s of a row's logits, in 32 bits or 64.
@@ -298,9 +351,7 @@ __device__ __forceinline__ void scores(const Args& a, const float (&x)[V], float
         if constexpr (sizeof(F) == 8) {
             s[i] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[i])) : exp((double)x[i] - (double)top);
         } else {
-            const float e = __builtin_amdgcn_exp2f(1.44269504f * (a.sigmoid ? -fabsf(x[i]) : x[i] - top));
-            const float r = __builtin_amdgcn_rcpf(1.0f + e);
-            s[i] = !a.sigmoid ? e : x[i] < 0.0f ? e * r : r;
+            s[i] = a.sigmoid ? sigmoid(x[i]) : exp_of(x[i] - top);
         }
         sum += s[i];
     }
@@ -314,12 +365,13 @@ __device__ __forceinline__ void scores(const Args& a, const float (&x)[V], float
 // kLogits: the logits are what is chosen by.  kScores: a bias, or groups worth a sum of scores.  What is chosen by
 // is then worked out in 32 bits; a row where two values that a choice or a group hangs on lie nearer than the
 // rounding, or are no numbers, is left to a second launch, kWide, which takes it in 64 (one of some hundred to
-// thousand).  In one launch the wide part's registers leave the other three waves a SIMD instead of
-// seven: 300,007 rows over 64 experts 104 us, these two 63.
+// thousand).  300,007 rows over 64 experts in groups, chosen with a bias: 57 and 18 us; in one launch, where the wide
+// part's registers leave the other three waves a SIMD, 92.  What bounds kScores is instructions, some thousand for a
+// wave's eight rows; five waves a SIMD are worth the registers that spill (57 us, four 72).
 enum { kLogits, kScores, kWide };
 
 template <typename T, int V, int HOW>
-__global__ __launch_bounds__(kThreads) void route_kernel(Args a)
+__global__ __launch_bounds__(kThreads, HOW == kScores && V <= 8 ? 5 : 1) void route_kernel(Args a)
 {
     constexpr bool SCORED = HOW != kLogits;
     using K = typename std::conditional<HOW == kWide, uint64_t, uint32_t>::type;
@@ -352,6 +404,21 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
     float bias[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) bias[i] = SCORED && a.bias && e0 + i < a.n ? a.bias[e0 + i] : 0.0f;
+    const Groups<V> groups(a, e0);
+    uint32_t never = 0;  // the lane's experts that no row takes
+    float most = 0.0f;   // of the biases
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const bool none = e0 + i >= a.n || bias[i] == -INFINITY;
+        never |= (uint32_t)none << i;
+        most = none ? most : fmaxf(most, fabsf(bias[i]));
+    }
+    over_lanes(a.lanes, [&](auto&& other) { most = fmaxf(most, as_float(other(as_bits(most)))); });
+    most += 1.0f;  // of a value
+    // How near two values may lie before 32 bits do not tell them apart: a sigmoid is within 6 2^-24, a softmax, whose
+    // sum has n terms, within 32 2^-24, their sum with the bias within another 2^-24 of itself; two values,
+    // each of them a sum of two; and the packed places.
+    const float apart = (a.sigmoid ? 2e-6f : 8e-6f) * (1.0f + most) + 2.4e-7f * V * most;
     for (int base = 0; base < rows; base += at_once) {
         const int at = base + in_block;
         bool live = at < rows;
@@ -370,35 +437,38 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
         if (!a.sigmoid && !a.renormalize) {
             float sum = 0;
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum += expf(x[i] - top);
+            for (int i = 0; i < V; ++i) sum += exp_of(x[i] - top);
             total = sum_lanes(sum, a.lanes);
         }
+        // (a row's keys: of its logits, where those are chosen by)
         uint32_t plain[V];
+        auto gone = [&](int i) { return x[i] == -INFINITY || (never >> i & 1); };
+        if (HOW != kScores || !a.bias) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) plain[i] = x[i] == -INFINITY || bias[i] == -INFINITY || e0 + i >= a.n ? 0 : key_of(x[i]);
+            for (int i = 0; i < V; ++i) plain[i] = gone(i) ? 0 : key_of(x[i]);
+        }
         bool poisoned = false;  // a softmax with a NaN or an infinity: every weight is one, whichever are chosen
         if constexpr (HOW == kScores) {
-            bool close = false;
-            float v[V], most = 0.0f;
+            float v[V], all = 0.0f;
             uint32_t key[V];
             scores<V>(a, x, top, v);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                v[i] = plain[i] ? v[i] + bias[i] : -INFINITY;
-                close = close || v[i] != v[i];
-                most = plain[i] ? fmaxf(most, fabsf(v[i])) : most;
-                key[i] = !a.bias || !plain[i] ? plain[i] : key_of(v[i]);
+                v[i] = gone(i) ? -INFINITY : v[i] + bias[i];
+                all += v[i];
+                key[i] = a.bias ? (gone(i) ? 0 : key_of(v[i])) : plain[i];
             }
-            over_lanes(a.lanes, [&](auto&& other) { most = fmaxf(most, as_float(other(as_bits(most)))); });
-            // (A sigmoid is within 6 2^-24, a softmax, whose sum has n terms, within 32 2^-24, and its sum with
-            // the bias within another 2^-24 of itself; two values, each of them a sum of two.)
-            const float apart = (a.sigmoid ? 2e-6f : 8e-6f) * (1.0f + most) + 2.4e-7f * V * most;  // (and the packed places)
+            bool close = all != all;  // (a NaN, or infinities of both signs)
             if (a.groups > 1) {
-                bool near = true;
-                const bool worthy = !a.group_lanes || mine_is_worthy<V>(a, v, lane, e0, (float*)s_worth, apart, near);
-                close = close || near;
+                bool near;
+                if (a.group_lanes) {
+                    const bool worthy = mine_is_worthy<V>(a, v, lane, e0, (float*)s_worth, apart, near);
 #pragma unroll
-                for (int i = 0; i < V; ++i) key[i] = worthy ? key[i] : 0;
+                    for (int i = 0; i < V; ++i) key[i] = worthy ? key[i] : 0;
+                } else {
+                    groups.keep(worthiest<V>(a, v, lane, e0, (float*)s_key, (float*)s_worth, apart, near), key);
+                }
+                close = close || near;
             }
             if (a.bias) {
                 sort_packed<V>(key);
@@ -426,10 +496,10 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
                 poisoned = poisoned || (!a.sigmoid && d[i] != d[i]);
             }
             poisoned = __ballot(poisoned) & of_row;
-            const uint64_t groups = a.groups > 1 ? worthiest<V>(a, key, lane, e0, s_key, s_worth) : ~0ull;
+            const uint64_t kept = a.groups > 1 ? worthiest<V>(a, key, lane, e0, s_key, s_worth) : ~0ull;
 #pragma unroll
             for (int i = 0; i < V; ++i) key[i] = a.bias ? key[i] : plain[i];
-            if (a.groups > 1) keep<V>(a, groups, e0, key);
+            if (a.groups > 1) groups.keep(kept, key);
             choose<V>(a, key, lane, e0, of_row, picks);
         } else {
             if (a.groups > 1 && a.group_lanes) {
@@ -437,7 +507,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
 #pragma unroll
                 for (int i = 0; i < V; ++i) plain[i] = worthy ? plain[i] : 0;
             } else if (a.groups > 1) {
-                keep<V>(a, worthiest<V>(a, plain, lane, e0, s_key, s_worth), e0, plain);
+                groups.keep(worthiest<V>(a, plain, lane, e0, s_key, s_worth), plain);
             }
             choose_logits<T, V>(a, plain, lane, e0, of_row, picks);
         }
@@ -456,11 +526,11 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a)
                 const float y = as_float(other(as_bits(m)));
                 m = y > m || y != y ? y : m;
             });
-            if (e >= 0) w = a.sigmoid && !(m < -30.0f) ? 1.0f / (1.0f + expf(-c)) : expf(c - m);
+            if (e >= 0) w = a.sigmoid && !(m < -30.0f) ? sigmoid(c) : exp_of(c - m);
             const float sum = sum_lanes(w, a.lanes);
-            if (e >= 0) w = w / sum;
+            if (e >= 0) w = w * __builtin_amdgcn_rcpf(sum);
         } else if (e >= 0) {
-            w = a.sigmoid ? 1.0f / (1.0f + expf(-c)) : expf(c - top) / total;
+            w = a.sigmoid ? sigmoid(c) : exp_of(c - top) * __builtin_amdgcn_rcpf(total);
         }
         if (mine) {
             a.experts[row * a.k + l] = e;
