@@ -16,6 +16,10 @@
 // The places are a stable counting sort in three launches: each workgroup's counts of its rows' choices, a
 // scan of them for each expert, and the ranks within a workgroup by matching lanes; nothing depends
 // on the order of atomics (counts alone are added up by them).
+//
+// Instructions bound it, not the bytes: 300,007 rows over 64 experts in 8 groups, 6 chosen with a bias, in float: 57 us
+// for the choices and 18 for the rows done again (98 MB: 19 us at a copy's rate), scan and places 5 and 12.  32,000
+// rows over 128 experts, 8 chosen, in bfloat16: 14, 3 and 5 us, backward 9.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
