@@ -124,6 +124,15 @@ variable_list once(variable_list grads, const char* what)
     return (*error)(std::move(in));
 }
 
+// A saved tensor as it comes back from a hook, which may have laid it out anew but is held to its shape, type and device.
+const Tensor& same(const Tensor& t, at::IntArrayRef sizes, int32_t type, at::Device device, const char* what)
+{
+    const bool typed = t.defined() && (type == DG_I32 ? t.scalar_type() == at::kInt : t.scalar_type() != at::kInt && type_of(t) == type);
+    if (!typed || t.sizes() != sizes || t.device() != device)
+        throw std::runtime_error(std::string(what) + ": a saved tensor came back with another shape, dtype or device");
+    return t;
+}
+
 std::string text(const void* d, size_t n) { return std::string((const char*)d, n); }
 
 // ---------------------------------------------------------------- rotate_heads
@@ -156,11 +165,23 @@ struct Rotate : torch::autograd::Function<Rotate> {
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const auto s = ctx->get_saved_variables();
-        const Tensor &q = s[0], &k = s[1], &positions = s[2], &frequencies = s[3], &q_weight = s[4], &k_weight = s[5];
-        c10::OptionalDeviceGuard guard(q.device());
-        Tensor gq = rows_16(grads[0]), gk = rows_16(grads[1]);
+        const at::Device dev = grads[0].device();
+        c10::OptionalDeviceGuard guard(dev);
         dg_rotate_desc d;
         memcpy(&d, ctx->saved_data["desc"].toStringRef().data(), sizeof d);
+        const char* const what = "rotate_heads";
+        int64_t pairs = 0;
+        for (int i = 0; i < d.axes; ++i) pairs += d.sections[i];
+        const Tensor q = rows_16(same(s[0], {d.n_targets, d.heads, d.dim}, d.dtype, dev, what));
+        const Tensor k = rows_16(same(s[1], {d.n_nodes, d.kv_heads, d.dim}, d.dtype, dev, what));
+        const Tensor positions = same(s[2], {d.n_nodes, d.axes}, d.pos_dtype, dev, what).contiguous();
+        const Tensor frequencies = same(s[3], {pairs}, DG_F32, dev, what).contiguous();
+        Tensor q_weight, k_weight;
+        if (s[4].defined()) q_weight = same(s[4], {d.dim}, d.weight_dtype, dev, what).contiguous();
+        if (s[5].defined()) k_weight = same(s[5], {d.dim}, d.weight_dtype, dev, what).contiguous();
+        const Tensor gq = rows_16(grads[0]), gk = rows_16(grads[1]);
+        d.ld_q = q.stride(0);
+        d.ld_k = k.stride(0);
         d.ld_gq = gq.stride(0);
         d.ld_gk = gk.stride(0);
         Tensor dq = plain(q), dk = plain(k), dpos, dqw, dkw, ws;
@@ -238,11 +259,15 @@ struct Route : torch::autograd::Function<Route> {
     {
         if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor()};
         const auto s = ctx->get_saved_variables();
-        c10::OptionalDeviceGuard guard(s[0].device());
+        const at::Device dev = grads[0].device();
+        c10::OptionalDeviceGuard guard(dev);
         dg_route_desc d;
         memcpy(&d, ctx->saved_data["desc"].toStringRef().data(), sizeof d);
-        Tensor g = grads[0].contiguous(), dlogits = plain(s[0]);
-        check(dg.route_backward(&d, s[0].data_ptr(), (const int32_t*)s[1].data_ptr(), (const float*)g.data_ptr(), dlogits.data_ptr(),
+        const Tensor logits = whole_rows(same(s[0], {d.n_rows, d.n_experts}, d.dtype, dev, "route_rows"));
+        const Tensor experts = same(s[1], {d.n_rows, d.k}, DG_I32, dev, "route_rows").contiguous();
+        d.ld = logits.stride(0);
+        Tensor g = grads[0].contiguous(), dlogits = plain(logits);
+        check(dg.route_backward(&d, logits.data_ptr(), (const int32_t*)experts.data_ptr(), (const float*)g.data_ptr(), dlogits.data_ptr(),
                                 stream_of(g)), "route_rows");
         return once({dlogits, Tensor(), Tensor()}, "route_rows");
     }
@@ -305,13 +330,17 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& places)
     {
         ctx->save_for_backward({places});
+        ctx->saved_data["rows"] = places.size(0);
         return dispatch_forward(x, places);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
-        c10::OptionalDeviceGuard guard(grads[0].device());
-        return once({combine_forward(grads[0].contiguous(), ctx->get_saved_variables()[0], Tensor(), Tensor(), "dispatch_rows"), Tensor()},
-                    "dispatch_rows");
+        const at::Device dev = grads[0].device();
+        c10::OptionalDeviceGuard guard(dev);
+        const auto s = ctx->get_saved_variables();
+        const int64_t rows = ctx->saved_data["rows"].toInt(), k = rows ? grads[0].size(0) / rows : s[0].size(1);
+        const Tensor places = same(s[0], {rows, k}, DG_I32, dev, "dispatch_rows").contiguous();
+        return once({combine_forward(grads[0].contiguous(), places, Tensor(), Tensor(), "dispatch_rows"), Tensor()}, "dispatch_rows");
     }
 };
 
@@ -328,13 +357,19 @@ struct Combine : torch::autograd::Function<Combine> {
     {
         ctx->save_for_backward({y, weights, places});
         ctx->saved_data["residual"] = residual.has_value();
+        ctx->saved_data["k"] = places.size(1);
         return combine_forward(y, places, weights, value(residual), "combine_rows");
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const auto s = ctx->get_saved_variables();
-        const Tensor &y = s[0], &weights = s[1], &places = s[2];
-        c10::OptionalDeviceGuard guard(y.device());
+        const at::Device dev = grads[0].device();
+        c10::OptionalDeviceGuard guard(dev);
+        const char* const what = "combine_rows";
+        const int64_t rows = grads[0].size(0), k = ctx->saved_data["k"].toInt();
+        const Tensor y = same(s[0], {rows * k, grads[0].size(1)}, type_of(grads[0]), dev, what).contiguous();
+        const Tensor weights = same(s[1], {rows, k}, DG_F32, dev, what).contiguous();
+        const Tensor places = same(s[2], {rows, k}, DG_I32, dev, what).contiguous();
         Tensor dy, dw, dr;
         if (ctx->needs_input_grad(0)) dy = plain(y);
         if (ctx->needs_input_grad(1)) dw = plain(weights);
@@ -388,26 +423,37 @@ struct Grouped : torch::autograd::Function<Grouped> {
         // (the backward pass makes z again: fewer bytes than keeping it)
         ctx->save_for_backward({x, weight, sizes, bias});
         ctx->saved_data["act"] = act;
+        ctx->saved_data["groups"] = weight.size(0);
+        ctx->saved_data["k"] = weight.size(2);
         ctx->saved_data["residual"] = residual.has_value();
         return grouped_forward(x, weight, sizes, bias, (int)act, value(residual));
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const auto s = ctx->get_saved_variables();
-        const Tensor &x = s[0], &weight = s[1], &sizes = s[2], &bias = s[3];
+        const at::Device dev = grads[0].device();
+        c10::OptionalDeviceGuard guard(dev);
+        const char* const what = "grouped_linear";
+        const int64_t rows = grads[0].size(0), n = grads[0].size(1);
+        const int64_t groups = ctx->saved_data["groups"].toInt(), depth = ctx->saved_data["k"].toInt();
+        const int32_t type = type_of(grads[0]);
+        const Tensor x = same(s[0], {rows, depth}, type, dev, what).contiguous();
+        const Tensor weight = same(s[1], {groups, n, depth}, type, dev, what).contiguous();
+        const Tensor sizes = same(s[2], {groups}, DG_I64, dev, what).contiguous();
+        Tensor bias;
+        if (s[3].defined()) bias = same(s[3], {groups, n}, type, dev, what).contiguous();
         const int act = (int)ctx->saved_data["act"].toInt();
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = bias.defined() && ctx->needs_input_grad(3);
         Tensor dx, dw, db, ws, dr;
         if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(bias.defined() ? 4 : 3)) dr = grads[0];
         if (need_x || need_w || need_b) {
-            c10::OptionalDeviceGuard guard(x.device());
             const auto d = grouped_of(x, weight);
-            const int64_t* n = (const int64_t*)sizes.data_ptr();
+            const int64_t* count = (const int64_t*)sizes.data_ptr();
             const hipStream_t stream = stream_of(x);
             Tensor g = grads[0].contiguous();
             if (act != DG_ACT_NONE) {
                 Tensor dz = plain(g);
-                check(dg.grouped_apply_backward(&d, act, x.data_ptr(), weight.data_ptr(), n, ptr(bias), g.data_ptr(), dz.data_ptr(), stream),
+                check(dg.grouped_apply_backward(&d, act, x.data_ptr(), weight.data_ptr(), count, ptr(bias), g.data_ptr(), dz.data_ptr(), stream),
                       "grouped_linear");
                 g = dz;
             }
@@ -418,7 +464,7 @@ struct Grouped : torch::autograd::Function<Grouped> {
                 ws = bytes(size = dg.grouped_workspace_size(&d), x);
             }
             if (need_b) db = plain(bias);
-            check(dg.grouped_backward(&d, x.data_ptr(), weight.data_ptr(), n, g.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(ws), size, stream),
+            check(dg.grouped_backward(&d, x.data_ptr(), weight.data_ptr(), count, g.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(ws), size, stream),
                   "grouped_linear");
         }
         return once({dx, need_w ? dw : Tensor(), Tensor(), db, Tensor(), dr}, "grouped_linear");

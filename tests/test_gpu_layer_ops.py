@@ -266,6 +266,52 @@ def test_hooks_and_anomalies(cuda):
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
 
 
+def test_hooks_that_lay_saved_tensors_out_anew(cuda):
+    """Rows that lie apart come back whole, whole ones apart or transposed: the same gradients."""
+    g = torch.Generator("cuda").manual_seed(6)
+    new = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    wide, scores, table = new(33, 400), new(33, 50), new(2, 33)
+    q = wide[:, :96].unflatten(1, (6, 16)).requires_grad_(True)
+    k = wide[:, 96:128].unflatten(1, (2, 16)).requires_grad_(True)
+    at, qw, kw = table.t().requires_grad_(True), new(16).requires_grad_(True), new(16).requires_grad_(True)
+    logits, x = scores[:, :6].requires_grad_(True), new(33, 32).requires_grad_(True)
+    w, b = new(6, 32, 32).requires_grad_(True), new(6, 32).requires_grad_(True)
+    freq = torch.linspace(0.1, 1.0, 6, device="cuda")
+    leaves = [q, k, at, qw, kw, logits, x, w, b]
+
+    def step():
+        a, c = ds.rotate_heads(q, k, at, freq, None, qw, kw)
+        r = ds.route_rows(logits, 2, renormalize=False)
+        y = ds.combine_rows(ds.grouped_linear(ds.dispatch_rows(x, r), w, r.sizes, b, activation="silu"), r, x)
+        out = [a, c, y]
+        return torch.autograd.grad(out, leaves, [torch.cos(torch.arange(t.numel(), device="cuda").float()).view_as(t) for t in out])
+
+    want = step()
+    turned = lambda t: t.movedim(0, -1).contiguous().movedim(-1, 0)  # noqa: E731
+    apart = lambda t: torch.stack([t, t], -1)[..., 0]  # noqa: E731
+    for back in (lambda t: t.contiguous(), lambda t: t.clone(memory_format=torch.contiguous_format), turned, apart):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+            assert all(torch.equal(m, n) for m, n in zip(step(), want))
+    with torch.autograd.graph.save_on_cpu():
+        assert all(torch.equal(m, n) for m, n in zip(step(), want))
+
+
+def test_hooks_that_change_saved_tensors_are_refused(cuda):
+    new = lambda *s: torch.randn(*s, device="cuda").requires_grad_(True)  # noqa: E731
+    logits, x, w = new(10, 4), new(10, 16), new(4, 16, 16)
+    r = ds.route_rows(logits, 2)
+    calls = {"rotate_heads": lambda: ds.rotate_heads(x.view(10, 1, 16), x.view(10, 1, 16), x[:, :2], torch.ones(8, device="cuda"))[0],
+             "route_rows": lambda: ds.route_rows(logits, 2).weights, "dispatch_rows": lambda: ds.dispatch_rows(x, r),
+             "combine_rows": lambda: ds.combine_rows(torch.cat([x, x]), r, x),
+             "grouped_linear": lambda: ds.grouped_linear(x, w, torch.tensor([1, 2, 3, 4], device="cuda"), None, "gelu")}
+    for change in (lambda t: t[:-1], lambda t: t.double(), lambda t: t.cpu()):
+        for name, call in calls.items():
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+                out = call()
+            with pytest.raises(RuntimeError, match=f"{name}: a saved tensor came back"):
+                torch.autograd.grad(out, [x, w, logits], torch.ones_like(out), allow_unused=True)
+
+
 def test_an_input_changed_in_place_is_noticed(cuda):
     x = torch.randn(10, 8, device="cuda")
     w = torch.randn(1, 8, 8, device="cuda", requires_grad=True)
