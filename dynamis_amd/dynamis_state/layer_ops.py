@@ -202,6 +202,16 @@ def route_rows(logits, k, scoring="softmax", bias=None, groups=1, top_groups=1, 
                                                           bool(renormalize), scale))
 
 
+def _check_routing(routing):
+    """Rows and choices of a routing, by the places that its users read: a Routing can be made or changed by anyone."""
+    _check(isinstance(routing, Routing), "routing must be a Routing")
+    places = routing.places
+    if not (type(places) in _TENSORS and places.is_cuda and places.dtype == torch.int32 and places.dim() == 2
+            and 1 <= places.size(1) <= 64):
+        raise RuntimeError("routing.places must be a CUDA tensor, int32 [rows, k]")
+    return places.shape
+
+
 def _check_rows(name, t, routing, rows):
     """The refusals of rows that go with a routing; their messages cost host time where one is due alone."""
     if type(t) in _TENSORS and t.dim() == 2 and t.size(0) == rows and t.dtype in _DTYPES \
@@ -224,8 +234,8 @@ def dispatch_rows(x, routing):
     """
     if forward_ad._current_level >= 0:
         _refuse_tangents("dispatch_rows", x)
-    _check(isinstance(routing, Routing), "routing must be a Routing")
-    _check_rows("x", x, routing, routing.rows)
+    rows, _ = _check_routing(routing)
+    _check_rows("x", x, routing, rows)
     return L.torch_layer().dispatch(x, routing.places)
 
 
@@ -237,16 +247,17 @@ def combine_rows(y, routing, residual=None):
     expert's rows.  Sums are 32 bits, in the choices' order, and rounded once.  Differentiable in y, the
     routing's weights (and so in the router's logits) and the residual, once, in reverse.
     """
-    _check(isinstance(routing, Routing), "routing must be a Routing")
+    rows, k = _check_routing(routing)
     if forward_ad._current_level >= 0:
         _refuse_tangents("combine_rows", y, routing.weights, residual)
-    _check_rows("y", y, routing, routing.rows * routing.k)
+    _check_rows("y", y, routing, rows * k)
     if residual is not None:
-        _check_rows("residual", residual, routing, routing.rows)
+        _check_rows("residual", residual, routing, rows)
         if residual.dtype != y.dtype or residual.size(1) != y.size(1):
-            raise RuntimeError(f"residual must be {y.dtype} [{routing.rows}, {y.size(1)}], "
+            raise RuntimeError(f"residual must be {y.dtype} [{rows}, {y.size(1)}], "
                                f"got {residual.dtype} {_shape(residual)}")
     weights = routing.weights
-    if weights.dtype != torch.float32 or weights.shape != routing.places.shape:
-        raise RuntimeError(f"routing.weights must be float32 {_shape(routing.places)}, got {weights.dtype} {_shape(weights)}")
+    if not (type(weights) in _TENSORS and weights.dtype == torch.float32 and weights.shape == routing.places.shape
+            and weights.device == y.device):
+        raise RuntimeError(f"routing.weights must be float32 {_shape(routing.places)} on {y.device}")
     return L.torch_layer().combine(y, weights, residual, routing.places)

@@ -196,6 +196,28 @@ def test_weights_of_another_make_are_refused(cuda):
     assert torch.equal(ds.combine_rows(y + 1, ds.Routing(4, turned, r.experts, r.sizes, r.places)), ds.combine_rows(y + 1, r))
 
 
+def test_a_changed_routing_is_refused(cuda):
+    """Weights elsewhere, places of another type, more or fewer rows than the operands have."""
+    r = ds.route_rows(torch.randn(10, 4, device="cuda"), 2)
+    x, y = torch.zeros(10, 8, device="cuda"), torch.zeros(20, 8, device="cuda")
+    for w in (r.weights.cpu(), None):
+        with pytest.raises(RuntimeError, match="routing.weights must be"):
+            ds.combine_rows(y, ds.Routing(4, w, r.experts, r.sizes, r.places))
+    for places in (r.places.long(), r.places.cpu(), r.places.float(), r.places.flatten()):
+        bad = ds.Routing(4, r.weights, r.experts, r.sizes, places)
+        with pytest.raises(RuntimeError, match="routing.places must be"):
+            ds.dispatch_rows(x, bad)
+        with pytest.raises(RuntimeError, match="routing.places must be"):
+            ds.combine_rows(y, bad)
+    for rows in (9, 11):
+        bad = ds.Routing(4, r.weights, r.experts, r.sizes, r.places)
+        bad.places = torch.zeros(rows, 2, dtype=torch.int32, device="cuda")
+        with pytest.raises(RuntimeError, match="x must have shape"):
+            ds.dispatch_rows(x, bad)
+        with pytest.raises(RuntimeError, match="y must have shape"):
+            ds.combine_rows(y, bad)
+
+
 def test_dispatched_bits_are_those_of_the_rows(cuda):
     """Every bit pattern of bfloat16, NaNs with their payloads, in whole chunks and one by one."""
     bits = torch.arange(-2 ** 15, 2 ** 15, device="cuda", dtype=torch.int32).to(torch.int16)

@@ -162,6 +162,17 @@ def test_python_calls_want_the_gpu():
         ds.grouped_linear(x, torch.zeros(1, 4, 8), [3], activation="tanh")
 
 
+def test_a_routing_of_another_make_is_refused():
+    """A Routing that was made, moved or changed by its user."""
+    x, e, n = torch.zeros(3, 8), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(4, dtype=torch.int64)
+    for places in (e, e.long(), e[0], None, torch.zeros(3, 65, dtype=torch.int32)):
+        r = ds.Routing(4, torch.zeros(3, 2), e, n, places)
+        with pytest.raises(RuntimeError, match="routing.places must be"):
+            ds.dispatch_rows(x, r)
+        with pytest.raises(RuntimeError, match="routing.places must be"):
+            ds.combine_rows(torch.zeros(6, 8), r)
+
+
 # ---------------------------------------------------------------- the definitions
 
 
