@@ -109,7 +109,8 @@ def rotate_heads(q, k, positions, frequencies, sections=None, q_weight=None, k_w
     the first sections[0] of them go with axis 0, the next sections[1] with axis 1 and so on (default:
     the same number for each axis).  Channels from 2 P on are not rotated.  q_weight and k_weight [dim],
     of the heads' type or float32 (default: ones).  Angles are worked out in 64 bits and squares summed in 32;
-    results are rounded once.  Returns (q, k) of the inputs' shapes and type, contiguous.
+    results are rounded once.  A mean square plus eps has to lie between 1e-38 and 3e38, or the head's result is
+    zeros or not finite.  Returns (q, k) of the inputs' shapes and type, contiguous.
 
     Differentiable in q, k, the weights and positions (in 32 bits, whatever their type), once, in reverse:
     a tensor with a forward-mode tangent is refused, and so are frequencies that require a gradient.  Sums have

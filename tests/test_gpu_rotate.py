@@ -290,3 +290,29 @@ def test_refusals(cuda):
     with forward_ad.dual_level():
         dual = forward_ad.make_dual(q, torch.ones_like(q))
         bad("forward-mode", dual, k, at, f)
+
+
+@LAYOUTS
+def test_offsets_past_32_bits(cuda, interleaved):
+    """Atoms whose heads lie past 2^31 elements, and past 2^32 where rows lie apart: the bits that the same atoms get by
+    themselves (a head's sums are its own lanes', however many atoms there are)."""
+    print("\n[case] far atoms", flush=True)
+    n, last, freq = (1 << 22) + 37, 50, torch.linspace(0.1, 1.0, 32, device="cuda")
+    g = torch.Generator("cuda").manual_seed(3)
+    piece = torch.randn(1 << 12, 8, 64, device="cuda", generator=g).bfloat16()
+    q = piece.repeat(n // (1 << 12) + 1, 1, 1)[:n].requires_grad_(True)
+    k, at, w = q.detach()[:, 3:4].clone(), torch.rand(n, 1, device="cuda", generator=g), torch.rand(64, device="cuda", generator=g)
+    assert q.numel() > 2 ** 31
+    y, z = ds.rotate_heads(q, k, at, freq, None, w, w, interleaved=interleaved)
+    few = q.detach()[-last:].clone().requires_grad_(True)
+    want, want_z = ds.rotate_heads(few, k[-last:], at[-last:], freq, None, w, w, interleaved=interleaved)
+    assert torch.equal(y[-last:], want) and torch.equal(z[-last:], want_z)
+    dq, = torch.autograd.grad(y, q, y.detach())
+    assert torch.equal(dq[-last:], torch.autograd.grad(want, few, want.detach())[0])
+    del q, y, z, dq
+    apart = torch.empty(1 << 12, (1 << 20) + 8, dtype=torch.bfloat16, device="cuda")[:, :512].unflatten(1, (8, 64))
+    apart.copy_(piece)
+    at = at[:1 << 12]
+    got, got_k = ds.rotate_heads(apart, apart[:, 2:4], at, freq, interleaved=interleaved)
+    want, want_k = ds.rotate_heads(piece, piece[:, 2:4], at, freq, interleaved=interleaved)
+    assert torch.equal(got, want) and torch.equal(got_k, want_k)

@@ -456,3 +456,20 @@ def test_refusals(cuda):
         bad("forward-mode", route, forward_ad.make_dual(x, x), 2)
         bad("forward-mode", ds.dispatch_rows, forward_ad.make_dual(x, x), r)
         bad("forward-mode", ds.combine_rows, y, r, forward_ad.make_dual(x, x))
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_logits_past_32_bits(cuda, renormalize):
+    """Rows that lie 2^20 elements apart: the bits of the same rows side by side, forward and backward."""
+    print("\n[case] far logits", flush=True)
+    close = torch.randn(4200, 24, device="cuda", generator=torch.Generator("cuda").manual_seed(8)).requires_grad_(True)
+    apart = torch.empty(4200, 1 << 20, device="cuda")[:, 5:29]
+    with torch.no_grad():
+        apart.copy_(close)
+    apart.requires_grad_(True)
+    bias = torch.linspace(-0.2, 0.2, 24, device="cuda")
+    a, b = (ds.route_rows(x, 3, bias=bias, renormalize=renormalize) for x in (close, apart))
+    for name in ("weights", "experts", "sizes", "places"):
+        assert torch.equal(getattr(a, name), getattr(b, name)), name
+    g = torch.arange(4200 * 3, device="cuda").float().cos().view(4200, 3)
+    assert torch.equal(torch.autograd.grad(a.weights, close, g)[0], torch.autograd.grad(b.weights, apart, g)[0])
