@@ -267,6 +267,8 @@ def lib():
         "dg_grouped_backward": (_i32, [GD] + [_p] * 8 + [_sz, _p]),
         "dg_grouped_apply": (_i32, [GD, _i32] + [_p] * 7),
         "dg_grouped_apply_backward": (_i32, [GD, _i32] + [_p] * 7),
+        "dg_grouped_apply_workspace_size": (_sz, [GD]),
+        "dg_grouped_apply_gradients": (_i32, [GD, _i32] + [_p] * 9 + [_sz, _p]),
         "dg_rotate_forward": (_i32, [RD] + [_p] * 9),
         "dg_rotate_workspace_size": (_sz, [RD]),
         "dg_rotate_backward": (_i32, [RD] + [_p] * 14 + [_sz, _p]),
@@ -290,8 +292,8 @@ def lib():
 _torch_layer = None
 _TORCH_LAYER = ("dg_last_error", "dg_rotate_forward", "dg_rotate_workspace_size", "dg_rotate_backward", "dg_route_workspace_size",
                 "dg_route_forward", "dg_route_backward", "dg_exchange_dispatch", "dg_exchange_combine",
-                "dg_exchange_combine_backward", "dg_grouped_forward", "dg_grouped_apply", "dg_grouped_apply_backward",
-                "dg_grouped_workspace_size", "dg_grouped_backward")
+                "dg_exchange_combine_backward", "dg_grouped_forward", "dg_grouped_apply", "dg_grouped_apply_workspace_size",
+                "dg_grouped_apply_gradients", "dg_grouped_workspace_size")
 
 
 def torch_layer():

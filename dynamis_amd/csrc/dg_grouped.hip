@@ -4,6 +4,9 @@
 //   dx[i] = W[g(i)]^T dy[i]   dW[g] = sum_{i in g} dy[i] x[i]^T   db[g] = sum_{i in g} dy[i]
 // and with an activation f and a residual r, in the epilogue of the same product (z is y above)
 //   y[i] = f(z[i]) + r[i]     dz[i] = dy[i] f'(z[i]), which takes dy's place above     dr = dy
+// In bfloat16 dz goes on as two of them, its rounding and what that left (16 bits and their sign), and the products
+// that take it sum over both: gradients are then as near to 64 bits as their own rounding (0.0017 of their norm; with dz
+// rounded to one 0.0024, and a training step of 128 groups of 250 rows of 256 by 256 in 117 us, with two 143).
 //
 // Tiles of 128 x 128 on the matrix units, 32 x 32 a step, sums in 32 bits.  Both operands pass
 // through LDS in rows of 128 bytes along the summed index (64 bfloat16 or 32 float), in chunks
@@ -57,9 +60,11 @@ constexpr int kSlab = kRowBytes / (int)sizeof(T);  // summed indices of a slab
 
 struct Args {
     const void* a;  // [rows, depth] (forward, dx); dy (dW)
+    const void* a_low;  // what is added to it, where it comes in two parts
     const void* b;  // weights [groups, ...]; x (dW)
     const void* bias;
     void* out;
+    void* out_low;    // (dz) what its rounding left, or NULL
     const void* aux;  // of out's layout: the residual, or dy (dz)
     int act;
     const int64_t* sizes;
@@ -280,13 +285,20 @@ __device__ __forceinline__ void begin_with(f32x16 (&acc)[2][2], const T* bias, i
         }
 }
 
+// What a rounding to bfloat16 leaves (of what is not finite then: nothing, or it would make a NaN of an infinity).
+__device__ __forceinline__ float left_over(float v)
+{
+    const float h = (float)(__bf16)v;
+    return fabsf(h) <= 3.4e38f ? v - h : 0.0f;
+}
+
 // A wave's 64 x 64 of the result to memory: in the accumulators a lane holds four neighbouring
-// columns of one row, which LDS turns into whole chunks of rows.  `s` is the wave's own.
+// columns of one row, which LDS turns into whole chunks of rows.  `s` is the wave's own.  LOW: what the rounding leaves.
 constexpr int kOutRows = 32;
 template <typename T>
 constexpr int kOutPitch = 64 * (int)sizeof(T) + 16;
 
-template <typename T, int EPI = kPlain>
+template <typename T, int EPI = kPlain, bool LOW = false>
 __device__ __forceinline__ void write_out(const f32x16 (&acc)[2][2], char* s, int lane, T* out, int64_t ld, int n_rows,
                                           int n_cols, const T* bias, const T* aux = nullptr, int act = 0)
 {
@@ -317,7 +329,7 @@ __device__ __forceinline__ void write_out(const f32x16 (&acc)[2][2], char* s, in
                     *(f32x4*)(s + x * kOutPitch<T> + col * 4) = v;
                 } else {
                     __attribute__((ext_vector_type(4))) __bf16 y;
-                    for (int c = 0; c < 4; ++c) y[c] = (__bf16)v[c];
+                    for (int c = 0; c < 4; ++c) y[c] = (__bf16)(LOW ? left_over(v[c]) : v[c]);
                     *(decltype(y)*)(s + x * kOutPitch<T> + col * 2) = y;
                 }
             }
@@ -455,8 +467,9 @@ __device__ __forceinline__ int64_t xcd_order(int64_t b, int64_t n)
     return b % kXcds * (n / kXcds) + b / kXcds;
 }
 
-// result[i, j] = sum_c a[i, c] W(j, c) (+ bias[j]), W(j, c) at weight[g][j][c], or (DX) [g][c][j].
-template <typename T, bool DX, int EPI>
+// result[i, j] = sum_c a[i, c] W(j, c) (+ bias[j]), W(j, c) at weight[g][j][c], or (DX) [g][c][j].  PARTS: of a, each
+// with all of the summed indices, one part after the other.
+template <typename T, bool DX, int EPI, int PARTS>
 __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
 {
     __shared__ __attribute__((aligned(16))) char s_a[kSlabBytes], s_b[kSlabBytes];
@@ -475,15 +488,17 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
     if (u < end) {
         Place p = locate<4>(a, cuts, u / col_tiles, s_w, &s_p);
         int64_t group = scalar64(p.group), piece = scalar64(p.piece), row = scalar64(p.row), size = scalar64(p.size);
-        const int slabs = (a.depth + kSlab<T> - 1) / kSlab<T>;
+        const int slabs = (a.depth + kSlab<T> - 1) / kSlab<T>, all_slabs = PARTS * slabs;
         using SA = Stage<T, false>;
         using SB = Stage<T, DX>;
         u32x4 r[8];
         auto fetch = [&](int64_t uu, int slab) {
             const int col = (int)(uu % col_tiles) * kTile;
             const int64_t r0 = row + piece * kTile;
+            const bool low = PARTS == 2 && slab >= slabs;
+            if (low) slab -= slabs;
             if (first_half)
-                SA::load(r, (const T*)a.a + r0 * a.depth, a.depth,
+                SA::load(r, (const T*)(low ? a.a_low : a.a) + r0 * a.depth, a.depth,
                         (int)max((int64_t)0, min(min(size - piece * kTile, a.rows - r0), (int64_t)kTile)), slab * kSlab<T>,
                         a.depth, t);
             else {
@@ -502,12 +517,12 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
             f32x16 acc[2][2] = {};
             if constexpr (EPI != kPlain)  // (as stream_kernel has it: the same bits)
                 if (a.bias) begin_with(acc, (const T*)a.bias + my_group * a.cols, col + (w / 2) * 64, a.cols, lane);
-            for (int slab = 0; slab < slabs; ++slab) {
+            for (int slab = 0; slab < all_slabs; ++slab) {
                 __syncthreads();
                 if (first_half) SA::store(r, s_a, t);
                 else SB::store(r, s_b, t);
                 __syncthreads();
-                if (slab + 1 < slabs) {
+                if (slab + 1 < all_slabs) {
                     fetch(u, slab + 1);
                 } else {  // the next unit's first slab
                     ++u;
@@ -530,6 +545,10 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
             write_out<T, EPI>(acc, s_out + w * kOutRows * kOutPitch<T>, lane, (T*)a.out + at, a.cols, n_rows - r0, a.cols - c0,
                               !DX && EPI == kPlain && a.bias ? (const T*)a.bias + my_group * a.cols + c0 : nullptr,
                               EPI != kPlain && a.aux ? (const T*)a.aux + at : nullptr, a.act);
+            if constexpr (EPI == kSlope && sizeof(T) == 2)
+                if (a.out_low)
+                    write_out<T, EPI, true>(acc, s_out + w * kOutRows * kOutPitch<T>, lane, (T*)a.out_low + at, a.cols, n_rows - r0,
+                                            a.cols - c0, nullptr, (const T*)a.aux + at, a.act);
         }
     }
     // rows of no group
@@ -563,7 +582,7 @@ __device__ __forceinline__ Buffer buffer_of(const void* p, int64_t bytes)
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)min(bytes, (int64_t)kOutside), 0x00020000);
 }
 
-template <typename T, bool DX, int PN, int EPI>
+template <typename T, bool DX, int PN, int EPI, int PARTS>
 __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool single)
 {
     __shared__ __attribute__((aligned(16))) char s_panel[65536];
@@ -621,7 +640,9 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
         // a lane loads a chunk of 16 bytes of each eighth row of 256: rows 4 i + quarter
         u32x4 r[8];
         auto fetch = [&](int64_t first_row, int n_rows, int step) {
-            const Buffer b = buffer_of((const char*)a.a + first_row * ld, n_rows * ld);
+            const bool low = PARTS == 2 && step >= steps;
+            if (low) step -= steps;
+            const Buffer b = buffer_of((const char*)(low ? a.a_low : a.a) + first_row * ld, n_rows * ld);
             const int at = step * kStepBytes + chunk * 16;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -646,14 +667,14 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                         const f32x4 f = *(const f32x4*)(s_bias + 32 * t + 8 * q + 4 * half);
                         for (int k = 0; k < 4; ++k) acc[t][4 * q + k] = f[k];
                     }
-            for (int step = 0; step < steps; ++step) {
+            for (int at_step = 0; at_step < PARTS * steps; ++at_step) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int rr = 4 * i + quarter;
                     *(u32x4*)(my_x + rr * kStepBytes + (chunk ^ (rr & 15)) * 16) = r[i];
                 }
-                if (step + 1 < steps) {
-                    fetch(r0, n_rows, step + 1);
+                if (at_step + 1 < PARTS * steps) {
+                    fetch(r0, n_rows, at_step + 1);
                 } else {
                     ++u;
                     if (u < end) {
@@ -668,6 +689,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                         fetch(r0, n_rows, 0);
                     }
                 }
+                const int step = PARTS == 2 && at_step >= steps ? at_step - steps : at_step;
                 const char* panel = s_panel + step * 2 * PN * kRowBytes;
                 const int inner = min(2, slabs - 2 * step);  // slabs of 128 bytes in this step
                 for (int b = 0; b < inner; ++b)
@@ -732,6 +754,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                 constexpr int kWide = PN < 64 ? PN : 64, kPieces = PN / kWide, kChunks = kWide / C, kEach = kStripRows * kChunks / 64;
                 const Buffer out = buffer_of((const char*)a.out + my_row * ld_out, my_rows * ld_out);
                 const Buffer in = buffer_of((const char*)a.aux + my_row * ld_out, a.aux ? my_rows * ld_out : 0);
+                const Buffer low = buffer_of((const char*)a.out_low + my_row * ld_out, a.out_low ? my_rows * ld_out : 0);
                 const int c = lane % kChunks, r_first = lane / kChunks;
 #pragma unroll
                 for (int piece_at = 0; piece_at < kPieces; ++piece_at) {
@@ -774,6 +797,13 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
                             y = __builtin_bit_cast(u32x4, f);
                         }
                         __builtin_amdgcn_raw_buffer_store_b128(y, out, at == kOutside ? at : rr * (int)ld_out + at, 0, 0);
+                        if constexpr (EPI == kSlope && sizeof(T) == 2)
+                            if (a.out_low) {
+                                bf16x8 f;
+                                for (int i = 0; i < 8; ++i) f[i] = (__bf16)left_over(v[i]);
+                                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f), low,
+                                                                       at == kOutside ? at : rr * (int)ld_out + at, 0, 0);
+                            }
                     }
                     wave_sync();
                 }
@@ -791,8 +821,8 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args a, bool 
 // first column tile's workgroups sum dy itself.  Groups of one item write their result,
 // others partial sums that weight_join_kernel adds up in order.  128 groups of 250 rows, 256 by 512:
 // 40 us, bound by the turning of both operands in registers (each is read twice to four times, from
-// L2): 83 MB in and out, 2.1 TB/s.
-template <typename T>
+// L2): 83 MB in and out, 2.1 TB/s.  PARTS of dy: its rows once for each, and x's again.
+template <typename T, int PARTS>
 __global__ __launch_bounds__(256, 2) void weight_kernel(Args a, int64_t max_items)
 {
     __shared__ __attribute__((aligned(16))) char s_a[kSlabBytes], s_b[kSlabBytes];
@@ -819,16 +849,19 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(Args a, int64_t max_item
     using S = Stage<T, true>;
     u32x4 st[S::R];
     float col_sum[8 / C][C] = {};
+    const int64_t span = PARTS == 1 ? n_rows : (n_rows + kSlab<T> - 1) / kSlab<T> * kSlab<T>, end = PARTS * span;
     auto fetch = [&](int64_t r) {
+        const bool low = PARTS == 2 && r >= span;
+        if (low) r -= span;
         const int left = (int)min(n_rows - r, (int64_t)kSlab<T>);
         if (first_half)
-            S::load(st, (const T*)a.a + (r0 + r) * a.cols + n0, a.cols, min(a.cols - n0, kTile), 0, left, t);
+            S::load(st, (const T*)(low ? a.a_low : a.a) + (r0 + r) * a.cols + n0, a.cols, min(a.cols - n0, kTile), 0, left, t);
         else
             S::load(st, (const T*)a.b + (r0 + r) * a.depth + k0, a.depth, min(a.depth - k0, kTile), 0, left, t);
     };
     f32x16 acc[2][2] = {};
     if (n_rows > 0) fetch(0);
-    for (int64_t r = 0; r < n_rows; r += kSlab<T>) {
+    for (int64_t r = 0; r < end; r += kSlab<T>) {
         __syncthreads();
         S::store(st, first_half ? s_a : s_b, t);
         if (sums && first_half) {
@@ -843,7 +876,7 @@ __global__ __launch_bounds__(256, 2) void weight_kernel(Args a, int64_t max_item
                     }
         }
         __syncthreads();
-        if (r + kSlab<T> < n_rows) fetch(r + kSlab<T>);
+        if (r + kSlab<T> < end) fetch(r + kSlab<T>);
         multiply<T>(s_b, s_a, (w / 2) * 64, (w % 2) * 64, lane, acc);
     }
     const bool whole = cuts.of(size) == 1;
@@ -987,16 +1020,16 @@ dg_status launched(const char* what)
 constexpr int kCus = 256;
 int64_t stream_tiles(const Args& a) { return a.rows / kStreamRows + std::min(a.groups, a.rows) + 1; }
 
-template <typename T, bool DX, int PN, int EPI>
+template <typename T, bool DX, int PN, int EPI, int PARTS>
 void run_stream(const Args& a, hipStream_t s)
 {
     const int64_t panels = (a.cols + PN - 1) / PN, tiles = stream_tiles(a);
     const int64_t lanes = std::max<int64_t>(1, std::min<int64_t>(tiles, kCus / panels));
-    hipLaunchKernelGGL((stream_kernel<T, DX, PN, EPI>), dim3((unsigned)(panels * lanes)), dim3(64 * kStreamWaves), 0, s, a,
+    hipLaunchKernelGGL((stream_kernel<T, DX, PN, EPI, PARTS>), dim3((unsigned)(panels * lanes)), dim3(64 * kStreamWaves), 0, s, a,
                        lanes == tiles);
 }
 
-template <typename T, bool DX, int EPI = kPlain>
+template <typename T, bool DX, int EPI = kPlain, int PARTS = 1>
 void run_rows(const Args& a, hipStream_t s)
 {
     // Whole chunks and a panel that fits: the streaming kernel (128 by 128 in bfloat16, 864 rows: 6.3
@@ -1006,29 +1039,30 @@ void run_rows(const Args& a, hipStream_t s)
     // rows 13.9, 12.6 and 11.1 us).  Rows of more than 512 bytes leave the panel's LDS 64 columns.
     const int64_t bytes = a.depth * (int64_t)sizeof(T);
     const bool whole = bytes % 16 == 0 && a.cols % kChunk<T> == 0 && ((uintptr_t)a.a & 15) == 0 &&
-                       ((uintptr_t)a.out & 15) == 0 && ((uintptr_t)a.aux & 15) == 0 && a.cols * (int64_t)sizeof(T) <= 1 << 24;
+                       ((uintptr_t)a.out & 15) == 0 && ((uintptr_t)a.aux & 15) == 0 && ((uintptr_t)a.a_low & 15) == 0 &&
+                       ((uintptr_t)a.out_low & 15) == 0 && a.cols * (int64_t)sizeof(T) <= 1 << 24;
     if (whole && bytes <= 1024) {
         const int64_t work = stream_tiles(a) * ((a.cols + 127) / 128);  // workgroups with panels of 128
-        if (work <= kCus / 4) run_stream<T, DX, 32, EPI>(a, s);
-        else if (bytes > 512 || work <= kCus / 2) run_stream<T, DX, 64, EPI>(a, s);
-        else run_stream<T, DX, 128, EPI>(a, s);
+        if (work <= kCus / 4) run_stream<T, DX, 32, EPI, PARTS>(a, s);
+        else if (bytes > 512 || work <= kCus / 2) run_stream<T, DX, 64, EPI, PARTS>(a, s);
+        else run_stream<T, DX, 128, EPI, PARTS>(a, s);
         return;
     }
 
     const int64_t tiles = (a.rows / kTile + std::min(a.groups, a.rows) + 1) * ((a.cols + kTile - 1) / kTile);
     unsigned grid = (unsigned)std::min<int64_t>(tiles, 256 * 2);
     if (grid > kXcds) grid = (grid + kXcds - 1) / kXcds * kXcds;
-    hipLaunchKernelGGL((rows_kernel<T, DX, EPI>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((rows_kernel<T, DX, EPI, PARTS>), dim3(grid), dim3(256), 0, s, a);
 }
 
-template <typename T>
+template <typename T, int PARTS = 1>
 void run_weight(const Args& a, hipStream_t s)
 {
     const int64_t tiles = (int64_t)((a.cols + kTile - 1) / kTile) * ((a.depth + kTile - 1) / kTile);
     const int64_t items = a.rows / a.chunk + a.groups;
     int64_t grid = items * tiles;
     if (grid > kXcds) grid = (grid + kXcds - 1) / kXcds * kXcds;
-    hipLaunchKernelGGL(weight_kernel<T>, workgroups(grid), dim3(256), 0, s, a, items);
+    hipLaunchKernelGGL((weight_kernel<T, PARTS>), workgroups(grid), dim3(256), 0, s, a, items);
     const int64_t split = std::min(a.groups, a.rows / a.chunk);  // groups above an item, at most
     if (split > 0) {
         // (most of a large number find no group: one round of workgroups, each with more to do)
@@ -1065,7 +1099,7 @@ dg_status dg_grouped_forward(const dg_grouped_desc* d, const void* x, const void
 }
 
 static dg_status apply(const dg_grouped_desc* d, int32_t act, bool slope, const void* x, const void* weight, const int64_t* sizes,
-                       const void* bias, const void* aux, void* out, hipStream_t s)
+                       const void* bias, const void* aux, void* out, void* out_low, hipStream_t s)
 {
     dg_status st = check(d);
     if (st != DG_OK) return st;
@@ -1079,6 +1113,7 @@ static dg_status apply(const dg_grouped_desc* d, int32_t act, bool slope, const 
     a.aux = aux;
     a.act = act;
     a.out = out;
+    a.out_low = out_low;
     a.sizes = sizes;
     a.rows = d->n_rows;
     a.groups = d->n_groups;
@@ -1097,13 +1132,13 @@ static dg_status apply(const dg_grouped_desc* d, int32_t act, bool slope, const 
 dg_status dg_grouped_apply(const dg_grouped_desc* d, int32_t act, const void* x, const void* weight, const int64_t* sizes,
                            const void* bias, const void* residual, void* y, hipStream_t s)
 {
-    return apply(d, act, false, x, weight, sizes, bias, residual, y, s);
+    return apply(d, act, false, x, weight, sizes, bias, residual, y, nullptr, s);
 }
 
 dg_status dg_grouped_apply_backward(const dg_grouped_desc* d, int32_t act, const void* x, const void* weight,
                                     const int64_t* sizes, const void* bias, const void* grad_y, void* dz, hipStream_t s)
 {
-    return apply(d, act, true, x, weight, sizes, bias, grad_y, dz, s);
+    return apply(d, act, true, x, weight, sizes, bias, grad_y, dz, nullptr, s);
 }
 
 size_t dg_grouped_workspace_size(const dg_grouped_desc* d)
@@ -1112,31 +1147,28 @@ size_t dg_grouped_workspace_size(const dg_grouped_desc* d)
     return layout(d).total;
 }
 
-dg_status dg_grouped_backward(const dg_grouped_desc* d, const void* x, const void* weight, const int64_t* sizes,
-                              const void* grad_y, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes,
-                              hipStream_t s)
+// The gradients from those of the product's results, in one part or two (grad_low; 8 and 16 bits apart, bfloat16).
+static dg_status backward(const dg_grouped_desc* d, const void* x, const void* weight, const int64_t* sizes, const void* grad,
+                          const void* grad_low, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes, hipStream_t s)
 {
-    dg_status st = check(d);
-    if (st != DG_OK) return st;
     const Layout L = layout(d);
-    if (!sizes || (d->n_rows > 0 && (!x || !weight || !grad_y)))
-        return fail(DG_ERR_INVALID, "inputs are NULL");
     Args a = {};
     a.sizes = sizes;
     a.rows = d->n_rows;
     a.groups = d->n_groups;
+    a.a = grad;
+    a.a_low = grad_low;
     if (dx && d->n_rows > 0) {
-        a.a = grad_y;
         a.b = weight;
         a.out = dx;
         a.cols = d->k;
         a.depth = d->n;
-        if (d->dtype == DG_BF16) run_rows<__bf16, true>(a, s);
-        else run_rows<float, true>(a, s);
+        if (d->dtype != DG_BF16) run_rows<float, true>(a, s);
+        else if (grad_low) run_rows<__bf16, true, kPlain, 2>(a, s);
+        else run_rows<__bf16, true>(a, s);
     }
     if (dweight) {
         if (!ws || ws_bytes < L.total) return fail(DG_ERR_WORKSPACE, "workspace too small");
-        a.a = grad_y;
         a.b = x;
         a.out = dweight;
         a.dbias = dbias;
@@ -1145,12 +1177,52 @@ dg_status dg_grouped_backward(const dg_grouped_desc* d, const void* x, const voi
         a.chunk = rows_of_item(d);
         a.part = (float*)((char*)ws + L.o_part);
         a.part_bias = (float*)((char*)ws + L.o_bias);
-        if (d->dtype == DG_BF16) run_weight<__bf16>(a, s);
-        else run_weight<float>(a, s);
+        if (d->dtype != DG_BF16) run_weight<float>(a, s);
+        else if (grad_low) run_weight<__bf16, 2>(a, s);
+        else run_weight<__bf16>(a, s);
     } else if (dbias) {
         return fail(DG_ERR_INVALID, "dbias comes with dweight");
     }
     return launched("dg_grouped_backward");
+}
+
+dg_status dg_grouped_backward(const dg_grouped_desc* d, const void* x, const void* weight, const int64_t* sizes,
+                              const void* grad_y, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes,
+                              hipStream_t s)
+{
+    dg_status st = check(d);
+    if (st != DG_OK) return st;
+    if (!sizes || (d->n_rows > 0 && (!x || !weight || !grad_y)))
+        return fail(DG_ERR_INVALID, "inputs are NULL");
+    return backward(d, x, weight, sizes, grad_y, nullptr, dx, dweight, dbias, ws, ws_bytes, s);
+}
+
+// dz: float, or two of bfloat16
+static size_t dz_bytes(const dg_grouped_desc* d) { return al((size_t)d->n_rows * d->n * (d->dtype == DG_BF16 ? 2 : 4)); }
+
+size_t dg_grouped_apply_workspace_size(const dg_grouped_desc* d)
+{
+    if (check(d) != DG_OK) return 0;
+    return layout(d).total + dz_bytes(d) * (d->dtype == DG_BF16 ? 2 : 1);
+}
+
+dg_status dg_grouped_apply_gradients(const dg_grouped_desc* d, int32_t act, const void* x, const void* weight, const int64_t* sizes,
+                                     const void* bias, const void* grad_y, void* dx, void* dweight, void* dbias, void* ws,
+                                     size_t ws_bytes, hipStream_t s)
+{
+    dg_status st = check(d);
+    if (st != DG_OK) return st;
+    if (act == DG_ACT_NONE) return dg_grouped_backward(d, x, weight, sizes, grad_y, dx, dweight, dbias, ws, ws_bytes, s);
+    if (act != DG_ACT_SILU && act != DG_ACT_GELU) return fail(DG_ERR_INVALID, "unknown activation");
+    if (!sizes || (d->n_rows > 0 && (!x || !weight || !grad_y))) return fail(DG_ERR_INVALID, "inputs are NULL");
+    if (dbias && !dweight) return fail(DG_ERR_INVALID, "dbias comes with dweight");
+    const size_t each = dz_bytes(d), sums = dweight ? layout(d).total : 0, dzs = dg_grouped_apply_workspace_size(d) - layout(d).total;
+    if (!ws || ws_bytes < dzs + sums) return fail(DG_ERR_WORKSPACE, "workspace too small");
+    char* const dz = (char*)ws;
+    char* const low = d->dtype == DG_BF16 ? dz + each : nullptr;
+    st = apply(d, act, true, x, weight, sizes, bias, grad_y, dz, low, s);
+    if (st != DG_OK) return st;
+    return backward(d, x, weight, sizes, dz, low, dx, dweight, dbias, dz + dzs, sums, s);
 }
 
 }  // extern "C"

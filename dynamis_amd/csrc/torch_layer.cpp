@@ -39,9 +39,9 @@ struct Entries {
     decltype(&dg_exchange_combine_backward) exchange_combine_backward;
     decltype(&dg_grouped_forward) grouped_forward;
     decltype(&dg_grouped_apply) grouped_apply;
-    decltype(&dg_grouped_apply_backward) grouped_apply_backward;
+    decltype(&dg_grouped_apply_workspace_size) grouped_apply_workspace_size;
+    decltype(&dg_grouped_apply_gradients) grouped_apply_gradients;
     decltype(&dg_grouped_workspace_size) grouped_workspace_size;
-    decltype(&dg_grouped_backward) grouped_backward;
 } dg;
 
 void load(const std::map<std::string, uintptr_t>& at)
@@ -59,9 +59,9 @@ void load(const std::map<std::string, uintptr_t>& at)
     get(dg.exchange_combine_backward, "dg_exchange_combine_backward");
     get(dg.grouped_forward, "dg_grouped_forward");
     get(dg.grouped_apply, "dg_grouped_apply");
-    get(dg.grouped_apply_backward, "dg_grouped_apply_backward");
+    get(dg.grouped_apply_workspace_size, "dg_grouped_apply_workspace_size");
+    get(dg.grouped_apply_gradients, "dg_grouped_apply_gradients");
     get(dg.grouped_workspace_size, "dg_grouped_workspace_size");
-    get(dg.grouped_backward, "dg_grouped_backward");
 }
 
 void check(dg_status status, const char* what)
@@ -420,7 +420,7 @@ struct Grouped : torch::autograd::Function<Grouped> {
                           int64_t act, const OptTensor& residual)
     {
         const Tensor bias = value(bias_);
-        // (the backward pass makes z again: fewer bytes than keeping it)
+        // (the backward pass makes z again)
         ctx->save_for_backward({x, weight, sizes, bias});
         ctx->saved_data["act"] = act;
         ctx->saved_data["groups"] = weight.size(0);
@@ -448,23 +448,16 @@ struct Grouped : torch::autograd::Function<Grouped> {
         if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(bias.defined() ? 4 : 3)) dr = grads[0];
         if (need_x || need_w || need_b) {
             const auto d = grouped_of(x, weight);
-            const int64_t* count = (const int64_t*)sizes.data_ptr();
-            const hipStream_t stream = stream_of(x);
-            Tensor g = grads[0].contiguous();
-            if (act != DG_ACT_NONE) {
-                Tensor dz = plain(g);
-                check(dg.grouped_apply_backward(&d, act, x.data_ptr(), weight.data_ptr(), count, ptr(bias), g.data_ptr(), dz.data_ptr(), stream),
-                      "grouped_linear");
-                g = dz;
-            }
-            size_t size = 0;
+            const Tensor g = grads[0].contiguous();
             if (need_x) dx = plain(x);
-            if (need_w || need_b) {
-                dw = plain(weight);
-                ws = bytes(size = dg.grouped_workspace_size(&d), x);
-            }
+            if (need_w || need_b) dw = plain(weight);
             if (need_b) db = plain(bias);
-            check(dg.grouped_backward(&d, x.data_ptr(), weight.data_ptr(), count, g.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(ws), size, stream),
+            // (dz, and what the sums of the weight's gradient need)
+            const size_t sums = dg.grouped_workspace_size(&d);
+            const size_t size = (act == DG_ACT_NONE ? sums : dg.grouped_apply_workspace_size(&d)) - (need_w || need_b ? 0 : sums);
+            if (size) ws = bytes(size, x);
+            check(dg.grouped_apply_gradients(&d, act, x.data_ptr(), weight.data_ptr(), (const int64_t*)sizes.data_ptr(), ptr(bias),
+                                             g.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(ws), size, stream_of(x)),
                   "grouped_linear");
         }
         return once({dx, need_w ? dw : Tensor(), Tensor(), db, Tensor(), dr}, "grouped_linear");

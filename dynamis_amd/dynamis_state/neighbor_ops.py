@@ -471,7 +471,8 @@ def grouped_linear(x, weight, sizes, bias=None, activation=None, residual=None):
     activation f: None, "silu" (z / (1 + exp(-z))) or "gelu" (z times the normal distribution's share below z,
     by its error function); residual [rows, n] of x's type.  Both are taken in 32 bits on the way to
     memory, and y is rounded once.  Rows behind the last group give their residual.  The backward pass with an
-    activation makes z again from x and the weights, and rounds its gradient to x's type before the other products.
+    activation makes z again from x and the weights; z's gradient goes into the other products in 32 bits, for bfloat16
+    in two parts of 16.
 
     Differentiable in x, weight, bias and residual (once, in reverse: a tensor with a forward-mode tangent is
     refused).  Sums are float32, in a fixed order: results

@@ -509,8 +509,11 @@ dg_status dg_grouped_backward(const dg_grouped_desc* desc, const void* x, const 
  *   y[i] = f(z[i]) + residual[i]       residual like y or NULL (zeros)
  *   dz[i] = grad_y[i] f'(z[i])         z made again from x and the weights
  * DG_ACT_SILU: z / (1 + exp(-z)); DG_ACT_GELU: z times the normal distribution's share below z.  Rows behind
- * the last group give their residual; their dz is zero.  dz, rounded to dtype, is the grad_y of
- * dg_grouped_backward for the other gradients; that of the residual is grad_y itself. */
+ * the last group give their residual; their dz is zero.  dg_grouped_apply_backward gives dz rounded to
+ * dtype; dg_grouped_apply_gradients the gradients of dg_grouped_backward that go with dz, which it holds in its
+ * workspace (of dg_grouped_apply_workspace_size bytes, aligned to 256; without dweight
+ * dg_grouped_workspace_size fewer) in 32 bits, for DG_BF16 in two parts of 16; that of the residual is
+ * grad_y itself. */
 #define DG_ACT_NONE 0
 #define DG_ACT_SILU 1
 #define DG_ACT_GELU 2
@@ -520,6 +523,11 @@ dg_status dg_grouped_apply(const dg_grouped_desc* desc, int32_t activation, cons
 dg_status dg_grouped_apply_backward(const dg_grouped_desc* desc, int32_t activation, const void* x,
                                     const void* weight, const int64_t* sizes, const void* bias,
                                     const void* grad_y, void* dz, hipStream_t stream);
+size_t dg_grouped_apply_workspace_size(const dg_grouped_desc* desc);
+dg_status dg_grouped_apply_gradients(const dg_grouped_desc* desc, int32_t activation, const void* x,
+                                     const void* weight, const int64_t* sizes, const void* bias,
+                                     const void* grad_y, void* dx, void* dweight, void* dbias, void* workspace,
+                                     size_t workspace_bytes, hipStream_t stream);
 
 /* Heads of queries and keys, normalised one by one and rotated by their nodes' positions:
  *   n[c] = x[c] / sqrt(mean_c x[c]^2 + eps) * weight[c]     (norm != 0; else n = x)
