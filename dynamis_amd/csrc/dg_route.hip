@@ -222,7 +222,15 @@ __device__ __forceinline__ bool mine_is_worthy(const Args& a, const uint32_t (&k
     wave_sync();
     return rank < a.top_groups;
 }
-// By sums in 32 bits; near: whether another group's lies nearer than `apart`.
+// A group's worth in 32 bits, the sum of its two largest where there are two; past: whether it is no 32-bit number though
+// the group has members (infinities lie nowhere apart, and 64 bits may tell two such sums from each other).
+__device__ __forceinline__ float worth_of(const Args& a, float best, float second, bool& past)
+{
+    const float worth = a.group_best == 2 && second > -INFINITY ? best + second : best;
+    past = best > -INFINITY && !(fabsf(worth) < INFINITY);
+    return worth;
+}
+// By sums in 32 bits; near: whether another group's lies nearer than `apart`, or the group's is past 32 bits.
 template <int V>
 __device__ __forceinline__ bool mine_is_worthy(const Args& a, const float (&v)[V], int lane, int e0, float* s_worth, float apart,
                                                bool& near)
@@ -238,7 +246,8 @@ __device__ __forceinline__ bool mine_is_worthy(const Args& a, const float (&v)[V
         second = fmaxf(fminf(best, b), fmaxf(second, t));
         best = fmaxf(best, b);
     });
-    const float worth = a.group_best == 2 && second > -INFINITY ? best + second : best;
+    bool past;
+    const float worth = worth_of(a, best, second, past);
     if (e0 < a.n) s_worth[(lane & (a.lanes - 1)) / a.group_lanes] = worth;
     wave_sync();
     int rank = 0, around = 0;
@@ -248,7 +257,7 @@ __device__ __forceinline__ bool mine_is_worthy(const Args& a, const float (&v)[V
         around += fabsf(x - worth) <= apart;  // (its own among them)
     }
     wave_sync();
-    near = around > 1;
+    near = past || around > 1;
     return rank < a.top_groups;
 }
 
@@ -283,7 +292,7 @@ __device__ __forceinline__ uint64_t worthiest(const Args& a, const K (&worth)[V]
     wave_sync();
     return __ballot(l < a.groups && mine && rank < a.top_groups) >> (lane & ~(a.lanes - 1));
 }
-// The same by sums in 32 bits; near: whether the lane's group and another lie nearer than `apart`.
+// The same by sums in 32 bits; near: whether the lane's group and another lie nearer than `apart`, or its own is past them.
 template <int V>
 __device__ __forceinline__ uint64_t worthiest(const Args& a, const float (&v)[V], int lane, int e0, float* s_value, float* s_worth,
                                               float apart, bool& near)
@@ -294,6 +303,7 @@ __device__ __forceinline__ uint64_t worthiest(const Args& a, const float (&v)[V]
         if (e0 + i < a.n) s_value[e0 + i] = v[i];
     wave_sync();
     float worth = -INFINITY;
+    bool past = false;
     if (l < a.groups) {
         float best = -INFINITY, second = -INFINITY;
         for (int i = l * per; i < (l + 1) * per; ++i) {
@@ -301,7 +311,7 @@ __device__ __forceinline__ uint64_t worthiest(const Args& a, const float (&v)[V]
             second = __builtin_amdgcn_fmed3f(best, second, x);
             best = fmaxf(best, x);
         }
-        worth = a.group_best == 2 && second > -INFINITY ? best + second : best;
+        worth = worth_of(a, best, second, past);
         s_worth[l] = worth;
     }
     wave_sync();
@@ -313,7 +323,7 @@ __device__ __forceinline__ uint64_t worthiest(const Args& a, const float (&v)[V]
             around += fabsf(x - worth) <= apart;  // (its own among them)
         }
     wave_sync();
-    near = around > 1;
+    near = past || around > 1;
     return __ballot(l < a.groups && rank < a.top_groups) >> (lane & ~(a.lanes - 1));
 }
 
