@@ -346,13 +346,32 @@ struct Groups {
     }
 };
 
-// exp, from that of 2: its argument's rounding is |x| 2^-24 of it.  The sigmoid from exp(-|x|), which overflows
-// nowhere (where it is 0, at -103 and below, so is the sigmoid in 32 bits).
+// For what is chosen by: exp, from that of 2 (its argument's rounding is |x| 2^-24 of it, and beneath 2^-126 it is 0),
+// and the sigmoid from exp(-|x|), which overflows nowhere.  A row whose choice hangs on either's error is done again.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(1.44269504f * x); }
 __device__ __forceinline__ float sigmoid(float x)
 {
     const float e = exp_of(-fabsf(x)), r = __builtin_amdgcn_rcpf(1.0f + e);
     return x < 0.0f ? e * r : r;
+}
+
+// For what is returned: exp(x - y), the difference in two parts (exact together, so that a weight's digits do not go
+// with its logit's distance from the largest), and the sigmoid, which is 0 where it is in 32 bits.
+__device__ __forceinline__ float exp_between(float x, float y)
+{
+    const float d = x - y, b = d - x, e = expf(d);
+    return d > -200.0f ? fmaf(e, (x - (d - b)) - (y + b), e) : e;
+}
+__device__ __forceinline__ float exact_sigmoid(float x)
+{
+    const float e = expf(-fabsf(x));
+    return (x < 0.0f ? e : 1.0f) / (1.0f + e);
+}
+// A weight of logit c up to a factor that is the row's: 1 for the largest chosen, m, or above 1/2 (a sigmoid's, whose
+// exponential is taken relative to the largest's: far below zero all of them would vanish).
+__device__ __forceinline__ float share_of(const Args& a, float c, float m)
+{
+    return a.sigmoid ? exp_between(fminf(c, 0.0f), fminf(m, 0.0f)) / (1.0f + expf(-fabsf(c))) : exp_between(c, m);
 }
 
 // s of a row's logits, in 32 bits or 64.
@@ -533,18 +552,17 @@ __global__ __launch_bounds__(kThreads, HOW == kScores && V <= 8 ? 5 : 1) void ro
         const float c = !mine || e < 0 ? -INFINITY : SCORED && a.bias ? logit<T>(a, row, e) : pick.x;
         float w = 0.0f;
         if (a.renormalize) {
-            // (relative to the largest chosen: a sum that vanishes in 32 bits has no ratio.  Far below
-            // zero a sigmoid is exp(x) to 32 bits.)
+            // (relative to the largest chosen: a sum that vanishes in 32 bits has no ratio)
             float m = c;
             over_lanes(a.lanes, [&](auto&& other) {
                 const float y = as_float(other(as_bits(m)));
                 m = y > m || y != y ? y : m;
             });
-            if (e >= 0) w = a.sigmoid && !(m < -30.0f) ? sigmoid(c) : exp_of(c - m);
+            if (e >= 0) w = share_of(a, c, m);
             const float sum = sum_lanes(w, a.lanes);
-            if (e >= 0) w = w * __builtin_amdgcn_rcpf(sum);
+            if (e >= 0) w = w / sum;
         } else if (e >= 0) {
-            w = a.sigmoid ? sigmoid(c) : exp_of(c - top) * __builtin_amdgcn_rcpf(total);
+            w = a.sigmoid ? exact_sigmoid(c) : exp_between(c, top) / total;
         }
         if (mine) {
             a.experts[row * a.k + l] = e;
@@ -701,8 +719,8 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(Args a)
         float sum = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
+            sum += exp_of(x[i] - top);  // (as the forward pass has it)
             x[i] = expf(x[i] - top);
-            sum += x[i];
         }
         total = sum_lanes(sum, a.lanes);
     }
@@ -720,18 +738,18 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(Args a)
             m = y > m || y != y ? y : m;
         });
         float u = 0.0f;
-        if (taken) u = a.sigmoid && !(m < -30.0f) ? 1.0f / (1.0f + expf(-c)) : expf(c - m);
+        if (taken) u = share_of(a, c, m);
         const float sum = sum_lanes(u, a.lanes);
         if (taken) u = u / sum;
         dot = sum_lanes(u * g, a.lanes);
         d = u * (g - dot);
-        if (a.sigmoid) d = d / (1.0f + expf(c));  // 1 - s
+        if (a.sigmoid) d = d * exact_sigmoid(-c);  // 1 - s
     } else if (a.sigmoid) {
         // s (1 - s), from the smaller of the two sides' exponentials
         const float z = expf(-fabsf(c));
         d = g * z / ((1.0f + z) * (1.0f + z));
     } else {
-        d = taken ? g * (expf(c - top) / total) : 0.0f;
+        d = taken ? g * (exp_between(c, top) / total) : 0.0f;
         dot = sum_lanes(d, a.lanes);
     }
     if (taken) s_row[e] = d;
