@@ -1,5 +1,8 @@
 """Compile libdynamis_graph.so (gfx950) in-tree with hipcc, and _torch_layer.so, which calls it from torch.
 
+The library needs no torch: it is linked first, whatever becomes of _torch_layer.so.  Where there is no torch at
+all it is all that is built.
+
     python -m dynamis_amd.build            # or dynamis_amd.build.build()
 
 Flags: -ffp-contract=off keeps the canonical fp64 predicate's operation order exactly
@@ -42,7 +45,7 @@ def _run(cmd):
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     out = "\n".join(l for l in r.stdout.splitlines() if "packed-fp32-ops" not in l)
     if r.returncode != 0:
-        raise RuntimeError("hipcc failed:\n" + " ".join(cmd) + "\n" + out)
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n" + " ".join(cmd) + "\n" + out)
     return out
 
 
@@ -50,7 +53,10 @@ def _torch_layer() -> str:
     """The operators' calls from torch (host code alone): a module of the interpreter, on torch's C++ interface."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        return "no torch: _torch_layer.so is not built"
     from torch.utils import cpp_extension
 
     tmp = TORCH_LAYER + ".tmp"
@@ -70,15 +76,15 @@ def build(verbose: bool = False) -> str:
     os.makedirs(bdir, exist_ok=True)
     objs = [os.path.join(bdir, src.replace(".hip", ".o")) for src in SOURCES]
     with ThreadPoolExecutor(4) as pool:
-        jobs = [pool.submit(_torch_layer)]
-        jobs += [pool.submit(_run, [HIPCC, *FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]) for src, obj in zip(SOURCES, objs)]
-        for job in jobs:
-            out = job.result()
-            if verbose and out.strip():
-                print(out)
-    tmp = LIB + ".tmp"
-    _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs])
-    os.replace(tmp, LIB)
+        layer = pool.submit(_torch_layer)
+        jobs = [pool.submit(_run, [HIPCC, *FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]) for src, obj in zip(SOURCES, objs)]
+        out = [job.result() for job in jobs]
+        tmp = LIB + ".tmp"
+        out.append(_run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]))
+        os.replace(tmp, LIB)
+        out.append(layer.result())
+    if verbose:
+        print(*(text for text in out if text.strip()), sep="\n")
     return LIB
 
 
