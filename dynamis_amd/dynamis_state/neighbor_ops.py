@@ -188,6 +188,13 @@ def _rows_16(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _came_back(what, dev, *saved):
+    """Refuses a saved tensor that a hook gives back with another shape, dtype or device; its strides may be others."""
+    for t, shape, dtype in saved:
+        if t.shape != shape or t.dtype != dtype or t.device != dev:
+            raise RuntimeError(f"{what}: a saved tensor came back with another shape, dtype or device")
+
+
 def _new_like(t):
     """A contiguous tensor like t."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
@@ -253,10 +260,17 @@ class _Attention(torch.autograd.Function):
         dev = plan.device
         if plan.by_source is None:
             raise RuntimeError("neighbor_attention: the plan was made with backward=False")
-        grad = _rows_16(grad)
         # (its own: another backward pass of the same graph may be under way with another stride)
         d = L.AttentionDesc.from_buffer_copy(ctx.desc)
-        d.ld_g = grad.stride(0)
+        dtype, (targets, heads, dim) = grad.dtype, grad.shape
+        kv = (plan.num_nodes, d.kv_heads, dim)
+        _came_back("neighbor_attention", dev, (q, grad.shape, dtype), (k, kv, dtype), (v, kv, dtype),
+                   (out32, grad.shape, torch.float32), (norm, (targets, heads, 2), torch.float32))
+        if table is not None:
+            _came_back("neighbor_attention", dev, (table, (d.n_buckets, heads), torch.float32))
+            table = table.contiguous()
+        q, k, v, grad, out32, norm = _rows_16(q), _rows_16(k), _rows_16(v), _rows_16(grad), out32.contiguous(), norm.contiguous()
+        d.ld_q, d.ld_k, d.ld_v, d.ld_g = q.stride(0), k.stride(0), v.stride(0), grad.stride(0)
         to, fro = plan.by_target.byref, plan.by_source.byref
         with L.on_device(dev):
             stream = L.raw_stream(dev)
@@ -391,8 +405,11 @@ class _Grouped(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight, sizes = ctx.saved_tensors
         need_x, need_w, _, need_b = ctx.needs_input_grad
-        lib, dev, grad = L.lib(), x.device, grad.contiguous()
-        d = ctx.desc
+        d, dev, dtype = ctx.desc, grad.device, grad.dtype
+        _came_back("grouped_linear", dev, (x, (d.n_rows, d.k), dtype), (weight, (d.n_groups, d.n, d.k), dtype),
+                   (sizes, (d.n_groups,), torch.int64))
+        x, weight, sizes, grad = x.contiguous(), weight.contiguous(), sizes.contiguous(), grad.contiguous()
+        lib = L.lib()
         with L.on_device(dev):
             dx = torch.empty_like(x) if need_x else None
             dw = torch.empty_like(weight) if need_w or need_b else None
