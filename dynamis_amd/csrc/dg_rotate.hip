@@ -15,7 +15,8 @@
 // angles' sines are made once for an atom and serve all of its heads from LDS.  An angle is
 // worked out in turns in 64 bits and brought into half a turn before it is rounded: positions are
 // as far away as they like.  Where pairs lie P channels apart a channel's partner, at any P,
-// comes through LDS, in 32 bits.  All sums have one owner and one order.
+// comes through LDS, in 32 bits.  All sums have one owner and one order.  The gradient of positions that have
+// 64 bits is worked out in them from the inputs on, sines and mean squares included.
 //
 // 8 + 8 heads of 32 in bfloat16, 1M atoms: 396 us, 5.2 TB/s, what a copy reaches.  16 + 4 heads of 64, 32,000
 // atoms: forward 37 us (4.4 TB/s), backward 74 (3.3 TB/s), which its instructions bound (some 250 for a lane's
@@ -27,6 +28,7 @@
 #include <algorithm>
 #include <initializer_list>
 #include <string>
+#include <type_traits>
 
 #include "../../include/dynamis_graph.h"
 #include "dg_lanes.hpp"
@@ -44,12 +46,15 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 
 constexpr int kWaves = 4;
 constexpr int kMaxAxes = 8;
-// Workgroups, as many as are resident at once by their registers: each takes as many atoms as the others, so a
-// second round would leave most of the card idle (1M atoms forward: 404 us with 1536, 451 with 2048; backward of
-// 32,000 in bfloat16, three waves a SIMD: 73 us with 768, 89 with 1024).
+// Workgroups: each takes as many atoms as the others, so a second round of them would leave most of the card idle.
+// Measured in bfloat16: 1M atoms forward, interleaved, 404 us with 1536, 451 with 2048; backward of 32,000, pairs
+// apart, three waves a SIMD, 73 us with 768, 89 with 1024.  The other instances have the same or, backward,
+// as many as their registers let reside (float three to five waves a SIMD; wide two, in float three); 32,000 atoms,
+// 16 + 4 heads of 64, pairs apart and interleaved: forward 31 and 29 us, in float 62 and 62 (328 MB, a copy's rate); backward 66 and 56,
+// in float 103 and 102 (492 MB, 95 at a copy's rate), wide 114 and 103, in float 139 and 133.
 constexpr int kForwardBlocks = 1536;
 constexpr int kMaxBlocks = 1024;
-inline int backward_blocks(int32_t dtype) { return dtype == DG_BF16 ? 768 : kMaxBlocks; }
+inline int backward_blocks(int32_t dtype, bool wide) { return dtype == DG_BF16 ? (wide ? 512 : 768) : wide ? 768 : kMaxBlocks; }
 
 template <typename T>
 constexpr int kC = 16 / (int)sizeof(T);  // channels of a lane
@@ -110,10 +115,11 @@ __device__ __forceinline__ int axis_of(const Args& a, int j)
     return x;
 }
 
-// LDS of a wave: its atoms' cosines and sines (at most 32 C of them, whatever the head), and a word for each
-// channel in flight.  One word in nine is spare, so that lanes eight apart do not meet.
-template <typename T>
+// LDS of a wave: its atoms' cosines and sines (at most 32 C of them, whatever the head; WIDE: in 64 bits too), and
+// a word for each channel in flight.  One word in nine is spare, so that lanes eight apart do not meet.
+template <typename T, bool WIDE>
 struct Shared {
+    double2 turn64[WIDE ? 32 * kC<T> : 1];
     float2 turn[32 * kC<T>];
     float row[64 * kC<T> + 64 * kC<T> / 8];
 };
@@ -158,18 +164,26 @@ __device__ __forceinline__ float2 cos_sin(double turns)
     sincospif(2.0f * (float)(turns - rint(turns)), &sine, &cosine);
     return make_float2(cosine, sine);
 }
-template <typename T>
-__device__ __forceinline__ void make_turns(const Args& a, Angles& g, int64_t first, int64_t after, int lane, Shared<T>& s)
+template <typename T, bool WIDE>
+__device__ __forceinline__ void make_turns(const Args& a, Angles& g, int64_t first, int64_t after, int lane, Shared<T, WIDE>& s)
 {
+    auto put = [&](int i, double turns) {
+        s.turn[i] = cos_sin(turns);
+        if constexpr (WIDE) {
+            double sine, cosine;
+            sincospi(2.0 * (turns - rint(turns)), &sine, &cosine);
+            s.turn64[i] = make_double2(cosine, sine);
+        }
+    };
     if (a.batch * a.pairs <= 64) {
         const double at = g.next;
         prefetch(a, g, after);
-        if (g.t < a.batch) s.turn[lane] = cos_sin(at * g.freq);
+        if (g.t < a.batch) put(lane, at * g.freq);
     } else {
         for (int i = lane; i < a.batch * a.pairs; i += 64) {
             const int t = i / a.pairs, j = i - t * a.pairs;
             const double at = first + t < a.nodes ? position(a, (first + t) * a.axes + axis_of(a, j)) : 0.0;
-            s.turn[i] = cos_sin(at * ((double)a.freq[j] * Angles::kInverse));
+            put(i, at * ((double)a.freq[j] * Angles::kInverse));
         }
     }
     wave_sync();
@@ -202,8 +216,8 @@ struct Seat {
 // The lane's channels v turned by the angles (BACK: by their opposites), with HALVES through LDS.  BACK: `across`
 // is what a channel's n is multiplied by in the angle's gradient, g'_b for a pair's first and -g'_a for its
 // second (a lane makes its partner's g' itself, and needs not its n).
-template <typename T, bool HALVES, bool BACK>
-__device__ __forceinline__ void turn(const Args& a, const Seat<T, HALVES>& at, const float2* turns, Shared<T>& s,
+template <typename T, bool HALVES, bool BACK, bool WIDE>
+__device__ __forceinline__ void turn(const Args& a, const Seat<T, HALVES>& at, const float2* turns, Shared<T, WIDE>& s,
                                      const float (&v)[kC<T>], float (&y)[kC<T>], float (&across)[kC<T>])
 {
     constexpr int C = kC<T>;
@@ -242,6 +256,32 @@ __device__ __forceinline__ void turn(const Args& a, const Seat<T, HALVES>& at, c
     }
 }
 
+// What turn<BACK> calls `across`, times n, in 64 bits, added to `sum`: of gradients g and inputs x, r = 1 / rms.  The
+// partners' g are where turn left them.
+template <typename T, bool HALVES>
+__device__ __forceinline__ void add_slopes(const Args& a, const Seat<T, HALVES>& at, const double2* turns, const Shared<T, true>& s,
+                                           const float (&g)[kC<T>], const float (&x)[kC<T>], double r, const float* wt,
+                                           double (&sum)[kC<T>])
+{
+#pragma unroll
+    for (int i = 0; i < kC<T>; ++i) {
+        const int c = at.c0 + i;
+        if (c >= 2 * a.pairs) continue;
+        const double2 z = HALVES ? turns[at.partner[HALVES ? i : 0] >> 19] : turns[c / 2];
+        const double other = HALVES ? *(const float*)((const char*)s.row + (at.partner[HALVES ? i : 0] & 0xffff)) : g[i ^ 1];
+        const bool second = HALVES ? c >= a.pairs : i & 1;
+        const double theirs = fma(other, z.x, second ? g[i] * z.y : -(g[i] * z.y));
+        sum[i] = fma((double)x[i] * r * (double)wt[i], second ? -theirs : theirs, sum[i]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ double inverse_rms64(const Args& a, const float (&x)[kC<T>])
+{
+    double ss = 0;
+    for (int i = 0; i < kC<T>; ++i) ss = fma((double)x[i], (double)x[i], ss);
+    return 1.0 / sqrt(sum_lanes(ss, a.per) / a.dim + (double)a.eps);
+}
 template <typename T>
 __device__ __forceinline__ float inverse_rms(const Args& a, const float (&x)[kC<T>])
 {
@@ -285,11 +325,11 @@ __device__ __forceinline__ Part part_of(const Args& a, const Seat<T, HALVES>& at
 template <typename T, bool HALVES>
 __global__ __launch_bounds__(64 * kWaves) void forward_kernel(Args a)
 {
-    __shared__ Shared<T> shared[kWaves];
+    __shared__ Shared<T, false> shared[kWaves];
     __shared__ __attribute__((aligned(16))) float s_w[2 * 256];
     constexpr int C = kC<T>;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Shared<T>& s = shared[w];
+    Shared<T, false>& s = shared[w];
     load_weights<T>(a, s_w);
     const Seat<T, HALVES> at(a, lane);
     const int64_t stride = (int64_t)gridDim.x * kWaves * a.batch;
@@ -327,15 +367,16 @@ __global__ __launch_bounds__(64 * kWaves) void forward_kernel(Args a)
     }
 }
 
-template <typename T, bool HALVES>
+// WIDE: the positions' gradient in 64 bits, that of positions which have them.
+template <typename T, bool HALVES, bool WIDE>
 __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
 {
-    __shared__ Shared<T> shared[kWaves];
+    __shared__ Shared<T, WIDE> shared[kWaves];
     __shared__ __attribute__((aligned(16))) float s_w[2 * 256];
     __shared__ float s_sum[64 * kWaves * kC<T>];
     constexpr int C = kC<T>;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Shared<T>& s = shared[w];
+    Shared<T, WIDE>& s = shared[w];
     load_weights<T>(a, s_w);
     const Seat<T, HALVES> at(a, lane);
     const int group = a.per * a.at_once;
@@ -356,7 +397,9 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
     };
     uint32_t axes = 0;
     for (int i = 0; i < C; ++i) axes |= (uint32_t)(at.c0 + i < 2 * a.pairs ? axis_of(a, pair_of(i)) : 15) << 4 * i;
-    float sum_q[C] = {}, sum_k[C] = {}, dtheta[C] = {};
+    using F = typename std::conditional<WIDE, double, float>::type;
+    float sum_q[C] = {}, sum_k[C] = {};
+    F dtheta[C] = {};
     Cursor cursor{first, 0, 0};
     Part next = part_of(a, at, cursor);
     u32x4 next_x, next_g;
@@ -377,13 +420,19 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
             turn<T, HALVES, true>(a, at, turns, s, g, back, across);
             // (a lane without a head adds nothing: an angle or a scale that is not finite would make a NaN of its zeros)
             const float* wt = s_w + (p.is_q ? 0 : a.dim) + (at.c0 < a.dim ? at.c0 : 0);
+            if constexpr (WIDE) {
+                const double r = a.norm ? inverse_rms64<T>(a, x) : 1.0;
+                if (p.live) add_slopes<T, HALVES>(a, at, s.turn64 + (turns - s.turn), s, g, x, r, wt, dtheta);
+                wave_sync();
+            }
             float r = 1.0f;
             if (a.norm) {
                 r = inverse_rms<T>(a, x);
                 for (int i = 0; i < C; ++i) x[i] *= r;
             }
-            if (a.dpos && p.live)
-                for (int i = 0; i < C; ++i) dtheta[i] = fmaf(x[i] * wt[i], across[i], dtheta[i]);
+            if constexpr (!WIDE)
+                if (a.dpos && p.live)
+                    for (int i = 0; i < C; ++i) dtheta[i] = fmaf(x[i] * wt[i], across[i], dtheta[i]);
             if (a.norm) {
                 if (a.part && p.live) {
                     if (p.is_q)
@@ -402,17 +451,14 @@ __global__ __launch_bounds__(64 * kWaves) void backward_kernel(Args a)
             if (p.live)
                 *(u32x4*)((T*)(p.is_q ? a.oq : a.ok) + (p.node * (p.is_q ? a.heads : a.kv) + p.head) * a.dim + at.c0) = pack<T>(back);
             if (a.dpos && last) {
-                for (int i = 0; i < C; ++i) dtheta[i] *= a.freq[pair_of(i)];
+                for (int i = 0; i < C; ++i) dtheta[i] *= (F)a.freq[pair_of(i)];
                 for (int axis = 0; axis < a.axes; ++axis) {
-                    float sum = 0;
-                    for (int i = 0; i < C; ++i) sum += (axes >> 4 * i & 15) == (uint32_t)axis ? dtheta[i] : 0.0f;
+                    F sum = 0;
+                    for (int i = 0; i < C; ++i) sum += (axes >> 4 * i & 15) == (uint32_t)axis ? dtheta[i] : (F)0;
                     sum = sum_lanes(sum, group);
-                    if ((lane & (group - 1)) == 0 && p.node < a.nodes) {
-                        if (a.pos_dtype == DG_F64) ((double*)a.dpos)[p.node * a.axes + axis] = sum;
-                        else ((float*)a.dpos)[p.node * a.axes + axis] = sum;
-                    }
+                    if ((lane & (group - 1)) == 0 && p.node < a.nodes) ((F*)a.dpos)[p.node * a.axes + axis] = sum;
                 }
-                for (int i = 0; i < C; ++i) dtheta[i] = 0.0f;
+                for (int i = 0; i < C; ++i) dtheta[i] = 0;
             }
         }
         wave_sync();
@@ -564,11 +610,14 @@ void run_forward(const Args& a, bool interleaved, hipStream_t s)
 template <typename T>
 void run_backward(const Args& a, bool interleaved, void* dqw, void* dkw, hipStream_t s)
 {
-    const int64_t blocks = a.nodes ? blocks_of(a, backward_blocks(sizeof(T) == 2 ? DG_BF16 : DG_F32)) : 0;
+    const bool wide = a.dpos && a.pos_dtype == DG_F64;
+    const int64_t blocks = a.nodes ? blocks_of(a, backward_blocks(sizeof(T) == 2 ? DG_BF16 : DG_F32, wide)) : 0;
     if (blocks) {
         const dim3 grid((unsigned)blocks);
-        if (interleaved) hipLaunchKernelGGL((backward_kernel<T, false>), grid, dim3(64 * kWaves), 0, s, a);
-        else hipLaunchKernelGGL((backward_kernel<T, true>), grid, dim3(64 * kWaves), 0, s, a);
+        if (interleaved && wide) hipLaunchKernelGGL((backward_kernel<T, false, true>), grid, dim3(64 * kWaves), 0, s, a);
+        else if (interleaved) hipLaunchKernelGGL((backward_kernel<T, false, false>), grid, dim3(64 * kWaves), 0, s, a);
+        else if (wide) hipLaunchKernelGGL((backward_kernel<T, true, true>), grid, dim3(64 * kWaves), 0, s, a);
+        else hipLaunchKernelGGL((backward_kernel<T, true, false>), grid, dim3(64 * kWaves), 0, s, a);
     }
     if (a.part)
         hipLaunchKernelGGL(join_kernel<T>, dim3((a.dim + 15) / 16, 2), dim3(1024), 0, s, a.part, (int)blocks, a.dim, dqw, dkw,
@@ -608,7 +657,7 @@ size_t dg_rotate_workspace_size(const dg_rotate_desc* d)
 {
     if (check(d) != DG_OK) return 0;
     const Args a = make_args(d);
-    return (size_t)blocks_of(a, backward_blocks(d->dtype)) * 2 * a.dim * sizeof(float);
+    return (size_t)blocks_of(a, backward_blocks(d->dtype, false)) * 2 * a.dim * sizeof(float);  // (wide: no more)
 }
 
 dg_status dg_rotate_backward(const dg_rotate_desc* d, const void* q, const void* k, const void* positions,

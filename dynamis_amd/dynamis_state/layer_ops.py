@@ -112,7 +112,7 @@ def rotate_heads(q, k, positions, frequencies, sections=None, q_weight=None, k_w
     results are rounded once.  A mean square plus eps has to lie between 1e-38 and 3e38, or the head's result is
     zeros or not finite.  Returns (q, k) of the inputs' shapes and type, contiguous.
 
-    Differentiable in q, k, the weights and positions (in 32 bits, whatever their type), once, in reverse:
+    Differentiable in q, k, the weights and positions (in 32 bits, float64 positions in 64), once, in reverse:
     a tensor with a forward-mode tangent is refused, and so are frequencies that require a gradient.  Sums have
     a fixed order: results repeat bit for bit.
     """

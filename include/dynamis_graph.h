@@ -543,7 +543,7 @@ dg_status dg_grouped_apply_gradients(const dg_grouped_desc* desc, int32_t activa
  *   q_out, k_out contiguous, of dtype, rounded once.
  * Backward: dq, dk contiguous, of dtype; dpositions like positions or NULL; dq_weight, dk_weight like
  * the weights or NULL, for which the workspace of dg_rotate_workspace_size bytes is needed.  Sums are
- * float32 and in a fixed order: results repeat bit for bit.  Both enqueue work only. */
+ * float32 (dpositions of DG_F64: float64) and in a fixed order: results repeat bit for bit.  Both enqueue work only. */
 typedef struct dg_rotate_desc {
     int64_t n_targets;
     int64_t n_nodes;
