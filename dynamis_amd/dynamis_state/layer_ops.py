@@ -2,7 +2,7 @@
 normalised and rotated by the atoms' positions, rows routed to experts, taken into their order and
 back.
 
-    q, k = rotate_heads(q, k, positions, frequencies)     # before neighbor_attention
+    q, k = rotate_heads(q, k, positions, frequencies)     # before neighbor_attention (periodic cells: see there)
     routing = route_rows(grouped_linear(x, router, natoms), k=2)
     rows = dispatch_rows(x, routing)                      # in the experts' order
     rows = grouped_linear(rows, weight, routing.sizes)    # a weight for each expert
@@ -112,6 +112,10 @@ def rotate_heads(q, k, positions, frequencies, sections=None, q_weight=None, k_w
     results are rounded once.  A mean square plus eps has to lie between 1e-38 and 3e38, or the head's result is
     zeros or not finite.  Returns (q, k) of the inputs' shapes and type, contiguous.
 
+    Positions count as they are: an edge across the boundary of a periodic cell has the angle between the atoms
+    themselves, not that to the image, unless all images of an atom have the same angles: fractional
+    coordinates, positions @ inv(cell), and frequencies of 2 pi times whole numbers.
+
     Differentiable in q, k, the weights and positions (in 32 bits, float64 positions in 64), once, in reverse:
     a tensor with a forward-mode tangent is refused, and so are frequencies that require a gradient.  Sums have
     a fixed order: results repeat bit for bit.
@@ -136,7 +140,13 @@ class Routing:
     rows, num_experts, k;  weights [rows, k] float32;  experts [rows, k] int32 (-1: none);
     sizes [num_experts] int64, the rows of each expert, as ``grouped_linear`` takes them;
     places [rows, k] int32, where a choice lies in the experts' order (of a choice of none, -1 minus
-    its place behind the last)."""
+    its place behind the last): together a permutation of [0, rows * k).
+
+    ``dispatch_rows`` and ``combine_rows`` go by places and weights alone, which a caller may change or make.  A
+    place past the rows is left out and none is read or written out of bounds; but a row of the experts'
+    order that no place points to is not written (``dispatch_rows``' result there, and y's gradient in
+    ``combine_rows``, are what the memory held), and one that two point to holds either.  A choice is
+    dropped by turning its place p into -1 - p, which keeps the permutation."""
 
     def __init__(self, num_experts, weights, experts, sizes, places):
         (self.rows, self.k), self.num_experts = experts.shape, num_experts

@@ -607,7 +607,8 @@ dg_status dg_route_backward(const dg_route_desc* desc, const void* logits, const
                             const float* grad_weights, void* grad_logits, hipStream_t stream);
 
 /* Rows into the experts' order and back, by the places of dg_route_forward (a permutation of
- * [0, n_rows * k); one that points past them is left out):
+ * [0, n_rows * k); one that points past them is left out, and a row of the experts' order that none points
+ * to is not written):
  *   dispatch  out[places[i, j]] = x[i]; zeros in the rows of choices of none
  *   combine   out[i] = residual[i] + sum_j weights[i, j] y[places[i, j]] over the choices that are not
  *             of none; weights NULL: ones (so the gradient of a dispatch), residual NULL: zeros

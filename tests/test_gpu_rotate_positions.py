@@ -76,3 +76,22 @@ def test_other_gradients_are_the_same_bits(cuda, interleaved):
     d = step(at2, at2)[-1]
     keep = torch.arange(60) != 7
     assert torch.equal(d[keep], got[-1][keep]) and d[7].isnan().any()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_images_of_a_periodic_cell(cuda, interleaved):
+    """Fractional coordinates and whole waves: an atom's images have its angles, and a query and a key the same product
+    wherever the cell's boundary lies between them.  A frequency is off by half a step, 2^-24 of itself, a turn of it by 2 pi m
+    2^-24 for a wave number m; three turns of 4 waves, and 8 roundings of 2^-24 of the results' own."""
+    print(f"\n[case] images {interleaved}", flush=True)
+    g = torch.Generator().manual_seed(5)
+    q, k = torch.randn(30, 4, 32, generator=g).cuda(), torch.randn(30, 4, 32, generator=g).cuda()
+    frac = torch.rand(30, 3, generator=g, dtype=torch.float64).cuda()
+    freq = (2 * np.pi * torch.arange(5, dtype=torch.float64).repeat(3)).float().cuda()
+    shift = torch.randint(-3, 4, (30, 3), generator=g).cuda()
+    a, b = ds.rotate_heads(q, k, frac, freq, norm=False, interleaved=interleaved)
+    c, d = ds.rotate_heads(q, k, frac + shift, freq, norm=False, interleaved=interleaved)
+    tol = (3 * 2 * np.pi * 4 + 8) * 2.0 ** -24
+    for x, y, z in ((a, c, q), (b, d, k)):
+        pair = z.abs().amax(-1, keepdim=True) * 2
+        assert ((x - y).abs() <= tol * pair).all()

@@ -1,5 +1,5 @@
 """route_rows where its 32-bit arithmetic has little room: biases near the largest numbers, logits that lie far
-apart, sigmoids that vanish.
+apart, sigmoids that vanish; and choices that a caller drops.
 
 Tolerances, EPS = 2^-24 of a weight.  An exponential of a difference of logits, which is taken in two parts: 2 for
 the exponential and 1 for the second part.  A sigmoid's denominator 4 more (2 for its exponential, a sum and a quotient).  The
@@ -121,3 +121,23 @@ def test_sigmoids_that_vanish_beside_others(cuda):
             dx, = torch.autograd.grad(r.weights, xd, grad.cuda())
             dx = dx.double().cpu().numpy()
             assert (np.abs(dx - want["dlogits"]) <= 60 * EPS * want["mag"] + 16 * lost).all(), (renormalize, scale, dx, want["dlogits"])
+
+
+def test_a_dropped_choice_keeps_the_permutation(cuda):
+    """Its place p as -1 - p: its row is zeros, it adds nothing, and nothing is left unwritten."""
+    r = ds.route_rows(torch.randn(12, 4, device="cuda", generator=torch.Generator("cuda").manual_seed(1)), 2)
+    x = torch.randn(12, 24, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).requires_grad_(True)
+    places, weights = r.places.clone(), r.weights.detach().clone().requires_grad_(True)
+    places[5, 1] = -1 - places[5, 1]
+    few = ds.Routing(4, weights, r.experts, r.sizes, places)
+    rows = ds.dispatch_rows(x, few)
+    want = ds.dispatch_rows(x, r).detach().clone()
+    want[int(r.places[5, 1])] = 0
+    assert torch.equal(rows, want)
+    y = want.clone().requires_grad_(True)
+    out = ds.combine_rows(y, few)
+    assert torch.equal(out[5], weights[5, 0] * x[5])
+    dy, dw = torch.autograd.grad(out, [y, weights], torch.ones_like(out))
+    assert not dy[int(r.places[5, 1])].any() and dw[5, 1] == 0 and torch.isfinite(dy).all()
+    dx, = torch.autograd.grad(rows, x, torch.ones_like(rows))
+    assert (dx[5] == 1).all() and (dx[:5] == 2).all()
