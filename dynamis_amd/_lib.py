@@ -292,8 +292,8 @@ def lib():
 _torch_layer = None
 _TORCH_LAYER = ("dg_last_error", "dg_rotate_forward", "dg_rotate_workspace_size", "dg_rotate_backward", "dg_route_workspace_size",
                 "dg_route_forward", "dg_route_backward", "dg_exchange_dispatch", "dg_exchange_combine",
-                "dg_exchange_combine_backward", "dg_grouped_forward", "dg_grouped_apply", "dg_grouped_apply_workspace_size",
-                "dg_grouped_apply_gradients", "dg_grouped_workspace_size")
+                "dg_exchange_combine_backward", "dg_grouped_apply", "dg_grouped_apply_workspace_size", "dg_grouped_apply_gradients",
+                "dg_grouped_workspace_size")
 
 
 def torch_layer():

@@ -17,9 +17,10 @@
 // scan of them for each expert, and the ranks within a workgroup by matching lanes; nothing depends
 // on the order of atomics (counts alone are added up by them).
 //
-// Instructions bound it, not the bytes: 300,007 rows over 64 experts in 8 groups, 6 chosen with a bias, in float: 57 us
-// for the choices and 18 for the rows done again (98 MB: 19 us at a copy's rate), scan and places 5 and 12.  32,000
-// rows over 128 experts, 8 chosen, in bfloat16: 14, 3 and 5 us, backward 9.
+// Instructions bound it, not the bytes: 300,007 rows over 64 experts in 8 groups, 6 chosen with a bias, in float: 60 us
+// for the choices and 18 for the rows done again (98 MB: 19 us at a copy's rate), scan and places 5 and 11.  32,000
+// rows over 128 experts, 8 chosen, in bfloat16 (8 MB): 14, 5 and 4 us, backward 9: rounds of maxima over 16
+// lanes, one after the other, and launches.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -149,8 +150,8 @@ __device__ __forceinline__ void choose(const Args& a, K (&key)[V], int lane, int
 
 // Keys whose low bits may go hold their place among the lane's in them (the first the largest), in falling order:
 // then a round looks at each lane's first alone, and the winner's others move up.  The low bits may go where they say
-// nothing (a bfloat16's), or no more than `apart` allows for.  (300,007 rows over 64 experts, 8 a lane, 6 rounds: 64
-// us, 70 where each round looks through all.)
+// nothing (a bfloat16's), or no more than `apart` allows for.  (300,007 rows over 64 experts, 8 a lane, 6 rounds: 60
+// us; when it came, 64, and 70 where each round looked through all.)
 template <int V>
 __device__ __forceinline__ void sort_packed(uint32_t (&key)[V])
 {
@@ -397,10 +398,12 @@ __device__ __forceinline__ void scores(const Args& a, const float (&x)[V], float
 
 // kLogits: the logits are what is chosen by.  kScores: a bias, or groups worth a sum of scores.  What is chosen by
 // is then worked out in 32 bits; a row where two values that a choice or a group hangs on lie nearer than the
-// rounding, or are no numbers, is left to a second launch, kWide, which takes it in 64 (one of some hundred to
-// thousand).  300,007 rows over 64 experts in groups, chosen with a bias: 57 and 18 us; in one launch, where the wide
-// part's registers leave the other three waves a SIMD, 92.  What bounds kScores is instructions, some thousand for a
-// wave's eight rows; five waves a SIMD are worth the registers that spill (57 us, four 72).
+// rounding, or are no numbers, is left to a second launch, kWide, which takes it in 64.  That is one of some hundred to
+// thousand while the biases are small; what counts as near goes by the largest |bias| of all, so that one large entry
+// sends more there.  300,007 rows over 64 experts in groups, biases of some 0.1: 60 and 18 us, a call 89; with one entry of
+// -10 93, -100 101, -1e3 164, -1e4 (every row) 192 (a bias of -inf takes an expert out at no cost).  In one
+// launch, where the wide part's registers leave the other three waves a SIMD, 92.  What bounds kScores is
+// instructions, some thousand for a wave's eight rows; five waves a SIMD are worth the registers that spill (57 us, four 72).
 enum { kLogits, kScores, kWide };
 
 template <typename T, int V, int HOW>

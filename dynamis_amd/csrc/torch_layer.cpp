@@ -37,7 +37,6 @@ struct Entries {
     decltype(&dg_exchange_dispatch) exchange_dispatch;
     decltype(&dg_exchange_combine) exchange_combine;
     decltype(&dg_exchange_combine_backward) exchange_combine_backward;
-    decltype(&dg_grouped_forward) grouped_forward;
     decltype(&dg_grouped_apply) grouped_apply;
     decltype(&dg_grouped_apply_workspace_size) grouped_apply_workspace_size;
     decltype(&dg_grouped_apply_gradients) grouped_apply_gradients;
@@ -57,7 +56,6 @@ void load(const std::map<std::string, uintptr_t>& at)
     get(dg.exchange_dispatch, "dg_exchange_dispatch");
     get(dg.exchange_combine, "dg_exchange_combine");
     get(dg.exchange_combine_backward, "dg_exchange_combine_backward");
-    get(dg.grouped_forward, "dg_grouped_forward");
     get(dg.grouped_apply, "dg_grouped_apply");
     get(dg.grouped_apply_workspace_size, "dg_grouped_apply_workspace_size");
     get(dg.grouped_apply_gradients, "dg_grouped_apply_gradients");
