@@ -83,3 +83,50 @@ def test_what_is_not_finite_shows_as_such(cuda, k, n, act):
             assert (dx[50] == value).all() and torch.equal(dx[keep], want[0][keep])
             assert (dw[1, 7] == value).all() and db[1, 7] == value and torch.equal(dw[0], want[1][0])
             assert torch.equal(db[0], want[2][0])
+
+
+@ACTS
+@pytest.mark.parametrize("k,n", [(64, 96), (50, 70)])
+def test_only_what_is_asked(cuda, k, n, act):
+    """Each gradient alone has the bits that it has among the others (without the weight's the workspace is smaller)."""
+    x, w, b, grad = (t.cuda() for t in _make([33, 100, 0, 300], k, n, 4))
+    sizes = torch.tensor([33, 100, 0, 300]).cuda()
+    want = _grads(x, w, b, [33, 100, 0, 300], act, grad)
+    for i in range(3):
+        leaves = [t.detach().clone().requires_grad_(i == j) for j, t in enumerate((x, w, b))]
+        got, = torch.autograd.grad(ds.grouped_linear(*leaves[:2], sizes, leaves[2], activation=act), leaves[i], grad)
+        assert torch.equal(got, want[i])
+
+
+def test_steps_from_graphs_and_streams(cuda):
+    """Two captured training steps replayed in turn and on two streams, with eager work between, against eager steps."""
+    sizes = [60, 0, 130, 7]
+    n_rows = torch.tensor(sizes).cuda()
+    sets = [[t.cuda() for t in _make(sizes, 64, 96, seed)] for seed in (1, 2)]
+
+    def step(x, w, b, grad):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = ds.grouped_linear(leaves[0], leaves[1], n_rows, leaves[2], activation="gelu")
+        return [y.detach(), *torch.autograd.grad(y, leaves, grad)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*sets[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(*s))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(4):
+        for s in sets:
+            s[0].copy_(torch.randn(197, 64, device="cuda"))
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for s, out in zip(sets, outs):
+            assert all(torch.equal(a, b) for a, b in zip(out, step(*s))), i

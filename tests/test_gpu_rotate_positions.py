@@ -95,3 +95,28 @@ def test_images_of_a_periodic_cell(cuda, interleaved):
     for x, y, z in ((a, c, q), (b, d, k)):
         pair = z.abs().amax(-1, keepdim=True) * 2
         assert ((x - y).abs() <= tol * pair).all()
+
+
+def test_steps_from_graphs(cuda):
+    """Captured steps with float64 positions, replayed with eager work between, against eager steps."""
+    q, k, at, freq, qw, kw, gq, gk = (t.cuda() for t in _inputs(300, 400, 4, 2, 32, (5, 5, 5), torch.bfloat16, 10.0, 4))
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, at, qw, kw)]
+        out = ds.rotate_heads(*leaves[:3], freq, None, *leaves[3:])
+        return torch.autograd.grad(out, leaves, [gq, gk])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(4):
+        at.add_(0.37)
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
