@@ -568,9 +568,9 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Args a)
 // 2.2M rows of 128 by 128 in bfloat16: 232 us, 4.86 TB/s, what a copy reaches (4.9).  100,000 rows of
 // 256 by 256 floats: 135 us, 97 TFLOP/s of the 153 that a product of 8192 cubed reaches.
 // With an epilogue (200,003 rows of 256 by 512 in bfloat16, 16 groups; bytes at a copy's rate 60 us, products 44 at a
-// library's): silu 105 us, gelu 138, a residual 117; in float silu 462, gelu 494.  864 rows, 8 groups: 8 us, in float 17.  Four panels read x four times, from L2; the rest is
-// instructions, 14 a value for silu and 25 for gelu, next to the products at two waves a SIMD (16 waves with panels half
-// as wide: 168).
+// library's): silu 105 us, gelu 138, a residual 117; in float silu 462, gelu 494.  864 rows, 8 groups: 8 us, in float 17.
+// Four panels read x four times, from L2; the rest is instructions, 14 a value for silu and 25 for gelu, next to the
+// products at two waves a SIMD (16 waves with panels half as wide: 168).
 constexpr int kStreamWaves = 8;
 constexpr int kStripRows = 32;
 constexpr int kStreamRows = kStreamWaves * kStripRows;

@@ -50,8 +50,10 @@ constexpr int kMaxAxes = 8;
 // Measured in bfloat16: 1M atoms forward, interleaved, 404 us with 1536, 451 with 2048; backward of 32,000, pairs
 // apart, three waves a SIMD, 73 us with 768, 89 with 1024.  The other instances have the same or, backward,
 // as many as their registers let reside (float three to five waves a SIMD; wide two, in float three); 32,000 atoms,
-// 16 + 4 heads of 64, pairs apart and interleaved: forward 31 and 29 us, in float 62 and 62 (328 MB, a copy's rate); backward 66 and 56,
-// in float 103 and 102 (492 MB, 95 at a copy's rate), wide 114 and 103, in float 139 and 133.
+// 16 + 4 heads of 64, pairs apart and interleaved: forward 31 and 29 us, in float 62 and 62 (328 MB, a copy's rate);
+// backward 66 and 56, in float 103 and 102 (492 MB, 95 at a copy's rate), wide 114 and 103, in float 139 and 133 (with as many as without
+// 145 and 131, 173 and 163).  The norms' weights' gradients are summed by workgroup, so above 512 of them their last bits go
+// with whether float64 positions want a gradient.
 constexpr int kForwardBlocks = 1536;
 constexpr int kMaxBlocks = 1024;
 inline int backward_blocks(int32_t dtype, bool wide) { return dtype == DG_BF16 ? (wide ? 512 : 768) : wide ? 768 : kMaxBlocks; }

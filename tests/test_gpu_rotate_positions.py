@@ -78,6 +78,24 @@ def test_other_gradients_are_the_same_bits(cuda, interleaved):
     assert torch.equal(d[keep], got[-1][keep]) and d[7].isnan().any()
 
 
+def test_other_gradients_of_many_atoms(cuda):
+    """More atoms than workgroups at once: the heads' gradients have the same bits; the weights' are summed in another order,
+    each of 30,000 atoms and 4 heads' terms once, 2^-24 of their magnitudes for a term's place in a chain of some 200."""
+    q, k, at, freq, qw, kw, gq, gk = (t.cuda() for t in _inputs(30000, 30000, 4, 4, 32, (5, 5, 5), torch.float32, 10.0, 6))
+    leaves = [t.requires_grad_(True) for t in (q, k, qw, kw)]
+    atd = at.clone().requires_grad_(True)
+    out = []
+    for positions in (at, atd):
+        y = ds.rotate_heads(q, k, positions, freq, None, qw, kw)
+        out.append(torch.autograd.grad(y, leaves + ([positions] if positions is atd else []), [gq, gk]))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    for x, g, a, b in ((q, gq, out[0][2], out[1][2]), (k, gk, out[0][3], out[1][3])):
+        # (a turned gradient is at most |g_a| + |g_b|, a normalised channel at most sqrt(32) times its mean size)
+        hat = x.detach() / x.detach().pow(2).mean(-1, keepdim=True).sqrt()
+        mag = (hat.abs() * 2 * g.abs().amax(-1, keepdim=True)).sum((0, 1))
+        assert ((a - b).abs() <= 400 * 2.0 ** -24 * mag).all()
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_images_of_a_periodic_cell(cuda, interleaved):
     """Fractional coordinates and whole waves: an atom's images have its angles, and a query and a key the same product
